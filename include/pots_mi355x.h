@@ -406,6 +406,86 @@ int pots_store_load(uint32_t n_files, const char *const *paths, uint32_t n_segs,
                     const pots_store_segment *segs, void *dst, int dst_device, void *staging,
                     uint64_t staging_bytes, uint32_t n_threads);
 
+/* ---- The training pass's own operators ---------------------------------------------------
+ *
+ * Attention, the loss over a vocabulary and the embedding, each with its gradient, for a pass
+ * that is not captured: no attention probability and no logit is kept. Every pointer is device
+ * memory of the current device; the calls enqueue on `stream` and allocate nothing; `work` is
+ * scratch of at least the size the matching *_work call returns, aligned to 256 bytes, its
+ * contents neither read before nor kept after a call. Results do not depend on the order in
+ * which blocks run. They return POTS_E_OK, POTS_E_ARG (a size, type or stride out of range; no
+ * work enqueued) or POTS_E_HIP. */
+
+#define POTS_OP_F32 0
+#define POTS_OP_BF16 1
+
+#define POTS_ATTENTION_MAX_DIM 128
+
+/* One operand [batch, heads, n, head_dim]: elements between batches, heads and positions (a
+ * position's values are consecutive). */
+typedef struct pots_heads {
+  void *ptr;
+  int64_t batch, head, row;
+} pots_heads;
+
+/* Softmax attention of `batch` sequences of n positions over their own keys: `heads` query
+ * heads, each `heads / kv_heads` consecutive ones sharing a key head. Position i sees j where
+ * j < length, i < length and (causal) j <= i; lengths is int32 [batch] (values past n count as
+ * n, negative ones as 0), or null for n. A position that sees nothing has an output of zero,
+ * lse -inf and gradients of zero; what lies past a sequence's length is not read. lse and delta
+ * are fp32 [batch, heads, n], natural logarithms. */
+typedef struct pots_attention {
+  pots_heads q, k, v, out;
+  pots_heads dout, dq, dk, dv; /* backward only */
+  float *lse;                  /* forward: written; backward: read */
+  const int32_t *lengths;
+  uint32_t batch, heads, kv_heads, n, head_dim;
+  uint32_t dtype, causal;
+  float scale;
+} pots_attention;
+
+int pots_attention_forward(const pots_attention *a, void *stream);
+uint64_t pots_attention_backward_work(const pots_attention *a);
+int pots_attention_backward(const pots_attention *a, void *work, void *stream);
+
+/* Softmax cross entropy of feature rows x [rows, dim] against a vocabulary matrix w
+ * [vocab, dim]: loss_r = lse_r - x_r.w_t, fp32, with t the row's int64 target; 0 where t < 0, NaN where
+ * t >= vocab. Backward: dx and dw of sum_r weights_r loss_r; a row of weight zero or without a
+ * target counts for nothing, whatever its features. Rows of x, w, dx and dw are `*_row`
+ * elements apart. */
+typedef struct pots_vocab_loss {
+  const void *x, *w;
+  const int64_t *targets;
+  float *loss, *lse;    /* [rows]; forward: both written; backward: lse is read */
+  const float *weights; /* [rows], backward only */
+  void *dx, *dw;        /* backward only */
+  int64_t x_row, w_row, dx_row, dw_row;
+  uint32_t rows, dim, vocab, dtype;
+} pots_vocab_loss;
+
+uint64_t pots_vocab_loss_forward_work(const pots_vocab_loss *a);
+int pots_vocab_loss_forward(const pots_vocab_loss *a, void *work, void *stream);
+uint64_t pots_vocab_loss_backward_work(const pots_vocab_loss *a);
+int pots_vocab_loss_backward(const pots_vocab_loss *a, void *work, void *stream);
+
+/* Rows of a table [vocab, dim] by token, times scale: out_i = scale * table[ids_i] (NaN where
+ * ids_i is outside the table). Backward: table_v (+)= scale * the sum of rows_i over ids_i = v,
+ * taken in the order of i in fp32; with `add` it is added to what the table holds, without it
+ * every row is written. An id outside the table adds to nothing. */
+typedef struct pots_embedding {
+  const int64_t *ids;
+  void *table;
+  void *rows; /* forward: written; backward: read */
+  int64_t table_row, rows_row;
+  uint32_t tokens, dim, vocab, dtype;
+  uint32_t add;
+  float scale;
+} pots_embedding;
+
+int pots_embedding_forward(const pots_embedding *a, void *stream);
+uint64_t pots_embedding_backward_work(const pots_embedding *a);
+int pots_embedding_backward(const pots_embedding *a, void *work, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,607 @@
+// Softmax attention of a batch of sequences over their own keys, with its gradient, for
+// passes that keep no probabilities.
+//
+//   s_ij = scale·q_i·k_j over the j that i sees, lse_i = log Σ_j e^{s_ij}, p_ij = e^{s_ij − lse_i}
+//   o_i = Σ_j p_ij v_j
+//   D_i = do_i·o_i,  dp_ij = do_i·v_j,  ds_ij = p_ij (dp_ij − D_i)
+//   dq_i = scale Σ_j ds_ij k_j,  dk_j = scale Σ_i ds_ij q_i,  dv_j = Σ_i p_ij do_i
+//
+// with k and v shared by heads / kv_heads query heads, over which dk and dv are summed.
+//
+// Forward: one pass over the keys with a running maximum and sum. A wave holds 32 query rows as
+// the columns of its products (tiles.h): Sᵀ = K·Qᵀ leaves a row's scores in one lane and its
+// other half, and those registers are the right operand of Oᵀ += Vᵀ·Pᵀ as they are. K and V go
+// through LDS, shared by a block's waves; V is read transposed from it.
+//
+// Backward: the probabilities are recomputed from lse. dq sums over keys and dk, dv over
+// queries, so each has a kernel of its own whose sums stay in registers (attn_dq, which also
+// makes D, and attn_dkv): seven products of a tile where one kernel with atomics on dq would
+// take five, for results that do not depend on the order of blocks. Few key heads leave
+// attn_dkv with few blocks: then the query heads of a group are split over blocks, each with
+// fp32 sums of its own that attn_fold adds in order.
+//
+// Roundings: bf16 p and ds (the right operands of the second products) are rounded to bf16,
+// half a step 2^-9 each, random over the terms of a sum whose result is rounded the same;
+// scores, statistics and sums are fp32.
+#include <math.h>
+
+#include "common.h"
+#include "gmem.h"
+#include "tiles.h"
+
+namespace pots {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Sixteen bytes of row r (zero from `rows` on) from column c on (zero from `d` on). vec: rows
+// are 16-byte aligned and d is a multiple of a chunk.
+template <class T>
+__device__ __forceinline__ u32x4v load_chunk(const typename T::elem* base, int64_t stride,
+                                             uint32_t r, uint32_t rows, uint32_t c, uint32_t d,
+                                             bool vec) {
+  constexpr uint32_t CE = 16 / sizeof(typename T::elem);
+  u32x4v x = {0, 0, 0, 0};
+  if (r >= rows || c >= d) return x;
+  const typename T::elem* p = base + (int64_t)r * stride + c;
+  if (vec) return gload<u32x4v>(p);
+#pragma unroll
+  for (uint32_t j = 0; j < CE; j++) {
+    if (c + j >= d) continue;
+    if constexpr (sizeof(typename T::elem) == 2) {
+      const uint32_t e = gload<uint16_t>(p + j);
+      x[j / 2] |= e << (16 * (j % 2));
+    } else {
+      x[j] = gload<uint32_t>(p + j);
+    }
+  }
+  return x;
+}
+
+template <class T>
+__device__ __forceinline__ typename T::frag load_frag(const typename T::elem* base,
+                                                      int64_t stride, uint32_t r, uint32_t rows,
+                                                      uint32_t c, uint32_t d, bool vec) {
+  if constexpr (sizeof(typename T::elem) == 2) {
+    return __builtin_bit_cast(bf16x8, load_chunk<T>(base, stride, r, rows, c, d, vec));
+  } else {
+    const f32x4 a = __builtin_bit_cast(f32x4, load_chunk<T>(base, stride, r, rows, c, d, vec));
+    const f32x4 b =
+        __builtin_bit_cast(f32x4, load_chunk<T>(base, stride, r, rows, c + 4, d, vec));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// Eight values of an LDS tile's row from column c on.
+template <class T>
+__device__ __forceinline__ typename T::frag lds_row(const typename T::elem* tile,
+                                                    uint32_t stride, uint32_t r, uint32_t c) {
+  const typename T::elem* p = tile + r * stride + c;
+  if constexpr (sizeof(typename T::elem) == 2) {
+    return *reinterpret_cast<const bf16x8*>(p);
+  } else {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0];
+    const f32x4 b = reinterpret_cast<const f32x4*>(p)[1];
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// Column c + i of an LDS tile at the rows that a D's registers 8t .. 8t + 7 hold: r0 + 4h +
+// (0..3) and r0 + 8 + 4h + (0..3), r0 = 16t.
+template <class T>
+__device__ __forceinline__ typename T::frag lds_col(const typename T::elem* tile,
+                                                    uint32_t stride, uint32_t r0, uint32_t c,
+                                                    uint32_t lane) {
+  const uint32_t h = lane / 32;
+  if constexpr (sizeof(typename T::elem) == 2) {
+    const uint32_t m = lane % 16;
+    const uint16_t* p = tile + (r0 + 4 * h + m / 4) * stride + c + (lane & 16) + 4 * (m % 4);
+    return join(read_tr(p), read_tr(p + 8 * stride));
+  } else {
+    f32x8 f;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; j++)
+      f[j] = tile[(r0 + 4 * h + j % 4 + 8 * (j / 4)) * stride + c + lane % 32];
+    return f;
+  }
+}
+
+// KT rows from r0 on into an LDS tile, the columns past d and the rows past `rows` zero.
+template <class T, uint32_t DP, uint32_t KT, uint32_t NT>
+__device__ __forceinline__ void stage(typename T::elem* tile, uint32_t lds_stride,
+                                      const typename T::elem* base, int64_t stride, uint32_t r0,
+                                      uint32_t rows, uint32_t d, bool vec) {
+  constexpr uint32_t CE = 16 / sizeof(typename T::elem), CPR = DP / CE;
+#pragma unroll
+  for (uint32_t c0 = 0; c0 < KT * CPR; c0 += NT) {
+    const uint32_t c = c0 + threadIdx.x;
+    if (KT * CPR % NT && c >= KT * CPR) break;
+    const uint32_t r = c / CPR, col = c % CPR * CE;
+    *reinterpret_cast<u32x4v*>(tile + r * lds_stride + col) =
+        load_chunk<T>(base, stride, r0 + r, rows, col, d, vec);
+  }
+}
+
+template <class T>
+struct Head {
+  const typename T::elem* p;
+  int64_t row;
+  __device__ Head(const pots_heads& x, uint32_t b, uint32_t h)
+      : p(reinterpret_cast<const typename T::elem*>(x.ptr) + b * x.batch + h * x.head),
+        row(x.row) {}
+};
+
+__device__ __forceinline__ uint32_t length_of(const pots_attention& a, uint32_t b) {
+  if (!a.lengths) return a.n;
+  const int32_t l = gload<int32_t>(a.lengths + b);
+  return l < 0 ? 0 : min((uint32_t)l, a.n);
+}
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+// A wave's D of [d_head × 32 rows] as rows of a tensor: lane (i, h) holds row r0 + i, four
+// consecutive columns at a time.
+template <class T, uint32_t NB>
+__device__ __forceinline__ void store_rows(const pots_heads& x, uint32_t b, uint32_t head,
+                                           uint32_t row, uint32_t n, uint32_t d,
+                                           const f32x16 (&acc)[NB], float mul, bool vec,
+                                           uint32_t h) {
+  if (row >= n) return;
+  typename T::elem* p = reinterpret_cast<typename T::elem*>(x.ptr) + b * x.batch +
+                        head * x.head + (int64_t)row * x.row;
+#pragma unroll
+  for (uint32_t db = 0; db < NB; db++)
+#pragma unroll
+    for (uint32_t g = 0; g < 4; g++) {
+      const uint32_t c = 32 * db + 8 * g + 4 * h;
+      if (c >= d) continue;
+      const f32x16& v = acc[db];
+      if (vec) {
+        T::store4(p + c, v[4 * g] * mul, v[4 * g + 1] * mul, v[4 * g + 2] * mul,
+                  v[4 * g + 3] * mul);
+      } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++)
+          if (c + e < d) p[c + e] = T::put(v[4 * g + e] * mul);
+      }
+    }
+}
+
+// Rows of a tile that is read by rows (16-byte reads, eight lanes of them in a cycle: 16 bytes
+// past a multiple of 128 leaves their banks apart) and of one that is read transposed (32 lanes
+// read four rows of 64 bytes: rows 64 bytes past a multiple of 256, or half of that, do).
+template <class T, uint32_t DP>
+constexpr uint32_t row_stride() { return DP + 16 / sizeof(typename T::elem); }
+template <class T, uint32_t DP>
+constexpr uint32_t col_stride() {
+  return sizeof(typename T::elem) == 4 ? DP : DP % 64 == 0 ? DP + 32 : DP;
+}
+
+template <class T, uint32_t DP, uint32_t NW, uint32_t KT>
+__global__ __launch_bounds__(64 * NW) void attn_fwd(pots_attention a, uint32_t tiles, bool vec,
+                                                    bool vec_out) {
+  typedef typename T::elem elem;
+  typedef typename T::frag frag;
+  constexpr uint32_t NT = 64 * NW, QB = 32 * NW, KS = DP / 16, NB = DP / 32;
+  constexpr uint32_t SK = row_stride<T, DP>(), SV = col_stride<T, DP>();
+  __shared__ __attribute__((aligned(16))) elem s_k[KT * SK];
+  __shared__ __attribute__((aligned(16))) elem s_v[KT * SV];
+  const uint32_t unit = xcd_block(blockIdx.x, gridDim.x);
+  const uint32_t bh = unit / tiles, tile = tiles - 1 - unit % tiles;  // the long tiles first
+  const uint32_t b = bh / a.heads, head = bh % a.heads;
+  const uint32_t kvh = head / (a.heads / a.kv_heads);
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, i = lane % 32, h = lane / 32;
+  const uint32_t len = length_of(a, b), d = a.head_dim;
+  const Head<T> Q(a.q, b, head), K(a.k, b, kvh), V(a.v, b, kvh);
+  const uint32_t q0 = tile * QB, qw = q0 + 32 * wave, q = qw + i;
+  frag qf[KS];
+#pragma unroll
+  for (uint32_t ks = 0; ks < KS; ks++)
+    qf[ks] = load_frag<T>(Q.p, Q.row, q, len, 16 * ks + 8 * h, d, vec);
+  f32x16 o[NB];
+#pragma unroll
+  for (uint32_t db = 0; db < NB; db++) o[db] = zero16();
+  const float c = a.scale * kLog2e;
+  float m = -INFINITY, mc = 0.f, l = 0.f;
+  // keys that the block's rows see, and the wave's
+  const uint32_t end = q0 >= len ? 0 : a.causal ? min(len, q0 + QB) : len;
+  const uint32_t wend = qw >= len ? 0 : a.causal ? min(len, qw + 32) : len;
+  for (uint32_t k0 = 0; k0 < end; k0 += KT) {
+    __syncthreads();
+    stage<T, DP, KT, NT>(s_k, SK, K.p, K.row, k0, len, d, vec);
+    stage<T, DP, KT, NT>(s_v, SV, V.p, V.row, k0, len, d, vec);
+    __syncthreads();
+    if (k0 >= wend) continue;
+    f32x16 s[KT / 32];
+#pragma unroll
+    for (uint32_t u = 0; u < KT / 32; u++) {
+      s[u] = zero16();
+#pragma unroll
+      for (uint32_t ks = 0; ks < KS; ks++)
+        s[u] = mma(lds_row<T>(s_k, SK, 32 * u + i, 16 * ks + 8 * h), qf[ks], s[u]);
+    }
+    // a tile that some row sees in part, or rows that see nothing
+    if (k0 + KT > len || qw + 32 > len || (a.causal && k0 + KT - 1 > qw)) {
+      const uint32_t seen = q >= len ? 0 : a.causal ? min(len, q + 1) : len;
+#pragma unroll
+      for (uint32_t u = 0; u < KT / 32; u++)
+#pragma unroll
+        for (uint32_t r = 0; r < 16; r++)
+          if (k0 + 32 * u + d_row(r, h) >= seen) s[u][r] = -INFINITY;
+    }
+    float top = m;
+#pragma unroll
+    for (uint32_t u = 0; u < KT / 32; u++)
+#pragma unroll
+      for (uint32_t r = 0; r < 16; r++) top = fmaxf(top, s[u][r]);
+    top = fmaxf(top, other_half(top));
+    if (__any(top > m)) {
+      const float tc = top == -INFINITY ? 0.f : top * c;
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - tc);
+      m = top;
+      mc = tc;
+      l *= f;
+#pragma unroll
+      for (uint32_t db = 0; db < NB; db++)
+#pragma unroll
+        for (uint32_t r = 0; r < 16; r++) o[db][r] *= f;
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < KT / 32; u++) {
+#pragma unroll
+      for (uint32_t r = 0; r < 16; r++) {
+        s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], c, -mc));
+        l += s[u][r];
+      }
+#pragma unroll
+      for (uint32_t t = 0; t < 2; t++) {
+        const frag p = T::pack(s[u], 8 * t);
+#pragma unroll
+        for (uint32_t db = 0; db < NB; db++)
+          o[db] = mma(lds_col<T>(s_v, SV, 32 * u + 16 * t, 32 * db, lane), p, o[db]);
+      }
+    }
+  }
+  l += other_half(l);
+  store_rows<T, NB>(a.out, b, head, q, a.n, d, o, l > 0.f || l != l ? 1.f / l : 0.f, vec_out, h);
+  if (h == 0 && q < a.n)
+    a.lse[(int64_t)bh * a.n + q] =
+        l == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// dq, and D for attn_dkv. A wave holds 32 query rows as columns, as in the forward pass:
+// Sᵀ = K·Qᵀ and dPᵀ = V·dOᵀ from one LDS tile each, dQᵀ += Kᵀ·dSᵀ with K read transposed.
+template <class T, uint32_t DP, uint32_t NW, uint32_t KT>
+__global__ __launch_bounds__(64 * NW) void attn_dq(pots_attention a, float* __restrict__ delta,
+                                                   uint32_t tiles, bool vec, bool vec_out) {
+  typedef typename T::elem elem;
+  typedef typename T::frag frag;
+  constexpr uint32_t NT = 64 * NW, QB = 32 * NW, KS = DP / 16, NB = DP / 32;
+  constexpr uint32_t ST = row_stride<T, DP>();
+  __shared__ __attribute__((aligned(16))) elem s_k[KT * ST];
+  __shared__ __attribute__((aligned(16))) elem s_v[KT * ST];
+  const uint32_t unit = xcd_block(blockIdx.x, gridDim.x);
+  const uint32_t bh = unit / tiles, tile = tiles - 1 - unit % tiles;
+  const uint32_t b = bh / a.heads, head = bh % a.heads;
+  const uint32_t kvh = head / (a.heads / a.kv_heads);
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, i = lane % 32, h = lane / 32;
+  const uint32_t len = length_of(a, b), d = a.head_dim;
+  const Head<T> Q(a.q, b, head), K(a.k, b, kvh), V(a.v, b, kvh), O(a.out, b, head),
+      G(a.dout, b, head);
+  const uint32_t q0 = tile * QB, qw = q0 + 32 * wave, q = qw + i;
+  frag qf[KS], gf[KS];
+  float dl = 0.f;
+#pragma unroll
+  for (uint32_t ks = 0; ks < KS; ks++) {
+    qf[ks] = load_frag<T>(Q.p, Q.row, q, len, 16 * ks + 8 * h, d, vec);
+    gf[ks] = load_frag<T>(G.p, G.row, q, len, 16 * ks + 8 * h, d, vec);
+    const frag of = load_frag<T>(O.p, O.row, q, len, 16 * ks + 8 * h, d, vec);
+#pragma unroll
+    for (int j = 0; j < 8; j++) dl = __builtin_fmaf(T::at(gf[ks], j), T::at(of, j), dl);
+  }
+  dl += other_half(dl);
+  float lse2 = INFINITY;  // a row that sees nothing has probabilities of zero
+  if (q < a.n) {
+    const int64_t at = (int64_t)bh * a.n + q;
+    if (h == 0) delta[at] = dl;
+    const float x = q < len ? gload<float>(a.lse + at) : -INFINITY;
+    if (x != -INFINITY) lse2 = x * kLog2e;
+  }
+  f32x16 acc[NB];
+#pragma unroll
+  for (uint32_t db = 0; db < NB; db++) acc[db] = zero16();
+  const float c = a.scale * kLog2e;
+  const uint32_t end = q0 >= len ? 0 : a.causal ? min(len, q0 + QB) : len;
+  const uint32_t wend = qw >= len ? 0 : a.causal ? min(len, qw + 32) : len;
+  const uint32_t seen = q >= len ? 0 : a.causal ? min(len, q + 1) : len;
+  for (uint32_t k0 = 0; k0 < end; k0 += KT) {
+    __syncthreads();
+    stage<T, DP, KT, NT>(s_k, ST, K.p, K.row, k0, len, d, vec);
+    stage<T, DP, KT, NT>(s_v, ST, V.p, V.row, k0, len, d, vec);
+    __syncthreads();
+#pragma unroll
+    for (uint32_t u = 0; u < KT / 32; u++) {
+      const uint32_t ku = k0 + 32 * u;
+      if (ku >= wend) break;
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (uint32_t ks = 0; ks < KS; ks++) {
+        s = mma(lds_row<T>(s_k, ST, 32 * u + i, 16 * ks + 8 * h), qf[ks], s);
+        dp = mma(lds_row<T>(s_v, ST, 32 * u + i, 16 * ks + 8 * h), gf[ks], dp);
+      }
+      const bool part = ku + 32 > len || qw + 32 > len || (a.causal && ku + 31 > qw);
+#pragma unroll
+      for (uint32_t r = 0; r < 16; r++) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse2));
+        s[r] = p * (dp[r] - dl);
+        if (part && ku + d_row(r, h) >= seen) s[r] = 0.f;
+      }
+#pragma unroll
+      for (uint32_t t = 0; t < 2; t++) {
+        const frag p = T::pack(s, 8 * t);
+#pragma unroll
+        for (uint32_t db = 0; db < NB; db++)
+          acc[db] = mma(lds_col<T>(s_k, ST, 32 * u + 16 * t, 32 * db, lane), p, acc[db]);
+      }
+    }
+  }
+  store_rows<T, NB>(a.dq, b, head, q, a.n, d, acc, a.scale, vec_out, h);
+}
+
+// dk and dv of 32·NW keys, over `per` query heads of their group and the queries that see
+// them. A wave holds 32 keys as columns: S = Q·Kᵀ and dP = dO·Vᵀ from LDS rows, dVᵀ += dOᵀ·P and
+// dKᵀ += Qᵀ·dS from the same tiles read transposed. With `part`, the sums go to fp32 slices
+// [2][split][batch][kv_heads][n][d].
+template <class T, uint32_t DP, uint32_t NW, uint32_t QT>
+__global__ __launch_bounds__(64 * NW) void attn_dkv(pots_attention a,
+                                                    const float* __restrict__ delta,
+                                                    float* __restrict__ part, uint32_t tiles,
+                                                    uint32_t splits, uint32_t per, bool vec,
+                                                    bool vec_out) {
+  typedef typename T::elem elem;
+  typedef typename T::frag frag;
+  constexpr uint32_t NT = 64 * NW, KB = 32 * NW, KS = DP / 16, NB = DP / 32;
+  constexpr uint32_t ST = row_stride<T, DP>();
+  __shared__ __attribute__((aligned(16))) elem s_q[QT * ST];
+  __shared__ __attribute__((aligned(16))) elem s_g[QT * ST];
+  __shared__ __attribute__((aligned(16))) float s_lse[QT];
+  __shared__ __attribute__((aligned(16))) float s_dl[QT];
+  const uint32_t unit = xcd_block(blockIdx.x, gridDim.x);
+  const uint32_t tile = unit % tiles, split = unit / tiles % splits;  // the long tiles first
+  const uint32_t bk = unit / tiles / splits, b = bk / a.kv_heads, kvh = bk % a.kv_heads;
+  const uint32_t rep = a.heads / a.kv_heads;
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, i = lane % 32, h = lane / 32;
+  const uint32_t len = length_of(a, b), d = a.head_dim;
+  const Head<T> K(a.k, b, kvh), V(a.v, b, kvh);
+  const uint32_t k0 = tile * KB, kw = k0 + 32 * wave, key = kw + i;
+  frag kf[KS], vf[KS];
+#pragma unroll
+  for (uint32_t ks = 0; ks < KS; ks++) {
+    kf[ks] = load_frag<T>(K.p, K.row, key, len, 16 * ks + 8 * h, d, vec);
+    vf[ks] = load_frag<T>(V.p, V.row, key, len, 16 * ks + 8 * h, d, vec);
+  }
+  f32x16 dk[NB], dv[NB];
+#pragma unroll
+  for (uint32_t db = 0; db < NB; db++) {
+    dk[db] = zero16();
+    dv[db] = zero16();
+  }
+  const float c = a.scale * kLog2e;
+  const uint32_t last = min(rep, (split + 1) * per);
+  for (uint32_t e = split * per; e < last && k0 < len; e++) {
+    const uint32_t head = kvh * rep + e;
+    const Head<T> Q(a.q, b, head), G(a.dout, b, head);
+    const int64_t stat = (int64_t)(b * a.heads + head) * a.n;
+    for (uint32_t q0 = a.causal ? k0 / QT * QT : 0; q0 < len; q0 += QT) {
+      __syncthreads();
+      stage<T, DP, QT, NT>(s_q, ST, Q.p, Q.row, q0, len, d, vec);
+      stage<T, DP, QT, NT>(s_g, ST, G.p, G.row, q0, len, d, vec);
+      if (threadIdx.x < QT) {
+        const uint32_t q = q0 + threadIdx.x;
+        const float x = q < len ? gload<float>(a.lse + stat + q) : -INFINITY;
+        s_lse[threadIdx.x] = x != -INFINITY ? x * kLog2e : INFINITY;
+        s_dl[threadIdx.x] = q < len ? gload<float>(delta + stat + q) : 0.f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (uint32_t u = 0; u < QT / 32; u++) {
+        const uint32_t qu = q0 + 32 * u;
+        if (qu >= len || kw >= len || (a.causal && qu + 31 < kw)) continue;
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (uint32_t ks = 0; ks < KS; ks++) {
+          s = mma(lds_row<T>(s_q, ST, 32 * u + i, 16 * ks + 8 * h), kf[ks], s);
+          dp = mma(lds_row<T>(s_g, ST, 32 * u + i, 16 * ks + 8 * h), vf[ks], dp);
+        }
+        const bool some = kw + 32 > len || qu + 32 > len || (a.causal && qu < kw + 31);
+#pragma unroll
+        for (uint32_t g = 0; g < 4; g++) {
+          const f32x4 ls = *reinterpret_cast<const f32x4*>(s_lse + 32 * u + 8 * g + 4 * h);
+          const f32x4 dl = *reinterpret_cast<const f32x4*>(s_dl + 32 * u + 8 * g + 4 * h);
+#pragma unroll
+          for (uint32_t x = 0; x < 4; x++) {
+            const uint32_t r = 4 * g + x;
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ls[x]));
+            const uint32_t q = qu + d_row(r, h);
+            const bool out = some && (key >= len || q >= len || (a.causal && q < key));
+            s[r] = out ? 0.f : p;
+            dp[r] = out ? 0.f : p * (dp[r] - dl[x]);
+          }
+        }
+#pragma unroll
+        for (uint32_t t = 0; t < 2; t++) {
+          const frag p = T::pack(s, 8 * t), ds = T::pack(dp, 8 * t);
+#pragma unroll
+          for (uint32_t db = 0; db < NB; db++) {
+            dv[db] = mma(lds_col<T>(s_g, ST, 32 * u + 16 * t, 32 * db, lane), p, dv[db]);
+            dk[db] = mma(lds_col<T>(s_q, ST, 32 * u + 16 * t, 32 * db, lane), ds, dk[db]);
+          }
+        }
+      }
+    }
+  }
+  if (part) {
+    pots_heads x;
+    x.row = d;
+    x.head = (int64_t)a.n * d;
+    x.batch = x.head * a.kv_heads;
+    x.ptr = part + split * x.batch * a.batch;
+    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dk, a.scale, d % 4 == 0, h);
+    x.ptr = part + (splits + split) * x.batch * a.batch;
+    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dv, 1.f, d % 4 == 0, h);
+  } else {
+    store_rows<T, NB>(a.dk, b, kvh, key, a.n, d, dk, a.scale, vec_out, h);
+    store_rows<T, NB>(a.dv, b, kvh, key, a.n, d, dv, 1.f, vec_out, h);
+  }
+}
+
+// dk (blockIdx.y = 0) and dv (1) from the splits' sums, in order.
+template <class T>
+__global__ __launch_bounds__(256) void attn_fold(pots_attention a,
+                                                 const float* __restrict__ part,
+                                                 uint32_t splits) {
+  const uint64_t each = (uint64_t)a.batch * a.kv_heads * a.n * a.head_dim;
+  const float* p = part + blockIdx.y * splits * each;
+  const pots_heads& x = blockIdx.y ? a.dv : a.dk;
+  for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < each;
+       e += (uint64_t)gridDim.x * 256) {
+    float sum = p[e];
+    for (uint32_t s = 1; s < splits; s++) sum += p[s * each + e];
+    const uint32_t col = e % a.head_dim;
+    const uint64_t row = e / a.head_dim, bk = row / a.n;
+    reinterpret_cast<typename T::elem*>(
+        x.ptr)[(int64_t)(bk / a.kv_heads) * x.batch + (int64_t)(bk % a.kv_heads) * x.head +
+               (int64_t)(row % a.n) * x.row + col] = T::put(sum);
+  }
+}
+
+namespace {
+
+bool bad(const pots_attention* a) {
+  return !a || a->dtype > POTS_OP_BF16 || a->kv_heads == 0 || a->heads == 0 ||
+         a->heads % a->kv_heads || a->head_dim == 0 || a->head_dim > POTS_ATTENTION_MAX_DIM ||
+         !(a->scale > 0.f) || !isfinite(a->scale) || a->n > 0x40000000u ||
+         (uint64_t)a->batch * a->heads > 0x100000u;
+}
+
+bool aligned(const pots_attention* a, const pots_heads& x, uint32_t bytes) {
+  const int64_t e = a->dtype == POTS_OP_BF16 ? 2 : 4;
+  return reinterpret_cast<uint64_t>(x.ptr) % bytes == 0 && x.batch * e % bytes == 0 &&
+         x.head * e % bytes == 0 && x.row * e % bytes == 0 && a->head_dim * e % bytes == 0;
+}
+
+// Waves in a block: as many as four (which share a K or V tile) while that leaves a block for
+// every compute unit.
+uint32_t waves(uint64_t sequences, uint32_t n) {
+  for (uint32_t w = 4; w > 1; w /= 2)
+    if (sequences * ((n + 32 * w - 1) / (32 * w)) >= 256) return w;
+  return 1;
+}
+
+struct Dkv {
+  uint32_t nw, tiles, splits, per;
+};
+
+Dkv dkv_cut(const pots_attention* a) {
+  Dkv r;
+  const uint32_t rep = a->heads / a->kv_heads;
+  r.nw = waves((uint64_t)a->batch * a->heads, a->n);
+  r.tiles = (a->n + 32 * r.nw - 1) / (32 * r.nw);
+  const uint64_t blocks = (uint64_t)a->batch * a->kv_heads * r.tiles;
+  r.splits = 1;
+  while (r.splits < rep && blocks * r.splits < 512) r.splits++;
+  r.per = (rep + r.splits - 1) / r.splits;
+  r.splits = (rep + r.per - 1) / r.per;
+  return r;
+}
+
+template <class T, uint32_t DP, uint32_t NW>
+int forward(const pots_attention* a, hipStream_t s) {
+  const uint32_t tiles = (a->n + 32 * NW - 1) / (32 * NW);
+  const uint64_t blocks = (uint64_t)a->batch * a->heads * tiles;
+  if (blocks > 0x7FFFFFFFu) return POTS_E_ARG;
+  const bool vec = aligned(a, a->q, 16) && aligned(a, a->k, 16) && aligned(a, a->v, 16);
+  hipLaunchKernelGGL((attn_fwd<T, DP, NW, NW == 4 ? 64 : 32>), dim3((uint32_t)blocks),
+                     dim3(64 * NW), 0, s, *a, tiles, vec,
+                     aligned(a, a->out, 4 * sizeof(typename T::elem)));
+  POTS_HIP(hipGetLastError());
+  return POTS_E_OK;
+}
+
+template <class T, uint32_t DP, uint32_t NW>
+int backward(const pots_attention* a, char* work, hipStream_t s) {
+  const Dkv cut = dkv_cut(a);
+  const uint64_t qblocks = (uint64_t)a->batch * a->heads * cut.tiles;
+  const uint64_t kblocks = (uint64_t)a->batch * a->kv_heads * cut.tiles * cut.splits;
+  if (qblocks > 0x7FFFFFFFu || kblocks > 0x7FFFFFFFu) return POTS_E_ARG;
+  float* delta = reinterpret_cast<float*>(work);
+  float* part = cut.splits == 1 ? nullptr
+                                : reinterpret_cast<float*>(
+                                      work + align_up((size_t)a->batch * a->heads * a->n * 4,
+                                                      256));
+  const bool vec = aligned(a, a->q, 16) && aligned(a, a->k, 16) && aligned(a, a->v, 16) &&
+                   aligned(a, a->out, 16) && aligned(a, a->dout, 16);
+  const uint32_t four = 4 * sizeof(typename T::elem);
+  hipLaunchKernelGGL((attn_dq<T, DP, NW, NW == 4 ? 64 : 32>), dim3((uint32_t)qblocks),
+                     dim3(64 * NW), 0, s, *a, delta, cut.tiles, vec, aligned(a, a->dq, four));
+  POTS_HIP(hipGetLastError());
+  hipLaunchKernelGGL((attn_dkv<T, DP, NW, NW == 4 ? 64 : 32>), dim3((uint32_t)kblocks),
+                     dim3(64 * NW), 0, s, *a, delta, part, cut.tiles, cut.splits, cut.per, vec,
+                     aligned(a, a->dk, four) && aligned(a, a->dv, four));
+  POTS_HIP(hipGetLastError());
+  if (part) {
+    const uint64_t each = (uint64_t)a->batch * a->kv_heads * a->n * a->head_dim;
+    const uint64_t nb = (each + 255) / 256;
+    hipLaunchKernelGGL((attn_fold<T>), dim3((uint32_t)(nb < 4096 ? nb : 4096), 2), dim3(256), 0,
+                       s, *a, part, cut.splits);
+    POTS_HIP(hipGetLastError());
+  }
+  return POTS_E_OK;
+}
+
+#define POTS_WAVES(T, DP, F, ...)          \
+  (nw == 4   ? F<T, DP, 4>(__VA_ARGS__)    \
+   : nw == 2 ? F<T, DP, 2>(__VA_ARGS__)    \
+             : F<T, DP, 1>(__VA_ARGS__))
+#define POTS_DIMS(T, F, ...)                                     \
+  (a->head_dim <= 32   ? POTS_WAVES(T, 32, F, __VA_ARGS__)       \
+   : a->head_dim <= 64 ? POTS_WAVES(T, 64, F, __VA_ARGS__)       \
+   : a->head_dim <= 96 ? POTS_WAVES(T, 96, F, __VA_ARGS__)       \
+                       : POTS_WAVES(T, 128, F, __VA_ARGS__))
+
+}  // namespace
+
+}  // namespace pots
+
+using namespace pots;
+
+extern "C" int pots_attention_forward(const pots_attention* a, void* stream) {
+  if (bad(a)) return POTS_E_ARG;
+  if (a->batch == 0 || a->n == 0) return POTS_E_OK;
+  if (!a->q.ptr || !a->k.ptr || !a->v.ptr || !a->out.ptr || !a->lse) return POTS_E_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const uint32_t nw = waves((uint64_t)a->batch * a->heads, a->n);
+  return a->dtype == POTS_OP_BF16 ? POTS_DIMS(Bf16, forward, a, s)
+                                  : POTS_DIMS(Fp32, forward, a, s);
+}
+
+extern "C" uint64_t pots_attention_backward_work(const pots_attention* a) {
+  if (bad(a) || a->batch == 0 || a->n == 0) return 0;
+  const Dkv cut = dkv_cut(a);
+  uint64_t bytes = align_up((size_t)a->batch * a->heads * a->n * 4, 256);
+  if (cut.splits > 1)
+    bytes += 2ull * cut.splits * a->batch * a->kv_heads * a->n * a->head_dim * 4;
+  return bytes;
+}
+
+extern "C" int pots_attention_backward(const pots_attention* a, void* work, void* stream) {
+  if (bad(a)) return POTS_E_ARG;
+  if (a->batch == 0 || a->n == 0) return POTS_E_OK;
+  if (!a->q.ptr || !a->k.ptr || !a->v.ptr || !a->out.ptr || !a->lse || !a->dout.ptr ||
+      !a->dq.ptr || !a->dk.ptr || !a->dv.ptr || !work)
+    return POTS_E_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const uint32_t nw = dkv_cut(a).nw;
+  char* w = static_cast<char*>(work);
+  return a->dtype == POTS_OP_BF16 ? POTS_DIMS(Bf16, backward, a, w, s)
+                                  : POTS_DIMS(Fp32, backward, a, w, s);
+}

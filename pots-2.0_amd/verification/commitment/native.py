@@ -152,6 +152,18 @@ class Native:
             "pots_update_plan_run": ([_vp, _vp, _vp], _int),
             "pots_update_plan_bytes": ([_vp], _u64),
             "pots_update_plan_destroy": ([_vp], None),
+            # the operators' argument blocks travel as packed bytes (verification.computation.
+            # operators), which a char pointer takes as they are
+            "pots_attention_forward": ([ctypes.c_char_p, _vp], _int),
+            "pots_attention_backward_work": ([ctypes.c_char_p], _u64),
+            "pots_attention_backward": ([ctypes.c_char_p, _vp, _vp], _int),
+            "pots_vocab_loss_forward_work": ([ctypes.c_char_p], _u64),
+            "pots_vocab_loss_forward": ([ctypes.c_char_p, _vp, _vp], _int),
+            "pots_vocab_loss_backward_work": ([ctypes.c_char_p], _u64),
+            "pots_vocab_loss_backward": ([ctypes.c_char_p, _vp, _vp], _int),
+            "pots_embedding_forward": ([ctypes.c_char_p, _vp], _int),
+            "pots_embedding_backward_work": ([ctypes.c_char_p], _u64),
+            "pots_embedding_backward": ([ctypes.c_char_p, _vp, _vp], _int),
         }
         for name, (args, res) in sigs.items():
             fn = getattr(lib, name)
@@ -171,6 +183,26 @@ class Native:
             raise ValueError(f"{what}: argument rejected by libpots_mi355x")
         msg = self._lib.pots_last_error().decode()
         raise NativeError(f"{what} failed with {rc}: {msg}")
+
+    def operator(self, name: str, args: bytes, device: torch.device, *,
+                 work: bool = True) -> None:
+        """Enqueue ``pots_<name>(args, …)`` on ``device``'s current stream; with ``work``, with
+        the scratch that ``pots_<name>_work`` asks for, taken from torch's allocator on that
+        stream."""
+        lib = self._lib
+        if device.index != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                return self.operator(name, args, device, work=work)
+        stream = torch.cuda.current_stream().cuda_stream
+        if not work:
+            rc = getattr(lib, "pots_" + name)(args, stream)
+        else:
+            nbytes = getattr(lib, f"pots_{name}_work")(args)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+            rc = getattr(lib, "pots_" + name)(args, None if scratch is None
+                                              else scratch.data_ptr(), stream)
+        if rc != E_OK:
+            self._check(rc, "pots_" + name)
 
     # ---- the reference's methods ---------------------------------------------------------
 
