@@ -13,7 +13,7 @@
 // All three products are one tiled kernel over the matrix cores (Tile), each operand stored
 // either with the contraction along its rows or with its rows along the contraction (W of dx,
 // G and X of dW); the latter are read transposed from LDS. bf16 is multiplied as it is. An fp32
-// value is the exact sum of three bf16 terms of eight bits each (split3), and a product of two
+// value is the exact sum of three bf16 terms of eight bits each (take_term), and a product of two
 // takes the six products of terms that reach 2^-24 of it: at six bf16 products' cost that is
 // 2.6 times the rate of the fp32 matrix instructions, with their accuracy (the three products
 // left out are below 2^-24 of |x||w|). G is rounded to the inputs' type as an operand: half a
@@ -43,38 +43,57 @@ __device__ __forceinline__ void pair_of(uint32_t pairs, uint32_t t, uint32_t* pa
   *pb = (0x001012u >> (4 * j)) & 15;
 }
 
+// Sixteen bytes a lane from a buffer to consecutive places from `lds` on, which is the same for
+// the wave. (The host's pass of the compiler knows no such builtin.)
+__device__ __forceinline__ void load_lds16(brsrc rsrc, uint16_t* lds, uint32_t off) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (POTS_LDS void*)lds, 16, off, 0, 0, 0);
+#endif
+}
+
 // T rows of an operand and BK of the contraction in LDS, in 16-byte chunks that one
 // instruction brings in for 64 lanes, straight from memory. TR: stored [contraction][rows], so
 // a stage is BK rows of T columns; else T rows of BK columns. A chunk is exchanged within its
 // row by the row's number, so that the reads of a fragment fall on different banks: eight
-// lanes' 16-byte reads of eight rows, or 32 lanes' transposing reads of four rows.
+// lanes' 16-byte reads of eight rows, or 32 lanes' transposing reads of four rows. A lane's
+// offsets are the same at every stage; the stage moves the buffer's base, in scalar registers.
 template <bool TR, uint32_t T, uint32_t NT>
 struct Stage {
-  static constexpr uint32_t kChunks = T * BK / 8 / NT;
-  static_assert(T * BK / 8 % NT == 0, "a stage is whole instructions");
+  static constexpr uint32_t kAll = T * BK / 8, kChunks = (kAll + NT - 1) / NT;
   static_assert(!TR || T >= 128, "the exchange of a transposed tile needs 16 chunks a row");
+  uint32_t off[kChunks], wide;
 
-  // r0, rows: the tile's first row and their number (for TR: columns, a multiple of 8); k0,
-  // ks: the contraction's. Rows and contraction past the end repeat the last.
-  static __device__ __forceinline__ void load(uint16_t* lds, const Mat& m, uint32_t plane,
-                                              uint32_t r0, uint32_t rows, uint32_t k0,
-                                              uint32_t ks) {
-    const uint16_t* base = m.p + (int64_t)plane * m.plane;
-    const uint32_t wave = threadIdx.x / 64;
+  // r0, rows: the tile's first row and their number; rows past it repeat the last (for TR:
+  // columns, whose last eight repeat).
+  __device__ __forceinline__ void init(const Mat& m, uint32_t r0, uint32_t rows) {
+    wide = 2 * min(T, rows - r0);
 #pragma unroll
     for (uint32_t u = 0; u < kChunks; u++) {
-      const uint32_t first = (u * NT / 64 + wave) * 64, c = first + threadIdx.x % 64;
-      const uint16_t* src;
+      const uint32_t c = u * NT + threadIdx.x;
       if constexpr (TR) {
         const uint32_t r = c / (T / 8), at = (c % (T / 8)) ^ (4 * (r & 3));
-        src = base + (int64_t)min(k0 + r, ks - 1) * m.ld + min(r0 + 8 * at, rows - 8);
+        off[u] = 2 * (r * (uint32_t)m.ld + min(r0 + 8 * at, rows - 8) - r0);
       } else {
         const uint32_t r = c / (BK / 8), at = (c % (BK / 8)) ^ (r & 7);
-        src = base + (int64_t)min(r0 + r, rows - 1) * m.ld + k0 + 8 * at;
+        off[u] = 2 * (min(r, rows - 1 - r0) * (uint32_t)m.ld + 8 * at);
       }
-      __builtin_amdgcn_global_load_lds((const POTS_GLOBAL void*)src,
-                                       (POTS_LDS void*)(lds + first * 8), 16, 0, 0);
     }
+  }
+
+  // The stage of contraction k0 .. k0 + BK; for TR, zero from `ks` on.
+  __device__ __forceinline__ void load(uint16_t* lds, const Mat& m, uint32_t plane, uint32_t r0,
+                                       uint32_t k0, uint32_t ks) const {
+    const uint16_t* base = m.p + (int64_t)plane * m.plane +
+                           (TR ? (int64_t)k0 * m.ld + r0 : (int64_t)r0 * m.ld + k0);
+    const uint32_t range =
+        TR ? (min(BK, ks - k0) - 1) * (uint32_t)m.ld * 2 + wide : 0x7FFFFFFF;
+    const brsrc rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), (short)0,
+                                                         range, 0x00020000);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+#pragma unroll
+    for (uint32_t u = 0; u < kChunks; u++)
+      if (kAll % NT == 0 || u * NT + wave * 64 < kAll)
+        load_lds16(rsrc, lds + (u * NT + wave * 64) * 8, off[u]);
   }
 
   // Rows c .. c + 31 at step ks of the stage: contraction 16ks + 8h + (0..7).
@@ -84,11 +103,11 @@ struct Stage {
     if constexpr (TR) {
       const uint32_t m = lane % 16, r = 16 * ks + 8 * h + m / 4;
       const uint32_t col = c + (lane & 16) + 4 * (m % 4);
-      const uint16_t* p = lds + r * T + (((col / 8) ^ (4 * (r & 3))) * 8 + col % 8);
+      const uint16_t* p = lds + r * T + (((col / 8) ^ (4 * (m / 4))) * 8 + 4 * (m % 2));
       return join(read_tr(p), read_tr(p + 4 * T));
     } else {
       const uint32_t r = c + lane % 32;
-      return *reinterpret_cast<const bf16x8*>(lds + r * BK + (((2 * ks + h) ^ (r & 7)) * 8));
+      return *reinterpret_cast<const bf16x8*>(lds + r * BK + (((2 * ks + h) ^ (lane & 7)) * 8));
     }
   }
 };
@@ -99,10 +118,18 @@ __device__ __forceinline__ void loads_done() {
   __syncthreads();
 }
 
+// The stages in LDS: objects of their own, so that the compiler knows a load into one from the
+// reads of another and need not wait for it; one set for all the products of a kernel.
+template <uint32_t WHICH, uint32_t SIZE>
+__device__ __forceinline__ uint16_t* lds_buffer() {
+  __shared__ __attribute__((aligned(16))) uint16_t s_buf[SIZE];
+  return s_buf;
+}
+
 // A block's TM x TN of A·Bᵀ over K (a multiple of BK), WM x WN waves of MB x NB products of 32.
-template <bool ATR, bool BTR, uint32_t TM_, uint32_t TN_, uint32_t WM, uint32_t WN>
+template <bool ATR, bool BTR, uint32_t TM_, uint32_t TN_, uint32_t WM_, uint32_t WN_>
 struct Tile {
-  static constexpr uint32_t TM = TM_, TN = TN_, NT = 64 * WM * WN;
+  static constexpr uint32_t TM = TM_, TN = TN_, WM = WM_, WN = WN_, NT = 64 * WM * WN;
   static constexpr uint32_t MB = TM / WM / 32, NB = TN / WN / 32;
   typedef Stage<ATR, TM, NT> SA;
   typedef Stage<BTR, TN, NT> SB;
@@ -124,12 +151,14 @@ struct Tile {
     }
   }
 
-  // ka: the contraction's length where an operand is stored along it and may end inside K.
+  // The contraction is k0 .. k0 + K; ka, kb: its end where an operand is stored along it.
   __device__ __forceinline__ void run(const Mat& A, const Mat& B, uint32_t m0, uint32_t M,
-                                      uint32_t n0, uint32_t N, uint32_t K, uint32_t ka,
-                                      uint32_t kb, uint32_t pairs) {
-    __shared__ __attribute__((aligned(16))) uint16_t s_a0[TM * BK], s_b0[TN * BK];
-    __shared__ __attribute__((aligned(16))) uint16_t s_a1[TM * BK], s_b1[TN * BK];
+                                      uint32_t n0, uint32_t N, uint32_t k0, uint32_t K,
+                                      uint32_t ka, uint32_t kb, uint32_t pairs) {
+    uint16_t* const s_a0 = lds_buffer<0, TM * BK>();
+    uint16_t* const s_a1 = lds_buffer<1, TM * BK>();
+    uint16_t* const s_b0 = lds_buffer<2, TN * BK>();
+    uint16_t* const s_b1 = lds_buffer<3, TN * BK>();
     lane = threadIdx.x % 64;
     wm = threadIdx.x / 64 / WN * (TM / WM);
     wn = threadIdx.x / 64 % WN * (TN / WN);
@@ -138,31 +167,47 @@ struct Tile {
 #pragma unroll
       for (uint32_t n = 0; n < NB; n++) acc[m][n] = zero16();
     const uint32_t steps = K / BK * pairs;
-    uint32_t k = 0, pair = 0;
+    uint32_t k = k0, pair = 0;
+    SA sa;
+    SB sb;
+    sa.init(A, m0, M);
+    sb.init(B, n0, N);
     auto load = [&](uint16_t* a, uint16_t* b) {
       uint32_t pa, pb;
       pair_of(pairs, pair, &pa, &pb);
-      SA::load(a, A, pa, m0, M, k, ka);
-      SB::load(b, B, pb, n0, N, k, kb);
+      sa.load(a, A, pa, m0, k, ka);
+      sb.load(b, B, pb, n0, k, kb);
       k += BK;
-      if (k == K) {
-        k = 0;
+      if (k == k0 + K) {
+        k = k0;
         pair++;
       }
     };
     if (steps) load(s_a0, s_b0);
-    for (uint32_t t = 0; t < steps; t += 2) {
+    uint32_t t = 0;
+    for (; t + 2 <= steps; t += 2) {  // the next stage is on its way while one is multiplied
       loads_done();
-      if (t + 1 < steps) load(s_a1, s_b1);
+      load(s_a1, s_b1);
       step(s_a0, s_b0);
-      if (t + 1 == steps) break;
       loads_done();
       if (t + 2 < steps) load(s_a0, s_b0);
       step(s_a1, s_b1);
     }
+    if (t < steps) {
+      loads_done();
+      step(s_a0, s_b0);
+    }
   }
 
-  // f(m, n, acc, row of A of register 0 of the lane, row of B of the lane)
+  // A part of A's stages for each wave to itself, once the block has passed a barrier after run().
+  static constexpr uint32_t kScratch = TM * BK * 2 / (WM_ * WN_);  // values
+  __device__ __forceinline__ uint16_t* scratch() const {
+    constexpr uint32_t half = WM * WN / 2;
+    const uint32_t w = threadIdx.x / 64, in = w % half * kScratch;
+    return w < half ? lds_buffer<0, TM * BK>() + in : lds_buffer<1, TM * BK>() + in;
+  }
+
+  // f(acc, row of A of register 0 of the lane, row of B of the lane)
   template <class F>
   __device__ __forceinline__ void each(uint32_t m0, uint32_t n0, F f) {
 #pragma unroll
@@ -175,8 +220,9 @@ struct Tile {
 
 // Tiles of a launch: an XCD's blocks are neighbours, groups of eight tiles of B by all of A's,
 // so that the 32 that run at once read four and eight tiles' operands through their L2.
-__device__ __forceinline__ void tile_of(uint32_t mt, uint32_t nt, uint32_t* m, uint32_t* n) {
-  const uint32_t u = xcd_block(blockIdx.x, mt * nt), g = u / (8 * mt), in = u % (8 * mt);
+__device__ __forceinline__ void tile_of(uint32_t block, uint32_t mt, uint32_t nt, uint32_t* m,
+                                        uint32_t* n) {
+  const uint32_t u = xcd_block(block, mt * nt), g = u / (8 * mt), in = u % (8 * mt);
   const uint32_t w = min(8u, nt - 8 * g);
   *m = in / w;
   *n = 8 * g + in % w;
@@ -184,19 +230,15 @@ __device__ __forceinline__ void tile_of(uint32_t mt, uint32_t nt, uint32_t* m, u
 
 // ---- laying operands out --------------------------------------------------------------------
 
-__device__ __forceinline__ void split3(float x, uint16_t* t) {
-  const uint32_t u = __float_as_uint(x);
+// The leading eight bits of x as bf16; x is left with the rest, exactly.
+__device__ __forceinline__ uint16_t take_term(float* x) {
+  const uint32_t u = __float_as_uint(*x);
   if ((u & 0x7F800000u) == 0x7F800000u) {  // one term; a NaN keeps a bit of its fraction
-    t[0] = (u >> 16) | ((u & 0x7FFFFFu) ? 0x40 : 0);
-    t[1] = t[2] = 0;
-    return;
+    *x = 0.f;
+    return (u >> 16) | ((u & 0x7FFFFFu) ? 0x40 : 0);
   }
-  const float r = x - __uint_as_float(u & 0xFFFF0000u);  // the lower 16 bits, exact
-  const uint32_t v = __float_as_uint(r);
-  const float q = r - __uint_as_float(v & 0xFFFF0000u);  // eight bits at most
-  t[0] = u >> 16;
-  t[1] = v >> 16;
-  t[2] = __float_as_uint(q) >> 16;
+  *x = *x - __uint_as_float(u & 0xFFFF0000u);
+  return u >> 16;
 }
 
 // dst [terms][rows_pad][dp] of src rows (through idx where given, rows from *count on zero).
@@ -219,10 +261,13 @@ __global__ __launch_bounds__(256) void lay_out(const typename T::elem* __restric
 #pragma unroll
       for (uint32_t j = 0; j < 4; j++)
         if (c + j < d) {
-          if constexpr (kTerms == 3)
-            split3(p[c + j], t[j]);
-          else
+          if constexpr (kTerms == 3) {
+            float x = p[c + j];
+#pragma unroll
+            for (uint32_t k = 0; k < 3; k++) t[j][k] = take_term(&x);
+          } else {
             t[j][0] = p[c + j];
+          }
         }
     }
 #pragma unroll
@@ -235,16 +280,27 @@ __global__ __launch_bounds__(256) void lay_out(const typename T::elem* __restric
 }
 
 // The rows that carry a gradient, in order: idx, their number, each row's place (or ~0), and
-// their weights, targets and lse (in units of log2) gathered.
+// their weights, targets and lse (in units of log2) gathered. G is held in units of the largest
+// weight, `unit`, which its products are multiplied by at the end: rows that weigh the same (a
+// mean over the batch) then have a weight of 1, which rounds no entry of G.
 __global__ __launch_bounds__(1024) void live_rows(pots_vocab_loss a, uint32_t* __restrict__ idx,
                                                   uint32_t* __restrict__ pos,
                                                   uint32_t* __restrict__ count,
                                                   float* __restrict__ weight,
                                                   float* __restrict__ lse2,
-                                                  uint32_t* __restrict__ target) {
+                                                  uint32_t* __restrict__ target,
+                                                  float* __restrict__ unit) {
   __shared__ uint32_t s_wave[16];
+  __shared__ float s_top[16];
   uint32_t base = 0;
   const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  float top = 0.f;
+  for (uint32_t r = threadIdx.x; r < a.rows; r += 1024) top = fmaxf(top, fabsf(a.weights[r]));
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (lane == 0) s_top[wave] = top;
+  __syncthreads();
+  for (uint32_t v = 0; v < 16; v++) top = fmaxf(top, s_top[v]);
+  if (!(top >= 0x1p-100f && top <= 0x1p100f)) top = 1.f;
   for (uint32_t r0 = 0; r0 < a.rows; r0 += 1024) {
     const uint32_t r = r0 + threadIdx.x;
     const float w = r < a.rows ? a.weights[r] : 0.f;
@@ -263,32 +319,35 @@ __global__ __launch_bounds__(1024) void live_rows(pots_vocab_loss a, uint32_t* _
     if (r < a.rows) pos[r] = live ? at : ~0u;
     if (live) {
       idx[at] = r;
-      weight[at] = t < a.vocab ? w : NAN;
+      weight[at] = t < a.vocab ? w / top : NAN;
       lse2[at] = a.lse[r] * kLog2e;
       target[at] = (uint32_t)t;
     }
     base += all;
   }
-  if (threadIdx.x == 0) *count = base;
+  if (threadIdx.x == 0) {
+    *count = base;
+    *unit = top;
+  }
 }
 
 // ---- the products ---------------------------------------------------------------------------
 
 // A piece of the vocabulary from v0 on, `nv` rows of it, against rows of x: a maximum (times
-// log2 e) and a sum of 2^(s - maximum) per row and wave, part[chunk][row], and the targets' s.
+// log2 e) and a sum of 2^(s - maximum) per row and tile, part[chunk][row], and the targets' s.
 template <class C>
 __global__ __launch_bounds__(C::NT) void loss_scores(Mat W, Mat X, uint32_t v0, uint32_t nv,
                                                      uint32_t rows, uint32_t K, uint32_t pairs,
                                                      uint32_t mt, uint32_t nt,
                                                      const int64_t* __restrict__ targets,
                                                      float2* __restrict__ part,
-                                                     uint32_t part_ld,
                                                      float* __restrict__ hit) {
+  __shared__ float2 s_part[C::WM][C::TN];
   uint32_t m, n;
-  tile_of(mt, nt, &m, &n);
+  tile_of(blockIdx.x, mt, nt, &m, &n);
   C c;
   const uint32_t m0 = m * C::TM, n0 = n * C::TN;
-  c.run(W, X, m0, nv, n0, rows, K, 0, 0, pairs);
+  c.run(W, X, m0, nv, n0, rows, 0, K, 0, 0, pairs);
   const uint32_t mw = m0 + c.wm;  // the wave's vocabulary rows: 32·MB of them
   if (mw + 32 * C::MB > nv)
     c.each(m0, n0, [&](f32x16& s, uint32_t v, uint32_t) {
@@ -312,8 +371,9 @@ __global__ __launch_bounds__(C::NT) void loss_scores(Mat W, Mat X, uint32_t v0, 
       for (uint32_t r = 0; r < 16; r++)
         sum += __builtin_amdgcn_exp2f(__builtin_fmaf(c.acc[x][b][r], kLog2e, -tc));
     sum += __shfl_xor(sum, 32);
-    if (row < rows && c.lane < 32)
-      part[(uint64_t)((v0 + mw) / (32 * C::MB)) * part_ld + row] = {tc, sum};
+    if (c.lane < 32)
+      s_part[c.wm / (C::TM / C::WM)][c.wn + 32 * b + c.lane] =
+          make_float2(top == -INFINITY ? -INFINITY : tc, sum);
     const int64_t t = row < rows ? targets[row] - v0 - mw : -1;
     const bool here = t >= 0 && t < 32 * C::MB && mw + t < nv;
     if (__any(here)) {
@@ -324,41 +384,56 @@ __global__ __launch_bounds__(C::NT) void loss_scores(Mat W, Mat X, uint32_t v0, 
           if (here && t == 32 * x + d_row(r, c.lane / 32)) hit[row] = c.acc[x][b][r];
     }
   }
+  __syncthreads();
+  for (uint32_t x = threadIdx.x; x < C::TN && n0 + x < rows; x += C::NT) {
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (uint32_t w = 0; w < C::WM; w++) top = fmaxf(top, s_part[w][x].x);
+#pragma unroll
+    for (uint32_t w = 0; w < C::WM; w++)
+      sum += s_part[w][x].y *
+             __builtin_amdgcn_exp2f(s_part[w][x].x == top ? 0.f : s_part[w][x].x - top);
+    part[(uint64_t)(v0 / C::TM + m) * rows + n0 + x] = make_float2(top, sum);
+  }
 }
 
-// 32 rows a block, the chunks over 32 groups of lanes, joined in a fixed order.
+// RB rows a block, the chunks over 1024 / RB groups of lanes, joined in a fixed order.
+template <uint32_t RB>
 __global__ __launch_bounds__(1024) void loss_rows(const float2* __restrict__ part,
-                                                  uint32_t part_ld, uint32_t chunks,
+                                                  uint32_t chunks,
                                                   const float* __restrict__ hit,
                                                   pots_vocab_loss a) {
-  __shared__ float2 s_part[32][33];
-  const uint32_t i = threadIdx.x % 32, g = threadIdx.x / 32, row = blockIdx.x * 32 + i;
+  constexpr uint32_t G = 1024 / RB;
+  __shared__ float2 s_part[G][RB + 1];
+  const uint32_t i = threadIdx.x % RB, g = threadIdx.x / RB, row = blockIdx.x * RB + i;
   float m = -INFINITY, l = 0.f;
-  if (row < a.rows)
-    for (uint32_t c = g; c < chunks; c += 32) {
-      const float2 p = part[(uint64_t)c * part_ld + row];
-      if (p.x > m) {
-        l *= __builtin_amdgcn_exp2f(m - p.x);
-        m = p.x;
-      }
-      l += p.y * __builtin_amdgcn_exp2f(p.x - m);
+  auto join = [&](float2 p) {
+    const float top = fmaxf(m, p.x);
+    if (top == -INFINITY) {  // no finite score yet; a NaN among them stays in the sum
+      l += p.y;
+      return;
     }
-  s_part[g][i] = {m, l};
-  __syncthreads();
-  if (g != 0 || row >= a.rows) return;
-  for (uint32_t x = 0; x < 32; x++) m = fmaxf(m, s_part[x][i].x);
-  l = 0.f;
-  for (uint32_t x = 0; x < 32; x++) {
-    const float2 p = s_part[x][i];
-    if (p.x != -INFINITY) l += p.y * __builtin_amdgcn_exp2f(p.x - m);
+    l = l * __builtin_amdgcn_exp2f(m - top) + p.y * __builtin_amdgcn_exp2f(p.x - top);
+    m = top;
+  };
+  if (row < a.rows)
+    for (uint32_t c = g; c < chunks; c += G) join(part[(uint64_t)c * a.rows + row]);
+  for (uint32_t half = G / 2; half > 0; half /= 2) {
+    s_part[g][i] = make_float2(m, l);
+    __syncthreads();
+    if (g < half) join(s_part[g + half][i]);
+    __syncthreads();
   }
+  if (g != 0 || row >= a.rows) return;
   const float lse = (m + __builtin_amdgcn_logf(l)) * kLn2;
   const int64_t t = a.targets[row];
   a.lse[row] = lse;
   a.loss[row] = t < 0 ? 0.f : t < a.vocab ? lse - hit[row] : NAN;
 }
 
-// The piece's G, [terms][live rows][ld], zero past the live rows and the vocabulary.
+// The piece's G in units of the largest weight, [terms][live rows][ld], zero past the live rows
+// and the vocabulary. A lane's results are four vocabulary rows at a time of a row of G; they
+// are gathered in LDS to whole 256-byte spans.
 template <class T, class C>
 __global__ __launch_bounds__(C::NT) void loss_grad(Mat W, Mat X, uint32_t v0, uint32_t nv,
                                                    const uint32_t* __restrict__ count,
@@ -370,78 +445,109 @@ __global__ __launch_bounds__(C::NT) void loss_grad(Mat W, Mat X, uint32_t v0, ui
                                                    uint16_t* __restrict__ g, uint32_t ld,
                                                    uint64_t plane) {
   uint32_t m, n;
-  tile_of(mt, nt, &m, &n);
+  tile_of(blockIdx.x, mt, nt, &m, &n);
   const uint32_t live = gload<uint32_t>(count);
   const uint32_t m0 = m * C::TM, n0 = n * C::TN;
   if (n0 >= live) return;
   C c;
-  c.run(W, X, m0, nv, n0, live, K, 0, 0, pairs);
-  c.each(m0, n0, [&](f32x16& s, uint32_t v, uint32_t row) {
+  c.run(W, X, m0, nv, n0, live, 0, K, 0, 0, pairs);
+  constexpr uint32_t kTerms = sizeof(typename T::elem) == 4 ? 3 : 1;
+  constexpr uint32_t CW = 4 * C::MB;  // 16-byte chunks of a wave's row of G
+  static_assert(CW * 8 * 32 <= C::kScratch, "a wave's 32 rows fit");
+  uint16_t* const s = c.scratch();
+  const uint32_t i = c.lane % 32, h = c.lane / 32;
+  __syncthreads();  // the last stage has been read
+#pragma unroll
+  for (uint32_t b = 0; b < C::NB; b++) {
+    const uint32_t row = n0 + c.wn + 32 * b + i;
     const bool on = row < live;
     const float w = on ? weight[row] : 0.f, l2 = on ? lse2[row] : 0.f;
-    const uint32_t t = on ? target[row] - v0 : ~0u;
+    const uint32_t t = on ? target[row] - v0 - m0 - c.wm : ~0u;
+    const uint32_t left = on && nv > m0 + c.wm ? nv - m0 - c.wm : 0;
 #pragma unroll
-    for (uint32_t q = 0; q < 4; q++) {
-      uint16_t e[4][3];
+    for (uint32_t x = 0; x < C::MB; x++)
 #pragma unroll
-      for (uint32_t x = 0; x < 4; x++) {
-        const uint32_t at = v + 8 * q + x;
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + x], kLog2e, -l2));
-        const float y = on && at < nv ? w * (at == t ? p - 1.f : p) : 0.f;
-        if constexpr (sizeof(typename T::elem) == 4)
-          split3(y, e[x]);
-        else
-          e[x][0] = f32_to_bf16(y);
+      for (uint32_t r = 0; r < 16; r++) {
+        const uint32_t at = 32 * x + d_row(r, h);
+        const float p =
+            __builtin_amdgcn_exp2f(__builtin_fmaf(c.acc[x][b][r], kLog2e, -l2));
+        c.acc[x][b][r] = at < left ? w * (at == t ? p - 1.f : p) : 0.f;
       }
 #pragma unroll
-      for (uint32_t k = 0; k < (sizeof(typename T::elem) == 4 ? 3 : 1); k++) {
-        const u32x2v o = {(uint32_t)e[0][k] | (uint32_t)e[1][k] << 16,
-                          (uint32_t)e[2][k] | (uint32_t)e[3][k] << 16};
-        *reinterpret_cast<u32x2v*>(g + k * plane + (uint64_t)row * ld + v + 8 * q) = o;
-      }
-    }
-  });
-}
-
-// dx's share of the piece: Wᵀ (stored along the contraction) by G, added to sums [rows][dp].
-template <class C>
-__global__ __launch_bounds__(C::NT) void loss_dx(Mat W, Mat G, uint32_t dp, uint32_t nv,
-                                                 const uint32_t* __restrict__ count, uint32_t K,
-                                                 uint32_t pairs, uint32_t mt, uint32_t nt,
-                                                 float* __restrict__ sums, bool first) {
-  uint32_t m, n;
-  tile_of(mt, nt, &m, &n);
-  const uint32_t live = gload<uint32_t>(count);
-  const uint32_t m0 = m * C::TM, n0 = n * C::TN;
-  if (n0 >= live) return;
-  C c;
-  c.run(W, G, m0, dp, n0, live, K, nv, 0, pairs);
-  c.each(m0, n0, [&](f32x16& s, uint32_t col, uint32_t row) {
-    if (row >= live) return;
+    for (uint32_t k = 0; k < kTerms; k++) {
 #pragma unroll
-    for (uint32_t q = 0; q < 4; q++) {
-      if (col + 8 * q >= dp) continue;
-      f32x4* p = reinterpret_cast<f32x4*>(sums + (uint64_t)row * dp + col + 8 * q);
-      f32x4 y = {s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
-      if (!first) y += *p;
-      *p = y;
+      for (uint32_t x = 0; x < C::MB; x++)
+#pragma unroll
+        for (uint32_t q = 0; q < 4; q++) {
+          uint16_t e[4];
+#pragma unroll
+          for (uint32_t y = 0; y < 4; y++) {
+            if constexpr (kTerms == 3) {
+              float v = c.acc[x][b][4 * q + y];
+              e[y] = take_term(&v);
+              c.acc[x][b][4 * q + y] = v;
+            } else {
+              e[y] = f32_to_bf16(c.acc[x][b][4 * q + y]);
+            }
+          }
+          const u32x2v o = {(uint32_t)e[0] | (uint32_t)e[1] << 16,
+                            (uint32_t)e[2] | (uint32_t)e[3] << 16};
+          *reinterpret_cast<u32x2v*>(s + i * 8 * CW + ((4 * x + q) ^ (i % CW)) * 8 + 4 * h) = o;
+        }
+      // (a wave's own LDS: its writes and reads are in order)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (uint32_t y = 0; y < CW / 2; y++) {
+        const uint32_t r = (c.lane + 64 * y) / CW, ch = c.lane % CW;
+        const u32x4v o = *reinterpret_cast<const u32x4v*>(s + r * 8 * CW + (ch ^ (r % CW)) * 8);
+        gstore<u32x4v>(g + k * plane + (uint64_t)(n0 + c.wn + 32 * b + r) * ld + m0 + c.wm +
+                           8 * ch,
+                       o);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-  });
+  }
 }
 
-// The piece's rows of dW: Xᵀ by Gᵀ, both stored along the contraction (the live rows).
-template <class T, class C>
-__global__ __launch_bounds__(C::NT) void loss_dw(Mat X, Mat G, uint32_t dp, uint32_t nv,
-                                                 const uint32_t* __restrict__ count,
-                                                 uint32_t pairs, uint32_t mt, uint32_t nt,
-                                                 uint32_t d, typename T::elem* __restrict__ dw,
-                                                 int64_t ld, bool vec) {
-  uint32_t m, n;
-  tile_of(mt, nt, &m, &n);
+// Both products of a piece of G in one launch, so that the tiles of one fill the GPU's places
+// beside the other's. Blocks below mt·nt·splits: a share of dx, Wᵀ (stored along the
+// contraction, the piece's vocabulary) by G, added to the split's sums [rows][dp]. The others:
+// the piece's rows of dW, Xᵀ by Gᵀ, both stored along the contraction (the live rows).
+template <class T, class CX, class CW>
+__global__ __launch_bounds__(CX::NT) void loss_products(
+    Mat W, Mat X, Mat G, uint32_t dp, uint32_t nv, const uint32_t* __restrict__ count,
+    const float* __restrict__ unit, uint32_t pairs, uint32_t mt, uint32_t nt, uint32_t splits,
+    uint32_t per, float* __restrict__ sums, uint64_t slice, bool first, uint32_t wmt,
+    uint32_t wnt, uint32_t d, typename T::elem* __restrict__ dw, int64_t ld, bool vec) {
   const uint32_t live = gload<uint32_t>(count);
-  const uint32_t m0 = m * C::TM, n0 = n * C::TN, K = (live + BK - 1) / BK * BK;
-  C c;
-  c.run(X, G, m0, dp, n0, (nv + 7) & ~7u, K, K, K, pairs);
+  uint32_t m, n;
+  if (blockIdx.x < mt * nt * splits) {
+    const uint32_t split = blockIdx.x / (mt * nt);
+    tile_of(blockIdx.x % (mt * nt), mt, nt, &m, &n);
+    const uint32_t m0 = m * CX::TM, n0 = n * CX::TN, k0 = split * per;
+    if (n0 >= live) return;
+    CX c;
+    const uint32_t all = (nv + BK - 1) / BK * BK;
+    c.run(W, G, m0, dp, n0, live, k0, k0 < all ? min(per, all - k0) : 0, nv, 0, pairs);
+    float* out = sums + split * slice;
+    c.each(m0, n0, [&](f32x16& s, uint32_t col, uint32_t row) {
+      if (row >= live) return;
+#pragma unroll
+      for (uint32_t q = 0; q < 4; q++) {
+        if (col + 8 * q >= dp) continue;
+        f32x4* p = reinterpret_cast<f32x4*>(out + (uint64_t)row * dp + col + 8 * q);
+        f32x4 y = {s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+        if (!first) y += *p;
+        *p = y;
+      }
+    });
+    return;
+  }
+  tile_of(blockIdx.x - mt * nt * splits, wmt, wnt, &m, &n);
+  const uint32_t m0 = m * CW::TM, n0 = n * CW::TN, K = (live + BK - 1) / BK * BK;
+  CW c;
+  c.run(X, G, m0, dp, n0, (nv + 7) & ~7u, 0, K, live, live, pairs);
+  const float mul = *unit;
   c.each(m0, n0, [&](f32x16& s, uint32_t col, uint32_t v) {
     if (v >= nv) return;
     typename T::elem* p = dw + (int64_t)v * ld;
@@ -450,40 +556,67 @@ __global__ __launch_bounds__(C::NT) void loss_dw(Mat X, Mat G, uint32_t dp, uint
       const uint32_t at = col + 8 * q;
       if (at >= d) continue;
       if (vec) {
-        T::store4(p + at, s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]);
+        T::store4(p + at, s[4 * q] * mul, s[4 * q + 1] * mul, s[4 * q + 2] * mul,
+                  s[4 * q + 3] * mul);
       } else {
 #pragma unroll
         for (uint32_t x = 0; x < 4; x++)
-          if (at + x < d) p[at + x] = T::put(s[4 * q + x]);
+          if (at + x < d) p[at + x] = T::put(s[4 * q + x] * mul);
       }
     }
   });
 }
 
-// dx from the sums: a block a row, zero for the rows left out.
+// dx from the splits' sums: a block a row, zero for the rows left out.
 template <class T>
 __global__ __launch_bounds__(256) void loss_dx_rows(const float* __restrict__ sums, uint32_t dp,
+                                                    uint32_t splits, uint64_t slice,
                                                     const uint32_t* __restrict__ pos,
-                                                    uint32_t d, typename T::elem* dx,
-                                                    int64_t ld) {
+                                                    const float* __restrict__ unit, uint32_t d,
+                                                    typename T::elem* dx, int64_t ld) {
   const uint32_t row = blockIdx.x, at = pos[row];
-  for (uint32_t c = threadIdx.x; c < d; c += 256)
-    dx[(int64_t)row * ld + c] = T::put(at == ~0u ? 0.f : sums[(uint64_t)at * dp + c]);
+  const float mul = *unit;
+  typename T::elem* out = dx + (int64_t)row * ld;
+  for (uint32_t c = threadIdx.x * 4; c < d; c += 1024) {
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    if (at != ~0u)
+      for (uint32_t s = 0; s < splits; s++)
+        y += gload<f32x4>(sums + s * slice + (uint64_t)at * dp + c);
+#pragma unroll
+    for (uint32_t x = 0; x < 4; x++)
+      if (c + x < d) out[c + x] = T::put(y[x] * mul);
+  }
 }
 
 namespace {
 
-typedef Tile<false, false, 128, 128, 2, 2> Scores;
-typedef Tile<true, false, 128, 128, 2, 2> DxTile;
-typedef Tile<true, true, 128, 128, 2, 2> DwTile;
+// Tiles. Large ones read each operand half as often and reach 1.1 PFLOP/s where there are enough of
+// them for the GPU; up to 32 rows the product is bound by reading W, and a tile as narrow as
+// the rows leaves its multiplications out of the way.
+template <bool ATR, bool BTR>
+using Large = Tile<ATR, BTR, 256, 256, 2, 4>;
+template <bool ATR, bool BTR>
+using Medium = Tile<ATR, BTR, 128, 128, 2, 2>;
+template <bool ATR, bool BTR>
+using Narrow = Tile<ATR, BTR, 256, 32, 8, 1>;
+enum Shape { kLarge, kMedium, kNarrow };
+
+constexpr uint32_t kCus = 256;
 
 uint32_t cdiv(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
+
+Shape scores_shape(uint32_t rows, uint32_t piece) {
+  if (rows <= 32) return kNarrow;
+  return rows > 128 && (uint64_t)cdiv(rows, 256) * cdiv(piece, 256) >= kCus ? kLarge : kMedium;
+}
 
 // Sizes and the workspace's parts.
 struct Plan {
   uint32_t dp, terms, pairs, rows_pad, piece;
+  Shape scores, products;
+  uint32_t splits, per;  // of dx's contraction
   bool copy_w, copy_x;
-  uint64_t w, x, part, hit, idx, pos, count, weight, lse2, target, g, sums, bytes;
+  uint64_t w, x, part, hit, idx, pos, count, unit, weight, lse2, target, g, sums, bytes;
 };
 
 uint64_t take(Plan* p, uint64_t bytes) {
@@ -498,27 +631,47 @@ bool as_is(const pots_vocab_loss* a, const void* p, int64_t row) {
 }
 
 Plan plan(const pots_vocab_loss* a, bool backward) {
+  constexpr uint64_t kRoom = 512ull << 20;  // bytes of a piece of G, and of a copied one of W
   Plan p = {};
   p.terms = a->dtype == POTS_OP_BF16 ? 1 : 3;
   p.pairs = a->dtype == POTS_OP_BF16 ? 1 : 6;
   p.dp = cdiv(a->dim, BK) * BK;
-  p.rows_pad = cdiv(a->rows, 128) * 128;
+  p.rows_pad = cdiv(a->rows, 256) * 256;
   p.copy_w = !as_is(a, a->w, a->w_row);
   p.copy_x = backward || !as_is(a, a->x, a->x_row);
-  const uint32_t all = cdiv(a->vocab, 128) * 128;
-  p.piece = backward || p.copy_w ? min(all, 16384u) : all;
+  const uint32_t all = cdiv(a->vocab, 256) * 256;
+  uint64_t most = all;
+  if (p.copy_w) most = min(most, kRoom / (2ull * p.terms * p.dp));
+  if (backward && a->rows) most = min(most, kRoom / (2ull * p.terms * p.rows_pad));
+  most = max(most, (uint64_t)2048);
+  const uint32_t pieces = (uint32_t)((all + most - 1) / most);
+  p.piece = cdiv(cdiv(all, pieces), 256) * 256;
+  p.scores = scores_shape(a->rows, p.piece);
   if (p.copy_w) p.w = take(&p, 2ull * p.terms * p.piece * p.dp);
   if (p.copy_x) p.x = take(&p, 2ull * p.terms * p.rows_pad * p.dp);
   if (!backward) {
-    p.part = take(&p, 8ull * (all / (32 * Scores::MB)) * a->rows);
+    p.part = take(&p, 8ull * (all / 128) * a->rows);
     p.hit = take(&p, 4ull * a->rows);
-  } else {
-    for (uint64_t* q : {&p.idx, &p.pos, &p.weight, &p.lse2, &p.target})
-      *q = take(&p, 4ull * p.rows_pad);
-    p.count = take(&p, 4);
-    p.g = take(&p, 2ull * p.terms * p.rows_pad * p.piece);
-    p.sums = take(&p, 4ull * p.rows_pad * p.dp);
+    return p;
   }
+  for (uint64_t* q : {&p.idx, &p.pos, &p.weight, &p.lse2, &p.target})
+    *q = take(&p, 4ull * p.rows_pad);
+  p.count = take(&p, 4);
+  p.unit = take(&p, 4);
+  p.g = take(&p, 2ull * p.terms * p.rows_pad * p.piece);
+  // Shares of dx's contraction about as long as dW's, so that the launch's blocks are alike, and
+  // shorter ones where the GPU would not be full; each share has sums of its own.
+  p.products = p.scores;
+  const uint32_t tm = p.products == kMedium ? 128 : 256, tn = p.products == kNarrow ? 32 : tm;
+  const uint32_t k_dx = p.piece / BK, k_dw = p.rows_pad / BK;
+  const uint32_t dx_tiles = cdiv(p.dp, tm) * cdiv(a->rows, tn);
+  const uint32_t dw_tiles = cdiv(p.dp, tm) * cdiv(p.piece, tm);
+  p.splits = k_dw ? min(max((k_dx + k_dw / 2) / k_dw, 1u), 16u) : 1;
+  while (p.splits < 16 && dx_tiles * p.splits + dw_tiles < 2 * kCus && k_dx / p.splits > 8)
+    p.splits++;
+  p.per = cdiv(k_dx, p.splits) * BK;
+  p.splits = cdiv(p.piece, p.per);
+  p.sums = take(&p, 4ull * p.splits * p.rows_pad * p.dp);
   return p;
 }
 
@@ -555,6 +708,17 @@ int piece_of_w(const pots_vocab_loss* a, const Plan& p, char* work, uint32_t v0,
   return lay<T>(src, a->w_row, a->dim, nv, nullptr, nullptr, dst, p, W->plane, nv, s);
 }
 
+template <class C>
+int scores(const pots_vocab_loss* a, const Plan& p, const Mat& W, const Mat& X, uint32_t v0,
+           uint32_t nv, char* work, hipStream_t s) {
+  const uint32_t mt = cdiv(nv, C::TM), nt = cdiv(a->rows, C::TN);
+  hipLaunchKernelGGL((loss_scores<C>), dim3(mt * nt), dim3(C::NT), 0, s, W, X, v0, nv, a->rows,
+                     p.dp, p.pairs, mt, nt, a->targets, reinterpret_cast<float2*>(work + p.part),
+                     reinterpret_cast<float*>(work + p.hit));
+  POTS_HIP(hipGetLastError());
+  return POTS_E_OK;
+}
+
 template <class T>
 int forward(const pots_vocab_loss* a, char* work, hipStream_t s) {
   const Plan p = plan(a, false);
@@ -566,20 +730,56 @@ int forward(const pots_vocab_loss* a, char* work, hipStream_t s) {
                           a->rows, s);
     if (rc) return rc;
   }
-  float2* part = reinterpret_cast<float2*>(work + p.part);
-  float* hit = reinterpret_cast<float*>(work + p.hit);
   for (uint32_t v0 = 0; v0 < a->vocab; v0 += p.piece) {
-    const uint32_t nv = a->vocab - v0 < p.piece ? a->vocab - v0 : p.piece;
+    const uint32_t nv = min(a->vocab - v0, p.piece);
     Mat W;
-    const int rc = piece_of_w<T>(a, p, work, v0, nv, &W, s);
+    int rc = piece_of_w<T>(a, p, work, v0, nv, &W, s);
     if (rc) return rc;
-    const uint32_t mt = cdiv(nv, Scores::TM), nt = cdiv(a->rows, Scores::TN);
-    hipLaunchKernelGGL((loss_scores<Scores>), dim3(mt * nt), dim3(Scores::NT), 0, s, W, X, v0,
-                       nv, a->rows, p.dp, p.pairs, mt, nt, a->targets, part, a->rows, hit);
+    rc = p.scores == kLarge    ? scores<Large<false, false>>(a, p, W, X, v0, nv, work, s)
+         : p.scores == kMedium ? scores<Medium<false, false>>(a, p, W, X, v0, nv, work, s)
+                               : scores<Narrow<false, false>>(a, p, W, X, v0, nv, work, s);
+    if (rc) return rc;
+  }
+  const float2* part = reinterpret_cast<const float2*>(work + p.part);
+  const float* hit = reinterpret_cast<const float*>(work + p.hit);
+  const uint32_t chunks = cdiv(a->vocab, p.scores == kMedium ? 128 : 256);
+  // four rows a block, in 32-byte reads, where 32 a block would not fill the GPU
+  if (a->rows < 32 * kCus)
+    hipLaunchKernelGGL(loss_rows<4>, dim3(cdiv(a->rows, 4)), dim3(1024), 0, s, part, chunks, hit,
+                       *a);
+  else
+    hipLaunchKernelGGL(loss_rows<32>, dim3(cdiv(a->rows, 32)), dim3(1024), 0, s, part, chunks,
+                       hit, *a);
+  POTS_HIP(hipGetLastError());
+  return POTS_E_OK;
+}
+
+template <class T, template <bool, bool> class S, template <bool, bool> class SW>
+int piece_grads(const pots_vocab_loss* a, const Plan& p, const Mat& W, const Mat& X, uint32_t v0,
+                uint32_t nv, char* work, hipStream_t s) {
+  auto f32 = [&](uint64_t at) { return reinterpret_cast<float*>(work + at); };
+  const uint32_t* count = reinterpret_cast<const uint32_t*>(work + p.count);
+  typedef S<false, false> C;
+  typedef S<true, false> CX;
+  typedef SW<true, true> CW;
+  uint16_t* g = reinterpret_cast<uint16_t*>(work + p.g);
+  const Mat G = {g, (int64_t)p.piece, (int64_t)p.rows_pad * p.piece};
+  const uint32_t mt = cdiv(nv, C::TM), nt = cdiv(a->rows, C::TN);
+  if (mt * nt) {
+    hipLaunchKernelGGL((loss_grad<T, C>), dim3(mt * nt), dim3(C::NT), 0, s, W, X, v0, nv, count,
+                       p.dp, p.pairs, mt, nt, f32(p.weight), f32(p.lse2),
+                       reinterpret_cast<const uint32_t*>(work + p.target), g, p.piece, G.plane);
     POTS_HIP(hipGetLastError());
   }
-  hipLaunchKernelGGL(loss_rows, dim3(cdiv(a->rows, 32)), dim3(1024), 0, s, part, a->rows,
-                     cdiv(a->vocab, Scores::TM) * (Scores::TM / (32 * Scores::MB)), hit, *a);
+  typedef typename T::elem elem;
+  const bool vec = a->dim % 4 == 0 && a->dw_row % 4 == 0 &&
+                   reinterpret_cast<uint64_t>(a->dw) % (4 * sizeof(elem)) == 0;
+  const uint32_t xmt = cdiv(p.dp, CX::TM), wmt = cdiv(p.dp, CW::TM), wnt = cdiv(nv, CW::TN);
+  hipLaunchKernelGGL((loss_products<T, CX, CW>), dim3(xmt * nt * p.splits + wmt * wnt),
+                     dim3(CX::NT), 0, s, W, X, G, p.dp, nv, count, f32(p.unit), p.pairs, xmt, nt,
+                     p.splits, p.per, f32(p.sums), (uint64_t)p.rows_pad * p.dp, v0 == 0, wmt,
+                     wnt, a->dim, reinterpret_cast<elem*>(a->dw) + (int64_t)v0 * a->dw_row,
+                     a->dw_row, vec);
   POTS_HIP(hipGetLastError());
   return POTS_E_OK;
 }
@@ -589,47 +789,30 @@ int backward(const pots_vocab_loss* a, char* work, hipStream_t s) {
   const Plan p = plan(a, true);
   auto u32 = [&](uint64_t at) { return reinterpret_cast<uint32_t*>(work + at); };
   auto f32 = [&](uint64_t at) { return reinterpret_cast<float*>(work + at); };
-  uint32_t* count = u32(p.count);
-  hipLaunchKernelGGL(live_rows, dim3(1), dim3(1024), 0, s, *a, u32(p.idx), u32(p.pos), count,
-                     f32(p.weight), f32(p.lse2), u32(p.target));
+  hipLaunchKernelGGL(live_rows, dim3(1), dim3(1024), 0, s, *a, u32(p.idx), u32(p.pos),
+                     u32(p.count), f32(p.weight), f32(p.lse2), u32(p.target), f32(p.unit));
   POTS_HIP(hipGetLastError());
   uint16_t* xs = reinterpret_cast<uint16_t*>(work + p.x);
   const Mat X = {xs, (int64_t)p.dp, (int64_t)p.rows_pad * p.dp};
-  int rc = a->rows == 0 ? POTS_E_OK
-                        : lay<T>(a->x, a->x_row, a->dim, a->rows, u32(p.idx), count, xs, p,
-                                 X.plane, p.rows_pad, s);
-  if (rc) return rc;
-  uint16_t* g = reinterpret_cast<uint16_t*>(work + p.g);
-  const Mat G = {g, (int64_t)p.piece, (int64_t)p.rows_pad * p.piece};
-  const int64_t esize = sizeof(typename T::elem);
-  const bool vec = a->dim % 4 == 0 && a->dw_row % 4 == 0 &&
-                   reinterpret_cast<uint64_t>(a->dw) % (4 * esize) == 0;
-  for (uint32_t v0 = 0; v0 < a->vocab; v0 += p.piece) {
-    const uint32_t nv = a->vocab - v0 < p.piece ? a->vocab - v0 : p.piece;
-    const uint32_t wmt = cdiv(p.dp, DwTile::TM), wnt = cdiv(nv, DwTile::TN);
-    const uint32_t mt = cdiv(nv, Scores::TM), nt = cdiv(a->rows, Scores::TN);
-    const uint32_t dmt = cdiv(p.dp, DxTile::TM), dnt = cdiv(a->rows, DxTile::TN);
-    if (a->rows) {
-    Mat W;
-    rc = piece_of_w<T>(a, p, work, v0, nv, &W, s);
+  if (a->rows) {
+    const int rc = lay<T>(a->x, a->x_row, a->dim, a->rows, u32(p.idx), u32(p.count), xs, p,
+                          X.plane, p.rows_pad, s);
     if (rc) return rc;
-    hipLaunchKernelGGL((loss_grad<T, Scores>), dim3(mt * nt), dim3(Scores::NT), 0, s, W, X, v0,
-                       nv, count, p.dp, p.pairs, mt, nt, f32(p.weight), f32(p.lse2),
-                       u32(p.target), g, p.piece, G.plane);
-    POTS_HIP(hipGetLastError());
-    hipLaunchKernelGGL((loss_dx<DxTile>), dim3(dmt * dnt), dim3(DxTile::NT), 0, s, W, G, p.dp,
-                       nv, count, cdiv(nv, BK) * BK, p.pairs, dmt, dnt, f32(p.sums), v0 == 0);
-    POTS_HIP(hipGetLastError());
-    }
-    hipLaunchKernelGGL((loss_dw<T, DwTile>), dim3(wmt * wnt), dim3(DwTile::NT), 0, s, X, G,
-                       p.dp, nv, count, p.pairs, wmt, wnt, a->dim,
-                       reinterpret_cast<typename T::elem*>(a->dw) + (int64_t)v0 * a->dw_row,
-                       a->dw_row, vec);
-    POTS_HIP(hipGetLastError());
+  }
+  for (uint32_t v0 = 0; v0 < a->vocab; v0 += p.piece) {
+    const uint32_t nv = min(a->vocab - v0, p.piece);
+    Mat W = {};
+    int rc = a->rows ? piece_of_w<T>(a, p, work, v0, nv, &W, s) : POTS_E_OK;
+    if (rc) return rc;
+    rc = p.products == kLarge    ? piece_grads<T, Large, Large>(a, p, W, X, v0, nv, work, s)
+         : p.products == kMedium ? piece_grads<T, Medium, Medium>(a, p, W, X, v0, nv, work, s)
+                                 : piece_grads<T, Narrow, Large>(a, p, W, X, v0, nv, work, s);
+    if (rc) return rc;
   }
   if (a->rows == 0) return POTS_E_OK;
   hipLaunchKernelGGL((loss_dx_rows<T>), dim3(a->rows), dim3(256), 0, s, f32(p.sums), p.dp,
-                     u32(p.pos), a->dim, reinterpret_cast<typename T::elem*>(a->dx), a->dx_row);
+                     p.splits, (uint64_t)p.rows_pad * p.dp, u32(p.pos), f32(p.unit), a->dim,
+                     reinterpret_cast<typename T::elem*>(a->dx), a->dx_row);
   POTS_HIP(hipGetLastError());
   return POTS_E_OK;
 }
