@@ -27,7 +27,8 @@
 namespace pots {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr uint32_t BK = 64;  // contraction per stage: 128 bytes of a row
+
+constexpr uint32_t kStep = 64;  // contractions are padded to 128 bytes of a row
 
 // A matrix of bf16 terms: rows `ld` elements apart, term planes `plane` elements apart.
 struct Mat {
@@ -51,17 +52,22 @@ __device__ __forceinline__ void load_lds16(brsrc rsrc, uint16_t* lds, uint32_t o
 #endif
 }
 
-// T rows of an operand and BK of the contraction in LDS, in 16-byte chunks that one
+// T rows of an operand and BK (32 or 64) of the contraction in LDS, in 16-byte chunks that one
 // instruction brings in for 64 lanes, straight from memory. TR: stored [contraction][rows], so
 // a stage is BK rows of T columns; else T rows of BK columns. A chunk is exchanged within its
 // row by the row's number, so that the reads of a fragment fall on different banks: eight
 // lanes' 16-byte reads of eight rows, or 32 lanes' transposing reads of four rows. A lane's
 // offsets are the same at every stage; the stage moves the buffer's base, in scalar registers.
-template <bool TR, uint32_t T, uint32_t NT>
+template <bool TR, uint32_t T, uint32_t NT, uint32_t BK>
 struct Stage {
   static constexpr uint32_t kAll = T * BK / 8, kChunks = (kAll + NT - 1) / NT;
   static_assert(!TR || T >= 128, "the exchange of a transposed tile needs 16 chunks a row");
   uint32_t off[kChunks], wide;
+
+  // What row r's chunks are exchanged by.
+  static __device__ __forceinline__ uint32_t swap(uint32_t r) {
+    return TR ? 4 * (r & 3) : BK == 64 ? r & 7 : (r >> 1) & 3;
+  }
 
   // r0, rows: the tile's first row and their number; rows past it repeat the last (for TR:
   // columns, whose last eight repeat).
@@ -71,10 +77,10 @@ struct Stage {
     for (uint32_t u = 0; u < kChunks; u++) {
       const uint32_t c = u * NT + threadIdx.x;
       if constexpr (TR) {
-        const uint32_t r = c / (T / 8), at = (c % (T / 8)) ^ (4 * (r & 3));
+        const uint32_t r = c / (T / 8), at = (c % (T / 8)) ^ swap(r);
         off[u] = 2 * (r * (uint32_t)m.ld + min(r0 + 8 * at, rows - 8) - r0);
       } else {
-        const uint32_t r = c / (BK / 8), at = (c % (BK / 8)) ^ (r & 7);
+        const uint32_t r = c / (BK / 8), at = (c % (BK / 8)) ^ swap(r);
         off[u] = 2 * (min(r, rows - 1 - r0) * (uint32_t)m.ld + 8 * at);
       }
     }
@@ -103,11 +109,11 @@ struct Stage {
     if constexpr (TR) {
       const uint32_t m = lane % 16, r = 16 * ks + 8 * h + m / 4;
       const uint32_t col = c + (lane & 16) + 4 * (m % 4);
-      const uint16_t* p = lds + r * T + (((col / 8) ^ (4 * (m / 4))) * 8 + 4 * (m % 2));
+      const uint16_t* p = lds + r * T + (((col / 8) ^ swap(m / 4)) * 8 + 4 * (m % 2));
       return join(read_tr(p), read_tr(p + 4 * T));
     } else {
       const uint32_t r = c + lane % 32;
-      return *reinterpret_cast<const bf16x8*>(lds + r * BK + (((2 * ks + h) ^ (lane & 7)) * 8));
+      return *reinterpret_cast<const bf16x8*>(lds + r * BK + (((2 * ks + h) ^ swap(lane % 32)) * 8));
     }
   }
 };
@@ -127,12 +133,13 @@ __device__ __forceinline__ uint16_t* lds_buffer() {
 }
 
 // A block's TM x TN of A·Bᵀ over K (a multiple of BK), WM x WN waves of MB x NB products of 32.
-template <bool ATR, bool BTR, uint32_t TM_, uint32_t TN_, uint32_t WM_, uint32_t WN_>
+template <bool ATR, bool BTR, uint32_t TM_, uint32_t TN_, uint32_t WM_, uint32_t WN_,
+          uint32_t BK>
 struct Tile {
   static constexpr uint32_t TM = TM_, TN = TN_, WM = WM_, WN = WN_, NT = 64 * WM * WN;
   static constexpr uint32_t MB = TM / WM / 32, NB = TN / WN / 32;
-  typedef Stage<ATR, TM, NT> SA;
-  typedef Stage<BTR, TN, NT> SB;
+  typedef Stage<ATR, TM, NT, BK> SA;
+  typedef Stage<BTR, TN, NT, BK> SB;
   f32x16 acc[MB][NB];
   uint32_t wm, wn, lane;
 
@@ -438,17 +445,16 @@ template <class T, class C>
 __global__ __launch_bounds__(C::NT) void loss_grad(Mat W, Mat X, uint32_t v0, uint32_t nv,
                                                    const uint32_t* __restrict__ count,
                                                    uint32_t K, uint32_t pairs, uint32_t mt,
-                                                   uint32_t nt,
                                                    const float* __restrict__ weight,
                                                    const float* __restrict__ lse2,
                                                    const uint32_t* __restrict__ target,
                                                    uint16_t* __restrict__ g, uint32_t ld,
                                                    uint64_t plane) {
   uint32_t m, n;
+  const uint32_t live = gload<uint32_t>(count), nt = (live + C::TN - 1) / C::TN;
+  if (blockIdx.x >= mt * nt) return;
   tile_of(blockIdx.x, mt, nt, &m, &n);
-  const uint32_t live = gload<uint32_t>(count);
   const uint32_t m0 = m * C::TM, n0 = n * C::TN;
-  if (n0 >= live) return;
   C c;
   c.run(W, X, m0, nv, n0, live, 0, K, 0, 0, pairs);
   constexpr uint32_t kTerms = sizeof(typename T::elem) == 4 ? 3 : 1;
@@ -516,18 +522,18 @@ __global__ __launch_bounds__(C::NT) void loss_grad(Mat W, Mat X, uint32_t v0, ui
 template <class T, class CX, class CW>
 __global__ __launch_bounds__(CX::NT) void loss_products(
     Mat W, Mat X, Mat G, uint32_t dp, uint32_t nv, const uint32_t* __restrict__ count,
-    const float* __restrict__ unit, uint32_t pairs, uint32_t mt, uint32_t nt, uint32_t splits,
+    const float* __restrict__ unit, uint32_t pairs, uint32_t mt, uint32_t splits,
     uint32_t per, float* __restrict__ sums, uint64_t slice, bool first, uint32_t wmt,
     uint32_t wnt, uint32_t d, typename T::elem* __restrict__ dw, int64_t ld, bool vec) {
-  const uint32_t live = gload<uint32_t>(count);
+  // (the tiles of the live rows alone, dealt over all XCDs; the launch has room for every row)
+  const uint32_t live = gload<uint32_t>(count), nt = (live + CX::TN - 1) / CX::TN;
   uint32_t m, n;
   if (blockIdx.x < mt * nt * splits) {
     const uint32_t split = blockIdx.x / (mt * nt);
     tile_of(blockIdx.x % (mt * nt), mt, nt, &m, &n);
     const uint32_t m0 = m * CX::TM, n0 = n * CX::TN, k0 = split * per;
-    if (n0 >= live) return;
     CX c;
-    const uint32_t all = (nv + BK - 1) / BK * BK;
+    const uint32_t all = (nv + kStep - 1) / kStep * kStep;
     c.run(W, G, m0, dp, n0, live, k0, k0 < all ? min(per, all - k0) : 0, nv, 0, pairs);
     float* out = sums + split * slice;
     c.each(m0, n0, [&](f32x16& s, uint32_t col, uint32_t row) {
@@ -543,8 +549,9 @@ __global__ __launch_bounds__(CX::NT) void loss_products(
     });
     return;
   }
+  if (blockIdx.x >= mt * nt * splits + wmt * wnt) return;
   tile_of(blockIdx.x - mt * nt * splits, wmt, wnt, &m, &n);
-  const uint32_t m0 = m * CW::TM, n0 = n * CW::TN, K = (live + BK - 1) / BK * BK;
+  const uint32_t m0 = m * CW::TM, n0 = n * CW::TN, K = (live + kStep - 1) / kStep * kStep;
   CW c;
   c.run(X, G, m0, dp, n0, (nv + 7) & ~7u, 0, K, live, live, pairs);
   const float mul = *unit;
@@ -594,11 +601,11 @@ namespace {
 // them for the GPU; up to 32 rows the product is bound by reading W, and a tile as narrow as
 // the rows leaves its multiplications out of the way.
 template <bool ATR, bool BTR>
-using Large = Tile<ATR, BTR, 256, 256, 2, 4>;
+using Large = Tile<ATR, BTR, 256, 256, 2, 4, 64>;
 template <bool ATR, bool BTR>
-using Medium = Tile<ATR, BTR, 128, 128, 2, 2>;
+using Medium = Tile<ATR, BTR, 128, 128, 2, 2, 64>;
 template <bool ATR, bool BTR>
-using Narrow = Tile<ATR, BTR, 256, 32, 8, 1>;
+using Narrow = Tile<ATR, BTR, 256, 32, 8, 1, 64>;
 enum Shape { kLarge, kMedium, kNarrow };
 
 constexpr uint32_t kCus = 256;
@@ -626,7 +633,7 @@ uint64_t take(Plan* p, uint64_t bytes) {
 }
 
 bool as_is(const pots_vocab_loss* a, const void* p, int64_t row) {
-  return a->dtype == POTS_OP_BF16 && a->dim % BK == 0 &&
+  return a->dtype == POTS_OP_BF16 && a->dim % kStep == 0 &&
          reinterpret_cast<uint64_t>(p) % 16 == 0 && row % 8 == 0;
 }
 
@@ -635,7 +642,7 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
   Plan p = {};
   p.terms = a->dtype == POTS_OP_BF16 ? 1 : 3;
   p.pairs = a->dtype == POTS_OP_BF16 ? 1 : 6;
-  p.dp = cdiv(a->dim, BK) * BK;
+  p.dp = cdiv(a->dim, kStep) * kStep;
   p.rows_pad = cdiv(a->rows, 256) * 256;
   p.copy_w = !as_is(a, a->w, a->w_row);
   p.copy_x = backward || !as_is(a, a->x, a->x_row);
@@ -663,13 +670,13 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
   // shorter ones where the GPU would not be full; each share has sums of its own.
   p.products = p.scores;
   const uint32_t tm = p.products == kMedium ? 128 : 256, tn = p.products == kNarrow ? 32 : tm;
-  const uint32_t k_dx = p.piece / BK, k_dw = p.rows_pad / BK;
+  const uint32_t k_dx = p.piece / kStep, k_dw = p.rows_pad / kStep;
   const uint32_t dx_tiles = cdiv(p.dp, tm) * cdiv(a->rows, tn);
   const uint32_t dw_tiles = cdiv(p.dp, tm) * cdiv(p.piece, tm);
   p.splits = k_dw ? min(max((k_dx + k_dw / 2) / k_dw, 1u), 16u) : 1;
   while (p.splits < 16 && dx_tiles * p.splits + dw_tiles < 2 * kCus && k_dx / p.splits > 8)
     p.splits++;
-  p.per = cdiv(k_dx, p.splits) * BK;
+  p.per = cdiv(k_dx, p.splits) * kStep;
   p.splits = cdiv(p.piece, p.per);
   p.sums = take(&p, 4ull * p.splits * p.rows_pad * p.dp);
   return p;
@@ -767,7 +774,7 @@ int piece_grads(const pots_vocab_loss* a, const Plan& p, const Mat& W, const Mat
   const uint32_t mt = cdiv(nv, C::TM), nt = cdiv(a->rows, C::TN);
   if (mt * nt) {
     hipLaunchKernelGGL((loss_grad<T, C>), dim3(mt * nt), dim3(C::NT), 0, s, W, X, v0, nv, count,
-                       p.dp, p.pairs, mt, nt, f32(p.weight), f32(p.lse2),
+                       p.dp, p.pairs, mt, f32(p.weight), f32(p.lse2),
                        reinterpret_cast<const uint32_t*>(work + p.target), g, p.piece, G.plane);
     POTS_HIP(hipGetLastError());
   }
@@ -776,7 +783,7 @@ int piece_grads(const pots_vocab_loss* a, const Plan& p, const Mat& W, const Mat
                    reinterpret_cast<uint64_t>(a->dw) % (4 * sizeof(elem)) == 0;
   const uint32_t xmt = cdiv(p.dp, CX::TM), wmt = cdiv(p.dp, CW::TM), wnt = cdiv(nv, CW::TN);
   hipLaunchKernelGGL((loss_products<T, CX, CW>), dim3(xmt * nt * p.splits + wmt * wnt),
-                     dim3(CX::NT), 0, s, W, X, G, p.dp, nv, count, f32(p.unit), p.pairs, xmt, nt,
+                     dim3(CX::NT), 0, s, W, X, G, p.dp, nv, count, f32(p.unit), p.pairs, xmt,
                      p.splits, p.per, f32(p.sums), (uint64_t)p.rows_pad * p.dp, v0 == 0, wmt,
                      wnt, a->dim, reinterpret_cast<elem*>(a->dw) + (int64_t)v0 * a->dw_row,
                      a->dw_row, vec);
