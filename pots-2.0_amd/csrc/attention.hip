@@ -71,55 +71,86 @@ __device__ __forceinline__ typename T::frag load_frag(const typename T::elem* ba
   }
 }
 
-// Eight values of an LDS tile's row from column c on.
-template <class T>
-__device__ __forceinline__ typename T::frag lds_row(const typename T::elem* tile,
-                                                    uint32_t stride, uint32_t r, uint32_t c) {
-  const typename T::elem* p = tile + r * stride + c;
-  if constexpr (sizeof(typename T::elem) == 2) {
-    return *reinterpret_cast<const bf16x8*>(p);
-  } else {
-    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0];
-    const f32x4 b = reinterpret_cast<const f32x4*>(p)[1];
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
-}
-
-// Column c + i of an LDS tile at the rows that a D's registers 8t .. 8t + 7 hold: r0 + 4h +
-// (0..3) and r0 + 8 + 4h + (0..3), r0 = 16t.
-template <class T>
-__device__ __forceinline__ typename T::frag lds_col(const typename T::elem* tile,
-                                                    uint32_t stride, uint32_t r0, uint32_t c,
-                                                    uint32_t lane) {
-  const uint32_t h = lane / 32;
-  if constexpr (sizeof(typename T::elem) == 2) {
-    const uint32_t m = lane % 16;
-    const uint16_t* p = tile + (r0 + 4 * h + m / 4) * stride + c + (lane & 16) + 4 * (m % 4);
-    return join(read_tr(p), read_tr(p + 8 * stride));
-  } else {
-    f32x8 f;
-#pragma unroll
-    for (uint32_t j = 0; j < 8; j++)
-      f[j] = tile[(r0 + 4 * h + j % 4 + 8 * (j / 4)) * stride + c + lane % 32];
-    return f;
-  }
-}
-
-// KT rows from r0 on into an LDS tile, the columns past d and the rows past `rows` zero.
+// A tile of KT rows of DP columns in LDS, in 16-byte chunks, each exchanged within its row by
+// swap(row) so that both of a tile's reads meet 64 different banks of four bytes: 16 lanes
+// reading a chunk of 16 rows, and 32 lanes reading 64 bytes of four rows transposed.
 template <class T, uint32_t DP, uint32_t KT, uint32_t NT>
-__device__ __forceinline__ void stage(typename T::elem* tile, uint32_t lds_stride,
-                                      const typename T::elem* base, int64_t stride, uint32_t r0,
-                                      uint32_t rows, uint32_t d, bool vec) {
-  constexpr uint32_t CE = 16 / sizeof(typename T::elem), CPR = DP / CE;
-#pragma unroll
-  for (uint32_t c0 = 0; c0 < KT * CPR; c0 += NT) {
-    const uint32_t c = c0 + threadIdx.x;
-    if (KT * CPR % NT && c >= KT * CPR) break;
-    const uint32_t r = c / CPR, col = c % CPR * CE;
-    *reinterpret_cast<u32x4v*>(tile + r * lds_stride + col) =
-        load_chunk<T>(base, stride, r0 + r, rows, col, d, vec);
+struct Rows {
+  typedef typename T::elem elem;
+  typedef typename T::frag frag;
+  static constexpr uint32_t CE = 16 / sizeof(elem), CPR = DP / CE, kAll = KT * CPR;
+  static constexpr uint32_t kChunks = (kAll + NT - 1) / NT, kBytes = DP * sizeof(elem);
+  uint32_t off[kChunks];
+
+  static __device__ __forceinline__ uint32_t swap(uint32_t r) {
+    const uint32_t low = (r >> 2) & 3;
+    return kBytes % 256 == 0 ? (r & 3) << 2 | low : kBytes % 128 == 0 ? (r & 2) << 1 | low : low;
   }
-}
+
+  // A lane's offsets into a tile's rows; columns past d are out of any buffer's range.
+  __device__ __forceinline__ void init(int64_t stride, uint32_t d) {
+#pragma unroll
+    for (uint32_t u = 0; u < kChunks; u++) {
+      const uint32_t c = u * NT + threadIdx.x, r = c / CPR, col = ((c % CPR) ^ swap(r)) * CE;
+      off[u] = col < d ? (r * (uint32_t)stride + col) * sizeof(elem) : 0x7FFFFFF0;
+    }
+  }
+
+  // Rows r0 .. r0 + KT; those past `rows` and the columns past d are zero. vec: straight into LDS,
+  // complete once the wave has waited for its loads; else through registers.
+  __device__ __forceinline__ void load(elem* tile, const elem* base, int64_t stride, uint32_t r0,
+                                       uint32_t rows, uint32_t d, bool vec) const {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    if (vec) {
+      const uint32_t range = ((min(KT, rows - r0) - 1) * (uint32_t)stride + d) * sizeof(elem);
+      const brsrc rsrc = make_rsrc(base + (int64_t)r0 * stride, range);
+#pragma unroll
+      for (uint32_t u = 0; u < kChunks; u++)
+        if (kAll % NT == 0 || u * NT + wave * 64 < kAll)
+          load_lds16(rsrc, tile + (u * NT + wave * 64) * CE, off[u]);
+    } else {
+#pragma unroll 1
+      for (uint32_t c = threadIdx.x; c < kAll; c += NT) {
+        const uint32_t r = c / CPR, col = ((c % CPR) ^ swap(r)) * CE;
+        *reinterpret_cast<u32x4v*>(tile + c * CE) =
+            load_chunk<T>(base, stride, r0 + r, rows, col, d, false);
+      }
+    }
+  }
+
+  // Eight values of row r from column c on.
+  static __device__ __forceinline__ frag row(const elem* tile, uint32_t r, uint32_t c) {
+    const elem* p = tile + r * DP;
+    if constexpr (sizeof(elem) == 2) {
+      return *reinterpret_cast<const bf16x8*>(p + ((c / 8) ^ swap(r)) * 8);
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(p + ((c / 4) ^ swap(r)) * 4);
+      const f32x4 b = *reinterpret_cast<const f32x4*>(p + ((c / 4 + 1) ^ swap(r)) * 4);
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+
+  // Column c + i at the rows that a D's registers 8t .. 8t + 7 hold: r0 + 4h + (0..3) and
+  // r0 + 8 + 4h + (0..3), r0 = 16t.
+  static __device__ __forceinline__ frag col(const elem* tile, uint32_t r0, uint32_t c,
+                                             uint32_t lane) {
+    const uint32_t h = lane / 32;
+    if constexpr (sizeof(elem) == 2) {
+      const uint32_t m = lane % 16, r = r0 + 4 * h + m / 4, at = c + (lane & 16) + 4 * (m % 4);
+      const uint16_t* p = tile + at % 8;
+      return join(read_tr(p + r * DP + ((at / 8) ^ swap(r)) * 8),
+                  read_tr(p + (r + 8) * DP + ((at / 8) ^ swap(r + 8)) * 8));
+    } else {
+      f32x8 f;
+#pragma unroll
+      for (uint32_t j = 0; j < 8; j++) {
+        const uint32_t r = r0 + 4 * h + j % 4 + 8 * (j / 4), at = c + lane % 32;
+        f[j] = tile[r * DP + ((at / 4) ^ swap(r)) * 4 + at % 4];
+      }
+      return f;
+    }
+  }
+};
 
 template <class T>
 struct Head {
@@ -166,33 +197,50 @@ __device__ __forceinline__ void store_rows(const pots_heads& x, uint32_t b, uint
     }
 }
 
-// Rows of a tile that is read by rows (16-byte reads, eight lanes of them in a cycle: 16 bytes
-// past a multiple of 128 leaves their banks apart) and of one that is read transposed (32 lanes
-// read four rows of 64 bytes: rows 64 bytes past a multiple of 256, or half of that, do).
-template <class T, uint32_t DP>
-constexpr uint32_t row_stride() { return DP + 16 / sizeof(typename T::elem); }
-template <class T, uint32_t DP>
-constexpr uint32_t col_stride() {
-  return sizeof(typename T::elem) == 4 ? DP : DP % 64 == 0 ? DP + 32 : DP;
+// The sequence (of `seqs`) and the tile of a block, long tiles first: a launch's blocks start in
+// order, and what is left at its end is short. Where the sequences divide over the XCDs, each
+// XCD has some of its own, and their shared rows in its L2.
+__device__ __forceinline__ void unit_of(uint32_t seqs, uint32_t* seq, uint32_t* place) {
+  if (seqs % kXcds == 0) {
+    const uint32_t per = seqs / kXcds, i = blockIdx.x / kXcds;
+    *seq = blockIdx.x % kXcds * per + i % per;
+    *place = i / per;
+  } else {
+    *seq = blockIdx.x % seqs;
+    *place = blockIdx.x / seqs;
+  }
 }
 
 template <class T, uint32_t DP, uint32_t NW, uint32_t KT>
-__global__ __launch_bounds__(64 * NW) void attn_fwd(pots_attention a, uint32_t tiles, bool vec,
-                                                    bool vec_out) {
+__global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 : 1) void attn_fwd(pots_attention a, uint32_t tiles,
+                                                       bool vec, bool vec_out) {
   typedef typename T::elem elem;
   typedef typename T::frag frag;
   constexpr uint32_t NT = 64 * NW, QB = 32 * NW, KS = DP / 16, NB = DP / 32;
-  constexpr uint32_t SK = row_stride<T, DP>(), SV = col_stride<T, DP>();
-  __shared__ __attribute__((aligned(16))) elem s_k[KT * SK];
-  __shared__ __attribute__((aligned(16))) elem s_v[KT * SV];
-  const uint32_t unit = xcd_block(blockIdx.x, gridDim.x);
-  const uint32_t bh = unit / tiles, tile = tiles - 1 - unit % tiles;  // the long tiles first
-  const uint32_t b = bh / a.heads, head = bh % a.heads;
+  typedef Rows<T, DP, KT, NT> R;
+  __shared__ __attribute__((aligned(16))) elem s_k0[KT * DP], s_k1[KT * DP];
+  __shared__ __attribute__((aligned(16))) elem s_v0[KT * DP], s_v1[KT * DP];
+  uint32_t bh, place;
+  unit_of(a.batch * a.heads, &bh, &place);
+  const uint32_t tile = tiles - 1 - place, b = bh / a.heads, head = bh % a.heads;
   const uint32_t kvh = head / (a.heads / a.kv_heads);
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, i = lane % 32, h = lane / 32;
+  const uint32_t lane = threadIdx.x % 64, i = lane % 32, h = lane / 32;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t len = length_of(a, b), d = a.head_dim;
   const Head<T> Q(a.q, b, head), K(a.k, b, kvh), V(a.v, b, kvh);
   const uint32_t q0 = tile * QB, qw = q0 + 32 * wave, q = qw + i;
+  // keys that the block's rows see, and the wave's
+  const uint32_t end = q0 >= len ? 0 : a.causal ? min(len, q0 + QB) : len;
+  const uint32_t wend = qw >= len ? 0 : a.causal ? min(len, qw + 32) : len;
+  const uint32_t seen = q >= len ? 0 : a.causal ? min(len, q + 1) : len;
+  R rk, rv;
+  rk.init(K.row, d);
+  rv.init(V.row, d);
+  auto load = [&](elem* k, elem* v, uint32_t k0) {
+    rk.load(k, K.p, K.row, k0, len, d, vec);
+    rv.load(v, V.p, V.row, k0, len, d, vec);
+  };
+  if (end) load(s_k0, s_v0, 0);
   frag qf[KS];
 #pragma unroll
   for (uint32_t ks = 0; ks < KS; ks++)
@@ -202,26 +250,18 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd(pots_attention a, uint32_t t
   for (uint32_t db = 0; db < NB; db++) o[db] = zero16();
   const float c = a.scale * kLog2e;
   float m = -INFINITY, mc = 0.f, l = 0.f;
-  // keys that the block's rows see, and the wave's
-  const uint32_t end = q0 >= len ? 0 : a.causal ? min(len, q0 + QB) : len;
-  const uint32_t wend = qw >= len ? 0 : a.causal ? min(len, qw + 32) : len;
-  for (uint32_t k0 = 0; k0 < end; k0 += KT) {
-    __syncthreads();
-    stage<T, DP, KT, NT>(s_k, SK, K.p, K.row, k0, len, d, vec);
-    stage<T, DP, KT, NT>(s_v, SV, V.p, V.row, k0, len, d, vec);
-    __syncthreads();
-    if (k0 >= wend) continue;
+  auto step = [&](const elem* s_k, const elem* s_v, uint32_t k0) {
+    if (k0 >= wend) return;
     f32x16 s[KT / 32];
 #pragma unroll
     for (uint32_t u = 0; u < KT / 32; u++) {
       s[u] = zero16();
 #pragma unroll
       for (uint32_t ks = 0; ks < KS; ks++)
-        s[u] = mma(lds_row<T>(s_k, SK, 32 * u + i, 16 * ks + 8 * h), qf[ks], s[u]);
+        s[u] = mma(R::row(s_k, 32 * u + i, 16 * ks + 8 * h), qf[ks], s[u]);
     }
     // a tile that some row sees in part, or rows that see nothing
     if (k0 + KT > len || qw + 32 > len || (a.causal && k0 + KT - 1 > qw)) {
-      const uint32_t seen = q >= len ? 0 : a.causal ? min(len, q + 1) : len;
 #pragma unroll
       for (uint32_t u = 0; u < KT / 32; u++)
 #pragma unroll
@@ -257,9 +297,22 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd(pots_attention a, uint32_t t
         const frag p = T::pack(s[u], 8 * t);
 #pragma unroll
         for (uint32_t db = 0; db < NB; db++)
-          o[db] = mma(lds_col<T>(s_v, SV, 32 * u + 16 * t, 32 * db, lane), p, o[db]);
+          o[db] = mma(R::col(s_v, 32 * u + 16 * t, 32 * db, lane), p, o[db]);
       }
     }
+  };
+  uint32_t k0 = 0;
+  for (; k0 + KT < end; k0 += 2 * KT) {  // the next tile is on its way while one is worked on
+    loads_done();
+    load(s_k1, s_v1, k0 + KT);
+    step(s_k0, s_v0, k0);
+    loads_done();
+    if (k0 + 2 * KT < end) load(s_k0, s_v0, k0 + 2 * KT);
+    step(s_k1, s_v1, k0 + KT);
+  }
+  if (k0 < end) {
+    loads_done();
+    step(s_k0, s_v0, k0);
   }
   l += other_half(l);
   store_rows<T, NB>(a.out, b, head, q, a.n, d, o, l > 0.f || l != l ? 1.f / l : 0.f, vec_out, h);
@@ -268,26 +321,39 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd(pots_attention a, uint32_t t
         l == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// dq, and D for attn_dkv. A wave holds 32 query rows as columns, as in the forward pass:
-// Sᵀ = K·Qᵀ and dPᵀ = V·dOᵀ from one LDS tile each, dQᵀ += Kᵀ·dSᵀ with K read transposed.
+// dq, and for attn_dkv each row's lse in units of log2 and D: stat [2][batch·heads][n]. A wave
+// holds 32 query rows as columns, as in the forward pass: Sᵀ = K·Qᵀ and dPᵀ = V·dOᵀ from the
+// tiles' rows, dQᵀ += Kᵀ·dSᵀ with K read transposed.
 template <class T, uint32_t DP, uint32_t NW, uint32_t KT>
-__global__ __launch_bounds__(64 * NW) void attn_dq(pots_attention a, float* __restrict__ delta,
-                                                   uint32_t tiles, bool vec, bool vec_out) {
+__global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 : 1) void attn_dq(pots_attention a, float* __restrict__ stat,
+                                                      uint32_t tiles, bool vec, bool vec_out) {
   typedef typename T::elem elem;
   typedef typename T::frag frag;
   constexpr uint32_t NT = 64 * NW, QB = 32 * NW, KS = DP / 16, NB = DP / 32;
-  constexpr uint32_t ST = row_stride<T, DP>();
-  __shared__ __attribute__((aligned(16))) elem s_k[KT * ST];
-  __shared__ __attribute__((aligned(16))) elem s_v[KT * ST];
-  const uint32_t unit = xcd_block(blockIdx.x, gridDim.x);
-  const uint32_t bh = unit / tiles, tile = tiles - 1 - unit % tiles;
-  const uint32_t b = bh / a.heads, head = bh % a.heads;
+  typedef Rows<T, DP, KT, NT> R;
+  __shared__ __attribute__((aligned(16))) elem s_k0[KT * DP], s_k1[KT * DP];
+  __shared__ __attribute__((aligned(16))) elem s_v0[KT * DP], s_v1[KT * DP];
+  uint32_t bh, place;
+  unit_of(a.batch * a.heads, &bh, &place);
+  const uint32_t tile = tiles - 1 - place, b = bh / a.heads, head = bh % a.heads;
   const uint32_t kvh = head / (a.heads / a.kv_heads);
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, i = lane % 32, h = lane / 32;
+  const uint32_t lane = threadIdx.x % 64, i = lane % 32, h = lane / 32;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t len = length_of(a, b), d = a.head_dim;
   const Head<T> Q(a.q, b, head), K(a.k, b, kvh), V(a.v, b, kvh), O(a.out, b, head),
       G(a.dout, b, head);
   const uint32_t q0 = tile * QB, qw = q0 + 32 * wave, q = qw + i;
+  const uint32_t end = q0 >= len ? 0 : a.causal ? min(len, q0 + QB) : len;
+  const uint32_t wend = qw >= len ? 0 : a.causal ? min(len, qw + 32) : len;
+  const uint32_t seen = q >= len ? 0 : a.causal ? min(len, q + 1) : len;
+  R rk, rv;
+  rk.init(K.row, d);
+  rv.init(V.row, d);
+  auto load = [&](elem* k, elem* v, uint32_t k0) {
+    rk.load(k, K.p, K.row, k0, len, d, vec);
+    rv.load(v, V.p, V.row, k0, len, d, vec);
+  };
+  if (end) load(s_k0, s_v0, 0);
   frag qf[KS], gf[KS];
   float dl = 0.f;
 #pragma unroll
@@ -302,77 +368,116 @@ __global__ __launch_bounds__(64 * NW) void attn_dq(pots_attention a, float* __re
   float lse2 = INFINITY;  // a row that sees nothing has probabilities of zero
   if (q < a.n) {
     const int64_t at = (int64_t)bh * a.n + q;
-    if (h == 0) delta[at] = dl;
     const float x = q < len ? gload<float>(a.lse + at) : -INFINITY;
     if (x != -INFINITY) lse2 = x * kLog2e;
+    if (h == 0) {
+      stat[at] = lse2;
+      stat[(int64_t)a.batch * a.heads * a.n + at] = dl;
+    }
   }
   f32x16 acc[NB];
 #pragma unroll
   for (uint32_t db = 0; db < NB; db++) acc[db] = zero16();
   const float c = a.scale * kLog2e;
-  const uint32_t end = q0 >= len ? 0 : a.causal ? min(len, q0 + QB) : len;
-  const uint32_t wend = qw >= len ? 0 : a.causal ? min(len, qw + 32) : len;
-  const uint32_t seen = q >= len ? 0 : a.causal ? min(len, q + 1) : len;
-  for (uint32_t k0 = 0; k0 < end; k0 += KT) {
-    __syncthreads();
-    stage<T, DP, KT, NT>(s_k, ST, K.p, K.row, k0, len, d, vec);
-    stage<T, DP, KT, NT>(s_v, ST, V.p, V.row, k0, len, d, vec);
-    __syncthreads();
+  auto step = [&](const elem* s_k, const elem* s_v, uint32_t k0) {
 #pragma unroll
     for (uint32_t u = 0; u < KT / 32; u++) {
       const uint32_t ku = k0 + 32 * u;
-      if (ku >= wend) break;
+      if (ku >= wend) return;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (uint32_t ks = 0; ks < KS; ks++) {
-        s = mma(lds_row<T>(s_k, ST, 32 * u + i, 16 * ks + 8 * h), qf[ks], s);
-        dp = mma(lds_row<T>(s_v, ST, 32 * u + i, 16 * ks + 8 * h), gf[ks], dp);
+        s = mma(R::row(s_k, 32 * u + i, 16 * ks + 8 * h), qf[ks], s);
+        dp = mma(R::row(s_v, 32 * u + i, 16 * ks + 8 * h), gf[ks], dp);
       }
-      const bool part = ku + 32 > len || qw + 32 > len || (a.causal && ku + 31 > qw);
 #pragma unroll
       for (uint32_t r = 0; r < 16; r++) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse2));
         s[r] = p * (dp[r] - dl);
-        if (part && ku + d_row(r, h) >= seen) s[r] = 0.f;
+      }
+      if (ku + 32 > len || qw + 32 > len || (a.causal && ku + 31 > qw)) {
+#pragma unroll
+        for (uint32_t r = 0; r < 16; r++)
+          if (ku + d_row(r, h) >= seen) s[r] = 0.f;
       }
 #pragma unroll
       for (uint32_t t = 0; t < 2; t++) {
         const frag p = T::pack(s, 8 * t);
 #pragma unroll
         for (uint32_t db = 0; db < NB; db++)
-          acc[db] = mma(lds_col<T>(s_k, ST, 32 * u + 16 * t, 32 * db, lane), p, acc[db]);
+          acc[db] = mma(R::col(s_k, 32 * u + 16 * t, 32 * db, lane), p, acc[db]);
       }
     }
+  };
+  uint32_t k0 = 0;
+  for (; k0 + KT < end; k0 += 2 * KT) {
+    loads_done();
+    load(s_k1, s_v1, k0 + KT);
+    step(s_k0, s_v0, k0);
+    loads_done();
+    if (k0 + 2 * KT < end) load(s_k0, s_v0, k0 + 2 * KT);
+    step(s_k1, s_v1, k0 + KT);
+  }
+  if (k0 < end) {
+    loads_done();
+    step(s_k0, s_v0, k0);
   }
   store_rows<T, NB>(a.dq, b, head, q, a.n, d, acc, a.scale, vec_out, h);
 }
 
 // dk and dv of 32·NW keys, over `per` query heads of their group and the queries that see
-// them. A wave holds 32 keys as columns: S = Q·Kᵀ and dP = dO·Vᵀ from LDS rows, dVᵀ += dOᵀ·P and
-// dKᵀ += Qᵀ·dS from the same tiles read transposed. With `part`, the sums go to fp32 slices
-// [2][split][batch][kv_heads][n][d].
+// them. A wave holds 32 keys as columns: S = Q·Kᵀ and dP = dO·Vᵀ from the tiles' rows, dVᵀ +=
+// dOᵀ·P and dKᵀ += Qᵀ·dS from the same tiles read transposed. With `part`, the sums go to fp32
+// slices [2][split][batch][kv_heads][n][d].
 template <class T, uint32_t DP, uint32_t NW, uint32_t QT>
-__global__ __launch_bounds__(64 * NW) void attn_dkv(pots_attention a,
-                                                    const float* __restrict__ delta,
-                                                    float* __restrict__ part, uint32_t tiles,
-                                                    uint32_t splits, uint32_t per, bool vec,
-                                                    bool vec_out) {
+__global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 128 ? 2 : 1) void attn_dkv(pots_attention a,
+                                                       const float* __restrict__ stat,
+                                                       float* __restrict__ part, uint32_t tiles,
+                                                       uint32_t splits, uint32_t per, bool vec,
+                                                       bool vec_out) {
   typedef typename T::elem elem;
   typedef typename T::frag frag;
   constexpr uint32_t NT = 64 * NW, KB = 32 * NW, KS = DP / 16, NB = DP / 32;
-  constexpr uint32_t ST = row_stride<T, DP>();
-  __shared__ __attribute__((aligned(16))) elem s_q[QT * ST];
-  __shared__ __attribute__((aligned(16))) elem s_g[QT * ST];
-  __shared__ __attribute__((aligned(16))) float s_lse[QT];
-  __shared__ __attribute__((aligned(16))) float s_dl[QT];
-  const uint32_t unit = xcd_block(blockIdx.x, gridDim.x);
-  const uint32_t tile = unit % tiles, split = unit / tiles % splits;  // the long tiles first
-  const uint32_t bk = unit / tiles / splits, b = bk / a.kv_heads, kvh = bk % a.kv_heads;
-  const uint32_t rep = a.heads / a.kv_heads;
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, i = lane % 32, h = lane / 32;
+  typedef Rows<T, DP, QT, NT> R;
+  __shared__ __attribute__((aligned(16))) elem s_q0[QT * DP], s_q1[QT * DP];
+  __shared__ __attribute__((aligned(16))) elem s_g0[QT * DP], s_g1[QT * DP];
+  __shared__ __attribute__((aligned(16))) float s_stat0[2 * 64], s_stat1[2 * 64];
+  uint32_t seq, tile;
+  unit_of(a.batch * a.kv_heads * splits, &seq, &tile);
+  const uint32_t split = seq % splits, bk = seq / splits, b = bk / a.kv_heads;
+  const uint32_t kvh = bk % a.kv_heads, rep = a.heads / a.kv_heads;
+  const uint32_t lane = threadIdx.x % 64, i = lane % 32, h = lane / 32;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t len = length_of(a, b), d = a.head_dim;
   const Head<T> K(a.k, b, kvh), V(a.v, b, kvh);
   const uint32_t k0 = tile * KB, kw = k0 + 32 * wave, key = kw + i;
+  // the block's steps: (head, tile of queries) in order
+  const uint32_t first = a.causal ? k0 / QT * QT : 0, e0 = split * per;
+  const uint32_t tiles_q = k0 < len ? (len - first + QT - 1) / QT : 0;
+  const uint32_t steps = tiles_q * (min(rep, e0 + per) - e0);
+  R rq, rg;
+  rq.init(a.q.row, d);
+  rg.init(a.dout.row, d);
+  const float* const stat1 = stat + (int64_t)a.batch * a.heads * a.n;
+  uint32_t le = e0, lq = first;  // the next step to load
+  auto load = [&](elem* s_q, elem* s_g, float* s_stat) {
+    const uint32_t head = kvh * rep + le;
+    const Head<T> Q(a.q, b, head), G(a.dout, b, head);
+    rq.load(s_q, Q.p, Q.row, lq, len, d, vec);
+    rg.load(s_g, G.p, G.row, lq, len, d, vec);
+    if (wave == 0) {  // lse and D of the tile's rows; zero past the length
+      const int64_t at = (int64_t)(b * a.heads + head) * a.n + lq;
+      const uint32_t range = 4 * min(64u, len - lq);
+      load_lds4(make_rsrc(stat + at, range), s_stat, 4 * lane);
+      load_lds4(make_rsrc(stat1 + at, range), s_stat + 64, 4 * lane);
+    }
+    lq += QT;
+    if (lq >= len) {
+      lq = first;
+      le++;
+    }
+  };
+  if (steps) load(s_q0, s_g0, s_stat0);
   frag kf[KS], vf[KS];
 #pragma unroll
   for (uint32_t ks = 0; ks < KS; ks++) {
@@ -386,58 +491,60 @@ __global__ __launch_bounds__(64 * NW) void attn_dkv(pots_attention a,
     dv[db] = zero16();
   }
   const float c = a.scale * kLog2e;
-  const uint32_t last = min(rep, (split + 1) * per);
-  for (uint32_t e = split * per; e < last && k0 < len; e++) {
-    const uint32_t head = kvh * rep + e;
-    const Head<T> Q(a.q, b, head), G(a.dout, b, head);
-    const int64_t stat = (int64_t)(b * a.heads + head) * a.n;
-    for (uint32_t q0 = a.causal ? k0 / QT * QT : 0; q0 < len; q0 += QT) {
-      __syncthreads();
-      stage<T, DP, QT, NT>(s_q, ST, Q.p, Q.row, q0, len, d, vec);
-      stage<T, DP, QT, NT>(s_g, ST, G.p, G.row, q0, len, d, vec);
-      if (threadIdx.x < QT) {
-        const uint32_t q = q0 + threadIdx.x;
-        const float x = q < len ? gload<float>(a.lse + stat + q) : -INFINITY;
-        s_lse[threadIdx.x] = x != -INFINITY ? x * kLog2e : INFINITY;
-        s_dl[threadIdx.x] = q < len ? gload<float>(delta + stat + q) : 0.f;
+  uint32_t q0 = first;
+  auto step = [&](const elem* s_q, const elem* s_g, const float* s_stat) {
+#pragma unroll
+    for (uint32_t u = 0; u < QT / 32; u++) {
+      const uint32_t qu = q0 + 32 * u;
+      if (qu >= len || kw >= len || (a.causal && qu + 31 < kw)) continue;
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (uint32_t ks = 0; ks < KS; ks++) {
+        s = mma(R::row(s_q, 32 * u + i, 16 * ks + 8 * h), kf[ks], s);
+        dp = mma(R::row(s_g, 32 * u + i, 16 * ks + 8 * h), vf[ks], dp);
       }
-      __syncthreads();
 #pragma unroll
-      for (uint32_t u = 0; u < QT / 32; u++) {
-        const uint32_t qu = q0 + 32 * u;
-        if (qu >= len || kw >= len || (a.causal && qu + 31 < kw)) continue;
-        f32x16 s = zero16(), dp = zero16();
+      for (uint32_t g = 0; g < 4; g++) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(s_stat + 32 * u + 8 * g + 4 * h);
+        const f32x4 dl = *reinterpret_cast<const f32x4*>(s_stat + 64 + 32 * u + 8 * g + 4 * h);
 #pragma unroll
-        for (uint32_t ks = 0; ks < KS; ks++) {
-          s = mma(lds_row<T>(s_q, ST, 32 * u + i, 16 * ks + 8 * h), kf[ks], s);
-          dp = mma(lds_row<T>(s_g, ST, 32 * u + i, 16 * ks + 8 * h), vf[ks], dp);
+        for (uint32_t x = 0; x < 4; x++) {
+          const uint32_t r = 4 * g + x;
+          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ls[x]));
+          dp[r] = s[r] * (dp[r] - dl[x]);
         }
-        const bool some = kw + 32 > len || qu + 32 > len || (a.causal && qu < kw + 31);
+      }
+      if (kw + 32 > len || qu + 32 > len || (a.causal && qu < kw + 31)) {
 #pragma unroll
-        for (uint32_t g = 0; g < 4; g++) {
-          const f32x4 ls = *reinterpret_cast<const f32x4*>(s_lse + 32 * u + 8 * g + 4 * h);
-          const f32x4 dl = *reinterpret_cast<const f32x4*>(s_dl + 32 * u + 8 * g + 4 * h);
-#pragma unroll
-          for (uint32_t x = 0; x < 4; x++) {
-            const uint32_t r = 4 * g + x;
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ls[x]));
-            const uint32_t q = qu + d_row(r, h);
-            const bool out = some && (key >= len || q >= len || (a.causal && q < key));
-            s[r] = out ? 0.f : p;
-            dp[r] = out ? 0.f : p * (dp[r] - dl[x]);
-          }
+        for (uint32_t r = 0; r < 16; r++) {
+          const uint32_t q = qu + d_row(r, h);
+          if (key >= len || q >= len || (a.causal && q < key)) s[r] = dp[r] = 0.f;
         }
+      }
 #pragma unroll
-        for (uint32_t t = 0; t < 2; t++) {
-          const frag p = T::pack(s, 8 * t), ds = T::pack(dp, 8 * t);
+      for (uint32_t t = 0; t < 2; t++) {
+        const frag p = T::pack(s, 8 * t), ds = T::pack(dp, 8 * t);
 #pragma unroll
-          for (uint32_t db = 0; db < NB; db++) {
-            dv[db] = mma(lds_col<T>(s_g, ST, 32 * u + 16 * t, 32 * db, lane), p, dv[db]);
-            dk[db] = mma(lds_col<T>(s_q, ST, 32 * u + 16 * t, 32 * db, lane), ds, dk[db]);
-          }
+        for (uint32_t db = 0; db < NB; db++) {
+          dv[db] = mma(R::col(s_g, 32 * u + 16 * t, 32 * db, lane), p, dv[db]);
+          dk[db] = mma(R::col(s_q, 32 * u + 16 * t, 32 * db, lane), ds, dk[db]);
         }
       }
     }
+    q0 = q0 + QT < len ? q0 + QT : first;
+  };
+  uint32_t t = 0;
+  for (; t + 2 <= steps; t += 2) {
+    loads_done();
+    load(s_q1, s_g1, s_stat1);
+    step(s_q0, s_g0, s_stat0);
+    loads_done();
+    if (t + 2 < steps) load(s_q0, s_g0, s_stat0);
+    step(s_q1, s_g1, s_stat1);
+  }
+  if (t < steps) {
+    loads_done();
+    step(s_q0, s_g0, s_stat0);
   }
   if (part) {
     pots_heads x;
@@ -483,10 +590,12 @@ bool bad(const pots_attention* a) {
          (uint64_t)a->batch * a->heads > 0x100000u;
 }
 
+// Whether x's rows start on multiples of `bytes`, and a tile of them spans less than 2 GiB.
 bool aligned(const pots_attention* a, const pots_heads& x, uint32_t bytes) {
   const int64_t e = a->dtype == POTS_OP_BF16 ? 2 : 4;
   return reinterpret_cast<uint64_t>(x.ptr) % bytes == 0 && x.batch * e % bytes == 0 &&
-         x.head * e % bytes == 0 && x.row * e % bytes == 0 && a->head_dim * e % bytes == 0;
+         x.head * e % bytes == 0 && x.row * e % bytes == 0 && a->head_dim * e % bytes == 0 &&
+         x.row >= 0 && x.row < (1 << 23);
 }
 
 // Waves in a block: as many as four (which share a K or V tile) while that leaves a block for
@@ -508,7 +617,7 @@ Dkv dkv_cut(const pots_attention* a) {
   r.tiles = (a->n + 32 * r.nw - 1) / (32 * r.nw);
   const uint64_t blocks = (uint64_t)a->batch * a->kv_heads * r.tiles;
   r.splits = 1;
-  while (r.splits < rep && blocks * r.splits < 512) r.splits++;
+  while (r.splits < rep && blocks * r.splits < 768) r.splits++;
   r.per = (rep + r.splits - 1) / r.splits;
   r.splits = (rep + r.per - 1) / r.per;
   return r;
@@ -520,7 +629,7 @@ int forward(const pots_attention* a, hipStream_t s) {
   const uint64_t blocks = (uint64_t)a->batch * a->heads * tiles;
   if (blocks > 0x7FFFFFFFu) return POTS_E_ARG;
   const bool vec = aligned(a, a->q, 16) && aligned(a, a->k, 16) && aligned(a, a->v, 16);
-  hipLaunchKernelGGL((attn_fwd<T, DP, NW, NW == 4 ? 64 : 32>), dim3((uint32_t)blocks),
+  hipLaunchKernelGGL((attn_fwd<T, DP, NW, sizeof(typename T::elem) == 2 && NW == 4 ? 64 : 32>), dim3((uint32_t)blocks),
                      dim3(64 * NW), 0, s, *a, tiles, vec,
                      aligned(a, a->out, 4 * sizeof(typename T::elem)));
   POTS_HIP(hipGetLastError());
@@ -533,19 +642,19 @@ int backward(const pots_attention* a, char* work, hipStream_t s) {
   const uint64_t qblocks = (uint64_t)a->batch * a->heads * cut.tiles;
   const uint64_t kblocks = (uint64_t)a->batch * a->kv_heads * cut.tiles * cut.splits;
   if (qblocks > 0x7FFFFFFFu || kblocks > 0x7FFFFFFFu) return POTS_E_ARG;
-  float* delta = reinterpret_cast<float*>(work);
+  float* stat = reinterpret_cast<float*>(work);
   float* part = cut.splits == 1 ? nullptr
                                 : reinterpret_cast<float*>(
-                                      work + align_up((size_t)a->batch * a->heads * a->n * 4,
+                                      work + align_up((size_t)a->batch * a->heads * a->n * 8,
                                                       256));
   const bool vec = aligned(a, a->q, 16) && aligned(a, a->k, 16) && aligned(a, a->v, 16) &&
                    aligned(a, a->out, 16) && aligned(a, a->dout, 16);
   const uint32_t four = 4 * sizeof(typename T::elem);
-  hipLaunchKernelGGL((attn_dq<T, DP, NW, NW == 4 ? 64 : 32>), dim3((uint32_t)qblocks),
-                     dim3(64 * NW), 0, s, *a, delta, cut.tiles, vec, aligned(a, a->dq, four));
+  hipLaunchKernelGGL((attn_dq<T, DP, NW, sizeof(typename T::elem) == 2 && NW == 4 ? 64 : 32>), dim3((uint32_t)qblocks),
+                     dim3(64 * NW), 0, s, *a, stat, cut.tiles, vec, aligned(a, a->dq, four));
   POTS_HIP(hipGetLastError());
-  hipLaunchKernelGGL((attn_dkv<T, DP, NW, NW == 4 ? 64 : 32>), dim3((uint32_t)kblocks),
-                     dim3(64 * NW), 0, s, *a, delta, part, cut.tiles, cut.splits, cut.per, vec,
+  hipLaunchKernelGGL((attn_dkv<T, DP, NW, sizeof(typename T::elem) == 2 && NW == 4 ? 64 : 32>), dim3((uint32_t)kblocks),
+                     dim3(64 * NW), 0, s, *a, stat, part, cut.tiles, cut.splits, cut.per, vec,
                      aligned(a, a->dk, four) && aligned(a, a->dv, four));
   POTS_HIP(hipGetLastError());
   if (part) {
@@ -587,7 +696,7 @@ extern "C" int pots_attention_forward(const pots_attention* a, void* stream) {
 extern "C" uint64_t pots_attention_backward_work(const pots_attention* a) {
   if (bad(a) || a->batch == 0 || a->n == 0) return 0;
   const Dkv cut = dkv_cut(a);
-  uint64_t bytes = align_up((size_t)a->batch * a->heads * a->n * 4, 256);
+  uint64_t bytes = align_up((size_t)a->batch * a->heads * a->n * 8, 256);
   if (cut.splits > 1)
     bytes += 2ull * cut.splits * a->batch * a->kv_heads * a->n * a->head_dim * 4;
   return bytes;

@@ -13,6 +13,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "gmem.h"
+
 namespace pots {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -66,6 +68,30 @@ __device__ __forceinline__ float bf16_to_f32(uint16_t x) {
 
 __device__ __forceinline__ uint16_t f32_to_bf16(float x) {  // to nearest, ties to even
   return __builtin_bit_cast(uint16_t, (__bf16)x);
+}
+
+// A buffer of `range` bytes: loads past it read zero.
+__device__ __forceinline__ brsrc make_rsrc(const void* base, uint32_t range) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, range, 0x00020000);
+}
+
+// Sixteen (or four) bytes a lane from a buffer to consecutive places from `lds` on, which is the
+// same for the wave. (The host's pass of the compiler knows no such builtin.)
+__device__ __forceinline__ void load_lds16(brsrc rsrc, void* lds, uint32_t off) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (POTS_LDS void*)lds, 16, off, 0, 0, 0);
+#endif
+}
+__device__ __forceinline__ void load_lds4(brsrc rsrc, void* lds, uint32_t off) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (POTS_LDS void*)lds, 4, off, 0, 0, 0);
+#endif
+}
+
+// Waits for the wave's own loads into LDS, then for the block: a stage is complete after it.
+__device__ __forceinline__ void loads_done() {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
 }
 
 // Element types of the operators' tensors.

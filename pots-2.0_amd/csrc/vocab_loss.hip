@@ -28,7 +28,7 @@ namespace pots {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-constexpr uint32_t kStep = 64;  // contractions are padded to 128 bytes of a row
+constexpr uint32_t BK = 64;  // contraction per stage, 128 bytes of a row; lengths are padded to it
 
 // A matrix of bf16 terms: rows `ld` elements apart, term planes `plane` elements apart.
 struct Mat {
@@ -44,21 +44,13 @@ __device__ __forceinline__ void pair_of(uint32_t pairs, uint32_t t, uint32_t* pa
   *pb = (0x001012u >> (4 * j)) & 15;
 }
 
-// Sixteen bytes a lane from a buffer to consecutive places from `lds` on, which is the same for
-// the wave. (The host's pass of the compiler knows no such builtin.)
-__device__ __forceinline__ void load_lds16(brsrc rsrc, uint16_t* lds, uint32_t off) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (POTS_LDS void*)lds, 16, off, 0, 0, 0);
-#endif
-}
-
-// T rows of an operand and BK (32 or 64) of the contraction in LDS, in 16-byte chunks that one
+// T rows of an operand and BK of the contraction in LDS, in 16-byte chunks that one
 // instruction brings in for 64 lanes, straight from memory. TR: stored [contraction][rows], so
 // a stage is BK rows of T columns; else T rows of BK columns. A chunk is exchanged within its
-// row by the row's number, so that the reads of a fragment fall on different banks: eight
-// lanes' 16-byte reads of eight rows, or 32 lanes' transposing reads of four rows. A lane's
+// row by the row's number, so that the reads of a fragment fall on different banks: 16 lanes'
+// 16-byte reads of 16 rows, or 32 lanes' transposing reads of four rows (64 banks of four bytes). A lane's
 // offsets are the same at every stage; the stage moves the buffer's base, in scalar registers.
-template <bool TR, uint32_t T, uint32_t NT, uint32_t BK>
+template <bool TR, uint32_t T, uint32_t NT>
 struct Stage {
   static constexpr uint32_t kAll = T * BK / 8, kChunks = (kAll + NT - 1) / NT;
   static_assert(!TR || T >= 128, "the exchange of a transposed tile needs 16 chunks a row");
@@ -66,7 +58,7 @@ struct Stage {
 
   // What row r's chunks are exchanged by.
   static __device__ __forceinline__ uint32_t swap(uint32_t r) {
-    return TR ? 4 * (r & 3) : BK == 64 ? r & 7 : (r >> 1) & 3;
+    return TR ? 4 * (r & 3) : (r >> 1) & 7;
   }
 
   // r0, rows: the tile's first row and their number; rows past it repeat the last (for TR:
@@ -93,8 +85,7 @@ struct Stage {
                            (TR ? (int64_t)k0 * m.ld + r0 : (int64_t)r0 * m.ld + k0);
     const uint32_t range =
         TR ? (min(BK, ks - k0) - 1) * (uint32_t)m.ld * 2 + wide : 0x7FFFFFFF;
-    const brsrc rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), (short)0,
-                                                         range, 0x00020000);
+    const brsrc rsrc = make_rsrc(base, range);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 #pragma unroll
     for (uint32_t u = 0; u < kChunks; u++)
@@ -118,12 +109,6 @@ struct Stage {
   }
 };
 
-// Waits for the wave's own loads into LDS, then for the block: a stage is complete after it.
-__device__ __forceinline__ void loads_done() {
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  __syncthreads();
-}
-
 // The stages in LDS: objects of their own, so that the compiler knows a load into one from the
 // reads of another and need not wait for it; one set for all the products of a kernel.
 template <uint32_t WHICH, uint32_t SIZE>
@@ -133,13 +118,12 @@ __device__ __forceinline__ uint16_t* lds_buffer() {
 }
 
 // A block's TM x TN of A·Bᵀ over K (a multiple of BK), WM x WN waves of MB x NB products of 32.
-template <bool ATR, bool BTR, uint32_t TM_, uint32_t TN_, uint32_t WM_, uint32_t WN_,
-          uint32_t BK>
+template <bool ATR, bool BTR, uint32_t TM_, uint32_t TN_, uint32_t WM_, uint32_t WN_>
 struct Tile {
   static constexpr uint32_t TM = TM_, TN = TN_, WM = WM_, WN = WN_, NT = 64 * WM * WN;
   static constexpr uint32_t MB = TM / WM / 32, NB = TN / WN / 32;
-  typedef Stage<ATR, TM, NT, BK> SA;
-  typedef Stage<BTR, TN, NT, BK> SB;
+  typedef Stage<ATR, TM, NT> SA;
+  typedef Stage<BTR, TN, NT> SB;
   f32x16 acc[MB][NB];
   uint32_t wm, wn, lane;
 
@@ -533,7 +517,7 @@ __global__ __launch_bounds__(CX::NT) void loss_products(
     tile_of(blockIdx.x % (mt * nt), mt, nt, &m, &n);
     const uint32_t m0 = m * CX::TM, n0 = n * CX::TN, k0 = split * per;
     CX c;
-    const uint32_t all = (nv + kStep - 1) / kStep * kStep;
+    const uint32_t all = (nv + BK - 1) / BK * BK;
     c.run(W, G, m0, dp, n0, live, k0, k0 < all ? min(per, all - k0) : 0, nv, 0, pairs);
     float* out = sums + split * slice;
     c.each(m0, n0, [&](f32x16& s, uint32_t col, uint32_t row) {
@@ -551,7 +535,7 @@ __global__ __launch_bounds__(CX::NT) void loss_products(
   }
   if (blockIdx.x >= mt * nt * splits + wmt * wnt) return;
   tile_of(blockIdx.x - mt * nt * splits, wmt, wnt, &m, &n);
-  const uint32_t m0 = m * CW::TM, n0 = n * CW::TN, K = (live + kStep - 1) / kStep * kStep;
+  const uint32_t m0 = m * CW::TM, n0 = n * CW::TN, K = (live + BK - 1) / BK * BK;
   CW c;
   c.run(X, G, m0, dp, n0, (nv + 7) & ~7u, 0, K, live, live, pairs);
   const float mul = *unit;
@@ -601,11 +585,11 @@ namespace {
 // them for the GPU; up to 32 rows the product is bound by reading W, and a tile as narrow as
 // the rows leaves its multiplications out of the way.
 template <bool ATR, bool BTR>
-using Large = Tile<ATR, BTR, 256, 256, 2, 4, 64>;
+using Large = Tile<ATR, BTR, 256, 256, 2, 4>;
 template <bool ATR, bool BTR>
-using Medium = Tile<ATR, BTR, 128, 128, 2, 2, 64>;
+using Medium = Tile<ATR, BTR, 128, 128, 2, 2>;
 template <bool ATR, bool BTR>
-using Narrow = Tile<ATR, BTR, 256, 32, 8, 1, 64>;
+using Narrow = Tile<ATR, BTR, 256, 32, 8, 1>;
 enum Shape { kLarge, kMedium, kNarrow };
 
 constexpr uint32_t kCus = 256;
@@ -633,7 +617,7 @@ uint64_t take(Plan* p, uint64_t bytes) {
 }
 
 bool as_is(const pots_vocab_loss* a, const void* p, int64_t row) {
-  return a->dtype == POTS_OP_BF16 && a->dim % kStep == 0 &&
+  return a->dtype == POTS_OP_BF16 && a->dim % BK == 0 &&
          reinterpret_cast<uint64_t>(p) % 16 == 0 && row % 8 == 0;
 }
 
@@ -642,7 +626,7 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
   Plan p = {};
   p.terms = a->dtype == POTS_OP_BF16 ? 1 : 3;
   p.pairs = a->dtype == POTS_OP_BF16 ? 1 : 6;
-  p.dp = cdiv(a->dim, kStep) * kStep;
+  p.dp = cdiv(a->dim, BK) * BK;
   p.rows_pad = cdiv(a->rows, 256) * 256;
   p.copy_w = !as_is(a, a->w, a->w_row);
   p.copy_x = backward || !as_is(a, a->x, a->x_row);
@@ -670,13 +654,13 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
   // shorter ones where the GPU would not be full; each share has sums of its own.
   p.products = p.scores;
   const uint32_t tm = p.products == kMedium ? 128 : 256, tn = p.products == kNarrow ? 32 : tm;
-  const uint32_t k_dx = p.piece / kStep, k_dw = p.rows_pad / kStep;
+  const uint32_t k_dx = p.piece / BK, k_dw = p.rows_pad / BK;
   const uint32_t dx_tiles = cdiv(p.dp, tm) * cdiv(a->rows, tn);
   const uint32_t dw_tiles = cdiv(p.dp, tm) * cdiv(p.piece, tm);
   p.splits = k_dw ? min(max((k_dx + k_dw / 2) / k_dw, 1u), 16u) : 1;
   while (p.splits < 16 && dx_tiles * p.splits + dw_tiles < 2 * kCus && k_dx / p.splits > 8)
     p.splits++;
-  p.per = cdiv(k_dx, p.splits) * kStep;
+  p.per = cdiv(k_dx, p.splits) * BK;
   p.splits = cdiv(p.piece, p.per);
   p.sums = take(&p, 4ull * p.splits * p.rows_pad * p.dp);
   return p;
