@@ -8,10 +8,11 @@
 // A row whose tokens lie within one piece is written right away; one that crosses pieces leaves
 // fp32 sums that embed_join adds in order.
 //
-// Sorting: a block sorts 2048 keys (id above position, so all differ) in LDS; runs are then
-// merged up to 32 at a time, where a key's place is its own index plus, for each other run,
-// the number of smaller keys there. A dense gradient's zeros are written by other blocks of the
-// sort's launch.
+// Sorting: the keys (id above position, so all differ) are placed by counting. A block holds 32 of
+// them and counts the smaller ones of their run, two instructions a pair: up to 16384 tokens are
+// one run (8192 tokens 14 us; sorting networks of 2048 in LDS and a merge took 24). More are runs of 2048, merged up to 32 at a time, where a key's place
+// is its own index plus, for each other run, the number of smaller keys there. A dense
+// gradient's zeros are written beside the sums, to the rows that no token has.
 #include <math.h>
 
 #include "common.h"
@@ -20,38 +21,46 @@
 
 namespace pots {
 
-constexpr uint32_t kRun = 2048;    // keys a block sorts
+constexpr uint32_t kOneRun = 16384, kRun = 2048;  // tokens of a single run; else of each run
 constexpr uint32_t kMerge = 32;    // runs a pass merges
+constexpr uint32_t kPiece = 16;    // sorted keys that a wave adds up, at the least
+constexpr uint32_t kFill = 16;     // rows that a block writes zeros to
 constexpr uint32_t kNoRow = ~0u;   // the id of a token outside the table; sorts last
 
 template <class T>
 constexpr uint32_t kPer = 16 / sizeof(typename T::elem);  // values in a 16-byte chunk
 
-// A chunk's values as floats, from column c of a row of d.
+template <class T>
+using Chunk = typename T::elem __attribute__((ext_vector_type(kPer<T>)));
+
+// A chunk from column c of a row of d, zero past its end.
+template <class T>
+__device__ __forceinline__ Chunk<T> load_chunk(const typename T::elem* p, uint32_t c, uint32_t d,
+                                               bool vec) {
+  if (vec) return gload<Chunk<T>>(p + c);
+  Chunk<T> x;
+#pragma unroll
+  for (uint32_t j = 0; j < kPer<T>; j++)
+    x[j] = c + j < d ? gload<typename T::elem>(p + c + j) : typename T::elem(0);
+  return x;
+}
+
 template <class T>
 __device__ __forceinline__ void get_chunk(const typename T::elem* p, uint32_t c, uint32_t d,
                                           bool vec, float (&v)[kPer<T>]) {
-  if (vec) {
-    typedef typename T::elem chunk __attribute__((ext_vector_type(kPer<T>)));
-    const chunk x = gload<chunk>(p + c);
+  const Chunk<T> x = load_chunk<T>(p, c, d, vec);
 #pragma unroll
-    for (uint32_t j = 0; j < kPer<T>; j++) v[j] = T::get(x[j]);
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < kPer<T>; j++)
-      v[j] = c + j < d ? T::get(gload<typename T::elem>(p + c + j)) : 0.f;
-  }
+  for (uint32_t j = 0; j < kPer<T>; j++) v[j] = T::get(x[j]);
 }
 
 template <class T>
 __device__ __forceinline__ void put_chunk(typename T::elem* p, uint32_t c, uint32_t d, bool vec,
                                           const float (&v)[kPer<T>]) {
   if (vec) {
-    typedef typename T::elem chunk __attribute__((ext_vector_type(kPer<T>)));
-    chunk x;
+    Chunk<T> x;
 #pragma unroll
     for (uint32_t j = 0; j < kPer<T>; j++) x[j] = T::put(v[j]);
-    gstore<chunk>(p + c, x);
+    gstore<Chunk<T>>(p + c, x);
   } else {
 #pragma unroll
     for (uint32_t j = 0; j < kPer<T>; j++)
@@ -79,46 +88,92 @@ __global__ __launch_bounds__(256) void embed_rows(pots_embedding a, uint32_t cpr
                vec, v);
 }
 
-// Blocks below `runs` sort a run each; the others write zeros to the table.
-template <class T>
-__global__ __launch_bounds__(1024) void embed_sort(pots_embedding a, uint64_t* __restrict__ keys,
-                                                   uint32_t runs, uint32_t cpr, bool vec) {
-  __shared__ uint64_t s_key[kRun];
-  if (blockIdx.x >= runs) {
-    const uint64_t all = (uint64_t)a.vocab * cpr, step = (uint64_t)(gridDim.x - runs) * 1024;
-    const float zero[kPer<T>] = {};
-    for (uint64_t e = (uint64_t)(blockIdx.x - runs) * 1024 + threadIdx.x; e < all; e += step) {
-      const uint32_t r = e / cpr, c = (e - (uint64_t)r * cpr) * kPer<T>;
-      put_chunk<T>(reinterpret_cast<typename T::elem*>(a.table) + (int64_t)r * a.table_row, c,
-                   a.dim, vec, zero);
+// Zeros to rows r0 .. r0 + kFill of a dense gradient (those before `end`), by a block; with keys,
+// only to the rows that no token has, each looked up in the sorted list by one lane.
+template <class T, uint32_t NT>
+__device__ __forceinline__ void fill_rows(const pots_embedding& a,
+                                          const uint64_t* __restrict__ keys, uint32_t r0,
+                                          uint32_t end, uint32_t cpr, bool vec) {
+  __shared__ uint32_t s_has[kFill];
+  const uint32_t n = r0 < end ? min(kFill, end - r0) : 0;
+  if (threadIdx.x < n) {
+    const uint64_t key = (uint64_t)(r0 + threadIdx.x) << 32;
+    uint32_t lo = 0, hi = keys ? a.tokens : 0;
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (keys[mid] < key)
+        lo = mid + 1;
+      else
+        hi = mid;
     }
+    s_has[threadIdx.x] =
+        keys && lo < a.tokens && (uint32_t)(keys[lo] >> 32) == r0 + threadIdx.x;
+  }
+  __syncthreads();
+  typename T::elem* table = reinterpret_cast<typename T::elem*>(a.table);
+  const float zero[kPer<T>] = {};
+  for (uint32_t e = threadIdx.x; e < n * cpr; e += NT) {
+    const uint32_t r = e / cpr, c = (e - r * cpr) * kPer<T>;
+    if (s_has[r]) continue;
+    typename T::elem* p = table + (int64_t)(r0 + r) * a.table_row;
+    if (vec)  // past the caches, which the sums' reads can use: 208 us a pass with plain stores, 201
+      __builtin_nontemporal_store(Chunk<T>{}, reinterpret_cast<Chunk<T>*>(p + c));
+    else
+      put_chunk<T>(p, c, a.dim, false, zero);
+  }
+}
+
+// Places 32 keys a block within their run, each of them in a lane of both halves of every wave:
+// 32 shares of the run. The run's keys before the block's own count where they are not above
+// (equal ids keep their order), the ones after it where they are below. The blocks after the
+// first `order` write zeros to the rows below `end`.
+template <class T>
+__global__ __launch_bounds__(1024) void embed_order(pots_embedding a,
+                                                    uint64_t* __restrict__ keys, uint32_t run,
+                                                    uint32_t order, uint32_t end, uint32_t cpr,
+                                                    bool vec) {
+  constexpr uint32_t kOwn = 32, G = 16;  // keys of a block; keys compared per step
+  __shared__ __attribute__((aligned(16))) uint32_t s_id[kOneRun];
+  __shared__ uint32_t s_count[32][kOwn];
+  if (blockIdx.x >= order) {
+    fill_rows<T, 1024>(a, nullptr, (blockIdx.x - order) * kFill, end, cpr, vec);
     return;
   }
-  const uint32_t base = blockIdx.x * kRun, t = threadIdx.x;
-#pragma unroll
-  for (uint32_t x = 0; x < kRun; x += 1024) {
-    const uint32_t i = base + x + t;
-    uint64_t key = ~0ull;
-    if (i < a.tokens) {
-      const int64_t id = gload<int64_t>(a.ids + i);
-      key = (uint64_t)(id >= 0 && id < a.vocab ? (uint32_t)id : kNoRow) << 32 | i;
-    }
-    s_key[x + t] = key;
+  const uint32_t t = threadIdx.x, lane = t % kOwn, part = t / kOwn;
+  const uint32_t own = blockIdx.x * kOwn, base = own / run * run, i = own + lane;
+  const uint32_t n = min(run, a.tokens - base), n_pad = (n + G - 1) / G * G;
+  for (uint32_t j = t; j < n_pad; j += 1024) {
+    const int64_t id = j < n ? gload<int64_t>(a.ids + base + j) : -1;
+    s_id[j] = id >= 0 && id < a.vocab ? (uint32_t)id : kNoRow;
   }
-  for (uint32_t size = 2; size <= kRun; size *= 2)
-    for (uint32_t gap = size / 2; gap > 0; gap /= 2) {
-      __syncthreads();
-      const uint32_t lo = t / gap * 2 * gap + t % gap, hi = lo + gap;
-      const uint64_t x = s_key[lo], y = s_key[hi];
-      if ((x > y) == ((lo & size) == 0)) {
-        s_key[lo] = y;
-        s_key[hi] = x;
-      }
-    }
   __syncthreads();
+  // (past the run's end a key compares as one that comes after all others)
+  const uint32_t id = s_id[min(own - base + lane, n_pad - 1)], o0 = (own - base) / G * G;
+  const uint32_t share = (n_pad / G + 31) / 32 * G;
+  const uint32_t j0 = min(part * share, n_pad), j1 = min(j0 + share, n_pad);
+  uint32_t count = 0;
+  for (uint32_t j = j0; j < j1; j += G) {
+    u32x4v o[G / 4];
 #pragma unroll
-  for (uint32_t x = 0; x < kRun; x += 1024)
-    if (base + x + t < a.tokens) keys[base + x + t] = s_key[x + t];
+    for (uint32_t x = 0; x < G / 4; x++) o[x] = reinterpret_cast<const u32x4v*>(s_id + j)[x];
+    if (j < o0) {
+#pragma unroll
+      for (uint32_t x = 0; x < G; x++) count += o[x / 4][x % 4] <= id;
+    } else if (j >= own - base + kOwn) {
+#pragma unroll
+      for (uint32_t x = 0; x < G; x++) count += o[x / 4][x % 4] < id;
+    } else {
+#pragma unroll
+      for (uint32_t x = 0; x < G; x++)
+        count += o[x / 4][x % 4] < id || (o[x / 4][x % 4] == id && base + j + x < i);
+    }
+  }
+  s_count[part][lane] = count;
+  __syncthreads();
+  if (part != 0 || i >= a.tokens) return;
+#pragma unroll
+  for (uint32_t w = 1; w < 32; w++) count += s_count[w][lane];
+  keys[base + count] = (uint64_t)id << 32 | i;
 }
 
 // Runs of `run` keys into runs of up to kMerge times as many.
@@ -144,49 +199,64 @@ __global__ __launch_bounds__(256) void embed_merge(const uint64_t* __restrict__ 
   to[group + at] = key;
 }
 
-// Adds up one piece of the sorted list for 64 chunks of columns. part: [piece][2][dim padded to
-// chunks]: the sum of the row that an earlier piece began, and of the one that goes on.
+// Below `sums` waves: one adds up one piece of the sorted list for 64 chunks of columns. part:
+// [piece][2][dim padded to chunks]: the sum of the row that an earlier piece began, and of the one
+// that goes on. The blocks after those write zeros to rows from `r0` to `end` that no token has.
 template <class T>
-__global__ __launch_bounds__(64) void embed_sum(pots_embedding a,
-                                                const uint64_t* __restrict__ keys,
-                                                uint32_t piece, uint32_t cpr,
-                                                float* __restrict__ part, bool vec) {
+__global__ __launch_bounds__(256) void embed_sum(pots_embedding a,
+                                                 const uint64_t* __restrict__ keys,
+                                                 uint32_t piece, uint32_t groups, uint32_t sums,
+                                                 uint32_t cpr, uint32_t r0, uint32_t end,
+                                                 float* __restrict__ part, bool vec) {
   constexpr uint32_t P = kPer<T>;
-  const uint32_t ch = blockIdx.y * 64 + threadIdx.x, c = ch * P;
-  const uint32_t k0 = blockIdx.x * piece, k1 = min(k0 + piece, a.tokens);
-  const bool on = ch < cpr;
   const typename T::elem* rows = reinterpret_cast<const typename T::elem*>(a.rows);
   typename T::elem* table = reinterpret_cast<typename T::elem*>(a.table);
+  const uint32_t blocks = (sums + 3) / 4;
+  if (blockIdx.x >= blocks) {
+    fill_rows<T, 256>(a, keys, r0 + (blockIdx.x - blocks) * kFill, end, cpr, vec);
+    return;
+  }
+  const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  if (unit >= sums) return;
+  const uint32_t b = unit / groups, ch = unit % groups * 64 + threadIdx.x % 64, c = ch * P;
+  const uint32_t k0 = b * piece, k1 = min(k0 + piece, a.tokens);
+  const bool on = ch < cpr;
   float sum[P] = {};
   // a row that an earlier piece began does not start here
   bool begun = k0 > 0 && (uint32_t)(keys[k0 - 1] >> 32) == (uint32_t)(keys[k0] >> 32);
-  constexpr uint32_t U = 8;
+  constexpr uint32_t U = kPiece;  // rows on their way at once
   for (uint32_t k = k0; k < k1; k += U) {
-    float v[U][P];
-    uint32_t id[U + 1];
+    Chunk<T> v[U], old[U];
+    uint32_t id[U + 1], at[U];
 #pragma unroll
-    for (uint32_t u = 0; u <= U; u++) id[u] = k + u < a.tokens ? keys[k + u] >> 32 : kNoRow;
+    for (uint32_t u = 0; u <= U; u++) {
+      const uint64_t key = k + u < a.tokens ? keys[k + u] : ~0ull;
+      id[u] = key >> 32;
+      if (u < U) at[u] = id[u] == kNoRow ? 0 : (uint32_t)key;
+    }
 #pragma unroll
-    for (uint32_t u = 0; u < U; u++)
-      if (on && k + u < k1 && id[u] != kNoRow)
-        get_chunk<T>(rows + (int64_t)(uint32_t)keys[k + u] * a.rows_row, c, a.dim, vec, v[u]);
+    for (uint32_t u = 0; u < U; u++) {
+      if (!on || id[u] == kNoRow) continue;
+      v[u] = load_chunk<T>(rows + (int64_t)at[u] * a.rows_row, c, a.dim, vec);
+      if (a.add && id[u + 1] != id[u])
+        old[u] = load_chunk<T>(table + (int64_t)id[u] * a.table_row, c, a.dim, vec);
+    }
 #pragma unroll
     for (uint32_t u = 0; u < U; u++) {
       if (k + u >= k1 || id[u] == kNoRow) continue;
 #pragma unroll
-      for (uint32_t j = 0; j < P; j++) sum[j] += v[u][j];
+      for (uint32_t j = 0; j < P; j++) sum[j] += T::get(v[u][j]);
       const bool ends = id[u + 1] != id[u], last = k + u + 1 == k1;
       if (!ends && !last) continue;
       if (on) {
         if (ends && !begun) {
-          typename T::elem* p = table + (int64_t)id[u] * a.table_row;
-          float y[P] = {};
-          if (a.add) get_chunk<T>(p, c, a.dim, vec, y);
+          float y[P];
 #pragma unroll
-          for (uint32_t j = 0; j < P; j++) y[j] = y[j] + sum[j] * a.scale;
-          put_chunk<T>(p, c, a.dim, vec, y);
+          for (uint32_t j = 0; j < P; j++)
+            y[j] = a.add ? T::get(old[u][j]) + sum[j] * a.scale : sum[j] * a.scale;
+          put_chunk<T>(table + (int64_t)id[u] * a.table_row, c, a.dim, vec, y);
         } else {
-          float* p = part + ((uint64_t)blockIdx.x * 2 + (begun ? 0 : 1)) * cpr * P + c;
+          float* p = part + ((uint64_t)b * 2 + (begun ? 0 : 1)) * cpr * P + c;
 #pragma unroll
           for (uint32_t j = 0; j < P; j++) p[j] = sum[j];
         }
@@ -198,29 +268,50 @@ __global__ __launch_bounds__(64) void embed_sum(pots_embedding a,
   }
 }
 
-// The rows that cross pieces, by the piece in which they begin.
+// The rows that cross pieces, by the piece in which they begin, a wave for 64 chunks of
+// columns; the blocks after the first `sums` waves' write zeros from `r0` on.
 template <class T>
-__global__ __launch_bounds__(64) void embed_join(pots_embedding a,
-                                                 const uint64_t* __restrict__ keys,
-                                                 uint32_t piece, uint32_t cpr,
-                                                 const float* __restrict__ part, bool vec) {
+__global__ __launch_bounds__(256) void embed_join(pots_embedding a,
+                                                  const uint64_t* __restrict__ keys,
+                                                  uint32_t piece, uint32_t groups, uint32_t sums,
+                                                  uint32_t cpr, uint32_t r0,
+                                                  const float* __restrict__ part, bool vec) {
   constexpr uint32_t P = kPer<T>;
-  const uint32_t ch = blockIdx.y * 64 + threadIdx.x, c = ch * P;
-  const uint32_t k0 = blockIdx.x * piece, k1 = min(k0 + piece, a.tokens);
+  const uint32_t blocks = (sums + 3) / 4;
+  if (blockIdx.x >= blocks) {
+    fill_rows<T, 256>(a, keys, r0 + (blockIdx.x - blocks) * kFill, a.vocab, cpr, vec);
+    return;
+  }
+  const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  if (unit >= sums) return;
+  const uint32_t own = unit / groups, ch = unit % groups * 64 + threadIdx.x % 64, c = ch * P;
+  const uint32_t k0 = own * piece, k1 = min(k0 + piece, a.tokens);
   if (k1 >= a.tokens || ch >= cpr) return;
   const uint32_t id = keys[k1 - 1] >> 32;
   if (id == kNoRow || (uint32_t)(keys[k1] >> 32) != id) return;       // ends here
   if ((uint32_t)(keys[k0] >> 32) == id && k0 > 0 && (uint32_t)(keys[k0 - 1] >> 32) == id)
     return;                                                           // began earlier
   float sum[P];
-  const float* p = part + ((uint64_t)blockIdx.x * 2 + 1) * cpr * P + c;
+  const float* p = part + ((uint64_t)own * 2 + 1) * cpr * P + c;
 #pragma unroll
   for (uint32_t j = 0; j < P; j++) sum[j] = p[j];
-  for (uint64_t k = k1, b = blockIdx.x + 1; k < a.tokens && (uint32_t)(keys[k] >> 32) == id;
-       k += piece, b++) {
-    const float* q = part + b * 2 * cpr * P + c;
+  constexpr uint32_t U = 8;  // pieces on their way at once
+  for (uint64_t k = k1, b = own + 1;; k += U * piece, b += U) {
+    bool in[U];
+    float v[U][P];
 #pragma unroll
-    for (uint32_t j = 0; j < P; j++) sum[j] += q[j];
+    for (uint32_t u = 0; u < U; u++) {
+      const uint64_t at = k + u * piece;
+      in[u] = at < a.tokens && (uint32_t)(keys[at] >> 32) == id;
+      const float* q = part + (at < a.tokens ? b + u : own) * 2 * cpr * P + c;
+#pragma unroll
+      for (uint32_t j = 0; j < P; j++) v[u][j] = q[j];
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++)
+#pragma unroll
+      for (uint32_t j = 0; j < P; j++) sum[j] += in[u] ? v[u][j] : 0.f;
+    if (!in[U - 1]) break;
   }
   typename T::elem* t = reinterpret_cast<typename T::elem*>(a.table) + (int64_t)id * a.table_row;
   float y[P] = {};
@@ -247,17 +338,20 @@ bool chunked(const pots_embedding* a) {
 }
 
 struct Cut {
-  uint32_t cpr, runs, piece, pieces;
+  uint32_t cpr, order, run, piece, pieces;
   uint64_t keys, part, bytes;  // `keys` bytes of one list; two of them, then the sums
 };
 
 // Pieces: short ones so that few tokens still spread over the GPU, longer ones so that their
-// sums stay a small part of the rows.
+// sums stay a small part of the rows; four times as long where the zeros of a dense gradient
+// (64 MiB or more) take longer than the sums beside them, for fewer rows to join after.
 Cut cut(const pots_embedding* a) {
   Cut c;
   c.cpr = (a->dim + per_chunk(a) - 1) / per_chunk(a);
-  c.runs = (a->tokens + kRun - 1) / kRun;
-  c.piece = 16;
+  c.order = (a->tokens + 31) / 32;
+  c.run = a->tokens <= kOneRun ? kOneRun : kRun;
+  c.piece = kPiece;
+  if (!a->add && (uint64_t)a->vocab * c.cpr * 16 >= 64ull << 20) c.piece *= 4;
   while (c.piece < 2048 && a->tokens / c.piece > 1024) c.piece *= 2;
   c.pieces = (a->tokens + c.piece - 1) / c.piece;
   c.keys = align_up(8ull * a->tokens, 256);
@@ -283,17 +377,18 @@ int backward(const pots_embedding* a, char* work, hipStream_t s) {
   uint64_t* from = reinterpret_cast<uint64_t*>(work);
   uint64_t* to = reinterpret_cast<uint64_t*>(work + c.keys);
   float* part = reinterpret_cast<float*>(work + 2 * c.keys);
-  uint32_t fill = 0;
-  if (!a->add) {
-    const uint64_t nb = ((uint64_t)a->vocab * c.cpr + 1023) / 1024;
-    fill = (uint32_t)(nb < 4096 ? nb : 4096);
+  // The zeros of a dense gradient: a share beside each of the three launches. Ordering and joining
+  // are short chains of dependent steps that would leave the memory idle, about as long as a
+  // twelfth of a large table takes to write.
+  const uint32_t r1 = a->add || !a->tokens ? 0 : a->vocab / 12;
+  const uint32_t r2 = a->add ? 0 : c.pieces > 1 ? a->vocab - r1 : a->vocab;
+  auto fills = [](uint32_t rows) { return (rows + kFill - 1) / kFill; };
+  if (a->tokens) {
+    hipLaunchKernelGGL((embed_order<T>), dim3(c.order + fills(r1)), dim3(1024), 0, s, *a, from,
+                       c.run, c.order, r1, c.cpr, vec);
+    POTS_HIP(hipGetLastError());
   }
-  if (c.runs + fill == 0) return POTS_E_OK;
-  hipLaunchKernelGGL((embed_sort<T>), dim3(c.runs + fill), dim3(1024), 0, s, *a, from, c.runs,
-                     c.cpr, vec);
-  POTS_HIP(hipGetLastError());
-  if (a->tokens == 0) return POTS_E_OK;
-  for (uint64_t run = kRun; run < a->tokens; run *= kMerge) {
+  for (uint64_t run = c.run; run < a->tokens; run *= kMerge) {
     hipLaunchKernelGGL(embed_merge, dim3((a->tokens + 255) / 256), dim3(256), 0, s, from, to,
                        a->tokens, run);
     POTS_HIP(hipGetLastError());
@@ -301,12 +396,15 @@ int backward(const pots_embedding* a, char* work, hipStream_t s) {
     from = to;
     to = t;
   }
-  const dim3 grid(c.pieces, (c.cpr + 63) / 64);
-  hipLaunchKernelGGL((embed_sum<T>), grid, dim3(64), 0, s, *a, from, c.piece, c.cpr, part, vec);
-  POTS_HIP(hipGetLastError());
+  const uint32_t groups = (c.cpr + 63) / 64, sums = c.pieces * groups, blocks = (sums + 3) / 4;
+  if (blocks + fills(r2 - r1)) {
+    hipLaunchKernelGGL((embed_sum<T>), dim3(blocks + fills(r2 - r1)), dim3(256), 0, s, *a, from,
+                       c.piece, groups, sums, c.cpr, r1, r2, part, vec);
+    POTS_HIP(hipGetLastError());
+  }
   if (c.pieces > 1) {
-    hipLaunchKernelGGL((embed_join<T>), grid, dim3(64), 0, s, *a, from, c.piece, c.cpr, part,
-                       vec);
+    hipLaunchKernelGGL((embed_join<T>), dim3(blocks + (a->add ? 0 : fills(a->vocab - r2))),
+                       dim3(256), 0, s, *a, from, c.piece, groups, sums, c.cpr, r2, part, vec);
     POTS_HIP(hipGetLastError());
   }
   return POTS_E_OK;
