@@ -170,17 +170,18 @@ __device__ __forceinline__ uint32_t length_of(const pots_attention& a, uint32_t 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 
 // A wave's D of [d_head × 32 rows] as rows of a tensor: lane (i, h) holds row r0 + i, four
-// consecutive columns at a time.
+// consecutive columns at a time (of the blocks of 32 columns `mine`, mine + step, ...).
 template <class T, uint32_t NB>
 __device__ __forceinline__ void store_rows(const pots_heads& x, uint32_t b, uint32_t head,
                                            uint32_t row, uint32_t n, uint32_t d,
                                            const f32x16 (&acc)[NB], float mul, bool vec,
-                                           uint32_t h) {
+                                           uint32_t h, uint32_t step = 1, uint32_t mine = 0) {
   if (row >= n) return;
   typename T::elem* p = reinterpret_cast<typename T::elem*>(x.ptr) + b * x.batch +
                         head * x.head + (int64_t)row * x.row;
 #pragma unroll
-  for (uint32_t db = 0; db < NB; db++)
+  for (uint32_t db = 0; db < NB; db++) {
+    if (db % step != mine) continue;
 #pragma unroll
     for (uint32_t g = 0; g < 4; g++) {
       const uint32_t c = 32 * db + 8 * g + 4 * h;
@@ -195,6 +196,7 @@ __device__ __forceinline__ void store_rows(const pots_heads& x, uint32_t b, uint
           if (c + e < d) p[c + e] = T::put(v[4 * g + e] * mul);
       }
     }
+  }
 }
 
 // The sequence (of `seqs`) and the tile of a block, long tiles first: a launch's blocks start in
@@ -211,15 +213,61 @@ __device__ __forceinline__ void unit_of(uint32_t seqs, uint32_t* seq, uint32_t* 
   }
 }
 
-template <class T, uint32_t DP, uint32_t NW, uint32_t KT>
-__global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 : 1) void attn_fwd(pots_attention a, uint32_t tiles,
-                                                       bool vec, bool vec_out) {
+// How a block divides its work. Rows: four waves of 32 rows each (queries; keys in attn_dkv) go
+// through the other side's tiles of 64 (32 in fp32) together. Split: where that leaves compute
+// units without a block, a block has 32 rows and each wave takes its own 32 of a tile's 32·NW; the
+// waves' sums are joined at the end, in order (two waves for wide fp32 heads, whose tiles would
+// not fit the LDS). The 135M decoder's layer (fp32, 36 query heads' sequences of 256), us:
+// blocks of one wave 24 (attn_fwd), 32 (attn_dq) and 47 (attn_dkv), split ones 15, 21 and 23.
+template <class T, uint32_t DP, bool SPLIT>
+struct Shape {
+  static constexpr uint32_t kWide = DP * sizeof(typename T::elem);  // bytes of a row
+  static constexpr uint32_t NW = SPLIT && kWide > 256 ? 2 : 4, NT = 64 * NW;
+  static constexpr uint32_t R = SPLIT ? 32 : 32 * NW;  // the block's rows
+  static constexpr uint32_t KT = SPLIT ? 32 * NW : sizeof(typename T::elem) == 2 ? 64 : 32;
+  static constexpr uint32_t U = SPLIT ? 1 : KT / 32;   // a wave's products in a tile
+  static constexpr uint32_t KS = DP / 16, NB = DP / 32;
+  typedef Rows<T, DP, KT, NT> Tile;
+  typedef typename T::elem Lds[KT * DP];  // at least 256 bytes a column: two sums of 32 rows
+};
+
+// The waves' sums of a split block, joined in order: wave w's at lds(w), of which the caller's
+// blocks db = wave, wave + NW, ... come back in acc. at: 0 or 1, two sums fit.
+template <uint32_t NB, uint32_t NW, class L>
+__device__ __forceinline__ void put_sums(f32x16 (&acc)[NB], L lds, uint32_t at, uint32_t wave,
+                                         uint32_t lane) {
+  float* p = lds(wave) + at * NB * 1024 + lane;
+#pragma unroll
+  for (uint32_t db = 0; db < NB; db++)
+#pragma unroll
+    for (uint32_t r = 0; r < 16; r++) p[(db * 16 + r) * 64] = acc[db][r];
+}
+template <uint32_t NB, uint32_t NW, class L>
+__device__ __forceinline__ void join_sums(f32x16 (&acc)[NB], L lds, uint32_t at, uint32_t wave,
+                                          uint32_t lane) {
+#pragma unroll
+  for (uint32_t db = 0; db < NB; db++) {
+    if (db % NW != wave) continue;
+#pragma unroll
+    for (uint32_t r = 0; r < 16; r++) {
+      float sum = 0.f;
+#pragma unroll
+      for (uint32_t w = 0; w < NW; w++) sum += lds(w)[at * NB * 1024 + (db * 16 + r) * 64 + lane];
+      acc[db][r] = sum;
+    }
+  }
+}
+
+template <class T, uint32_t DP, bool SPLIT>
+__global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
+                             (!SPLIT && Shape<T, DP, SPLIT>::kWide <= 256 ? 2 : 1)) void attn_fwd(
+    pots_attention a, uint32_t tiles, bool vec, bool vec_out) {
   typedef typename T::elem elem;
   typedef typename T::frag frag;
-  constexpr uint32_t NT = 64 * NW, QB = 32 * NW, KS = DP / 16, NB = DP / 32;
-  typedef Rows<T, DP, KT, NT> R;
-  __shared__ __attribute__((aligned(16))) elem s_k0[KT * DP], s_k1[KT * DP];
-  __shared__ __attribute__((aligned(16))) elem s_v0[KT * DP], s_v1[KT * DP];
+  typedef Shape<T, DP, SPLIT> S;
+  typedef typename S::Tile R;
+  constexpr uint32_t NW = S::NW, KT = S::KT, KS = S::KS, NB = S::NB, U = S::U;
+  __shared__ __attribute__((aligned(16))) typename S::Lds s_k0, s_k1, s_v0, s_v1;
   uint32_t bh, place;
   unit_of(a.batch * a.heads, &bh, &place);
   const uint32_t tile = tiles - 1 - place, b = bh / a.heads, head = bh % a.heads;
@@ -228,9 +276,9 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 :
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t len = length_of(a, b), d = a.head_dim;
   const Head<T> Q(a.q, b, head), K(a.k, b, kvh), V(a.v, b, kvh);
-  const uint32_t q0 = tile * QB, qw = q0 + 32 * wave, q = qw + i;
+  const uint32_t q0 = tile * S::R, qw = SPLIT ? q0 : q0 + 32 * wave, q = qw + i;
   // keys that the block's rows see, and the wave's
-  const uint32_t end = q0 >= len ? 0 : a.causal ? min(len, q0 + QB) : len;
+  const uint32_t end = q0 >= len ? 0 : a.causal ? min(len, q0 + S::R) : len;
   const uint32_t wend = qw >= len ? 0 : a.causal ? min(len, qw + 32) : len;
   const uint32_t seen = q >= len ? 0 : a.causal ? min(len, q + 1) : len;
   R rk, rv;
@@ -250,27 +298,28 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 :
   for (uint32_t db = 0; db < NB; db++) o[db] = zero16();
   const float c = a.scale * kLog2e;
   float m = -INFINITY, mc = 0.f, l = 0.f;
-  auto step = [&](const elem* s_k, const elem* s_v, uint32_t k0) {
+  auto step = [&](const elem* s_k, const elem* s_v, uint32_t t0) {
+    const uint32_t at = SPLIT ? 32 * wave : 0, k0 = t0 + at;  // of the tile, the wave's part
     if (k0 >= wend) return;
-    f32x16 s[KT / 32];
+    f32x16 s[U];
 #pragma unroll
-    for (uint32_t u = 0; u < KT / 32; u++) {
+    for (uint32_t u = 0; u < U; u++) {
       s[u] = zero16();
 #pragma unroll
       for (uint32_t ks = 0; ks < KS; ks++)
-        s[u] = mma(R::row(s_k, 32 * u + i, 16 * ks + 8 * h), qf[ks], s[u]);
+        s[u] = mma(R::row(s_k, at + 32 * u + i, 16 * ks + 8 * h), qf[ks], s[u]);
     }
     // a tile that some row sees in part, or rows that see nothing
-    if (k0 + KT > len || qw + 32 > len || (a.causal && k0 + KT - 1 > qw)) {
+    if (k0 + 32 * U > len || qw + 32 > len || (a.causal && k0 + 32 * U - 1 > qw)) {
 #pragma unroll
-      for (uint32_t u = 0; u < KT / 32; u++)
+      for (uint32_t u = 0; u < U; u++)
 #pragma unroll
         for (uint32_t r = 0; r < 16; r++)
           if (k0 + 32 * u + d_row(r, h) >= seen) s[u][r] = -INFINITY;
     }
     float top = m;
 #pragma unroll
-    for (uint32_t u = 0; u < KT / 32; u++)
+    for (uint32_t u = 0; u < U; u++)
 #pragma unroll
       for (uint32_t r = 0; r < 16; r++) top = fmaxf(top, s[u][r]);
     top = fmaxf(top, other_half(top));
@@ -286,7 +335,7 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 :
         for (uint32_t r = 0; r < 16; r++) o[db][r] *= f;
     }
 #pragma unroll
-    for (uint32_t u = 0; u < KT / 32; u++) {
+    for (uint32_t u = 0; u < U; u++) {
 #pragma unroll
       for (uint32_t r = 0; r < 16; r++) {
         s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], c, -mc));
@@ -297,7 +346,7 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 :
         const frag p = T::pack(s[u], 8 * t);
 #pragma unroll
         for (uint32_t db = 0; db < NB; db++)
-          o[db] = mma(R::col(s_v, 32 * u + 16 * t, 32 * db, lane), p, o[db]);
+          o[db] = mma(R::col(s_v, at + 32 * u + 16 * t, 32 * db, lane), p, o[db]);
       }
     }
   };
@@ -315,8 +364,35 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 :
     step(s_k0, s_v0, k0);
   }
   l += other_half(l);
-  store_rows<T, NB>(a.out, b, head, q, a.n, d, o, l > 0.f || l != l ? 1.f / l : 0.f, vec_out, h);
-  if (h == 0 && q < a.n)
+  if constexpr (SPLIT) {
+    // each wave's sums in units of the largest maximum of all, then added up
+    __shared__ float s_m[NW][32], s_l[NW][32];
+    auto lds = [&](uint32_t w) {
+      return reinterpret_cast<float*>(w == 0 ? s_k0 : w == 1 ? s_k1 : w == 2 ? s_v0 : s_v1);
+    };
+    if (h == 0) s_m[wave][i] = m == -INFINITY ? -INFINITY : mc;
+    __syncthreads();  // and every wave is done with its tiles
+    float top = -INFINITY;
+#pragma unroll
+    for (uint32_t w = 0; w < NW; w++) top = fmaxf(top, s_m[w][i]);
+    // (a sum without a finite maximum is zero, or NaN, which stays)
+    const float f = m == -INFINITY || mc == top ? 1.f : __builtin_amdgcn_exp2f(mc - top);
+    if (h == 0) s_l[wave][i] = l * f;
+#pragma unroll
+    for (uint32_t db = 0; db < NB; db++)
+#pragma unroll
+      for (uint32_t r = 0; r < 16; r++) o[db][r] *= f;
+    put_sums<NB, NW>(o, lds, 0, wave, lane);
+    __syncthreads();
+    l = 0.f;
+#pragma unroll
+    for (uint32_t w = 0; w < NW; w++) l += s_l[w][i];
+    mc = top == -INFINITY ? 0.f : top;
+    join_sums<NB, NW>(o, lds, 0, wave, lane);
+  }
+  store_rows<T, NB>(a.out, b, head, q, a.n, d, o, l > 0.f || l != l ? 1.f / l : 0.f, vec_out, h,
+                    SPLIT ? NW : 1, SPLIT ? wave : 0);
+  if (h == 0 && q < a.n && (!SPLIT || wave == 0))
     a.lse[(int64_t)bh * a.n + q] =
         l == 0.f ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * kLn2;
 }
@@ -324,15 +400,16 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 :
 // dq, and for attn_dkv each row's lse in units of log2 and D: stat [2][batch·heads][n]. A wave
 // holds 32 query rows as columns, as in the forward pass: Sᵀ = K·Qᵀ and dPᵀ = V·dOᵀ from the
 // tiles' rows, dQᵀ += Kᵀ·dSᵀ with K read transposed.
-template <class T, uint32_t DP, uint32_t NW, uint32_t KT>
-__global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 : 1) void attn_dq(pots_attention a, float* __restrict__ stat,
-                                                      uint32_t tiles, bool vec, bool vec_out) {
+template <class T, uint32_t DP, bool SPLIT>
+__global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
+                             (!SPLIT && Shape<T, DP, SPLIT>::kWide <= 256 ? 2 : 1)) void attn_dq(
+    pots_attention a, float* __restrict__ stat, uint32_t tiles, bool vec, bool vec_out) {
   typedef typename T::elem elem;
   typedef typename T::frag frag;
-  constexpr uint32_t NT = 64 * NW, QB = 32 * NW, KS = DP / 16, NB = DP / 32;
-  typedef Rows<T, DP, KT, NT> R;
-  __shared__ __attribute__((aligned(16))) elem s_k0[KT * DP], s_k1[KT * DP];
-  __shared__ __attribute__((aligned(16))) elem s_v0[KT * DP], s_v1[KT * DP];
+  typedef Shape<T, DP, SPLIT> S;
+  typedef typename S::Tile R;
+  constexpr uint32_t NW = S::NW, KT = S::KT, KS = S::KS, NB = S::NB, U = S::U;
+  __shared__ __attribute__((aligned(16))) typename S::Lds s_k0, s_k1, s_v0, s_v1;
   uint32_t bh, place;
   unit_of(a.batch * a.heads, &bh, &place);
   const uint32_t tile = tiles - 1 - place, b = bh / a.heads, head = bh % a.heads;
@@ -342,8 +419,8 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 :
   const uint32_t len = length_of(a, b), d = a.head_dim;
   const Head<T> Q(a.q, b, head), K(a.k, b, kvh), V(a.v, b, kvh), O(a.out, b, head),
       G(a.dout, b, head);
-  const uint32_t q0 = tile * QB, qw = q0 + 32 * wave, q = qw + i;
-  const uint32_t end = q0 >= len ? 0 : a.causal ? min(len, q0 + QB) : len;
+  const uint32_t q0 = tile * S::R, qw = SPLIT ? q0 : q0 + 32 * wave, q = qw + i;
+  const uint32_t end = q0 >= len ? 0 : a.causal ? min(len, q0 + S::R) : len;
   const uint32_t wend = qw >= len ? 0 : a.causal ? min(len, qw + 32) : len;
   const uint32_t seen = q >= len ? 0 : a.causal ? min(len, q + 1) : len;
   R rk, rv;
@@ -370,7 +447,7 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 :
     const int64_t at = (int64_t)bh * a.n + q;
     const float x = q < len ? gload<float>(a.lse + at) : -INFINITY;
     if (x != -INFINITY) lse2 = x * kLog2e;
-    if (h == 0) {
+    if (h == 0 && (!SPLIT || wave == 0)) {
       stat[at] = lse2;
       stat[(int64_t)a.batch * a.heads * a.n + at] = dl;
     }
@@ -381,8 +458,8 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 :
   const float c = a.scale * kLog2e;
   auto step = [&](const elem* s_k, const elem* s_v, uint32_t k0) {
 #pragma unroll
-    for (uint32_t u = 0; u < KT / 32; u++) {
-      const uint32_t ku = k0 + 32 * u;
+    for (uint32_t x = 0; x < U; x++) {
+      const uint32_t u = SPLIT ? wave : x, ku = k0 + 32 * u;
       if (ku >= wend) return;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -422,26 +499,36 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 256 ? 2 :
     loads_done();
     step(s_k0, s_v0, k0);
   }
-  store_rows<T, NB>(a.dq, b, head, q, a.n, d, acc, a.scale, vec_out, h);
+  if constexpr (SPLIT) {
+    auto lds = [&](uint32_t w) {
+      return reinterpret_cast<float*>(w == 0 ? s_k0 : w == 1 ? s_k1 : w == 2 ? s_v0 : s_v1);
+    };
+    __syncthreads();
+    put_sums<NB, NW>(acc, lds, 0, wave, lane);
+    __syncthreads();
+    join_sums<NB, NW>(acc, lds, 0, wave, lane);
+  }
+  store_rows<T, NB>(a.dq, b, head, q, a.n, d, acc, a.scale, vec_out, h, SPLIT ? NW : 1,
+                    SPLIT ? wave : 0);
 }
 
-// dk and dv of 32·NW keys, over `per` query heads of their group and the queries that see
+// dk and dv of a block's keys, over `per` query heads of their group and the queries that see
 // them. A wave holds 32 keys as columns: S = Q·Kᵀ and dP = dO·Vᵀ from the tiles' rows, dVᵀ +=
 // dOᵀ·P and dKᵀ += Qᵀ·dS from the same tiles read transposed. With `part`, the sums go to fp32
 // slices [2][split][batch][kv_heads][n][d].
-template <class T, uint32_t DP, uint32_t NW, uint32_t QT>
-__global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 128 ? 2 : 1) void attn_dkv(pots_attention a,
-                                                       const float* __restrict__ stat,
-                                                       float* __restrict__ part, uint32_t tiles,
-                                                       uint32_t splits, uint32_t per, bool vec,
-                                                       bool vec_out) {
+template <class T, uint32_t DP, bool SPLIT>
+__global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
+                             (!SPLIT && Shape<T, DP, SPLIT>::kWide <= 128 ? 2 : 1)) void attn_dkv(
+    pots_attention a, const float* __restrict__ stat, float* __restrict__ part, uint32_t tiles,
+    uint32_t splits, uint32_t per, bool vec, bool vec_out) {
   typedef typename T::elem elem;
   typedef typename T::frag frag;
-  constexpr uint32_t NT = 64 * NW, KB = 32 * NW, KS = DP / 16, NB = DP / 32;
-  typedef Rows<T, DP, QT, NT> R;
-  __shared__ __attribute__((aligned(16))) elem s_q0[QT * DP], s_q1[QT * DP];
-  __shared__ __attribute__((aligned(16))) elem s_g0[QT * DP], s_g1[QT * DP];
-  __shared__ __attribute__((aligned(16))) float s_stat0[2 * 64], s_stat1[2 * 64];
+  typedef Shape<T, DP, SPLIT> S;
+  typedef typename S::Tile R;
+  constexpr uint32_t NW = S::NW, QT = S::KT, KS = S::KS, NB = S::NB, U = S::U;
+  constexpr uint32_t kStat = QT < 64 ? 64 : QT;
+  __shared__ __attribute__((aligned(16))) typename S::Lds s_q0, s_q1, s_g0, s_g1;
+  __shared__ __attribute__((aligned(16))) float s_stat0[2 * kStat], s_stat1[2 * kStat];
   uint32_t seq, tile;
   unit_of(a.batch * a.kv_heads * splits, &seq, &tile);
   const uint32_t split = seq % splits, bk = seq / splits, b = bk / a.kv_heads;
@@ -450,7 +537,7 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 128 ? 2 :
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t len = length_of(a, b), d = a.head_dim;
   const Head<T> K(a.k, b, kvh), V(a.v, b, kvh);
-  const uint32_t k0 = tile * KB, kw = k0 + 32 * wave, key = kw + i;
+  const uint32_t k0 = tile * S::R, kw = SPLIT ? k0 : k0 + 32 * wave, key = kw + i;
   // the block's steps: (head, tile of queries) in order
   const uint32_t first = a.causal ? k0 / QT * QT : 0, e0 = split * per;
   const uint32_t tiles_q = k0 < len ? (len - first + QT - 1) / QT : 0;
@@ -465,11 +552,12 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 128 ? 2 :
     const Head<T> Q(a.q, b, head), G(a.dout, b, head);
     rq.load(s_q, Q.p, Q.row, lq, len, d, vec);
     rg.load(s_g, G.p, G.row, lq, len, d, vec);
-    if (wave == 0) {  // lse and D of the tile's rows; zero past the length
-      const int64_t at = (int64_t)(b * a.heads + head) * a.n + lq;
-      const uint32_t range = 4 * min(64u, len - lq);
-      load_lds4(make_rsrc(stat + at, range), s_stat, 4 * lane);
-      load_lds4(make_rsrc(stat1 + at, range), s_stat + 64, 4 * lane);
+    if (64 * wave < kStat) {  // lse and D of the tile's rows, 64 a wave; zero past the length
+      const uint32_t q = lq + 64 * wave;
+      const int64_t at = (int64_t)(b * a.heads + head) * a.n + q;
+      const uint32_t range = q < len ? 4 * min(64u, len - q) : 0;
+      load_lds4(make_rsrc(stat + at, range), s_stat + 64 * wave, 4 * lane);
+      load_lds4(make_rsrc(stat1 + at, range), s_stat + kStat + 64 * wave, 4 * lane);
     }
     lq += QT;
     if (lq >= len) {
@@ -494,8 +582,8 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 128 ? 2 :
   uint32_t q0 = first;
   auto step = [&](const elem* s_q, const elem* s_g, const float* s_stat) {
 #pragma unroll
-    for (uint32_t u = 0; u < QT / 32; u++) {
-      const uint32_t qu = q0 + 32 * u;
+    for (uint32_t y = 0; y < U; y++) {
+      const uint32_t u = SPLIT ? wave : y, qu = q0 + 32 * u;
       if (qu >= len || kw >= len || (a.causal && qu + 31 < kw)) continue;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -506,7 +594,7 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 128 ? 2 :
 #pragma unroll
       for (uint32_t g = 0; g < 4; g++) {
         const f32x4 ls = *reinterpret_cast<const f32x4*>(s_stat + 32 * u + 8 * g + 4 * h);
-        const f32x4 dl = *reinterpret_cast<const f32x4*>(s_stat + 64 + 32 * u + 8 * g + 4 * h);
+        const f32x4 dl = *reinterpret_cast<const f32x4*>(s_stat + kStat + 32 * u + 8 * g + 4 * h);
 #pragma unroll
         for (uint32_t x = 0; x < 4; x++) {
           const uint32_t r = 4 * g + x;
@@ -546,38 +634,65 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(typename T::elem) <= 128 ? 2 :
     loads_done();
     step(s_q0, s_g0, s_stat0);
   }
+  if constexpr (SPLIT) {
+    auto lds = [&](uint32_t w) {
+      return reinterpret_cast<float*>(w == 0 ? s_q0 : w == 1 ? s_q1 : w == 2 ? s_g0 : s_g1);
+    };
+    __syncthreads();
+    put_sums<NB, NW>(dk, lds, 0, wave, lane);
+    put_sums<NB, NW>(dv, lds, 1, wave, lane);
+    __syncthreads();
+    join_sums<NB, NW>(dk, lds, 0, wave, lane);
+    join_sums<NB, NW>(dv, lds, 1, wave, lane);
+  }
+  constexpr uint32_t kOf = SPLIT ? NW : 1;
+  const uint32_t mine = SPLIT ? wave : 0;
   if (part) {
     pots_heads x;
     x.row = d;
     x.head = (int64_t)a.n * d;
     x.batch = x.head * a.kv_heads;
     x.ptr = part + split * x.batch * a.batch;
-    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dk, a.scale, d % 4 == 0, h);
+    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dk, a.scale, d % 4 == 0, h, kOf, mine);
     x.ptr = part + (splits + split) * x.batch * a.batch;
-    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dv, 1.f, d % 4 == 0, h);
+    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dv, 1.f, d % 4 == 0, h, kOf, mine);
   } else {
-    store_rows<T, NB>(a.dk, b, kvh, key, a.n, d, dk, a.scale, vec_out, h);
-    store_rows<T, NB>(a.dv, b, kvh, key, a.n, d, dv, 1.f, vec_out, h);
+    store_rows<T, NB>(a.dk, b, kvh, key, a.n, d, dk, a.scale, vec_out, h, kOf, mine);
+    store_rows<T, NB>(a.dv, b, kvh, key, a.n, d, dv, 1.f, vec_out, h, kOf, mine);
   }
 }
 
-// dk (blockIdx.y = 0) and dv (1) from the splits' sums, in order.
+// dk (blockIdx.y = 0) and dv (1) from the splits' sums, in order, four values a thread.
 template <class T>
 __global__ __launch_bounds__(256) void attn_fold(pots_attention a,
                                                  const float* __restrict__ part,
-                                                 uint32_t splits) {
+                                                 uint32_t splits, bool vec_out) {
   const uint64_t each = (uint64_t)a.batch * a.kv_heads * a.n * a.head_dim;
   const float* p = part + blockIdx.y * splits * each;
   const pots_heads& x = blockIdx.y ? a.dv : a.dk;
-  for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < each;
-       e += (uint64_t)gridDim.x * 256) {
-    float sum = p[e];
-    for (uint32_t s = 1; s < splits; s++) sum += p[s * each + e];
-    const uint32_t col = e % a.head_dim;
-    const uint64_t row = e / a.head_dim, bk = row / a.n;
-    reinterpret_cast<typename T::elem*>(
-        x.ptr)[(int64_t)(bk / a.kv_heads) * x.batch + (int64_t)(bk % a.kv_heads) * x.head +
-               (int64_t)(row % a.n) * x.row + col] = T::put(sum);
+  const uint64_t step = (uint64_t)gridDim.x * 1024;
+  for (uint64_t e = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4; e < each; e += step) {
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    const bool four = vec_out && a.head_dim % 4 == 0;  // then also of one row
+    for (uint32_t s = 0; s < splits; s++) {
+      if (four) {
+        sum += gload<f32x4>(p + s * each + e);
+      } else {
+        for (uint32_t j = 0; j < 4 && e + j < each; j++) sum[j] += p[s * each + e + j];
+      }
+    }
+    for (uint32_t j = 0; j < 4 && e + j < each; j += four ? 4 : 1) {
+      const uint64_t row = (e + j) / a.head_dim, bk = row / a.n;
+      const uint32_t col = (e + j) - row * a.head_dim;
+      typename T::elem* q = reinterpret_cast<typename T::elem*>(x.ptr) +
+                            (int64_t)(bk / a.kv_heads) * x.batch +
+                            (int64_t)(bk % a.kv_heads) * x.head +
+                            (int64_t)(row - bk * a.n) * x.row + col;
+      if (four)
+        T::store4(q, sum[0], sum[1], sum[2], sum[3]);
+      else
+        *q = T::put(sum[j]);
+    }
   }
 }
 
@@ -598,84 +713,91 @@ bool aligned(const pots_attention* a, const pots_heads& x, uint32_t bytes) {
          x.row >= 0 && x.row < (1 << 23);
 }
 
-// Waves in a block: as many as four (which share a K or V tile) while that leaves a block for
-// every compute unit.
-uint32_t waves(uint64_t sequences, uint32_t n) {
-  for (uint32_t w = 4; w > 1; w /= 2)
-    if (sequences * ((n + 32 * w - 1) / (32 * w)) >= 256) return w;
-  return 1;
-}
+uint32_t cdiv(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
 
-struct Dkv {
-  uint32_t nw, tiles, splits, per;
+// Whether blocks of 128 rows leave compute units without one: blocks of 32 then.
+bool few(uint64_t sequences, uint32_t n) { return sequences * cdiv(n, 128) < 256; }
+
+struct Cut {
+  bool split;
+  uint32_t tiles, splits, per;  // of keys; of a group's query heads in attn_dkv
 };
 
-Dkv dkv_cut(const pots_attention* a) {
-  Dkv r;
+// The query heads of a group are shared out over blocks while there are fewer blocks than
+// compute units and a block has more than two tiles of queries to go through, or fewer than
+// three for each (causal tiles differ in length, and the launch ends with the short ones) and
+// more than eight tiles. us, two blocks for a unit at the least and three: the 0.5B shape 86 + 11 and
+// 64 + 12 (attn_dkv, attn_fold), the 1.5B shape 197 + 18 and 191 + 23.
+Cut cut(const pots_attention* a) {
+  Cut c;
   const uint32_t rep = a->heads / a->kv_heads;
-  r.nw = waves((uint64_t)a->batch * a->heads, a->n);
-  r.tiles = (a->n + 32 * r.nw - 1) / (32 * r.nw);
-  const uint64_t blocks = (uint64_t)a->batch * a->kv_heads * r.tiles;
-  r.splits = 1;
-  while (r.splits < rep && blocks * r.splits < 768) r.splits++;
-  r.per = (rep + r.splits - 1) / r.splits;
-  r.splits = (rep + r.per - 1) / r.per;
-  return r;
+  c.split = few((uint64_t)a->batch * a->heads, a->n);
+  c.tiles = cdiv(a->n, c.split ? 32 : 128);
+  const uint64_t blocks = (uint64_t)a->batch * a->kv_heads * c.tiles;
+  const uint32_t steps = cdiv(a->n, c.split ? 128 : 64);
+  c.splits = 1;
+  while (c.splits < rep) {
+    const uint64_t now = blocks * c.splits, left = (uint64_t)steps * cdiv(rep, c.splits);
+    if (!(now < 256 && left > 2) && !(now < 768 && left > 8)) break;
+    c.splits++;
+  }
+  c.per = cdiv(rep, c.splits);
+  c.splits = cdiv(rep, c.per);
+  return c;
 }
 
-template <class T, uint32_t DP, uint32_t NW>
+template <class T, uint32_t DP, bool SPLIT>
 int forward(const pots_attention* a, hipStream_t s) {
-  const uint32_t tiles = (a->n + 32 * NW - 1) / (32 * NW);
+  typedef Shape<T, DP, SPLIT> S;
+  const uint32_t tiles = cdiv(a->n, S::R);
   const uint64_t blocks = (uint64_t)a->batch * a->heads * tiles;
   if (blocks > 0x7FFFFFFFu) return POTS_E_ARG;
   const bool vec = aligned(a, a->q, 16) && aligned(a, a->k, 16) && aligned(a, a->v, 16);
-  hipLaunchKernelGGL((attn_fwd<T, DP, NW, sizeof(typename T::elem) == 2 && NW == 4 ? 64 : 32>), dim3((uint32_t)blocks),
-                     dim3(64 * NW), 0, s, *a, tiles, vec,
-                     aligned(a, a->out, 4 * sizeof(typename T::elem)));
+  hipLaunchKernelGGL((attn_fwd<T, DP, SPLIT>), dim3((uint32_t)blocks), dim3(S::NT), 0, s, *a,
+                     tiles, vec, aligned(a, a->out, 4 * sizeof(typename T::elem)));
   POTS_HIP(hipGetLastError());
   return POTS_E_OK;
 }
 
-template <class T, uint32_t DP, uint32_t NW>
+template <class T, uint32_t DP, bool SPLIT>
 int backward(const pots_attention* a, char* work, hipStream_t s) {
-  const Dkv cut = dkv_cut(a);
-  const uint64_t qblocks = (uint64_t)a->batch * a->heads * cut.tiles;
-  const uint64_t kblocks = (uint64_t)a->batch * a->kv_heads * cut.tiles * cut.splits;
+  typedef Shape<T, DP, SPLIT> S;
+  const Cut c = cut(a);
+  const uint64_t qblocks = (uint64_t)a->batch * a->heads * c.tiles;
+  const uint64_t kblocks = (uint64_t)a->batch * a->kv_heads * c.tiles * c.splits;
   if (qblocks > 0x7FFFFFFFu || kblocks > 0x7FFFFFFFu) return POTS_E_ARG;
   float* stat = reinterpret_cast<float*>(work);
-  float* part = cut.splits == 1 ? nullptr
-                                : reinterpret_cast<float*>(
-                                      work + align_up((size_t)a->batch * a->heads * a->n * 8,
-                                                      256));
+  float* part = nullptr;
+  if (c.splits > 1)
+    part = reinterpret_cast<float*>(work +
+                                    align_up((size_t)a->batch * a->heads * a->n * 8, 256));
   const bool vec = aligned(a, a->q, 16) && aligned(a, a->k, 16) && aligned(a, a->v, 16) &&
                    aligned(a, a->out, 16) && aligned(a, a->dout, 16);
   const uint32_t four = 4 * sizeof(typename T::elem);
-  hipLaunchKernelGGL((attn_dq<T, DP, NW, sizeof(typename T::elem) == 2 && NW == 4 ? 64 : 32>), dim3((uint32_t)qblocks),
-                     dim3(64 * NW), 0, s, *a, stat, cut.tiles, vec, aligned(a, a->dq, four));
+  hipLaunchKernelGGL((attn_dq<T, DP, SPLIT>), dim3((uint32_t)qblocks), dim3(S::NT), 0, s, *a,
+                     stat, c.tiles, vec, aligned(a, a->dq, four));
   POTS_HIP(hipGetLastError());
-  hipLaunchKernelGGL((attn_dkv<T, DP, NW, sizeof(typename T::elem) == 2 && NW == 4 ? 64 : 32>), dim3((uint32_t)kblocks),
-                     dim3(64 * NW), 0, s, *a, stat, part, cut.tiles, cut.splits, cut.per, vec,
+  hipLaunchKernelGGL((attn_dkv<T, DP, SPLIT>), dim3((uint32_t)kblocks), dim3(S::NT), 0, s, *a,
+                     stat, part, c.tiles, c.splits, c.per, vec,
                      aligned(a, a->dk, four) && aligned(a, a->dv, four));
   POTS_HIP(hipGetLastError());
   if (part) {
     const uint64_t each = (uint64_t)a->batch * a->kv_heads * a->n * a->head_dim;
-    const uint64_t nb = (each + 255) / 256;
+    const uint64_t nb = (each + 1023) / 1024;
     hipLaunchKernelGGL((attn_fold<T>), dim3((uint32_t)(nb < 4096 ? nb : 4096), 2), dim3(256), 0,
-                       s, *a, part, cut.splits);
+                       s, *a, part, c.splits, aligned(a, a->dk, four) && aligned(a, a->dv, four));
     POTS_HIP(hipGetLastError());
   }
   return POTS_E_OK;
 }
 
-#define POTS_WAVES(T, DP, F, ...)          \
-  (nw == 4   ? F<T, DP, 4>(__VA_ARGS__)    \
-   : nw == 2 ? F<T, DP, 2>(__VA_ARGS__)    \
-             : F<T, DP, 1>(__VA_ARGS__))
+#define POTS_SPLIT(T, DP, F, ...) \
+  (split ? F<T, DP, true>(__VA_ARGS__) : F<T, DP, false>(__VA_ARGS__))
 #define POTS_DIMS(T, F, ...)                                     \
-  (a->head_dim <= 32   ? POTS_WAVES(T, 32, F, __VA_ARGS__)       \
-   : a->head_dim <= 64 ? POTS_WAVES(T, 64, F, __VA_ARGS__)       \
-   : a->head_dim <= 96 ? POTS_WAVES(T, 96, F, __VA_ARGS__)       \
-                       : POTS_WAVES(T, 128, F, __VA_ARGS__))
+  (a->head_dim <= 32   ? POTS_SPLIT(T, 32, F, __VA_ARGS__)       \
+   : a->head_dim <= 64 ? POTS_SPLIT(T, 64, F, __VA_ARGS__)       \
+   : a->head_dim <= 96 ? POTS_SPLIT(T, 96, F, __VA_ARGS__)       \
+                       : POTS_SPLIT(T, 128, F, __VA_ARGS__))
 
 }  // namespace
 
@@ -688,17 +810,17 @@ extern "C" int pots_attention_forward(const pots_attention* a, void* stream) {
   if (a->batch == 0 || a->n == 0) return POTS_E_OK;
   if (!a->q.ptr || !a->k.ptr || !a->v.ptr || !a->out.ptr || !a->lse) return POTS_E_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const uint32_t nw = waves((uint64_t)a->batch * a->heads, a->n);
+  const bool split = few((uint64_t)a->batch * a->heads, a->n);
   return a->dtype == POTS_OP_BF16 ? POTS_DIMS(Bf16, forward, a, s)
                                   : POTS_DIMS(Fp32, forward, a, s);
 }
 
 extern "C" uint64_t pots_attention_backward_work(const pots_attention* a) {
   if (bad(a) || a->batch == 0 || a->n == 0) return 0;
-  const Dkv cut = dkv_cut(a);
+  const Cut c = cut(a);
   uint64_t bytes = align_up((size_t)a->batch * a->heads * a->n * 8, 256);
-  if (cut.splits > 1)
-    bytes += 2ull * cut.splits * a->batch * a->kv_heads * a->n * a->head_dim * 4;
+  if (c.splits > 1)
+    bytes += 2ull * c.splits * a->batch * a->kv_heads * a->n * a->head_dim * 4;
   return bytes;
 }
 
@@ -709,7 +831,7 @@ extern "C" int pots_attention_backward(const pots_attention* a, void* work, void
       !a->dq.ptr || !a->dk.ptr || !a->dv.ptr || !work)
     return POTS_E_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const uint32_t nw = dkv_cut(a).nw;
+  const bool split = cut(a).split;
   char* w = static_cast<char*>(work);
   return a->dtype == POTS_OP_BF16 ? POTS_DIMS(Bf16, backward, a, w, s)
                                   : POTS_DIMS(Fp32, backward, a, w, s);

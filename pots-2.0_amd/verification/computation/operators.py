@@ -120,7 +120,8 @@ def _attention_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 def _new_heads(b: int, h: int, n: int, d: int, ref: torch.Tensor) -> torch.Tensor:
     """``[b, h, n, d]`` over memory of ``[b, n, h, d]``: a position's heads beside each other,
     as the projections around attention read and write them."""
-    return torch.empty(b, n, h, d, dtype=ref.dtype, device=ref.device).transpose(1, 2)
+    return torch.empty_strided((b, h, n, d), (n * h * d, d, h * d, 1), dtype=ref.dtype,
+                               device=ref.device)
 
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
