@@ -53,12 +53,12 @@ __device__ __forceinline__ void pair_of(uint32_t pairs, uint32_t t, uint32_t* pa
 template <bool TR, uint32_t T, uint32_t NT>
 struct Stage {
   static constexpr uint32_t kAll = T * BK / 8, kChunks = (kAll + NT - 1) / NT;
-  static_assert(!TR || T >= 128, "the exchange of a transposed tile needs 16 chunks a row");
+  static_assert(!TR || (T % 64 == 0 && T > 64), "the exchange stays within a transposed row");
   uint32_t off[kChunks], wide;
 
   // What row r's chunks are exchanged by.
   static __device__ __forceinline__ uint32_t swap(uint32_t r) {
-    return TR ? 4 * (r & 3) : (r >> 1) & 7;
+    return !TR ? (r >> 1) & 7 : T % 128 == 0 ? 4 * (r & 3) : 2 * (r & 2);
   }
 
   // r0, rows: the tile's first row and their number; rows past it repeat the last (for TR:
@@ -587,10 +587,12 @@ namespace {
 template <bool ATR, bool BTR>
 using Large = Tile<ATR, BTR, 256, 256, 2, 4>;
 template <bool ATR, bool BTR>
+using Trimmed = Tile<ATR, BTR, 192, 256, 2, 4>;  // products' rows of 576 or 896 columns, say
+template <bool ATR, bool BTR>
 using Medium = Tile<ATR, BTR, 128, 128, 2, 2>;
 template <bool ATR, bool BTR>
 using Narrow = Tile<ATR, BTR, 256, 32, 8, 1>;
-enum Shape { kLarge, kMedium, kNarrow };
+enum Shape { kLarge, kTrimmed, kMedium, kNarrow };
 
 constexpr uint32_t kCus = 256;
 
@@ -653,10 +655,13 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
   // Shares of dx's contraction about as long as dW's, so that the launch's blocks are alike, and
   // shorter ones where the GPU would not be full; each share has sums of its own.
   p.products = p.scores;
-  const uint32_t tm = p.products == kMedium ? 128 : 256, tn = p.products == kNarrow ? 32 : tm;
+  if (p.products == kLarge && cdiv(p.dp, 192) * 192 < cdiv(p.dp, 256) * 256)
+    p.products = kTrimmed;  // fewer columns past the end
+  const uint32_t tn = p.products == kNarrow ? 32 : p.products == kMedium ? 128 : 256;
+  const uint32_t tm = p.products == kTrimmed ? 192 : p.products == kMedium ? 128 : 256;
   const uint32_t k_dx = p.piece / BK, k_dw = p.rows_pad / BK;
   const uint32_t dx_tiles = cdiv(p.dp, tm) * cdiv(a->rows, tn);
-  const uint32_t dw_tiles = cdiv(p.dp, tm) * cdiv(p.piece, tm);
+  const uint32_t dw_tiles = cdiv(p.dp, tm) * cdiv(p.piece, p.products == kMedium ? 128 : 256);
   p.splits = k_dw ? min(max((k_dx + k_dw / 2) / k_dw, 1u), 16u) : 1;
   while (p.splits < 16 && dx_tiles * p.splits + dw_tiles < 2 * kCus && k_dx / p.splits > 8)
     p.splits++;
@@ -745,13 +750,14 @@ int forward(const pots_vocab_loss* a, char* work, hipStream_t s) {
   return POTS_E_OK;
 }
 
-template <class T, template <bool, bool> class S, template <bool, bool> class SW>
+template <class T, template <bool, bool> class S, template <bool, bool> class SX,
+          template <bool, bool> class SW>
 int piece_grads(const pots_vocab_loss* a, const Plan& p, const Mat& W, const Mat& X, uint32_t v0,
                 uint32_t nv, char* work, hipStream_t s) {
   auto f32 = [&](uint64_t at) { return reinterpret_cast<float*>(work + at); };
   const uint32_t* count = reinterpret_cast<const uint32_t*>(work + p.count);
   typedef S<false, false> C;
-  typedef S<true, false> CX;
+  typedef SX<true, false> CX;
   typedef SW<true, true> CW;
   uint16_t* g = reinterpret_cast<uint16_t*>(work + p.g);
   const Mat G = {g, (int64_t)p.piece, (int64_t)p.rows_pad * p.piece};
@@ -795,9 +801,13 @@ int backward(const pots_vocab_loss* a, char* work, hipStream_t s) {
     Mat W = {};
     int rc = a->rows ? piece_of_w<T>(a, p, work, v0, nv, &W, s) : POTS_E_OK;
     if (rc) return rc;
-    rc = p.products == kLarge    ? piece_grads<T, Large, Large>(a, p, W, X, v0, nv, work, s)
-         : p.products == kMedium ? piece_grads<T, Medium, Medium>(a, p, W, X, v0, nv, work, s)
-                                 : piece_grads<T, Narrow, Large>(a, p, W, X, v0, nv, work, s);
+    rc = p.products == kLarge
+             ? piece_grads<T, Large, Large, Large>(a, p, W, X, v0, nv, work, s)
+         : p.products == kTrimmed
+             ? piece_grads<T, Large, Trimmed, Trimmed>(a, p, W, X, v0, nv, work, s)
+         : p.products == kMedium
+             ? piece_grads<T, Medium, Medium, Medium>(a, p, W, X, v0, nv, work, s)
+             : piece_grads<T, Narrow, Narrow, Large>(a, p, W, X, v0, nv, work, s);
     if (rc) return rc;
   }
   if (a->rows == 0) return POTS_E_OK;
