@@ -27,11 +27,15 @@ same computation.
 
 from __future__ import annotations
 
+import contextlib
+from collections.abc import Iterator
+
 import torch
 
-__all__ = ["ATTENTION", "register", "attention_forward"]
+__all__ = ["ATTENTION", "FUSED", "register", "attention_forward", "fused_forward", "fused"]
 
 ATTENTION = "pots_contiguous_bmm"
+FUSED = "pots_fused"
 
 
 def _check_right(b: torch.Tensor) -> None:
@@ -114,17 +118,49 @@ def attention_forward(module: torch.nn.Module, query: torch.Tensor, key: torch.T
     return out.view(b, h, n, d).transpose(1, 2).contiguous(), probs
 
 
+def fused_forward(module: torch.nn.Module, query: torch.Tensor, key: torch.Tensor,
+                  value: torch.Tensor, attention_mask: torch.Tensor | None, scaling: float,
+                  dropout: float = 0.0, **kwargs):
+    """The same attention for a pass that is not captured, without its probabilities
+    (``verification.computation.operators.attention``): causal, over whole sequences, so it
+    takes no mask. Returns ``(output [B, n, H, d_h], None)``."""
+    from verification.computation import operators
+    if dropout:
+        raise ValueError("attention dropout must be off: a step must be deterministic")
+    if attention_mask is not None:
+        raise ValueError("the uncaptured attention is causal over whole sequences: no mask")
+    dev = query.device.type
+    dt = torch.get_autocast_dtype(dev) if torch.is_autocast_enabled(dev) else query.dtype
+    out = operators.attention(query.to(dt), key.to(dt), value.to(dt), scale=scaling)
+    return out.transpose(1, 2), None
+
+
+@contextlib.contextmanager
+def fused(model: torch.nn.Module) -> Iterator[None]:
+    """``model`` with :func:`fused_forward` as its attention inside the block."""
+    register()
+    before = model.config._attn_implementation
+    model.config._attn_implementation = FUSED
+    try:
+        yield
+    finally:
+        model.config._attn_implementation = before
+
+
 _REGISTERED = False
 
 
 def register() -> str:
     """Register the core (and the eager causal mask it takes) with transformers under
-    :data:`ATTENTION`; idempotent. Returns the implementation name for a model config."""
+    :data:`ATTENTION`, and the uncaptured attention, which takes none, under :data:`FUSED`;
+    idempotent. Returns the core's name for a model config."""
     global _REGISTERED
     if not _REGISTERED:
         from transformers import AttentionInterface
         from transformers.masking_utils import AttentionMaskInterface, eager_mask
         AttentionInterface.register(ATTENTION, attention_forward)
         AttentionMaskInterface.register(ATTENTION, eager_mask)
+        AttentionInterface.register(FUSED, fused_forward)
+        AttentionMaskInterface.register(FUSED, lambda *args, **kwargs: None)
         _REGISTERED = True
     return ATTENTION

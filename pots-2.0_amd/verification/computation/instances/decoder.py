@@ -320,6 +320,25 @@ class DecoderComputation(DeclaredComputation):
             logits = model(input_ids=ids).logits
         return self._block_loss(logits, targets, mask, mask.sum())
 
+    def uncaptured_loss(self, model: torch.nn.Module, records) -> torch.Tensor:
+        """:meth:`loss` for a pass that leaves no transcript (a held-out batch, a step between
+        audits), on the GPU: the embedding, the attention and the loss run as the operators of
+        ``verification.computation.operators``, which keep no attention probability and no
+        logit, and the loss's backward recomputes the logits a piece of the vocabulary at a
+        time. The same mean over the masked tokens, and differentiable in the same weights; its
+        sums are taken in another order, so the bits are not the captured step's."""
+        from verification.computation import operators
+        from verification.computation.instances.attention import fused
+        dev = next(model.parameters()).device
+        ids, targets, mask = self._batch(records, dev)
+        with fused(model), self.autocast(dev):
+            rows = operators.embedding(ids, model.get_input_embeddings().weight)
+            f = model.model(inputs_embeds=rows).last_hidden_state
+        weights = mask.reshape(-1) / mask.sum()
+        return operators.vocab_loss(f.reshape(-1, self.d).to(self.compute_dtype),
+                                    model.get_output_embeddings().weight.to(self.compute_dtype),
+                                    targets.reshape(-1), weights)
+
     def forward_backward(self, model: torch.nn.Module, records, stage) -> torch.Tensor:
         """One training pass. With one head block, the loss over the whole batch and its
         backward. With ``B = head_blocks`` blocks (reference decoder.py:740-770): the features
