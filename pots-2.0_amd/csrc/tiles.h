@@ -88,10 +88,17 @@ __device__ __forceinline__ void load_lds4(brsrc rsrc, void* lds, uint32_t off) {
 #endif
 }
 
-// Waits for the wave's own loads into LDS, then for the block: a stage is complete after it.
+// Waits until at most LEFT of the wave's own loads (the last ones) are on their way, then for the
+// block: the stages loaded before those are complete after it.
+template <uint32_t LEFT = 0>
 __device__ __forceinline__ void loads_done() {
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  __syncthreads();
+  static_assert(LEFT < 64, "vmcnt has six bits");
+  // (a barrier of its own, since __syncthreads waits for every load into LDS; the empty statements
+  // keep the compiler from moving accesses over it)
+  __builtin_amdgcn_s_waitcnt(0x0070 | (LEFT & 15) | (LEFT >> 4) << 14);  // vmcnt(LEFT) lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // Element types of the operators' tensors.

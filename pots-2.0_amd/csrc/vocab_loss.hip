@@ -53,6 +53,7 @@ __device__ __forceinline__ void pair_of(uint32_t pairs, uint32_t t, uint32_t* pa
 template <bool TR, uint32_t T, uint32_t NT>
 struct Stage {
   static constexpr uint32_t kAll = T * BK / 8, kChunks = (kAll + NT - 1) / NT;
+  static_assert(kAll % 64 == 0 && (kAll % NT == 0 || NT % kAll == 0), "whole waves' loads");
   static_assert(!TR || (T % 64 == 0 && T > 64), "the exchange stays within a transposed row");
   uint32_t off[kChunks], wide;
 
@@ -67,7 +68,8 @@ struct Stage {
     wide = 2 * min(T, rows - r0);
 #pragma unroll
     for (uint32_t u = 0; u < kChunks; u++) {
-      const uint32_t c = u * NT + threadIdx.x;
+      // (a tile of less than a load for each wave is loaded by several, so that all wait alike)
+      const uint32_t c = (u * NT + threadIdx.x) % kAll;
       if constexpr (TR) {
         const uint32_t r = c / (T / 8), at = (c % (T / 8)) ^ swap(r);
         off[u] = 2 * (r * (uint32_t)m.ld + min(r0 + 8 * at, rows - 8) - r0);
@@ -78,19 +80,19 @@ struct Stage {
     }
   }
 
-  // The stage of contraction k0 .. k0 + BK; for TR, zero from `ks` on.
+  // The stage of contraction k0 .. k0 + BK; for TR, zero from `ks` on. Not `on`: zeros, and no
+  // memory is read.
   __device__ __forceinline__ void load(uint16_t* lds, const Mat& m, uint32_t plane, uint32_t r0,
-                                       uint32_t k0, uint32_t ks) const {
+                                       uint32_t k0, uint32_t ks, bool on) const {
     const uint16_t* base = m.p + (int64_t)plane * m.plane +
                            (TR ? (int64_t)k0 * m.ld + r0 : (int64_t)r0 * m.ld + k0);
     const uint32_t range =
         TR ? (min(BK, ks - k0) - 1) * (uint32_t)m.ld * 2 + wide : 0x7FFFFFFF;
-    const brsrc rsrc = make_rsrc(base, range);
+    const brsrc rsrc = make_rsrc(base, on ? range : 0);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 #pragma unroll
     for (uint32_t u = 0; u < kChunks; u++)
-      if (kAll % NT == 0 || u * NT + wave * 64 < kAll)
-        load_lds16(rsrc, lds + (u * NT + wave * 64) * 8, off[u]);
+      load_lds16(rsrc, lds + (u * NT + wave * 64) % kAll * 8, off[u]);
   }
 
   // Rows c .. c + 31 at step ks of the stage: contraction 16ks + 8h + (0..7).
@@ -118,7 +120,9 @@ __device__ __forceinline__ uint16_t* lds_buffer() {
 }
 
 // A block's TM x TN of A·Bᵀ over K (a multiple of BK), WM x WN waves of MB x NB products of 32.
-template <bool ATR, bool BTR, uint32_t TM_, uint32_t TN_, uint32_t WM_, uint32_t WN_>
+// NBUF stages in LDS: NBUF - 1 are on their way while one is multiplied.
+template <bool ATR, bool BTR, uint32_t TM_, uint32_t TN_, uint32_t WM_, uint32_t WN_,
+          uint32_t NBUF>
 struct Tile {
   static constexpr uint32_t TM = TM_, TN = TN_, WM = WM_, WN = WN_, NT = 64 * WM * WN;
   static constexpr uint32_t MB = TM / WM / 32, NB = TN / WN / 32;
@@ -146,10 +150,12 @@ struct Tile {
   __device__ __forceinline__ void run(const Mat& A, const Mat& B, uint32_t m0, uint32_t M,
                                       uint32_t n0, uint32_t N, uint32_t k0, uint32_t K,
                                       uint32_t ka, uint32_t kb, uint32_t pairs) {
-    uint16_t* const s_a0 = lds_buffer<0, TM * BK>();
-    uint16_t* const s_a1 = lds_buffer<1, TM * BK>();
-    uint16_t* const s_b0 = lds_buffer<2, TN * BK>();
-    uint16_t* const s_b1 = lds_buffer<3, TN * BK>();
+    uint16_t* const s_a[4] = {lds_buffer<0, TM * BK>(), lds_buffer<1, TM * BK>(),
+                              lds_buffer<NBUF == 4 ? 2 : 0, TM * BK>(),
+                              lds_buffer<NBUF == 4 ? 3 : 1, TM * BK>()};
+    uint16_t* const s_b[4] = {lds_buffer<4, TN * BK>(), lds_buffer<5, TN * BK>(),
+                              lds_buffer<NBUF == 4 ? 6 : 4, TN * BK>(),
+                              lds_buffer<NBUF == 4 ? 7 : 5, TN * BK>()};
     lane = threadIdx.x % 64;
     wm = threadIdx.x / 64 / WN * (TM / WM);
     wn = threadIdx.x / 64 % WN * (TN / WN);
@@ -158,39 +164,39 @@ struct Tile {
 #pragma unroll
       for (uint32_t n = 0; n < NB; n++) acc[m][n] = zero16();
     const uint32_t steps = K / BK * pairs;
-    uint32_t k = k0, pair = 0;
+    uint32_t k = k0, pair = 0, ahead = 0;
     SA sa;
     SB sb;
     sa.init(A, m0, M);
     sb.init(B, n0, N);
-    auto load = [&](uint16_t* a, uint16_t* b) {
+    auto load = [&](uint32_t j) {  // the next stage; past the last, nothing
+      const bool on = ahead < steps;
       uint32_t pa, pb;
-      pair_of(pairs, pair, &pa, &pb);
-      sa.load(a, A, pa, m0, k, ka);
-      sb.load(b, B, pb, n0, k, kb);
+      pair_of(pairs, on ? pair : 0, &pa, &pb);
+      sa.load(s_a[j], A, pa, m0, k, ka, on);
+      sb.load(s_b[j], B, pb, n0, k, kb, on);
+      ahead++;
       k += BK;
       if (k == k0 + K) {
         k = k0;
         pair++;
       }
     };
-    if (steps) load(s_a0, s_b0);
-    uint32_t t = 0;
-    for (; t + 2 <= steps; t += 2) {  // the next stage is on its way while one is multiplied
-      loads_done();
-      load(s_a1, s_b1);
-      step(s_a0, s_b0);
-      loads_done();
-      if (t + 2 < steps) load(s_a0, s_b0);
-      step(s_a1, s_b1);
+#pragma unroll
+    for (uint32_t j = 0; j + 1 < NBUF; j++) load(j);
+    constexpr uint32_t kLeft = (NBUF - 2) * (SA::kChunks + SB::kChunks);  // of later stages
+    for (uint32_t t = 0; t < steps; t += NBUF) {
+#pragma unroll
+      for (uint32_t j = 0; j < NBUF; j++) {
+        loads_done<kLeft>();
+        load((j + NBUF - 1) % NBUF);
+        if (t + j < steps) step(s_a[j], s_b[j]);
+      }
     }
-    if (t < steps) {
-      loads_done();
-      step(s_a0, s_b0);
-    }
+    loads_done();
   }
 
-  // A part of A's stages for each wave to itself, once the block has passed a barrier after run().
+  // A part of A's stages for each wave to itself, after run().
   static constexpr uint32_t kScratch = TM * BK * 2 / (WM_ * WN_);  // values
   __device__ __forceinline__ uint16_t* scratch() const {
     constexpr uint32_t half = WM * WN / 2;
@@ -446,7 +452,6 @@ __global__ __launch_bounds__(C::NT) void loss_grad(Mat W, Mat X, uint32_t v0, ui
   static_assert(CW * 8 * 32 <= C::kScratch, "a wave's 32 rows fit");
   uint16_t* const s = c.scratch();
   const uint32_t i = c.lane % 32, h = c.lane / 32;
-  __syncthreads();  // the last stage has been read
 #pragma unroll
   for (uint32_t b = 0; b < C::NB; b++) {
     const uint32_t row = n0 + c.wn + 32 * b + i;
@@ -502,13 +507,15 @@ __global__ __launch_bounds__(C::NT) void loss_grad(Mat W, Mat X, uint32_t v0, ui
 // Both products of a piece of G in one launch, so that the tiles of one fill the GPU's places
 // beside the other's. Blocks below mt·nt·splits: a share of dx, Wᵀ (stored along the
 // contraction, the piece's vocabulary) by G, added to the split's sums [rows][dp]. The others:
-// the piece's rows of dW, Xᵀ by Gᵀ, both stored along the contraction (the live rows).
+// the piece's rows of dW, Xᵀ by Gᵀ, both stored along the contraction (the live rows), or a
+// share of their contraction to sums of its own where there are few tiles.
 template <class T, class CX, class CW>
 __global__ __launch_bounds__(CX::NT) void loss_products(
     Mat W, Mat X, Mat G, uint32_t dp, uint32_t nv, const uint32_t* __restrict__ count,
     const float* __restrict__ unit, uint32_t pairs, uint32_t mt, uint32_t splits,
     uint32_t per, float* __restrict__ sums, uint64_t slice, bool first, uint32_t wmt,
-    uint32_t wnt, uint32_t d, typename T::elem* __restrict__ dw, int64_t ld, bool vec) {
+    uint32_t wnt, uint32_t wsplits, uint32_t wper, float* __restrict__ wsums, uint64_t wslice,
+    uint32_t d, typename T::elem* __restrict__ dw, int64_t ld, bool vec) {
   // (the tiles of the live rows alone, dealt over all XCDs; the launch has room for every row)
   const uint32_t live = gload<uint32_t>(count), nt = (live + CX::TN - 1) / CX::TN;
   uint32_t m, n;
@@ -533,11 +540,26 @@ __global__ __launch_bounds__(CX::NT) void loss_products(
     });
     return;
   }
-  if (blockIdx.x >= mt * nt * splits + wmt * wnt) return;
-  tile_of(blockIdx.x - mt * nt * splits, wmt, wnt, &m, &n);
-  const uint32_t m0 = m * CW::TM, n0 = n * CW::TN, K = (live + BK - 1) / BK * BK;
+  const uint32_t unit_w = blockIdx.x - mt * nt * splits;
+  if (unit_w >= wmt * wnt * wsplits) return;
+  tile_of(unit_w % (wmt * wnt), wmt, wnt, &m, &n);
+  const uint32_t m0 = m * CW::TM, n0 = n * CW::TN, all = (live + BK - 1) / BK * BK;
+  const uint32_t wsplit = unit_w / (wmt * wnt), k0 = wsplit * wper;
   CW c;
-  c.run(X, G, m0, dp, n0, (nv + 7) & ~7u, 0, K, live, live, pairs);
+  c.run(X, G, m0, dp, n0, (nv + 7) & ~7u, k0, k0 < all ? min(wper, all - k0) : 0, live, live,
+        pairs);
+  if (wsplits > 1) {
+    float* out = wsums + wsplit * wslice;
+    c.each(m0, n0, [&](f32x16& s, uint32_t col, uint32_t v) {
+      if (v >= nv) return;
+#pragma unroll
+      for (uint32_t q = 0; q < 4; q++) {
+        const f32x4 y = {s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+        if (col + 8 * q < dp) *reinterpret_cast<f32x4*>(out + (uint64_t)v * dp + col + 8 * q) = y;
+      }
+    });
+    return;
+  }
   const float mul = *unit;
   c.each(m0, n0, [&](f32x16& s, uint32_t col, uint32_t v) {
     if (v >= nv) return;
@@ -558,16 +580,17 @@ __global__ __launch_bounds__(CX::NT) void loss_products(
   });
 }
 
-// dx from the splits' sums: a block a row, zero for the rows left out.
+// Rows of dx or dW from the shares' sums, a block a row: row pos[r] of them (r without pos), zero
+// for the rows left out.
 template <class T>
-__global__ __launch_bounds__(256) void loss_dx_rows(const float* __restrict__ sums, uint32_t dp,
-                                                    uint32_t splits, uint64_t slice,
-                                                    const uint32_t* __restrict__ pos,
-                                                    const float* __restrict__ unit, uint32_t d,
-                                                    typename T::elem* dx, int64_t ld) {
-  const uint32_t row = blockIdx.x, at = pos[row];
+__global__ __launch_bounds__(256) void loss_join(const float* __restrict__ sums, uint32_t dp,
+                                                 uint32_t splits, uint64_t slice,
+                                                 const uint32_t* __restrict__ pos,
+                                                 const float* __restrict__ unit, uint32_t d,
+                                                 typename T::elem* out, int64_t ld) {
+  const uint32_t row = blockIdx.x, at = pos ? pos[row] : row;
   const float mul = *unit;
-  typename T::elem* out = dx + (int64_t)row * ld;
+  out += (int64_t)row * ld;
   for (uint32_t c = threadIdx.x * 4; c < d; c += 1024) {
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
     if (at != ~0u)
@@ -585,13 +608,15 @@ namespace {
 // them for the GPU; up to 32 rows the product is bound by reading W, and a tile as narrow as
 // the rows leaves its multiplications out of the way.
 template <bool ATR, bool BTR>
-using Large = Tile<ATR, BTR, 256, 256, 2, 4>;
+using Large = Tile<ATR, BTR, 256, 256, 2, 4, 2>;
 template <bool ATR, bool BTR>
-using Trimmed = Tile<ATR, BTR, 192, 256, 2, 4>;  // products' rows of 576 or 896 columns, say
+using Trimmed = Tile<ATR, BTR, 192, 256, 2, 4, 2>;  // products' rows of 576 or 896 columns, say
 template <bool ATR, bool BTR>
-using Medium = Tile<ATR, BTR, 128, 128, 2, 2>;
+using Medium = Tile<ATR, BTR, 128, 128, 2, 2, 2>;
 template <bool ATR, bool BTR>
-using Narrow = Tile<ATR, BTR, 256, 32, 8, 1>;
+using Narrow = Tile<ATR, BTR, 256, 32, 8, 1, 4>;
+template <bool ATR, bool BTR>
+using NarrowX = Tile<ATR, BTR, 256, 32, 8, 1, 2>;  // beside Large in one kernel's LDS
 enum Shape { kLarge, kTrimmed, kMedium, kNarrow };
 
 constexpr uint32_t kCus = 256;
@@ -607,9 +632,9 @@ Shape scores_shape(uint32_t rows, uint32_t piece) {
 struct Plan {
   uint32_t dp, terms, pairs, rows_pad, piece;
   Shape scores, products;
-  uint32_t splits, per;  // of dx's contraction
+  uint32_t splits, per, wsplits, wper;  // shares of dx's and of dW's contractions
   bool copy_w, copy_x;
-  uint64_t w, x, part, hit, idx, pos, count, unit, weight, lse2, target, g, sums, bytes;
+  uint64_t w, x, part, hit, idx, pos, count, unit, weight, lse2, target, g, sums, wsums, bytes;
 };
 
 uint64_t take(Plan* p, uint64_t bytes) {
@@ -659,15 +684,25 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
     p.products = kTrimmed;  // fewer columns past the end
   const uint32_t tn = p.products == kNarrow ? 32 : p.products == kMedium ? 128 : 256;
   const uint32_t tm = p.products == kTrimmed ? 192 : p.products == kMedium ? 128 : 256;
-  const uint32_t k_dx = p.piece / BK, k_dw = p.rows_pad / BK;
+  const uint32_t k_dx = p.piece / BK, k_dw = cdiv(a->rows, BK);
+  const uint32_t most_splits = p.products == kNarrow ? 64 : 16;
   const uint32_t dx_tiles = cdiv(p.dp, tm) * cdiv(a->rows, tn);
   const uint32_t dw_tiles = cdiv(p.dp, tm) * cdiv(p.piece, p.products == kMedium ? 128 : 256);
   p.splits = k_dw ? min(max((k_dx + k_dw / 2) / k_dw, 1u), 16u) : 1;
-  while (p.splits < 16 && dx_tiles * p.splits + dw_tiles < 2 * kCus && k_dx / p.splits > 8)
+  while (p.splits < most_splits && dx_tiles * p.splits + dw_tiles < 2 * kCus &&
+         k_dx * p.pairs / p.splits > 8)
     p.splits++;
   p.per = cdiv(k_dx, p.splits) * BK;
   p.splits = cdiv(p.piece, p.per);
   p.sums = take(&p, 4ull * p.splits * p.rows_pad * p.dp);
+  // dW's contraction in shares too, where its few tiles would be the launch's long end
+  p.wsplits = 1;
+  while (p.wsplits < 16 && dx_tiles * p.splits + dw_tiles * p.wsplits < kCus &&
+         k_dw * p.pairs / p.wsplits > 8)
+    p.wsplits *= 2;
+  p.wper = cdiv(max(k_dw, 1u), p.wsplits) * BK;
+  p.wsplits = max(cdiv(p.rows_pad, p.wper), 1u);
+  if (p.wsplits > 1) p.wsums = take(&p, 4ull * p.wsplits * p.piece * p.dp);
   return p;
 }
 
@@ -769,15 +804,21 @@ int piece_grads(const pots_vocab_loss* a, const Plan& p, const Mat& W, const Mat
     POTS_HIP(hipGetLastError());
   }
   typedef typename T::elem elem;
+  elem* const dw = reinterpret_cast<elem*>(a->dw) + (int64_t)v0 * a->dw_row;
   const bool vec = a->dim % 4 == 0 && a->dw_row % 4 == 0 &&
                    reinterpret_cast<uint64_t>(a->dw) % (4 * sizeof(elem)) == 0;
   const uint32_t xmt = cdiv(p.dp, CX::TM), wmt = cdiv(p.dp, CW::TM), wnt = cdiv(nv, CW::TN);
-  hipLaunchKernelGGL((loss_products<T, CX, CW>), dim3(xmt * nt * p.splits + wmt * wnt),
+  hipLaunchKernelGGL((loss_products<T, CX, CW>), dim3(xmt * nt * p.splits + wmt * wnt * p.wsplits),
                      dim3(CX::NT), 0, s, W, X, G, p.dp, nv, count, f32(p.unit), p.pairs, xmt,
                      p.splits, p.per, f32(p.sums), (uint64_t)p.rows_pad * p.dp, v0 == 0, wmt,
-                     wnt, a->dim, reinterpret_cast<elem*>(a->dw) + (int64_t)v0 * a->dw_row,
+                     wnt, p.wsplits, p.wper, f32(p.wsums), (uint64_t)p.piece * p.dp, a->dim, dw,
                      a->dw_row, vec);
   POTS_HIP(hipGetLastError());
+  if (p.wsplits > 1) {
+    hipLaunchKernelGGL((loss_join<T>), dim3(nv), dim3(256), 0, s, f32(p.wsums), p.dp, p.wsplits,
+                       (uint64_t)p.piece * p.dp, nullptr, f32(p.unit), a->dim, dw, a->dw_row);
+    POTS_HIP(hipGetLastError());
+  }
   return POTS_E_OK;
 }
 
@@ -807,11 +848,11 @@ int backward(const pots_vocab_loss* a, char* work, hipStream_t s) {
              ? piece_grads<T, Large, Trimmed, Trimmed>(a, p, W, X, v0, nv, work, s)
          : p.products == kMedium
              ? piece_grads<T, Medium, Medium, Medium>(a, p, W, X, v0, nv, work, s)
-             : piece_grads<T, Narrow, Narrow, Large>(a, p, W, X, v0, nv, work, s);
+             : piece_grads<T, Narrow, NarrowX, Large>(a, p, W, X, v0, nv, work, s);
     if (rc) return rc;
   }
   if (a->rows == 0) return POTS_E_OK;
-  hipLaunchKernelGGL((loss_dx_rows<T>), dim3(a->rows), dim3(256), 0, s, f32(p.sums), p.dp,
+  hipLaunchKernelGGL((loss_join<T>), dim3(a->rows), dim3(256), 0, s, f32(p.sums), p.dp,
                      p.splits, (uint64_t)p.rows_pad * p.dp, u32(p.pos), f32(p.unit), a->dim,
                      reinterpret_cast<typename T::elem*>(a->dx), a->dx_row);
   POTS_HIP(hipGetLastError());
