@@ -21,6 +21,7 @@
 
 namespace pots {
 
+constexpr uint32_t kFew = 256;                    // tokens that every block orders for itself
 constexpr uint32_t kOneRun = 16384, kRun = 2048;  // tokens of a single run; else of each run
 constexpr uint32_t kMerge = 32;    // runs a pass merges
 constexpr uint32_t kPiece = 16;    // sorted keys that a wave adds up, at the least
@@ -92,8 +93,8 @@ __global__ __launch_bounds__(256) void embed_rows(pots_embedding a, uint32_t cpr
 // only to the rows that no token has, each looked up in the sorted list by one lane.
 template <class T, uint32_t NT>
 __device__ __forceinline__ void fill_rows(const pots_embedding& a,
-                                          const uint64_t* __restrict__ keys, uint32_t r0,
-                                          uint32_t end, uint32_t cpr, bool vec) {
+                                          const uint64_t* keys, uint32_t r0, uint32_t end,
+                                          uint32_t cpr, bool vec) {
   __shared__ uint32_t s_has[kFill];
   const uint32_t n = r0 < end ? min(kFill, end - r0) : 0;
   if (threadIdx.x < n) {
@@ -202,18 +203,40 @@ __global__ __launch_bounds__(256) void embed_merge(const uint64_t* __restrict__ 
 // Below `sums` waves: one adds up one piece of the sorted list for 64 chunks of columns. part:
 // [piece][2][dim padded to chunks]: the sum of the row that an earlier piece began, and of the one
 // that goes on. The blocks after those write zeros to rows from `r0` to `end` that no token has.
-template <class T>
-__global__ __launch_bounds__(256) void embed_sum(pots_embedding a,
-                                                 const uint64_t* __restrict__ keys,
+// FEW: up to kFew tokens, whose order each block finds in its LDS (one launch less, 5 us); the
+// first leaves it in `keys` for embed_join.
+template <class T, bool FEW, bool ADD, bool VEC>
+__global__ __launch_bounds__(256) void embed_sum(pots_embedding a, uint64_t* __restrict__ list,
                                                  uint32_t piece, uint32_t groups, uint32_t sums,
                                                  uint32_t cpr, uint32_t r0, uint32_t end,
-                                                 float* __restrict__ part, bool vec) {
+                                                 float* __restrict__ part) {
   constexpr uint32_t P = kPer<T>;
   const typename T::elem* rows = reinterpret_cast<const typename T::elem*>(a.rows);
   typename T::elem* table = reinterpret_cast<typename T::elem*>(a.table);
   const uint32_t blocks = (sums + 3) / 4;
+  __shared__ uint64_t s_list[FEW ? kFew : 1];
+  if constexpr (FEW) {
+    __shared__ __attribute__((aligned(16))) uint32_t s_id[kFew];
+    const uint32_t t = threadIdx.x;
+    const int64_t own = t < a.tokens ? gload<int64_t>(a.ids + t) : -1;
+    const uint32_t id = own >= 0 && own < a.vocab ? (uint32_t)own : kNoRow;
+    s_id[t] = id;
+    __syncthreads();
+    uint32_t at = 0;
+    for (uint32_t j = 0; j < a.tokens; j += 4) {  // (what lies past the last token comes after it)
+      const u32x4v o = *reinterpret_cast<const u32x4v*>(s_id + j);
+#pragma unroll
+      for (uint32_t x = 0; x < 4; x++) at += o[x] < id || (o[x] == id && j + x < t);
+    }
+    if (t < a.tokens) {
+      s_list[at] = (uint64_t)id << 32 | t;
+      if (blockIdx.x == 0) list[at] = (uint64_t)id << 32 | t;
+    }
+    __syncthreads();
+  }
+  const uint64_t* const keys = FEW ? s_list : list;
   if (blockIdx.x >= blocks) {
-    fill_rows<T, 256>(a, keys, r0 + (blockIdx.x - blocks) * kFill, end, cpr, vec);
+    fill_rows<T, 256>(a, keys, r0 + (blockIdx.x - blocks) * kFill, end, cpr, VEC);
     return;
   }
   const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -221,6 +244,7 @@ __global__ __launch_bounds__(256) void embed_sum(pots_embedding a,
   const uint32_t b = unit / groups, ch = unit % groups * 64 + threadIdx.x % 64, c = ch * P;
   const uint32_t k0 = b * piece, k1 = min(k0 + piece, a.tokens);
   const bool on = ch < cpr;
+  const uint32_t cl = on ? c : 0;  // the columns that a lane without any loads
   float sum[P] = {};
   // a row that an earlier piece began does not start here
   bool begun = k0 > 0 && (uint32_t)(keys[k0 - 1] >> 32) == (uint32_t)(keys[k0] >> 32);
@@ -235,11 +259,12 @@ __global__ __launch_bounds__(256) void embed_sum(pots_embedding a,
       if (u < U) at[u] = id[u] == kNoRow ? 0 : (uint32_t)key;
     }
 #pragma unroll
-    for (uint32_t u = 0; u < U; u++) {
-      if (!on || id[u] == kNoRow) continue;
-      v[u] = load_chunk<T>(rows + (int64_t)at[u] * a.rows_row, c, a.dim, vec);
-      if (a.add && id[u + 1] != id[u])
-        old[u] = load_chunk<T>(table + (int64_t)id[u] * a.table_row, c, a.dim, vec);
+    for (uint32_t u = 0; u < U; u++) {  // (no branch between the loads: some are not used)
+      v[u] = load_chunk<T>(rows + (int64_t)at[u] * a.rows_row, cl, a.dim, VEC);
+      if (ADD) {
+        const uint32_t row = id[u] == kNoRow ? 0 : id[u];
+        old[u] = load_chunk<T>(table + (int64_t)row * a.table_row, cl, a.dim, VEC);
+      }
     }
 #pragma unroll
     for (uint32_t u = 0; u < U; u++) {
@@ -253,8 +278,8 @@ __global__ __launch_bounds__(256) void embed_sum(pots_embedding a,
           float y[P];
 #pragma unroll
           for (uint32_t j = 0; j < P; j++)
-            y[j] = a.add ? T::get(old[u][j]) + sum[j] * a.scale : sum[j] * a.scale;
-          put_chunk<T>(table + (int64_t)id[u] * a.table_row, c, a.dim, vec, y);
+            y[j] = ADD ? T::get(old[u][j]) + sum[j] * a.scale : sum[j] * a.scale;
+          put_chunk<T>(table + (int64_t)id[u] * a.table_row, c, a.dim, VEC, y);
         } else {
           float* p = part + ((uint64_t)b * 2 + (begun ? 0 : 1)) * cpr * P + c;
 #pragma unroll
@@ -371,6 +396,15 @@ int forward(const pots_embedding* a, hipStream_t s) {
 }
 
 template <class T>
+auto sum_kernel(bool few, bool add, bool vec) {
+  if (vec)
+    return few ? (add ? embed_sum<T, true, true, true> : embed_sum<T, true, false, true>)
+               : (add ? embed_sum<T, false, true, true> : embed_sum<T, false, false, true>);
+  return few ? (add ? embed_sum<T, true, true, false> : embed_sum<T, true, false, false>)
+             : (add ? embed_sum<T, false, true, false> : embed_sum<T, false, false, false>);
+}
+
+template <class T>
 int backward(const pots_embedding* a, char* work, hipStream_t s) {
   const Cut c = cut(a);
   const bool vec = chunked(a);
@@ -380,10 +414,11 @@ int backward(const pots_embedding* a, char* work, hipStream_t s) {
   // The zeros of a dense gradient: a share beside each of the three launches. Ordering and joining
   // are short chains of dependent steps that would leave the memory idle, about as long as a
   // twelfth of a large table takes to write.
-  const uint32_t r1 = a->add || !a->tokens ? 0 : a->vocab / 12;
+  const bool few = a->tokens <= kFew;
+  const uint32_t r1 = a->add || few ? 0 : a->vocab / 12;
   const uint32_t r2 = a->add ? 0 : c.pieces > 1 ? a->vocab - r1 : a->vocab;
   auto fills = [](uint32_t rows) { return (rows + kFill - 1) / kFill; };
-  if (a->tokens) {
+  if (!few) {
     hipLaunchKernelGGL((embed_order<T>), dim3(c.order + fills(r1)), dim3(1024), 0, s, *a, from,
                        c.run, c.order, r1, c.cpr, vec);
     POTS_HIP(hipGetLastError());
@@ -398,8 +433,9 @@ int backward(const pots_embedding* a, char* work, hipStream_t s) {
   }
   const uint32_t groups = (c.cpr + 63) / 64, sums = c.pieces * groups, blocks = (sums + 3) / 4;
   if (blocks + fills(r2 - r1)) {
-    hipLaunchKernelGGL((embed_sum<T>), dim3(blocks + fills(r2 - r1)), dim3(256), 0, s, *a, from,
-                       c.piece, groups, sums, c.cpr, r1, r2, part, vec);
+    const auto kernel = sum_kernel<T>(few, a->add, vec);
+    hipLaunchKernelGGL(kernel, dim3(blocks + fills(r2 - r1)), dim3(256), 0, s, *a, from, c.piece,
+                       groups, sums, c.cpr, r1, r2, part);
     POTS_HIP(hipGetLastError());
   }
   if (c.pieces > 1) {

@@ -170,6 +170,12 @@ class Native:
             fn.argtypes = args
             fn.restype = res
         self._lib = lib
+        # name: its entry point, and the one that says how much scratch it wants
+        self._operators = {
+            f"{op}_{way}": (getattr(lib, f"pots_{op}_{way}"),
+                            getattr(lib, f"pots_{op}_{way}_work", None)
+                            if f"pots_{op}_{way}_work" in sigs else None)
+            for op in ("attention", "vocab_loss", "embedding") for way in ("forward", "backward")}
         self.version = lib.pots_mi355x_version().decode()
         self.blake3_version = lib.pots_blake3_version().decode()
         self.simd_degree = int(lib.pots_simd_degree())
@@ -184,24 +190,26 @@ class Native:
         msg = self._lib.pots_last_error().decode()
         raise NativeError(f"{what} failed with {rc}: {msg}")
 
-    def operator(self, name: str, args: bytes, device: torch.device, *,
-                 work: bool = True) -> None:
-        """Enqueue ``pots_<name>(args, …)`` on ``device``'s current stream; with ``work``, with
-        the scratch that ``pots_<name>_work`` asks for, taken from torch's allocator on that
+    def operator(self, name: str, args: bytes, device: torch.device) -> None:
+        """Enqueue ``pots_<name>(args, …)`` on ``device``'s current stream, with the scratch that
+        ``pots_<name>_work`` asks for (where there is one) taken from torch's allocator on that
         stream."""
-        lib = self._lib
-        if device.index != torch.cuda.current_device():
+        index = device.index
+        if index != torch.cuda.current_device():
             with torch.cuda.device(device):
-                return self.operator(name, args, device, work=work)
+                return self.operator(name, args, device)
         # (torch.cuda.current_stream's Stream object costs more than a launch's own host time)
-        stream = torch._C._cuda_getCurrentRawStream(device.index)
-        if not work:
-            rc = getattr(lib, "pots_" + name)(args, stream)
+        stream = torch._C._cuda_getCurrentRawStream(index)
+        run, work = self._operators[name]
+        if work is None:
+            rc = run(args, stream)
         else:
-            nbytes = getattr(lib, f"pots_{name}_work")(args)
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-            rc = getattr(lib, "pots_" + name)(args, None if scratch is None
-                                              else scratch.data_ptr(), stream)
+            nbytes = work(args)
+            if nbytes:
+                scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                rc = run(args, scratch.data_ptr(), stream)
+            else:
+                rc = run(args, None, stream)
         if rc != E_OK:
             self._check(rc, "pots_" + name)
 

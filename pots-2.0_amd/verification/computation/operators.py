@@ -77,7 +77,9 @@ def _floats(t: torch.Tensor, device: torch.device, shape: tuple[int, ...],
 def _indices(t: torch.Tensor, device: torch.device, what: str) -> torch.Tensor:
     if t.dtype not in (torch.int64, torch.int32) or t.device != device:
         raise ValueError(f"{what} must be int64 or int32 on {device}")
-    return t.to(torch.int64).contiguous()
+    if t.dtype != torch.int64:
+        t = t.to(torch.int64)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 # ---- attention ------------------------------------------------------------------------------
@@ -146,7 +148,7 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                            *_NO_HEADS, *_NO_HEADS, *_NO_HEADS, lse.data_ptr(),
                            0 if lengths is None else lengths.data_ptr(), b, h, k.shape[1], n, d,
                            code, causal, scale)
-    native.get().operator("attention_forward", args, q.device, work=False)
+    native.get().operator("attention_forward", args, q.device)
     return out, lse
 
 
@@ -297,7 +299,7 @@ def embedding_forward(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 
     args = _EMBEDDING.pack(ids.data_ptr(), table.data_ptr(), out.data_ptr(), table.stride(0),
                            table.shape[1], ids.numel(), table.shape[1], table.shape[0], code, 0,
                            scale)
-    native.get().operator("embedding_forward", args, table.device, work=False)
+    native.get().operator("embedding_forward", args, table.device)
     return out
 
 
