@@ -422,14 +422,16 @@ int pots_store_load(uint32_t n_files, const char *const *paths, uint32_t n_segs,
 #define POTS_ATTENTION_MAX_DIM 128
 
 /* One operand [batch, heads, n, head_dim]: elements between batches, heads and positions (a
- * position's values are consecutive). */
+ * position's values are consecutive). The pointer and every stride are multiples of 16 bytes, and
+ * `row` is less than 2^22. */
 typedef struct pots_heads {
   void *ptr;
   int64_t batch, head, row;
 } pots_heads;
 
 /* Softmax attention of `batch` sequences of n positions over their own keys: `heads` query
- * heads, each `heads / kv_heads` consecutive ones sharing a key head. Position i sees j where
+ * heads, each `heads / kv_heads` consecutive ones sharing a key head, of a head_dim that is a
+ * multiple of 8 (a narrower head is one with columns of zeros). Position i sees j where
  * j < length, i < length and (causal) j <= i; lengths is int32 [batch] (values past n count as
  * n, negative ones as 0), or null for n. A position that sees nothing has an output of zero,
  * lse -inf and gradients of zero; what lies past a sequence's length is not read. lse and delta

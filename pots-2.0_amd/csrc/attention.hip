@@ -33,42 +33,22 @@ namespace pots {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Sixteen bytes of row r (zero from `rows` on) from column c on (zero from `d` on). vec: rows
-// are 16-byte aligned and d is a multiple of a chunk.
-template <class T>
-__device__ __forceinline__ u32x4v load_chunk(const typename T::elem* base, int64_t stride,
-                                             uint32_t r, uint32_t rows, uint32_t c, uint32_t d,
-                                             bool vec) {
-  constexpr uint32_t CE = 16 / sizeof(typename T::elem);
-  u32x4v x = {0, 0, 0, 0};
-  if (r >= rows || c >= d) return x;
-  const typename T::elem* p = base + (int64_t)r * stride + c;
-  if (vec) return gload<u32x4v>(p);
-#pragma unroll
-  for (uint32_t j = 0; j < CE; j++) {
-    if (c + j >= d) continue;
-    if constexpr (sizeof(typename T::elem) == 2) {
-      const uint32_t e = gload<uint16_t>(p + j);
-      x[j / 2] |= e << (16 * (j % 2));
-    } else {
-      x[j] = gload<uint32_t>(p + j);
-    }
-  }
-  return x;
-}
-
+// Eight values of row r from column c on; zero for rows from `rows` and columns from `d` (a multiple
+// of eight) on.
 template <class T>
 __device__ __forceinline__ typename T::frag load_frag(const typename T::elem* base,
                                                       int64_t stride, uint32_t r, uint32_t rows,
-                                                      uint32_t c, uint32_t d, bool vec) {
-  if constexpr (sizeof(typename T::elem) == 2) {
-    return __builtin_bit_cast(bf16x8, load_chunk<T>(base, stride, r, rows, c, d, vec));
-  } else {
-    const f32x4 a = __builtin_bit_cast(f32x4, load_chunk<T>(base, stride, r, rows, c, d, vec));
-    const f32x4 b =
-        __builtin_bit_cast(f32x4, load_chunk<T>(base, stride, r, rows, c + 4, d, vec));
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+                                                      uint32_t c, uint32_t d) {
+  typename T::frag f = {};
+  if (r < rows && c < d) {
+    const typename T::elem* p = base + (int64_t)r * stride + c;
+    if constexpr (sizeof(typename T::elem) == 2) {
+      f = gload<bf16x8>(p);
+    } else {
+      f = __builtin_shufflevector(gload<f32x4>(p), gload<f32x4>(p + 4), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
   }
+  return f;
 }
 
 // A tile of KT rows of DP columns in LDS, in 16-byte chunks, each exchanged within its row by
@@ -96,26 +76,17 @@ struct Rows {
     }
   }
 
-  // Rows r0 .. r0 + KT; those past `rows` and the columns past d are zero. vec: straight into LDS,
-  // complete once the wave has waited for its loads; else through registers.
+  // Rows r0 .. r0 + KT, straight into LDS (complete once the wave has waited for its loads); those
+  // past `rows` and the columns past d are zero.
   __device__ __forceinline__ void load(elem* tile, const elem* base, int64_t stride, uint32_t r0,
-                                       uint32_t rows, uint32_t d, bool vec) const {
+                                       uint32_t rows, uint32_t d) const {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    if (vec) {
-      const uint32_t range = ((min(KT, rows - r0) - 1) * (uint32_t)stride + d) * sizeof(elem);
-      const brsrc rsrc = make_rsrc(base + (int64_t)r0 * stride, range);
+    const uint32_t range = ((min(KT, rows - r0) - 1) * (uint32_t)stride + d) * sizeof(elem);
+    const brsrc rsrc = make_rsrc(base + (int64_t)r0 * stride, range);
 #pragma unroll
-      for (uint32_t u = 0; u < kChunks; u++)
-        if (kAll % NT == 0 || u * NT + wave * 64 < kAll)
-          load_lds16(rsrc, tile + (u * NT + wave * 64) * CE, off[u]);
-    } else {
-#pragma unroll 1
-      for (uint32_t c = threadIdx.x; c < kAll; c += NT) {
-        const uint32_t r = c / CPR, col = ((c % CPR) ^ swap(r)) * CE;
-        *reinterpret_cast<u32x4v*>(tile + c * CE) =
-            load_chunk<T>(base, stride, r0 + r, rows, col, d, false);
-      }
-    }
+    for (uint32_t u = 0; u < kChunks; u++)
+      if (kAll % NT == 0 || u * NT + wave * 64 < kAll)
+        load_lds16(rsrc, tile + (u * NT + wave * 64) * CE, off[u]);
   }
 
   // Eight values of row r from column c on.
@@ -174,8 +145,8 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32);
 template <class T, uint32_t NB>
 __device__ __forceinline__ void store_rows(const pots_heads& x, uint32_t b, uint32_t head,
                                            uint32_t row, uint32_t n, uint32_t d,
-                                           const f32x16 (&acc)[NB], float mul, bool vec,
-                                           uint32_t h, uint32_t step = 1, uint32_t mine = 0) {
+                                           const f32x16 (&acc)[NB], float mul, uint32_t h,
+                                           uint32_t step = 1, uint32_t mine = 0) {
   if (row >= n) return;
   typename T::elem* p = reinterpret_cast<typename T::elem*>(x.ptr) + b * x.batch +
                         head * x.head + (int64_t)row * x.row;
@@ -187,14 +158,8 @@ __device__ __forceinline__ void store_rows(const pots_heads& x, uint32_t b, uint
       const uint32_t c = 32 * db + 8 * g + 4 * h;
       if (c >= d) continue;
       const f32x16& v = acc[db];
-      if (vec) {
-        T::store4(p + c, v[4 * g] * mul, v[4 * g + 1] * mul, v[4 * g + 2] * mul,
-                  v[4 * g + 3] * mul);
-      } else {
-#pragma unroll
-        for (uint32_t e = 0; e < 4; e++)
-          if (c + e < d) p[c + e] = T::put(v[4 * g + e] * mul);
-      }
+      T::store4(p + c, v[4 * g] * mul, v[4 * g + 1] * mul, v[4 * g + 2] * mul,
+                v[4 * g + 3] * mul);
     }
   }
 }
@@ -261,7 +226,7 @@ __device__ __forceinline__ void join_sums(f32x16 (&acc)[NB], L lds, uint32_t at,
 template <class T, uint32_t DP, bool SPLIT>
 __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
                              (!SPLIT && Shape<T, DP, SPLIT>::kWide <= 256 ? 2 : 1)) void attn_fwd(
-    pots_attention a, uint32_t tiles, bool vec, bool vec_out) {
+    pots_attention a, uint32_t tiles) {
   typedef typename T::elem elem;
   typedef typename T::frag frag;
   typedef Shape<T, DP, SPLIT> S;
@@ -285,14 +250,14 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
   rk.init(K.row, d);
   rv.init(V.row, d);
   auto load = [&](elem* k, elem* v, uint32_t k0) {
-    rk.load(k, K.p, K.row, k0, len, d, vec);
-    rv.load(v, V.p, V.row, k0, len, d, vec);
+    rk.load(k, K.p, K.row, k0, len, d);
+    rv.load(v, V.p, V.row, k0, len, d);
   };
   if (end) load(s_k0, s_v0, 0);
   frag qf[KS];
 #pragma unroll
   for (uint32_t ks = 0; ks < KS; ks++)
-    qf[ks] = load_frag<T>(Q.p, Q.row, q, len, 16 * ks + 8 * h, d, vec);
+    qf[ks] = load_frag<T>(Q.p, Q.row, q, len, 16 * ks + 8 * h, d);
   f32x16 o[NB];
 #pragma unroll
   for (uint32_t db = 0; db < NB; db++) o[db] = zero16();
@@ -390,7 +355,7 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
     mc = top == -INFINITY ? 0.f : top;
     join_sums<NB, NW>(o, lds, 0, wave, lane);
   }
-  store_rows<T, NB>(a.out, b, head, q, a.n, d, o, l > 0.f || l != l ? 1.f / l : 0.f, vec_out, h,
+  store_rows<T, NB>(a.out, b, head, q, a.n, d, o, l > 0.f || l != l ? 1.f / l : 0.f, h,
                     SPLIT ? NW : 1, SPLIT ? wave : 0);
   if (h == 0 && q < a.n && (!SPLIT || wave == 0))
     a.lse[(int64_t)bh * a.n + q] =
@@ -403,7 +368,7 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
 template <class T, uint32_t DP, bool SPLIT>
 __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
                              (!SPLIT && Shape<T, DP, SPLIT>::kWide <= 256 ? 2 : 1)) void attn_dq(
-    pots_attention a, float* __restrict__ stat, uint32_t tiles, bool vec, bool vec_out) {
+    pots_attention a, float* __restrict__ stat, uint32_t tiles) {
   typedef typename T::elem elem;
   typedef typename T::frag frag;
   typedef Shape<T, DP, SPLIT> S;
@@ -427,17 +392,17 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
   rk.init(K.row, d);
   rv.init(V.row, d);
   auto load = [&](elem* k, elem* v, uint32_t k0) {
-    rk.load(k, K.p, K.row, k0, len, d, vec);
-    rv.load(v, V.p, V.row, k0, len, d, vec);
+    rk.load(k, K.p, K.row, k0, len, d);
+    rv.load(v, V.p, V.row, k0, len, d);
   };
   if (end) load(s_k0, s_v0, 0);
   frag qf[KS], gf[KS];
   float dl = 0.f;
 #pragma unroll
   for (uint32_t ks = 0; ks < KS; ks++) {
-    qf[ks] = load_frag<T>(Q.p, Q.row, q, len, 16 * ks + 8 * h, d, vec);
-    gf[ks] = load_frag<T>(G.p, G.row, q, len, 16 * ks + 8 * h, d, vec);
-    const frag of = load_frag<T>(O.p, O.row, q, len, 16 * ks + 8 * h, d, vec);
+    qf[ks] = load_frag<T>(Q.p, Q.row, q, len, 16 * ks + 8 * h, d);
+    gf[ks] = load_frag<T>(G.p, G.row, q, len, 16 * ks + 8 * h, d);
+    const frag of = load_frag<T>(O.p, O.row, q, len, 16 * ks + 8 * h, d);
 #pragma unroll
     for (int j = 0; j < 8; j++) dl = __builtin_fmaf(T::at(gf[ks], j), T::at(of, j), dl);
   }
@@ -508,7 +473,7 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
     __syncthreads();
     join_sums<NB, NW>(acc, lds, 0, wave, lane);
   }
-  store_rows<T, NB>(a.dq, b, head, q, a.n, d, acc, a.scale, vec_out, h, SPLIT ? NW : 1,
+  store_rows<T, NB>(a.dq, b, head, q, a.n, d, acc, a.scale, h, SPLIT ? NW : 1,
                     SPLIT ? wave : 0);
 }
 
@@ -520,7 +485,7 @@ template <class T, uint32_t DP, bool SPLIT>
 __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
                              (!SPLIT && Shape<T, DP, SPLIT>::kWide <= 128 ? 2 : 1)) void attn_dkv(
     pots_attention a, const float* __restrict__ stat, float* __restrict__ part, uint32_t tiles,
-    uint32_t splits, uint32_t per, bool vec, bool vec_out) {
+    uint32_t splits, uint32_t per) {
   typedef typename T::elem elem;
   typedef typename T::frag frag;
   typedef Shape<T, DP, SPLIT> S;
@@ -550,8 +515,8 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
   auto load = [&](elem* s_q, elem* s_g, float* s_stat) {
     const uint32_t head = kvh * rep + le;
     const Head<T> Q(a.q, b, head), G(a.dout, b, head);
-    rq.load(s_q, Q.p, Q.row, lq, len, d, vec);
-    rg.load(s_g, G.p, G.row, lq, len, d, vec);
+    rq.load(s_q, Q.p, Q.row, lq, len, d);
+    rg.load(s_g, G.p, G.row, lq, len, d);
     if (64 * wave < kStat) {  // lse and D of the tile's rows, 64 a wave; zero past the length
       const uint32_t q = lq + 64 * wave;
       const int64_t at = (int64_t)(b * a.heads + head) * a.n + q;
@@ -569,8 +534,8 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
   frag kf[KS], vf[KS];
 #pragma unroll
   for (uint32_t ks = 0; ks < KS; ks++) {
-    kf[ks] = load_frag<T>(K.p, K.row, key, len, 16 * ks + 8 * h, d, vec);
-    vf[ks] = load_frag<T>(V.p, V.row, key, len, 16 * ks + 8 * h, d, vec);
+    kf[ks] = load_frag<T>(K.p, K.row, key, len, 16 * ks + 8 * h, d);
+    vf[ks] = load_frag<T>(V.p, V.row, key, len, 16 * ks + 8 * h, d);
   }
   f32x16 dk[NB], dv[NB];
 #pragma unroll
@@ -653,12 +618,12 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
     x.head = (int64_t)a.n * d;
     x.batch = x.head * a.kv_heads;
     x.ptr = part + split * x.batch * a.batch;
-    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dk, a.scale, d % 4 == 0, h, kOf, mine);
+    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dk, a.scale, h, kOf, mine);
     x.ptr = part + (splits + split) * x.batch * a.batch;
-    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dv, 1.f, d % 4 == 0, h, kOf, mine);
+    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dv, 1.f, h, kOf, mine);
   } else {
-    store_rows<T, NB>(a.dk, b, kvh, key, a.n, d, dk, a.scale, vec_out, h, kOf, mine);
-    store_rows<T, NB>(a.dv, b, kvh, key, a.n, d, dv, 1.f, vec_out, h, kOf, mine);
+    store_rows<T, NB>(a.dk, b, kvh, key, a.n, d, dk, a.scale, h, kOf, mine);
+    store_rows<T, NB>(a.dv, b, kvh, key, a.n, d, dv, 1.f, h, kOf, mine);
   }
 }
 
@@ -666,33 +631,19 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
 template <class T>
 __global__ __launch_bounds__(256) void attn_fold(pots_attention a,
                                                  const float* __restrict__ part,
-                                                 uint32_t splits, bool vec_out) {
+                                                 uint32_t splits) {
   const uint64_t each = (uint64_t)a.batch * a.kv_heads * a.n * a.head_dim;
   const float* p = part + blockIdx.y * splits * each;
   const pots_heads& x = blockIdx.y ? a.dv : a.dk;
-  const uint64_t step = (uint64_t)gridDim.x * 1024;
-  for (uint64_t e = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4; e < each; e += step) {
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    const bool four = vec_out && a.head_dim % 4 == 0;  // then also of one row
-    for (uint32_t s = 0; s < splits; s++) {
-      if (four) {
-        sum += gload<f32x4>(p + s * each + e);
-      } else {
-        for (uint32_t j = 0; j < 4 && e + j < each; j++) sum[j] += p[s * each + e + j];
-      }
-    }
-    for (uint32_t j = 0; j < 4 && e + j < each; j += four ? 4 : 1) {
-      const uint64_t row = (e + j) / a.head_dim, bk = row / a.n;
-      const uint32_t col = (e + j) - row * a.head_dim;
-      typename T::elem* q = reinterpret_cast<typename T::elem*>(x.ptr) +
-                            (int64_t)(bk / a.kv_heads) * x.batch +
-                            (int64_t)(bk % a.kv_heads) * x.head +
-                            (int64_t)(row - bk * a.n) * x.row + col;
-      if (four)
-        T::store4(q, sum[0], sum[1], sum[2], sum[3]);
-      else
-        *q = T::put(sum[j]);
-    }
+  for (uint64_t e = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4; e < each;
+       e += (uint64_t)gridDim.x * 1024) {
+    f32x4 sum = gload<f32x4>(p + e);
+    for (uint32_t s = 1; s < splits; s++) sum += gload<f32x4>(p + s * each + e);
+    const uint64_t row = e / a.head_dim, bk = row / a.n;
+    T::store4(reinterpret_cast<typename T::elem*>(x.ptr) + (int64_t)(bk / a.kv_heads) * x.batch +
+                  (int64_t)(bk % a.kv_heads) * x.head + (int64_t)(row - bk * a.n) * x.row +
+                  (e - row * a.head_dim),
+              sum[0], sum[1], sum[2], sum[3]);
   }
 }
 
@@ -700,17 +651,17 @@ namespace {
 
 bool bad(const pots_attention* a) {
   return !a || a->dtype > POTS_OP_BF16 || a->kv_heads == 0 || a->heads == 0 ||
-         a->heads % a->kv_heads || a->head_dim == 0 || a->head_dim > POTS_ATTENTION_MAX_DIM ||
+         a->heads % a->kv_heads || a->head_dim == 0 || a->head_dim % 8 ||
+         a->head_dim > POTS_ATTENTION_MAX_DIM ||
          !(a->scale > 0.f) || !isfinite(a->scale) || a->n > 0x40000000u ||
          (uint64_t)a->batch * a->heads > 0x100000u;
 }
 
-// Whether x's rows start on multiples of `bytes`, and a tile of them spans less than 2 GiB.
-bool aligned(const pots_attention* a, const pots_heads& x, uint32_t bytes) {
+// Whether x's rows start on 16-byte borders, and a tile of them spans less than 2 GiB.
+bool aligned(const pots_attention* a, const pots_heads& x) {
   const int64_t e = a->dtype == POTS_OP_BF16 ? 2 : 4;
-  return reinterpret_cast<uint64_t>(x.ptr) % bytes == 0 && x.batch * e % bytes == 0 &&
-         x.head * e % bytes == 0 && x.row * e % bytes == 0 && a->head_dim * e % bytes == 0 &&
-         x.row >= 0 && x.row < (1 << 23);
+  return reinterpret_cast<uint64_t>(x.ptr) % 16 == 0 && x.batch * e % 16 == 0 &&
+         x.head * e % 16 == 0 && x.row * e % 16 == 0 && x.row >= 0 && x.row < (1 << 22);
 }
 
 uint32_t cdiv(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
@@ -752,9 +703,8 @@ int forward(const pots_attention* a, hipStream_t s) {
   const uint32_t tiles = cdiv(a->n, S::R);
   const uint64_t blocks = (uint64_t)a->batch * a->heads * tiles;
   if (blocks > 0x7FFFFFFFu) return POTS_E_ARG;
-  const bool vec = aligned(a, a->q, 16) && aligned(a, a->k, 16) && aligned(a, a->v, 16);
   hipLaunchKernelGGL((attn_fwd<T, DP, SPLIT>), dim3((uint32_t)blocks), dim3(S::NT), 0, s, *a,
-                     tiles, vec, aligned(a, a->out, 4 * sizeof(typename T::elem)));
+                     tiles);
   POTS_HIP(hipGetLastError());
   return POTS_E_OK;
 }
@@ -771,21 +721,17 @@ int backward(const pots_attention* a, char* work, hipStream_t s) {
   if (c.splits > 1)
     part = reinterpret_cast<float*>(work +
                                     align_up((size_t)a->batch * a->heads * a->n * 8, 256));
-  const bool vec = aligned(a, a->q, 16) && aligned(a, a->k, 16) && aligned(a, a->v, 16) &&
-                   aligned(a, a->out, 16) && aligned(a, a->dout, 16);
-  const uint32_t four = 4 * sizeof(typename T::elem);
   hipLaunchKernelGGL((attn_dq<T, DP, SPLIT>), dim3((uint32_t)qblocks), dim3(S::NT), 0, s, *a,
-                     stat, c.tiles, vec, aligned(a, a->dq, four));
+                     stat, c.tiles);
   POTS_HIP(hipGetLastError());
   hipLaunchKernelGGL((attn_dkv<T, DP, SPLIT>), dim3((uint32_t)kblocks), dim3(S::NT), 0, s, *a,
-                     stat, part, c.tiles, c.splits, c.per, vec,
-                     aligned(a, a->dk, four) && aligned(a, a->dv, four));
+                     stat, part, c.tiles, c.splits, c.per);
   POTS_HIP(hipGetLastError());
   if (part) {
     const uint64_t each = (uint64_t)a->batch * a->kv_heads * a->n * a->head_dim;
     const uint64_t nb = (each + 1023) / 1024;
     hipLaunchKernelGGL((attn_fold<T>), dim3((uint32_t)(nb < 4096 ? nb : 4096), 2), dim3(256), 0,
-                       s, *a, part, c.splits, aligned(a, a->dk, four) && aligned(a, a->dv, four));
+                       s, *a, part, c.splits);
     POTS_HIP(hipGetLastError());
   }
   return POTS_E_OK;
@@ -809,6 +755,8 @@ extern "C" int pots_attention_forward(const pots_attention* a, void* stream) {
   if (bad(a)) return POTS_E_ARG;
   if (a->batch == 0 || a->n == 0) return POTS_E_OK;
   if (!a->q.ptr || !a->k.ptr || !a->v.ptr || !a->out.ptr || !a->lse) return POTS_E_ARG;
+  for (const pots_heads* x : {&a->q, &a->k, &a->v, &a->out})
+    if (!aligned(a, *x)) return POTS_E_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool split = few((uint64_t)a->batch * a->heads, a->n);
   return a->dtype == POTS_OP_BF16 ? POTS_DIMS(Bf16, forward, a, s)
@@ -830,6 +778,8 @@ extern "C" int pots_attention_backward(const pots_attention* a, void* work, void
   if (!a->q.ptr || !a->k.ptr || !a->v.ptr || !a->out.ptr || !a->lse || !a->dout.ptr ||
       !a->dq.ptr || !a->dk.ptr || !a->dv.ptr || !work)
     return POTS_E_ARG;
+  for (const pots_heads* x : {&a->q, &a->k, &a->v, &a->out, &a->dout, &a->dq, &a->dk, &a->dv})
+    if (!aligned(a, *x)) return POTS_E_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool split = cut(a).split;
   char* w = static_cast<char*>(work);

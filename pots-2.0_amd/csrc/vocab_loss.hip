@@ -508,14 +508,15 @@ __global__ __launch_bounds__(C::NT) void loss_grad(Mat W, Mat X, uint32_t v0, ui
 // beside the other's. Blocks below mt·nt·splits: a share of dx, Wᵀ (stored along the
 // contraction, the piece's vocabulary) by G, added to the split's sums [rows][dp]. The others:
 // the piece's rows of dW, Xᵀ by Gᵀ, both stored along the contraction (the live rows), or a
-// share of their contraction to sums of its own where there are few tiles.
+// share of their contraction to sums of its own where there are few tiles (or dW's rows are not
+// whole fours of values).
 template <class T, class CX, class CW>
 __global__ __launch_bounds__(CX::NT) void loss_products(
     Mat W, Mat X, Mat G, uint32_t dp, uint32_t nv, const uint32_t* __restrict__ count,
     const float* __restrict__ unit, uint32_t pairs, uint32_t mt, uint32_t splits,
     uint32_t per, float* __restrict__ sums, uint64_t slice, bool first, uint32_t wmt,
     uint32_t wnt, uint32_t wsplits, uint32_t wper, float* __restrict__ wsums, uint64_t wslice,
-    uint32_t d, typename T::elem* __restrict__ dw, int64_t ld, bool vec) {
+    uint32_t d, typename T::elem* __restrict__ dw, int64_t ld) {
   // (the tiles of the live rows alone, dealt over all XCDs; the launch has room for every row)
   const uint32_t live = gload<uint32_t>(count), nt = (live + CX::TN - 1) / CX::TN;
   uint32_t m, n;
@@ -548,7 +549,7 @@ __global__ __launch_bounds__(CX::NT) void loss_products(
   CW c;
   c.run(X, G, m0, dp, n0, (nv + 7) & ~7u, k0, k0 < all ? min(wper, all - k0) : 0, live, live,
         pairs);
-  if (wsplits > 1) {
+  if (wsums) {
     float* out = wsums + wsplit * wslice;
     c.each(m0, n0, [&](f32x16& s, uint32_t col, uint32_t v) {
       if (v >= nv) return;
@@ -567,15 +568,9 @@ __global__ __launch_bounds__(CX::NT) void loss_products(
 #pragma unroll
     for (uint32_t q = 0; q < 4; q++) {
       const uint32_t at = col + 8 * q;
-      if (at >= d) continue;
-      if (vec) {
+      if (at < d)
         T::store4(p + at, s[4 * q] * mul, s[4 * q + 1] * mul, s[4 * q + 2] * mul,
                   s[4 * q + 3] * mul);
-      } else {
-#pragma unroll
-        for (uint32_t x = 0; x < 4; x++)
-          if (at + x < d) p[at + x] = T::put(s[4 * q + x] * mul);
-      }
     }
   });
 }
@@ -633,7 +628,7 @@ struct Plan {
   uint32_t dp, terms, pairs, rows_pad, piece;
   Shape scores, products;
   uint32_t splits, per, wsplits, wper;  // shares of dx's and of dW's contractions
-  bool copy_w, copy_x;
+  bool copy_w, copy_x, join_w;
   uint64_t w, x, part, hit, idx, pos, count, unit, weight, lse2, target, g, sums, wsums, bytes;
 };
 
@@ -702,7 +697,10 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
     p.wsplits *= 2;
   p.wper = cdiv(max(k_dw, 1u), p.wsplits) * BK;
   p.wsplits = max(cdiv(p.rows_pad, p.wper), 1u);
-  if (p.wsplits > 1) p.wsums = take(&p, 4ull * p.wsplits * p.piece * p.dp);
+  const uint64_t esize = a->dtype == POTS_OP_BF16 ? 2 : 4;
+  p.join_w = p.wsplits > 1 || a->dim % 4 || a->dw_row % 4 ||
+             reinterpret_cast<uint64_t>(a->dw) % (4 * esize);
+  if (p.join_w) p.wsums = take(&p, 4ull * p.wsplits * p.piece * p.dp);
   return p;
 }
 
@@ -805,16 +803,14 @@ int piece_grads(const pots_vocab_loss* a, const Plan& p, const Mat& W, const Mat
   }
   typedef typename T::elem elem;
   elem* const dw = reinterpret_cast<elem*>(a->dw) + (int64_t)v0 * a->dw_row;
-  const bool vec = a->dim % 4 == 0 && a->dw_row % 4 == 0 &&
-                   reinterpret_cast<uint64_t>(a->dw) % (4 * sizeof(elem)) == 0;
   const uint32_t xmt = cdiv(p.dp, CX::TM), wmt = cdiv(p.dp, CW::TM), wnt = cdiv(nv, CW::TN);
   hipLaunchKernelGGL((loss_products<T, CX, CW>), dim3(xmt * nt * p.splits + wmt * wnt * p.wsplits),
                      dim3(CX::NT), 0, s, W, X, G, p.dp, nv, count, f32(p.unit), p.pairs, xmt,
                      p.splits, p.per, f32(p.sums), (uint64_t)p.rows_pad * p.dp, v0 == 0, wmt,
-                     wnt, p.wsplits, p.wper, f32(p.wsums), (uint64_t)p.piece * p.dp, a->dim, dw,
-                     a->dw_row, vec);
+                     wnt, p.wsplits, p.wper, p.join_w ? f32(p.wsums) : nullptr,
+                     (uint64_t)p.piece * p.dp, a->dim, dw, a->dw_row);
   POTS_HIP(hipGetLastError());
-  if (p.wsplits > 1) {
+  if (p.join_w) {
     hipLaunchKernelGGL((loss_join<T>), dim3(nv), dim3(256), 0, s, f32(p.wsums), p.dp, p.wsplits,
                        (uint64_t)p.piece * p.dp, nullptr, f32(p.unit), a->dim, dw, a->dw_row);
     POTS_HIP(hipGetLastError());

@@ -84,9 +84,28 @@ def _indices(t: torch.Tensor, device: torch.device, what: str) -> torch.Tensor:
 
 # ---- attention ------------------------------------------------------------------------------
 
-def _rows_last(t: torch.Tensor) -> torch.Tensor:
-    """The kernels take any strides but the last, which is 1, and write no row twice."""
-    return t if t.stride(3) == 1 or t.shape[3] <= 1 else t.contiguous()
+# What the kernels take as it lies: 16-byte borders, consecutive values, rows under 2^22 values.
+_MAX_ROW = 1 << 22
+
+
+def _lies_well(t: torch.Tensor) -> bool:
+    sb, sh, sn, sd = t.stride()
+    size = t.element_size()
+    return (sd == 1 and sn < _MAX_ROW and t.data_ptr() % 16 == 0
+            and (sb | sh | sn) * size % 16 == 0)
+
+
+def _laid_out(t: torch.Tensor, d: int) -> torch.Tensor:
+    """``t`` as the kernels take it, its heads ``d`` wide: a copy where it lies otherwise, with
+    columns of zeros past its own."""
+    if t.shape[3] == d and _lies_well(t):
+        return t
+    b, h, n, own = t.shape
+    out = _new_heads(b, h, n, d, t)
+    out[..., :own] = t
+    if own < d:
+        out[..., own:] = 0
+    return out
 
 
 def _heads(t: torch.Tensor) -> tuple[int, int, int, int]:
@@ -131,7 +150,8 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                       scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Softmax attention of each sequence over its own keys: ``q [b, h, n, d]``, ``k`` and ``v
     [b, kv, n, d]`` with ``h`` a multiple of ``kv`` (consecutive query heads share a key head),
-    any strides, ``d`` up to 128; ``scale`` is ``1/√d`` unless given. ``causal``: position i sees
+    any strides (a tensor whose positions do not start on 16-byte borders is copied first, and so
+    is one whose ``d`` is no multiple of 8), ``d`` up to 128; ``scale`` is ``1/√d`` unless given. ``causal``: position i sees
     the positions up to i. ``lengths`` (int32 ``[b]``): positions from a sequence's length on
     are neither read nor seen; their outputs are zero.
 
@@ -140,8 +160,9 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     in memory as ``[b, n, h, d]``."""
     code, lengths, scale = _attention_args(q, k, v, lengths, scale)
     _on_gpu(q)
-    b, h, n, d = q.shape
-    q, k, v = _rows_last(q), _rows_last(k), _rows_last(v)
+    b, h, n, own = q.shape
+    d = (own + 7) & ~7
+    q, k, v = _laid_out(q, d), _laid_out(k, d), _laid_out(v, d)
     out = _new_heads(b, h, n, d, q)
     lse = torch.empty(b, h, n, dtype=torch.float32, device=q.device)
     args = _ATTENTION.pack(*_heads(q), *_heads(k), *_heads(v), *_heads(out), *_NO_HEADS,
@@ -149,7 +170,7 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                            0 if lengths is None else lengths.data_ptr(), b, h, k.shape[1], n, d,
                            code, causal, scale)
     native.get().operator("attention_forward", args, q.device)
-    return out, lse
+    return out if d == own else out[..., :own], lse
 
 
 def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -160,13 +181,14 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     ``lse``, in the inputs' type, lying in memory as ``[b, n, heads, d]``. The probabilities are
     recomputed; ``dk`` and ``dv`` are summed in fp32 over the query heads that share them."""
     code, lengths, scale = _attention_args(q, k, v, lengths, scale)
-    b, h, n, d = q.shape
+    b, h, n, own = q.shape
     kv = k.shape[1]
-    _like(dout, q, (b, h, n, d), "dout")
-    _like(out, q, (b, h, n, d), "out")
+    _like(dout, q, q.shape, "dout")
+    _like(out, q, q.shape, "out")
     lse = _floats(lse, q.device, (b, h, n), "lse")
     _on_gpu(q)
-    q, k, v, out, dout = (_rows_last(t) for t in (q, k, v, out, dout))
+    d = (own + 7) & ~7
+    q, k, v, out, dout = (_laid_out(t, d) for t in (q, k, v, out, dout))
     dq = _new_heads(b, h, n, d, q)
     dk = _new_heads(b, kv, n, d, q)
     dv = _new_heads(b, kv, n, d, q)
@@ -175,6 +197,8 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                            0 if lengths is None else lengths.data_ptr(), b, h, kv, n, d, code,
                            causal, scale)
     native.get().operator("attention_backward", args, q.device)
+    if d != own:
+        return dq[..., :own], dk[..., :own], dv[..., :own]
     return dq, dk, dv
 
 
