@@ -192,6 +192,8 @@ struct Shape {
   static constexpr uint32_t KT = SPLIT ? 32 * NW : sizeof(typename T::elem) == 2 ? 64 : 32;
   static constexpr uint32_t U = SPLIT ? 1 : KT / 32;   // a wave's products in a tile
   static constexpr uint32_t KS = DP / 16, NB = DP / 32;
+  static constexpr uint32_t kStat = KT < 64 ? 64 : KT;  // a tile's statistics, 64 to a load
+  static constexpr bool kApart = DP > 64;               // dk and dv in blocks of their own
   typedef Rows<T, DP, KT, NT> Tile;
   typedef typename T::elem Lds[KT * DP];  // at least 256 bytes a column: two sums of 32 rows
 };
@@ -481,21 +483,21 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
 // them. A wave holds 32 keys as columns: S = Q·Kᵀ and dP = dO·Vᵀ from the tiles' rows, dVᵀ +=
 // dOᵀ·P and dKᵀ += Qᵀ·dS from the same tiles read transposed. With `part`, the sums go to fp32
 // slices [2][split][batch][kv_heads][n][d].
-template <class T, uint32_t DP, bool SPLIT>
-__global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
-                             (!SPLIT && Shape<T, DP, SPLIT>::kWide <= 128 ? 2 : 1)) void attn_dkv(
-    pots_attention a, const float* __restrict__ stat, float* __restrict__ part, uint32_t tiles,
-    uint32_t splits, uint32_t per) {
+enum DkvWhat { kBoth, kOnlyDk, kOnlyDv };
+
+template <class T, uint32_t DP, bool SPLIT, DkvWhat WHAT>
+__device__ __forceinline__ void dkv_block(
+    const pots_attention& a, const float* __restrict__ stat, float* __restrict__ part,
+    uint32_t seq, uint32_t tile, uint32_t splits, uint32_t per, typename T::elem* s_q0,
+    typename T::elem* s_q1, typename T::elem* s_g0, typename T::elem* s_g1, float* s_stat0,
+    float* s_stat1) {
   typedef typename T::elem elem;
   typedef typename T::frag frag;
   typedef Shape<T, DP, SPLIT> S;
   typedef typename S::Tile R;
   constexpr uint32_t NW = S::NW, QT = S::KT, KS = S::KS, NB = S::NB, U = S::U;
-  constexpr uint32_t kStat = QT < 64 ? 64 : QT;
-  __shared__ __attribute__((aligned(16))) typename S::Lds s_q0, s_q1, s_g0, s_g1;
-  __shared__ __attribute__((aligned(16))) float s_stat0[2 * kStat], s_stat1[2 * kStat];
-  uint32_t seq, tile;
-  unit_of(a.batch * a.kv_heads * splits, &seq, &tile);
+  constexpr uint32_t kStat = S::kStat;
+  constexpr bool kDk = WHAT != kOnlyDv, kDv = WHAT != kOnlyDk;
   const uint32_t split = seq % splits, bk = seq / splits, b = bk / a.kv_heads;
   const uint32_t kvh = bk % a.kv_heads, rep = a.heads / a.kv_heads;
   const uint32_t lane = threadIdx.x % 64, i = lane % 32, h = lane / 32;
@@ -535,7 +537,7 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
 #pragma unroll
   for (uint32_t ks = 0; ks < KS; ks++) {
     kf[ks] = load_frag<T>(K.p, K.row, key, len, 16 * ks + 8 * h, d);
-    vf[ks] = load_frag<T>(V.p, V.row, key, len, 16 * ks + 8 * h, d);
+    if (kDk) vf[ks] = load_frag<T>(V.p, V.row, key, len, 16 * ks + 8 * h, d);
   }
   f32x16 dk[NB], dv[NB];
 #pragma unroll
@@ -546,43 +548,57 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
   const float c = a.scale * kLog2e;
   uint32_t q0 = first;
   auto step = [&](const elem* s_q, const elem* s_g, const float* s_stat) {
+    constexpr uint32_t C = 1;
 #pragma unroll
-    for (uint32_t y = 0; y < U; y++) {
-      const uint32_t u = SPLIT ? wave : y, qu = q0 + 32 * u;
-      if (qu >= len || kw >= len || (a.causal && qu + 31 < kw)) continue;
-      f32x16 s = zero16(), dp = zero16();
+    for (uint32_t y = 0; y < U; y += C) {
+      const uint32_t u0 = SPLIT ? wave : y, qu = q0 + 32 * u0;
+      if (qu >= len || kw >= len || (a.causal && qu + 32 * C - 1 < kw)) continue;
+      f32x16 s[C], dp[C];
 #pragma unroll
-      for (uint32_t ks = 0; ks < KS; ks++) {
-        s = mma(R::row(s_q, 32 * u + i, 16 * ks + 8 * h), kf[ks], s);
-        dp = mma(R::row(s_g, 32 * u + i, 16 * ks + 8 * h), vf[ks], dp);
-      }
+      for (uint32_t u = 0; u < C; u++) {
+        s[u] = zero16();
+        dp[u] = zero16();
 #pragma unroll
-      for (uint32_t g = 0; g < 4; g++) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(s_stat + 32 * u + 8 * g + 4 * h);
-        const f32x4 dl = *reinterpret_cast<const f32x4*>(s_stat + kStat + 32 * u + 8 * g + 4 * h);
-#pragma unroll
-        for (uint32_t x = 0; x < 4; x++) {
-          const uint32_t r = 4 * g + x;
-          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ls[x]));
-          dp[r] = s[r] * (dp[r] - dl[x]);
-        }
-      }
-      if (kw + 32 > len || qu + 32 > len || (a.causal && qu < kw + 31)) {
-#pragma unroll
-        for (uint32_t r = 0; r < 16; r++) {
-          const uint32_t q = qu + d_row(r, h);
-          if (key >= len || q >= len || (a.causal && q < key)) s[r] = dp[r] = 0.f;
+        for (uint32_t ks = 0; ks < KS; ks++) {
+          s[u] = mma(R::row(s_q, 32 * (u0 + u) + i, 16 * ks + 8 * h), kf[ks], s[u]);
+          if (kDk) dp[u] = mma(R::row(s_g, 32 * (u0 + u) + i, 16 * ks + 8 * h), vf[ks], dp[u]);
         }
       }
 #pragma unroll
-      for (uint32_t t = 0; t < 2; t++) {
-        const frag p = T::pack(s, 8 * t), ds = T::pack(dp, 8 * t);
+      for (uint32_t u = 0; u < C; u++)
 #pragma unroll
-        for (uint32_t db = 0; db < NB; db++) {
-          dv[db] = mma(R::col(s_g, 32 * u + 16 * t, 32 * db, lane), p, dv[db]);
-          dk[db] = mma(R::col(s_q, 32 * u + 16 * t, 32 * db, lane), ds, dk[db]);
+        for (uint32_t g = 0; g < 4; g++) {
+          const float* st = s_stat + 32 * (u0 + u) + 8 * g + 4 * h;
+          const f32x4 ls = *reinterpret_cast<const f32x4*>(st);
+          const f32x4 dl = *reinterpret_cast<const f32x4*>(st + kStat);
+#pragma unroll
+          for (uint32_t x = 0; x < 4; x++) {
+            const uint32_t r = 4 * g + x;
+            s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], c, -ls[x]));
+            if (kDk) dp[u][r] = s[u][r] * (dp[u][r] - dl[x]);
+          }
         }
+      if (kw + 32 > len || qu + 32 * C > len || (a.causal && qu < kw + 31)) {
+#pragma unroll
+        for (uint32_t u = 0; u < C; u++)
+#pragma unroll
+          for (uint32_t r = 0; r < 16; r++) {
+            const uint32_t q = qu + 32 * u + d_row(r, h);
+            if (key >= len || q >= len || (a.causal && q < key)) s[u][r] = dp[u][r] = 0.f;
+          }
       }
+#pragma unroll
+      for (uint32_t u = 0; u < C; u++)
+#pragma unroll
+        for (uint32_t t = 0; t < 2; t++) {
+          const frag p = T::pack(kDv ? s[u] : dp[u], 8 * t), ds = T::pack(dp[u], 8 * t);
+#pragma unroll
+          for (uint32_t db = 0; db < NB; db++) {
+            const uint32_t r0 = 32 * (u0 + u) + 16 * t;
+            if (kDv) dv[db] = mma(R::col(s_g, r0, 32 * db, lane), p, dv[db]);
+            if (kDk) dk[db] = mma(R::col(s_q, r0, 32 * db, lane), ds, dk[db]);
+          }
+        }
     }
     q0 = q0 + QT < len ? q0 + QT : first;
   };
@@ -604,11 +620,11 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
       return reinterpret_cast<float*>(w == 0 ? s_q0 : w == 1 ? s_q1 : w == 2 ? s_g0 : s_g1);
     };
     __syncthreads();
-    put_sums<NB, NW>(dk, lds, 0, wave, lane);
-    put_sums<NB, NW>(dv, lds, 1, wave, lane);
+    if (kDk) put_sums<NB, NW>(dk, lds, 0, wave, lane);
+    if (kDv) put_sums<NB, NW>(dv, lds, 1, wave, lane);
     __syncthreads();
-    join_sums<NB, NW>(dk, lds, 0, wave, lane);
-    join_sums<NB, NW>(dv, lds, 1, wave, lane);
+    if (kDk) join_sums<NB, NW>(dk, lds, 0, wave, lane);
+    if (kDv) join_sums<NB, NW>(dv, lds, 1, wave, lane);
   }
   constexpr uint32_t kOf = SPLIT ? NW : 1;
   const uint32_t mine = SPLIT ? wave : 0;
@@ -618,12 +634,42 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
     x.head = (int64_t)a.n * d;
     x.batch = x.head * a.kv_heads;
     x.ptr = part + split * x.batch * a.batch;
-    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dk, a.scale, h, kOf, mine);
+    if (kDk) store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dk, a.scale, h, kOf, mine);
     x.ptr = part + (splits + split) * x.batch * a.batch;
-    store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dv, 1.f, h, kOf, mine);
+    if (kDv) store_rows<Fp32, NB>(x, b, kvh, key, a.n, d, dv, 1.f, h, kOf, mine);
   } else {
-    store_rows<T, NB>(a.dk, b, kvh, key, a.n, d, dk, a.scale, h, kOf, mine);
-    store_rows<T, NB>(a.dv, b, kvh, key, a.n, d, dv, 1.f, h, kOf, mine);
+    if (kDk) store_rows<T, NB>(a.dk, b, kvh, key, a.n, d, dk, a.scale, h, kOf, mine);
+    if (kDv) store_rows<T, NB>(a.dv, b, kvh, key, a.n, d, dv, 1.f, h, kOf, mine);
+  }
+}
+
+
+// Wide heads have a block for dk and one for dv, which both make S: five products of a tile, not
+// four, but sums and fragments of one fit two waves a SIMD (1.5B shape: 194 us together, one
+// wave a SIMD, 188 apart; two heads of 675 in fp32, a launch of few blocks: 121 and 80).
+template <class T, uint32_t DP, bool SPLIT>
+__global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
+                             (!SPLIT && Shape<T, DP, SPLIT>::kWide <= 256 ? 2 : 1)) void attn_dkv(
+    pots_attention a, const float* __restrict__ stat, float* __restrict__ part, uint32_t splits,
+    uint32_t per) {
+  typedef Shape<T, DP, SPLIT> S;
+  __shared__ __attribute__((aligned(16))) typename S::Lds s_q0, s_q1, s_g0, s_g1;
+  __shared__ __attribute__((aligned(16))) float s_stat0[2 * S::kStat], s_stat1[2 * S::kStat];
+  const uint32_t seqs = a.batch * a.kv_heads * splits;
+  uint32_t seq, place;
+  if constexpr (S::kApart) {
+    unit_of(2 * seqs, &seq, &place);
+    const uint32_t tile = place;
+    if (seq % 2 == 0)
+      dkv_block<T, DP, SPLIT, kOnlyDk>(a, stat, part, seq / 2, tile, splits, per, s_q0, s_q1,
+                                       s_g0, s_g1, s_stat0, s_stat1);
+    else
+      dkv_block<T, DP, SPLIT, kOnlyDv>(a, stat, part, seq / 2, tile, splits, per, s_q0, s_q1,
+                                       s_g0, s_g1, s_stat0, s_stat1);
+  } else {
+    unit_of(seqs, &seq, &place);
+    dkv_block<T, DP, SPLIT, kBoth>(a, stat, part, seq, place, splits, per, s_q0, s_q1, s_g0, s_g1,
+                                   s_stat0, s_stat1);
   }
 }
 
@@ -684,7 +730,7 @@ Cut cut(const pots_attention* a) {
   const uint32_t rep = a->heads / a->kv_heads;
   c.split = few((uint64_t)a->batch * a->heads, a->n);
   c.tiles = cdiv(a->n, c.split ? 32 : 128);
-  const uint64_t blocks = (uint64_t)a->batch * a->kv_heads * c.tiles;
+  const uint64_t blocks = (uint64_t)a->batch * a->kv_heads * c.tiles * (a->head_dim > 64 ? 2 : 1);
   const uint32_t steps = cdiv(a->n, c.split ? 128 : 64);
   c.splits = 1;
   while (c.splits < rep) {
@@ -714,7 +760,8 @@ int backward(const pots_attention* a, char* work, hipStream_t s) {
   typedef Shape<T, DP, SPLIT> S;
   const Cut c = cut(a);
   const uint64_t qblocks = (uint64_t)a->batch * a->heads * c.tiles;
-  const uint64_t kblocks = (uint64_t)a->batch * a->kv_heads * c.tiles * c.splits;
+  const uint64_t kblocks =
+      (uint64_t)a->batch * a->kv_heads * c.tiles * c.splits * (S::kApart ? 2 : 1);
   if (qblocks > 0x7FFFFFFFu || kblocks > 0x7FFFFFFFu) return POTS_E_ARG;
   float* stat = reinterpret_cast<float*>(work);
   float* part = nullptr;
@@ -725,7 +772,7 @@ int backward(const pots_attention* a, char* work, hipStream_t s) {
                      stat, c.tiles);
   POTS_HIP(hipGetLastError());
   hipLaunchKernelGGL((attn_dkv<T, DP, SPLIT>), dim3((uint32_t)kblocks), dim3(S::NT), 0, s, *a,
-                     stat, part, c.tiles, c.splits, c.per);
+                     stat, part, c.splits, c.per);
   POTS_HIP(hipGetLastError());
   if (part) {
     const uint64_t each = (uint64_t)a->batch * a->kv_heads * a->n * a->head_dim;
