@@ -26,6 +26,9 @@ constexpr uint32_t kOneRun = 16384, kRun = 2048;  // tokens of a single run; els
 constexpr uint32_t kMerge = 32;    // runs a pass merges
 constexpr uint32_t kPiece = 16;    // sorted keys that a wave adds up, at the least
 constexpr uint32_t kFill = 16;     // rows that a block writes zeros to
+// The last cache before memory: a table that it holds is written through it (191 MB 25 us, past it
+// 31), a larger one past it, which leaves it to the sums' reads (933 MB 208 us through it, 201 past).
+constexpr uint64_t kCache = 256ull << 20;
 constexpr uint32_t kNoRow = ~0u;   // the id of a token outside the table; sorts last
 
 template <class T>
@@ -95,6 +98,7 @@ template <class T, uint32_t NT>
 __device__ __forceinline__ void fill_rows(const pots_embedding& a,
                                           const uint64_t* keys, uint32_t r0, uint32_t end,
                                           uint32_t cpr, bool vec) {
+  const bool past = (uint64_t)a.vocab * cpr * 16 > kCache;
   __shared__ uint32_t s_has[kFill];
   const uint32_t n = r0 < end ? min(kFill, end - r0) : 0;
   if (threadIdx.x < n) {
@@ -117,10 +121,10 @@ __device__ __forceinline__ void fill_rows(const pots_embedding& a,
     const uint32_t r = e / cpr, c = (e - r * cpr) * kPer<T>;
     if (s_has[r]) continue;
     typename T::elem* p = table + (int64_t)(r0 + r) * a.table_row;
-    if (vec)  // past the caches, which the sums' reads can use: 208 us a pass with plain stores, 201
+    if (vec && past)
       __builtin_nontemporal_store(Chunk<T>{}, reinterpret_cast<Chunk<T>*>(p + c));
     else
-      put_chunk<T>(p, c, a.dim, false, zero);
+      put_chunk<T>(p, c, a.dim, vec, zero);
   }
 }
 

@@ -331,6 +331,30 @@ def test_embedding(dtype, tokens, d, vocab):
     R.within(into, R.embedding(ids, dout, vocab, 1.0, table), "added gradient")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("tokens", [255, 256, 257, 16384, 16385])
+def test_embedding_around_the_counts_that_change_its_path(dtype, tokens):
+    g = _gen(tokens)
+    ids = (torch.rand(tokens, generator=g) ** 3 * 700).long().to(DEV)
+    dout = _rand(g, tokens, 24, dtype=dtype)
+    R.within(ops.embedding_backward(ids, dout, 701), R.embedding(ids, dout, 701, 1.0), "gradient")
+    into = _rand(g, 701, 24, dtype=dtype)
+    want = R.embedding(ids, dout, 701, 1.0, into)
+    R.within(ops.embedding_backward(ids, dout, 701, add_to=into), want, "added gradient")
+
+
+def test_embedding_gradient_of_a_large_table():
+    """A dense gradient too large for any cache: every row that no token has is zero."""
+    vocab, d = 70001, 1024
+    ids = torch.tensor([0, 70000, 35000, 0, 69999], device=DEV)
+    dout = _rand(_gen(33), 5, d, dtype=F32)
+    torch.full((vocab, d), math.nan, device=DEV)  # what the allocator may hand out again
+    got = ops.embedding_backward(ids, dout, vocab)
+    assert torch.equal(got[35000], dout[2]) and torch.equal(got[0], dout[0] + dout[3])
+    assert torch.equal(got[70000], dout[1]) and torch.equal(got[69999], dout[4])
+    assert int((got != 0).any(1).sum()) == 4
+
+
 def test_embedding_of_frequent_tokens():
     """One token for every position, and one that many pieces of the sorted list share."""
     g = _gen(31)
