@@ -94,11 +94,10 @@ __global__ __launch_bounds__(256) void embed_rows(pots_embedding a, uint32_t cpr
 
 // Zeros to rows r0 .. r0 + kFill of a dense gradient (those before `end`), by a block; with keys,
 // only to the rows that no token has, each looked up in the sorted list by one lane.
-template <class T, uint32_t NT>
-__device__ __forceinline__ void fill_rows(const pots_embedding& a,
-                                          const uint64_t* keys, uint32_t r0, uint32_t end,
-                                          uint32_t cpr, bool vec) {
-  const bool past = (uint64_t)a.vocab * cpr * 16 > kCache;
+template <class T, uint32_t NT, bool PAST>
+__device__ __forceinline__ void fill_rows_as(const pots_embedding& a, const uint64_t* keys,
+                                             uint32_t r0, uint32_t end, uint32_t cpr,
+                                             bool vec) {
   __shared__ uint32_t s_has[kFill];
   const uint32_t n = r0 < end ? min(kFill, end - r0) : 0;
   if (threadIdx.x < n) {
@@ -121,11 +120,21 @@ __device__ __forceinline__ void fill_rows(const pots_embedding& a,
     const uint32_t r = e / cpr, c = (e - r * cpr) * kPer<T>;
     if (s_has[r]) continue;
     typename T::elem* p = table + (int64_t)(r0 + r) * a.table_row;
-    if (vec && past)
+    if (vec && PAST)
       __builtin_nontemporal_store(Chunk<T>{}, reinterpret_cast<Chunk<T>*>(p + c));
     else
       put_chunk<T>(p, c, a.dim, vec, zero);
   }
+}
+
+// (two loops, since two stores of one loop that differ in this alone become one plain store)
+template <class T, uint32_t NT>
+__device__ __forceinline__ void fill_rows(const pots_embedding& a, const uint64_t* keys,
+                                          uint32_t r0, uint32_t end, uint32_t cpr, bool vec) {
+  if ((uint64_t)a.vocab * cpr * 16 > kCache)
+    fill_rows_as<T, NT, true>(a, keys, r0, end, cpr, vec);
+  else
+    fill_rows_as<T, NT, false>(a, keys, r0, end, cpr, vec);
 }
 
 // Places 32 keys a block within their run, each of them in a lane of both halves of every wave:

@@ -189,7 +189,7 @@ struct Tile {
 #pragma unroll
       for (uint32_t j = 0; j < NBUF; j++) {
         loads_done<kLeft>();
-        load((j + NBUF - 1) % NBUF);
+        if (NBUF > 2 || ahead < steps) load((j + NBUF - 1) % NBUF);
         if (t + j < steps) step(s_a[j], s_b[j]);
       }
     }
