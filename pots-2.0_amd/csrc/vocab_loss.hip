@@ -4,8 +4,8 @@
 //   s_rv = x_r·w_v,  lse_r = log Σ_v e^{s_rv},  loss_r = lse_r − s_{r,t_r}
 //   g_rv = weight_r (e^{s_rv − lse_r} − [v = t_r]),  dx = G·W,  dW = Gᵀ·X
 //
-// Forward: a tile of S is a product whose epilogue leaves a maximum and a sum of exponentials
-// per row and 32·MB vocabulary rows; loss_rows joins them. Backward, in pieces of the
+// Forward: a tile of S is a product whose epilogue leaves a maximum and a sum of exponentials per
+// row of x; loss_rows joins the tiles. Backward, in pieces of the
 // vocabulary: S again with the epilogue that writes the piece of G, then that piece's rows of
 // dW, and its share of dx added to fp32 sums. Rows that carry no weight are left out of the
 // products first (live_rows: prompts, rows without a target), and so is whatever they hold.
@@ -13,11 +13,18 @@
 // All three products are one tiled kernel over the matrix cores (Tile), each operand stored
 // either with the contraction along its rows or with its rows along the contraction (W of dx,
 // G and X of dW); the latter are read transposed from LDS. bf16 is multiplied as it is. An fp32
-// value is the exact sum of three bf16 terms of eight bits each (take_term), and a product of two
-// takes the six products of terms that reach 2^-24 of it: at six bf16 products' cost that is
-// 2.6 times the rate of the fp32 matrix instructions, with their accuracy (the three products
-// left out are below 2^-24 of |x||w|). G is rounded to the inputs' type as an operand: half a
-// step of bf16, 2^-9 of each term of sums that are rounded to bf16 themselves.
+// value is the exact sum of three bf16 terms (take_term), the second at most 2^-8 and the third 2^-16
+// of it. A product of two takes the six products of terms above 2^-24 of it; the three left out are
+// together below 2^-23. At six bf16 products' cost that is 1.3 times as fast as the library's
+// fp32 product (154 TFLOP/s). G is rounded to the inputs' type as an operand: half a step of
+// bf16, 2^-8, of each term of sums that are rounded to bf16 themselves.
+//
+// Bound by the matrix cores and what feeds them: a block's 256 x 256 tile needs 64 KiB a stage of 64,
+// and the loads alone (multiplications taken out, in a copy) take three quarters of the time;
+// multiplications alone two thirds. 8192 rows of 1536 against 151936 in bf16: 3.4 ms, 1.14 PFLOP/s,
+// of which exponentials and sums are about a tenth (the library's product without them:
+// 3.1 ms). What did not help: four stages of 32 (3.7 ms), four waves of 128 x 128 (4.0), one
+// operand past the LDS in fragments (3.7), loads issued later in a stage (3 to 7 % slower).
 #include <math.h>
 
 #include "common.h"
@@ -227,15 +234,18 @@ __device__ __forceinline__ void tile_of(uint32_t block, uint32_t mt, uint32_t nt
 
 // ---- laying operands out --------------------------------------------------------------------
 
-// The leading eight bits of x as bf16; x is left with the rest, exactly.
+// x to eight bits as bf16 (to nearest; down where that would be infinite); x is left with the
+// rest, exactly, at most 2^-8 of it.
 __device__ __forceinline__ uint16_t take_term(float* x) {
   const uint32_t u = __float_as_uint(*x);
   if ((u & 0x7F800000u) == 0x7F800000u) {  // one term; a NaN keeps a bit of its fraction
     *x = 0.f;
     return (u >> 16) | ((u & 0x7FFFFFu) ? 0x40 : 0);
   }
-  *x = *x - __uint_as_float(u & 0xFFFF0000u);
-  return u >> 16;
+  uint16_t t = f32_to_bf16(*x);
+  if ((t & 0x7F80u) == 0x7F80u) t = u >> 16;
+  *x = *x - bf16_to_f32(t);
+  return t;
 }
 
 // dst [terms][rows_pad][dp] of src rows (through idx where given, rows from *count on zero).
@@ -599,9 +609,10 @@ __global__ __launch_bounds__(256) void loss_join(const float* __restrict__ sums,
 
 namespace {
 
-// Tiles. Large ones read each operand half as often and reach 1.1 PFLOP/s where there are enough of
-// them for the GPU; up to 32 rows the product is bound by reading W, and a tile as narrow as
-// the rows leaves its multiplications out of the way.
+// Tiles. Large ones read each operand half as often, where there are enough of them for the GPU
+// (8192 rows of 1536: 3.4 ms, 4.0 in medium ones); up to 32 rows the product is bound by reading W,
+// and a tile as narrow as the rows leaves its multiplications out of the way (seven rows of 896
+// against 151936: 51 us, 5.3 TB/s).
 template <bool ATR, bool BTR>
 using Large = Tile<ATR, BTR, 256, 256, 2, 4, 2>;
 template <bool ATR, bool BTR>
@@ -772,8 +783,8 @@ int forward(const pots_vocab_loss* a, char* work, hipStream_t s) {
   const float2* part = reinterpret_cast<const float2*>(work + p.part);
   const float* hit = reinterpret_cast<const float*>(work + p.hit);
   const uint32_t chunks = cdiv(a->vocab, p.scores == kMedium ? 128 : 256);
-  // four rows a block, in 32-byte reads, where 32 a block would not fill the GPU
-  if (a->rows < 32 * kCus)
+  // four rows a block, in 32-byte reads, where blocks of 32 would be few (seven rows: 28 us and 4)
+  if (a->rows < 2048)
     hipLaunchKernelGGL(loss_rows<4>, dim3(cdiv(a->rows, 4)), dim3(1024), 0, s, part, chunks, hit,
                        *a);
   else
