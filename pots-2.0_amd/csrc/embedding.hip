@@ -3,8 +3,8 @@
 //   out_i = scale·table[id_i]        dtable_v (+)= scale · Σ_{i: id_i = v} dout_i
 //
 // Both are bound by memory: 8192 rows of 1536 in fp32 out of a table of 151936 take 14.6 us (6.9 TB/s,
-// part of it out of the last cache), the dense gradient of the same 185 us (983 MB, 5.3 TB/s; a fill
-// alone writes 6.8). Few tokens are bound by the launches, 5 us each. The gradient's sums are taken in the order of the positions, so no
+// part of it out of the last cache), the dense gradient of the same 185 us (983 MB, 5.3
+// TB/s, which a copy does not exceed). Few tokens are bound by the launches, 5 us each. The gradient's sums are taken in the order of the positions, so no
 // result depends on atomics: the tokens are sorted by (id, position), the sorted list is cut
 // into equal pieces whatever the ids' frequencies, and each piece adds up its rows in registers.
 // A row whose tokens lie within one piece is written right away; one that crosses pieces leaves
