@@ -2,18 +2,21 @@
 //
 //   out_i = scale·table[id_i]        dtable_v (+)= scale · Σ_{i: id_i = v} dout_i
 //
-// Both are bound by memory: 8192 rows of 1536 in fp32 out of a table of 151936 take 14.6 us (6.9 TB/s,
-// part of it out of the last cache), the dense gradient of the same 185 us (983 MB, 5.3
-// TB/s, which a copy does not exceed). Few tokens are bound by the launches, 5 us each. The gradient's sums are taken in the order of the positions, so no
-// result depends on atomics: the tokens are sorted by (id, position), the sorted list is cut
-// into equal pieces whatever the ids' frequencies, and each piece adds up its rows in registers.
-// A row whose tokens lie within one piece is written right away; one that crosses pieces leaves
-// fp32 sums that embed_join adds in order.
+// Both are bound by memory: 8192 rows of 1536 in fp32 out of a table of 151936 take 14.6 us (6.9
+// TB/s, part of it out of the last cache), the dense gradient of the same 185 us (983 MB, 5.3 TB/s,
+// which a copy does not exceed). Few tokens are bound by the launches, 5 us each.
+//
+// The gradient's sums are taken in the order of the positions, so no result depends on atomics: the
+// tokens are sorted by (id, position), the sorted list is cut into equal pieces whatever the ids'
+// frequencies, and each piece adds up its rows in registers. A row whose tokens lie within one
+// piece is written right away; one that crosses pieces leaves fp32 sums that embed_join adds in
+// order.
 //
 // Sorting: the keys (id above position, so all differ) are placed by counting. A block holds 32 of
 // them and counts the smaller ones of their run, two instructions a pair: up to 16384 tokens are
-// one run (8192 tokens 14 us; sorting networks of 2048 in LDS and a merge took 24). More are runs of 2048, merged up to 32 at a time, where a key's place
-// is its own index plus, for each other run, the number of smaller keys there. A dense
+// one run (8192 tokens 14 us; sorting networks of 2048 in LDS and a merge took 24). More are runs
+// of 2048, merged up to 32 at a time, where a key's place is its own index plus, for each other
+// run, the number of smaller keys there. A dense
 // gradient's zeros are written beside the sums, to the rows that no token has.
 #include <math.h>
 

@@ -649,9 +649,11 @@ uint64_t take(Plan* p, uint64_t bytes) {
   return at;
 }
 
+// Whether a matrix can be read where it lies: whole stages on 16-byte borders, and a tile of 256 of
+// its rows within 31 bits of offset.
 bool as_is(const pots_vocab_loss* a, const void* p, int64_t row) {
   return a->dtype == POTS_OP_BF16 && a->dim % BK == 0 &&
-         reinterpret_cast<uint64_t>(p) % 16 == 0 && row % 8 == 0;
+         reinterpret_cast<uint64_t>(p) % 16 == 0 && row % 8 == 0 && row >= 0 && row < 1 << 22;
 }
 
 Plan plan(const pots_vocab_loss* a, bool backward) {
@@ -717,7 +719,8 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
 
 bool bad(const pots_vocab_loss* a) {
   return !a || a->dtype > POTS_OP_BF16 || a->dim == 0 || a->vocab == 0 || a->dim > 65536 ||
-         a->rows > (1u << 24) || a->vocab > (1u << 24);
+         a->rows > (1u << 24) || a->vocab > (1u << 24) ||
+         (uint64_t)cdiv(a->rows, 32) * cdiv(a->vocab, 128) > 0x7FFFFFFFu;
 }
 
 template <class T>

@@ -255,6 +255,18 @@ def test_loss_strides(dtype):
     R.within(ops.vocab_loss_forward(x, w, t.int())[0], want["loss"], "int32 targets")
 
 
+@pytest.mark.parametrize("row", [(1 << 22) - 64, (1 << 22) + 64])
+def test_loss_of_rows_far_apart(row):
+    """Rows of the vocabulary on either side of what a tile's offsets reach."""
+    x, w, t, wt = _loss_inputs(28, BF, 40, 64, 600)
+    far = torch.empty(600 * row, dtype=BF, device=DEV).as_strided((600, 64), (row, 1)).copy_(w)
+    want = R.vocab_loss(x, w, t, wt)
+    loss, lse = ops.vocab_loss_forward(x, far, t)
+    dx, dw = ops.vocab_loss_backward(wt, x, far, t, lse)
+    for name, got in (("loss", loss), ("lse", lse), ("dx", dx), ("dw", dw)):
+        R.within(got, want[name], name)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 def test_loss_rows_that_count_for_nothing(dtype):
     """Rows of weight zero or without a target may hold anything."""

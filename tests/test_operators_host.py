@@ -129,7 +129,8 @@ def _loss(**kw):
 
 
 @pytest.mark.parametrize("kw", [dict(dim=0), dict(vocab=0), dict(dtype=2), dict(dim=65537),
-                                dict(rows=(1 << 24) + 1), dict(vocab=(1 << 24) + 1), {}])
+                                dict(rows=(1 << 24) + 1), dict(vocab=(1 << 24) + 1),
+                                dict(rows=1 << 24, vocab=1 << 24), {}])
 def test_vocab_loss_entry_points_refuse(abi, kw):
     a = _loss(**kw)
     assert abi.pots_vocab_loss_forward(a, None, None) == E_ARG
