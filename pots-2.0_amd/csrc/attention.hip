@@ -188,14 +188,16 @@ __device__ __forceinline__ void unit_of(uint32_t seqs, uint32_t* seq, uint32_t* 
 
 // How a block divides its work. Rows: four waves of 32 rows each (queries; keys in attn_dkv) go
 // through the other side's tiles of 64 (32 in fp32) together. Split: where that leaves compute
-// units without a block, a block has 32 rows and each wave takes its own 32 of a tile's 32·NW; the
-// waves' sums are joined at the end, in order (two waves for wide fp32 heads, whose tiles would
-// not fit the LDS). The 135M decoder's layer (fp32, 36 query heads' sequences of 256), us:
-// blocks of one wave 24 (attn_fwd), 32 (attn_dq) and 47 (attn_dkv), split ones 15, 21 and 23.
+// units without a block, a block has 32 rows and each wave takes its own 32 of a tile's 128; the
+// waves' sums are joined at the end, in order. A split block loads a tile when it has done with the
+// one before: its sequences are short, and two blocks to a compute unit cover for each other. The
+// 135M decoder's layer (fp32, 36 query heads' sequences of 256), us:
+// blocks of one wave 24 (attn_fwd), 32 (attn_dq) and 47 (attn_dkv), split ones 14, 21 and 22;
+// two sequences of 675 x 128 in fp32 56, 78 and 80 with two waves and a tile ahead, 37, 51 and 49.
 template <class T, uint32_t DP, bool SPLIT>
 struct Shape {
   static constexpr uint32_t kWide = DP * sizeof(typename T::elem);  // bytes of a row
-  static constexpr uint32_t NW = SPLIT && kWide > 256 ? 2 : 4, NT = 64 * NW;
+  static constexpr uint32_t NW = 4, NT = 64 * NW;
   static constexpr uint32_t R = SPLIT ? 32 : 32 * NW;  // the block's rows
   static constexpr uint32_t KT = SPLIT ? 32 * NW : sizeof(typename T::elem) == 2 ? 64 : 32;
   static constexpr uint32_t U = SPLIT ? 1 : KT / 32;   // a wave's products in a tile
@@ -203,31 +205,36 @@ struct Shape {
   static constexpr uint32_t kStat = KT < 64 ? 64 : KT;  // a tile's statistics, 64 to a load
   static constexpr bool kApart = DP > 64;               // dk and dv in blocks of their own
   typedef Rows<T, DP, KT, NT> Tile;
-  typedef typename T::elem Lds[KT * DP];  // at least 256 bytes a column: two sums of 32 rows
+  typedef typename T::elem Lds[KT * DP];
+  typedef typename T::elem Next[SPLIT ? 1 : KT * DP];  // the tile on its way; a split block has none
 };
 
-// The waves' sums of a split block, joined in order: wave w's at lds(w), of which the caller's
-// blocks db = wave, wave + NW, ... come back in acc. at: 0 or 1, two sums fit.
-template <uint32_t NB, uint32_t NW, class L>
-__device__ __forceinline__ void put_sums(f32x16 (&acc)[NB], L lds, uint32_t at, uint32_t wave,
+// The four waves' sums of a split block, joined in order: two waves' in each of its tiles, of which
+// the caller's blocks of 32 columns, wave, wave + 4, ..., come back in acc. Between two barriers.
+template <uint32_t NB>
+__device__ __forceinline__ float* sums_of(void* a, void* b, uint32_t wave) {
+  return reinterpret_cast<float*>(wave < 2 ? a : b) + wave % 2 * NB * 1024;
+}
+template <uint32_t NB>
+__device__ __forceinline__ void put_sums(f32x16 (&acc)[NB], void* a, void* b, uint32_t wave,
                                          uint32_t lane) {
-  float* p = lds(wave) + at * NB * 1024 + lane;
+  float* p = sums_of<NB>(a, b, wave) + lane;
 #pragma unroll
   for (uint32_t db = 0; db < NB; db++)
 #pragma unroll
     for (uint32_t r = 0; r < 16; r++) p[(db * 16 + r) * 64] = acc[db][r];
 }
-template <uint32_t NB, uint32_t NW, class L>
-__device__ __forceinline__ void join_sums(f32x16 (&acc)[NB], L lds, uint32_t at, uint32_t wave,
+template <uint32_t NB>
+__device__ __forceinline__ void join_sums(f32x16 (&acc)[NB], void* a, void* b, uint32_t wave,
                                           uint32_t lane) {
 #pragma unroll
   for (uint32_t db = 0; db < NB; db++) {
-    if (db % NW != wave) continue;
+    if (db % 4 != wave) continue;
 #pragma unroll
     for (uint32_t r = 0; r < 16; r++) {
       float sum = 0.f;
 #pragma unroll
-      for (uint32_t w = 0; w < NW; w++) sum += lds(w)[at * NB * 1024 + (db * 16 + r) * 64 + lane];
+      for (uint32_t w = 0; w < 4; w++) sum += sums_of<NB>(a, b, w)[(db * 16 + r) * 64 + lane];
       acc[db][r] = sum;
     }
   }
@@ -242,7 +249,8 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
   typedef Shape<T, DP, SPLIT> S;
   typedef typename S::Tile R;
   constexpr uint32_t NW = S::NW, KT = S::KT, KS = S::KS, NB = S::NB, U = S::U;
-  __shared__ __attribute__((aligned(16))) typename S::Lds s_k0, s_k1, s_v0, s_v1;
+  __shared__ __attribute__((aligned(16))) typename S::Lds s_k0, s_v0;
+  __shared__ __attribute__((aligned(16))) typename S::Next s_k1, s_v1;
   uint32_t bh, place;
   unit_of(a.batch * a.heads, &bh, &place);
   const uint32_t tile = tiles - 1 - place, b = bh / a.heads, head = bh % a.heads;
@@ -326,6 +334,12 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
     }
   };
   uint32_t k0 = 0;
+  for (; SPLIT && k0 + KT < end; k0 += KT) {
+    loads_done();
+    step(s_k0, s_v0, k0);
+    __syncthreads();
+    load(s_k0, s_v0, k0 + KT);
+  }
   for (; k0 + KT < end; k0 += 2 * KT) {  // the next tile is on its way while one is worked on
     loads_done();
     load(s_k1, s_v1, k0 + KT);
@@ -342,9 +356,6 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
   if constexpr (SPLIT) {
     // each wave's sums in units of the largest maximum of all, then added up
     __shared__ float s_m[NW][32], s_l[NW][32];
-    auto lds = [&](uint32_t w) {
-      return reinterpret_cast<float*>(w == 0 ? s_k0 : w == 1 ? s_k1 : w == 2 ? s_v0 : s_v1);
-    };
     if (h == 0) s_m[wave][i] = m == -INFINITY ? -INFINITY : mc;
     __syncthreads();  // and every wave is done with its tiles
     float top = -INFINITY;
@@ -357,13 +368,13 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
     for (uint32_t db = 0; db < NB; db++)
 #pragma unroll
       for (uint32_t r = 0; r < 16; r++) o[db][r] *= f;
-    put_sums<NB, NW>(o, lds, 0, wave, lane);
+    put_sums<NB>(o, s_k0, s_v0, wave, lane);
     __syncthreads();
     l = 0.f;
 #pragma unroll
     for (uint32_t w = 0; w < NW; w++) l += s_l[w][i];
     mc = top == -INFINITY ? 0.f : top;
-    join_sums<NB, NW>(o, lds, 0, wave, lane);
+    join_sums<NB>(o, s_k0, s_v0, wave, lane);
   }
   store_rows<T, NB>(a.out, b, head, q, a.n, d, o, l > 0.f || l != l ? 1.f / l : 0.f, h,
                     SPLIT ? NW : 1, SPLIT ? wave : 0);
@@ -384,7 +395,8 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
   typedef Shape<T, DP, SPLIT> S;
   typedef typename S::Tile R;
   constexpr uint32_t NW = S::NW, KT = S::KT, KS = S::KS, NB = S::NB, U = S::U;
-  __shared__ __attribute__((aligned(16))) typename S::Lds s_k0, s_k1, s_v0, s_v1;
+  __shared__ __attribute__((aligned(16))) typename S::Lds s_k0, s_v0;
+  __shared__ __attribute__((aligned(16))) typename S::Next s_k1, s_v1;
   uint32_t bh, place;
   unit_of(a.batch * a.heads, &bh, &place);
   const uint32_t tile = tiles - 1 - place, b = bh / a.heads, head = bh % a.heads;
@@ -462,6 +474,12 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
     }
   };
   uint32_t k0 = 0;
+  for (; SPLIT && k0 + KT < end; k0 += KT) {
+    loads_done();
+    step(s_k0, s_v0, k0);
+    __syncthreads();
+    load(s_k0, s_v0, k0 + KT);
+  }
   for (; k0 + KT < end; k0 += 2 * KT) {
     loads_done();
     load(s_k1, s_v1, k0 + KT);
@@ -475,13 +493,10 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
     step(s_k0, s_v0, k0);
   }
   if constexpr (SPLIT) {
-    auto lds = [&](uint32_t w) {
-      return reinterpret_cast<float*>(w == 0 ? s_k0 : w == 1 ? s_k1 : w == 2 ? s_v0 : s_v1);
-    };
     __syncthreads();
-    put_sums<NB, NW>(acc, lds, 0, wave, lane);
+    put_sums<NB>(acc, s_k0, s_v0, wave, lane);
     __syncthreads();
-    join_sums<NB, NW>(acc, lds, 0, wave, lane);
+    join_sums<NB>(acc, s_k0, s_v0, wave, lane);
   }
   store_rows<T, NB>(a.dq, b, head, q, a.n, d, acc, a.scale, h, SPLIT ? NW : 1,
                     SPLIT ? wave : 0);
@@ -611,6 +626,12 @@ __device__ __forceinline__ void dkv_block(
     q0 = q0 + QT < len ? q0 + QT : first;
   };
   uint32_t t = 0;
+  for (; SPLIT && t + 1 < steps; t++) {
+    loads_done();
+    step(s_q0, s_g0, s_stat0);
+    __syncthreads();
+    load(s_q0, s_g0, s_stat0);
+  }
   for (; t + 2 <= steps; t += 2) {
     loads_done();
     load(s_q1, s_g1, s_stat1);
@@ -624,15 +645,14 @@ __device__ __forceinline__ void dkv_block(
     step(s_q0, s_g0, s_stat0);
   }
   if constexpr (SPLIT) {
-    auto lds = [&](uint32_t w) {
-      return reinterpret_cast<float*>(w == 0 ? s_q0 : w == 1 ? s_q1 : w == 2 ? s_g0 : s_g1);
+    auto join = [&](f32x16(&acc)[NB]) {
+      __syncthreads();
+      put_sums<NB>(acc, s_q0, s_g0, wave, lane);
+      __syncthreads();
+      join_sums<NB>(acc, s_q0, s_g0, wave, lane);
     };
-    __syncthreads();
-    if (kDk) put_sums<NB, NW>(dk, lds, 0, wave, lane);
-    if (kDv) put_sums<NB, NW>(dv, lds, 1, wave, lane);
-    __syncthreads();
-    if (kDk) join_sums<NB, NW>(dk, lds, 0, wave, lane);
-    if (kDv) join_sums<NB, NW>(dv, lds, 1, wave, lane);
+    if (kDk) join(dk);
+    if (kDv) join(dv);
   }
   constexpr uint32_t kOf = SPLIT ? NW : 1;
   const uint32_t mine = SPLIT ? wave : 0;
@@ -661,7 +681,8 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
     pots_attention a, const float* __restrict__ stat, float* __restrict__ part, uint32_t splits,
     uint32_t per) {
   typedef Shape<T, DP, SPLIT> S;
-  __shared__ __attribute__((aligned(16))) typename S::Lds s_q0, s_q1, s_g0, s_g1;
+  __shared__ __attribute__((aligned(16))) typename S::Lds s_q0, s_g0;
+  __shared__ __attribute__((aligned(16))) typename S::Next s_q1, s_g1;
   __shared__ __attribute__((aligned(16))) float s_stat0[2 * S::kStat], s_stat1[2 * S::kStat];
   const uint32_t seqs = a.batch * a.kv_heads * splits;
   uint32_t seq, place;

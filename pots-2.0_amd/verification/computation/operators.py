@@ -84,23 +84,15 @@ def _indices(t: torch.Tensor, device: torch.device, what: str) -> torch.Tensor:
 
 # ---- attention ------------------------------------------------------------------------------
 
-# What the kernels take as it lies: 16-byte borders, consecutive values, rows under 2^22 values.
-_MAX_ROW = 1 << 22
-
-
-def _lies_well(t: torch.Tensor) -> bool:
-    sb, sh, sn, sd = t.stride()
-    size = t.element_size()
-    return (sd == 1 and sn < _MAX_ROW and t.data_ptr() % 16 == 0
-            and (sb | sh | sn) * size % 16 == 0)
-
-
 def _laid_out(t: torch.Tensor, d: int) -> torch.Tensor:
-    """``t`` as the kernels take it, its heads ``d`` wide: a copy where it lies otherwise, with
-    columns of zeros past its own."""
-    if t.shape[3] == d and _lies_well(t):
+    """``t`` as the kernels take it, its heads ``d`` wide (columns of zeros past its own): itself
+    where its values follow each other and its positions lie on 16-byte borders, else a copy."""
+    sb, sh, sn, sd = t.stride()
+    own = t.shape[3]
+    if (own == d and sd == 1 and sn < 1 << 22 and t.data_ptr() % 16 == 0
+            and (sb | sh | sn) * t.element_size() % 16 == 0):
         return t
-    b, h, n, own = t.shape
+    b, h, n, _ = t.shape
     out = _new_heads(b, h, n, d, t)
     out[..., :own] = t
     if own < d:
@@ -109,8 +101,26 @@ def _laid_out(t: torch.Tensor, d: int) -> torch.Tensor:
 
 
 def _heads(t: torch.Tensor) -> tuple[int, int, int, int]:
-    s = t.stride()
-    return t.data_ptr(), s[0], s[1], s[2]
+    sb, sh, sn, sd = t.stride()
+    if sd != 1:
+        raise ValueError("a position's values must follow each other")
+    return t.data_ptr(), sb, sh, sn
+
+
+def _call_attention(name: str, tensors: tuple[torch.Tensor, ...], d: int, pack) -> None:
+    """Enqueue on the tensors as they lie, which the library accepts almost always and checks
+    itself; where it does not, on copies."""
+    lib, device = native.get(), tensors[0].device
+    if tensors[0].shape[3] == d:
+        try:
+            return lib.operator(name, pack(*tensors), device)
+        except ValueError:
+            laid = [_laid_out(t, d) for t in tensors]
+            if all(a is b for a, b in zip(laid, tensors)):
+                raise
+    else:
+        laid = [_laid_out(t, d) for t in tensors]
+    lib.operator(name, pack(*laid), device)
 
 
 def _attention_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -151,9 +161,9 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     """Softmax attention of each sequence over its own keys: ``q [b, h, n, d]``, ``k`` and ``v
     [b, kv, n, d]`` with ``h`` a multiple of ``kv`` (consecutive query heads share a key head),
     any strides (a tensor whose positions do not start on 16-byte borders is copied first, and so
-    is one whose ``d`` is no multiple of 8), ``d`` up to 128; ``scale`` is ``1/√d`` unless given. ``causal``: position i sees
-    the positions up to i. ``lengths`` (int32 ``[b]``): positions from a sequence's length on
-    are neither read nor seen; their outputs are zero.
+    is one whose ``d`` is no multiple of 8), ``d`` up to 128; ``scale`` is ``1/√d`` unless given.
+    ``causal``: position i sees the positions up to i. ``lengths`` (int32 ``[b]``): positions
+    from a sequence's length on are neither read nor seen; their outputs are zero.
 
     Returns ``(out [b, h, n, d], lse fp32 [b, h, n])``, ``lse`` the logarithm of each row's sum
     of exponentials (−inf for a row that sees nothing), which the backward pass takes. ``out`` lies
@@ -162,14 +172,16 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     _on_gpu(q)
     b, h, n, own = q.shape
     d = (own + 7) & ~7
-    q, k, v = _laid_out(q, d), _laid_out(k, d), _laid_out(v, d)
     out = _new_heads(b, h, n, d, q)
     lse = torch.empty(b, h, n, dtype=torch.float32, device=q.device)
-    args = _ATTENTION.pack(*_heads(q), *_heads(k), *_heads(v), *_heads(out), *_NO_HEADS,
-                           *_NO_HEADS, *_NO_HEADS, *_NO_HEADS, lse.data_ptr(),
-                           0 if lengths is None else lengths.data_ptr(), b, h, k.shape[1], n, d,
-                           code, causal, scale)
-    native.get().operator("attention_forward", args, q.device)
+
+    def pack(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bytes:
+        return _ATTENTION.pack(*_heads(q), *_heads(k), *_heads(v), *_heads(out), *_NO_HEADS,
+                               *_NO_HEADS, *_NO_HEADS, *_NO_HEADS, lse.data_ptr(),
+                               0 if lengths is None else lengths.data_ptr(), b, h, k.shape[1], n,
+                               d, code, causal, scale)
+
+    _call_attention("attention_forward", (q, k, v), d, pack)
     return out if d == own else out[..., :own], lse
 
 
@@ -188,15 +200,18 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     lse = _floats(lse, q.device, (b, h, n), "lse")
     _on_gpu(q)
     d = (own + 7) & ~7
-    q, k, v, out, dout = (_laid_out(t, d) for t in (q, k, v, out, dout))
     dq = _new_heads(b, h, n, d, q)
     dk = _new_heads(b, kv, n, d, q)
     dv = _new_heads(b, kv, n, d, q)
-    args = _ATTENTION.pack(*_heads(q), *_heads(k), *_heads(v), *_heads(out), *_heads(dout),
-                           *_heads(dq), *_heads(dk), *_heads(dv), lse.data_ptr(),
-                           0 if lengths is None else lengths.data_ptr(), b, h, kv, n, d, code,
-                           causal, scale)
-    native.get().operator("attention_backward", args, q.device)
+
+    def pack(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+             dout: torch.Tensor) -> bytes:
+        return _ATTENTION.pack(*_heads(q), *_heads(k), *_heads(v), *_heads(out), *_heads(dout),
+                               *_heads(dq), *_heads(dk), *_heads(dv), lse.data_ptr(),
+                               0 if lengths is None else lengths.data_ptr(), b, h, kv, n, d, code,
+                               causal, scale)
+
+    _call_attention("attention_backward", (q, k, v, out, dout), d, pack)
     if d != own:
         return dq[..., :own], dk[..., :own], dv[..., :own]
     return dq, dk, dv
