@@ -7,8 +7,9 @@
 // Forward: a tile of S is a product whose epilogue leaves a maximum and a sum of exponentials per
 // row of x; loss_rows joins the tiles. Backward, in pieces of the vocabulary: S again with the
 // epilogue that writes the piece of G (1.1 PFLOP/s without its writes, 0.9 with them), then that
-// piece's rows of dW, and its share of dx added to fp32 sums (1.0 PFLOP/s together). Rows that carry no weight are left out of the
-// products first (live_rows: prompts, rows without a target), and so is whatever they hold.
+// piece's rows of dW, and its share of dx added to fp32 sums (1.0 PFLOP/s together). Rows that
+// carry no weight are left out of the products first (live_rows: prompts, rows without a target),
+// and so is whatever they hold.
 //
 // All three products are one tiled kernel over the matrix cores (Tile), each operand stored
 // either with the contraction along its rows or with its rows along the contraction (W of dx,
@@ -20,7 +21,7 @@
 // bf16, 2^-8, of each term of sums that are rounded to bf16 themselves.
 //
 // Bound by the matrix cores and what feeds them: a block's 256 x 256 tile needs 64 KiB a stage of 64,
-// and the loads alone (multiplications taken out, in a copy) take three quarters of the time;
+// and the loads alone (multiplications taken out, in a copy) take four fifths of the time;
 // multiplications alone two thirds. 8192 rows of 1536 against 151936 in bf16: 3.4 ms, 1.14 PFLOP/s,
 // of which exponentials and sums are about a tenth (the library's product without them:
 // 3.1 ms). What did not help: four stages of 32 (3.7 ms), four waves of 128 x 128 (4.0), one
