@@ -28,8 +28,8 @@
 // through registers into padded LDS, with no tile on its way, took 159, 207 and 467 us.
 //
 // Roundings: bf16 p and ds (the right operands of the second products) are rounded to bf16, off by
-// at most 2^-8 of each term of a sum whose result is rounded the same; scores, statistics and
-// sums are fp32. A value that is not finite, inside its sequence's length, may reach every row of
+// at most 2^-8 of each term of a sum whose result is rounded the same, and D is taken from out as
+// it was rounded, but where a row sees few keys (attn_dq); scores, statistics and sums are fp32. A value that is not finite, inside its sequence's length, may reach every row of
 // its tile (zero times infinity); what lies past a length is never read.
 #include <math.h>
 
@@ -386,9 +386,15 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
 // dq, and for attn_dkv each row's lse in units of log2 and D: stat [2][batch·heads][n]. A wave
 // holds 32 query rows as columns, as in the forward pass: Sᵀ = K·Qᵀ and dPᵀ = V·dOᵀ from the
 // tiles' rows, dQᵀ += Kᵀ·dSᵀ with K read transposed.
+//
+// D = Σ dO·out carries the rounding of out, which counts where a row sees few keys, since its out is
+// then as large as v and no average of many. Rows that see one product of 32 keys or less, the first
+// of causal sequences, take D = Σ p·dp from their registers instead, in no time that shows (the
+// gradients of the 0.5B shape are then off by 2.4e-3 of their norm, else 2.5e-3; with no rounding
+// but their own 1.7e-3).
 template <class T, uint32_t DP, bool SPLIT>
 __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
-                             (!SPLIT && Shape<T, DP, SPLIT>::kWide <= 256 ? 2 : 1)) void attn_dq(
+                             (Shape<T, DP, SPLIT>::kWide <= 256 ? 2 : 1)) void attn_dq(
     pots_attention a, float* __restrict__ stat, uint32_t tiles) {
   typedef typename T::elem elem;
   typedef typename T::frag frag;
@@ -455,10 +461,19 @@ __global__ __launch_bounds__((Shape<T, DP, SPLIT>::NT),
         dp = mma(R::row(s_v, 32 * u + i, 16 * ks + 8 * h), gf[ks], dp);
       }
 #pragma unroll
-      for (uint32_t r = 0; r < 16; r++) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse2));
-        s[r] = p * (dp[r] - dl);
+      for (uint32_t r = 0; r < 16; r++)
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse2));
+      if (wend <= 32) {  // all the keys of these rows are here
+        dl = 0.f;
+#pragma unroll
+        for (uint32_t r = 0; r < 16; r++)
+          if (d_row(r, h) < seen) dl = __builtin_fmaf(s[r], dp[r], dl);
+        dl += other_half(dl);
+        if (h == 0 && q < a.n)
+          stat[((int64_t)a.batch * a.heads + bh) * a.n + q] = dl;
       }
+#pragma unroll
+      for (uint32_t r = 0; r < 16; r++) s[r] *= dp[r] - dl;
       if (ku + 32 > len || qw + 32 > len || (a.causal && ku + 31 > qw)) {
 #pragma unroll
         for (uint32_t r = 0; r < 16; r++)
@@ -752,8 +767,8 @@ struct Cut {
 // The query heads of a group are shared out over blocks while there are fewer blocks than
 // compute units and a block has more than two tiles of queries to go through, or fewer than
 // three for each (causal tiles differ in length, and the launch ends with the short ones) and
-// more than eight tiles. us, two blocks for a unit at the least and three: the 0.5B shape 86 + 11 and
-// 64 + 12 (attn_dkv, attn_fold), the 1.5B shape 197 + 18 and 191 + 23.
+// more than eight tiles. us, attn_dkv and attn_fold, with half as many blocks asked for and so: the
+// 0.5B shape 75 + 7 and 57 + 8, the 1.5B shape 266 + 9 and 200 + 12; with twice as many no faster.
 Cut cut(const pots_attention* a) {
   Cut c;
   const uint32_t rep = a->heads / a->kv_heads;

@@ -127,6 +127,38 @@ def test_attention_scale_and_large_scores(dtype):
     assert bool(out.isfinite().all()) and bool(lse.isfinite().all())
 
 
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("h", [2, 96])
+def test_attention_gradients_where_few_keys_are_seen(d, h):
+    """What all values of such rows have in common changes no gradient of q and k: no more comes
+    of it than the rounding of fp32 sums, though out, rounded to bf16, is off by far more."""
+    q, k, v, g = _attention_inputs(d, BF, 8, h, 2, d, 32)
+    v = (v + 64).contiguous()
+    out, lse = ops.attention_forward(q, k, v)
+    dq, dk, _ = ops.attention_backward(g, q, k, v, out, lse)
+    want = R.attention(q, k, v, g, causal=True)
+    Q, K, V, G = (t.double().cpu() for t in (q, k, v, g))
+    rep, scale = h // 2, d ** -0.5
+    K, V = K.repeat_interleave(rep, 1), V.repeat_interleave(rep, 1)
+    s = (Q @ K.mT * scale).masked_fill(torch.ones(32, 32).triu(1).bool(), -math.inf)
+    p = s.softmax(-1)
+    dp = G @ V.mT
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    # scores and statistics as in the oracle; a relative error of all p of a row changes their sum
+    size = (Q.abs() @ K.abs().mT * scale).amax(-1, keepdim=True)
+    rp = (2 * (d + 4) * size + 32 + 8 + 8 * (size + s.logsumexp(-1, keepdim=True).abs())) * R.E32
+    edp = (d + 4) * R.E32 * (G.abs() @ V.abs().mT).amax(-1, keepdim=True)
+    eds = p * (3 * rp * dp.abs().amax(-1, keepdim=True) + 3 * edp)
+    eds = eds + (R.U[BF] + rep * 40 * R.E32) * (ds.abs() + eds)
+
+    def shared(t):
+        return t.view(8, 2, rep, 32, d).sum(2)
+
+    R.within(dq, (want["dq"][0], eds @ K.abs() * scale + R.U[BF] * want["dq"][0].abs()), "dq")
+    R.within(dk, (want["dk"][0], shared(eds.mT @ Q.abs()) * scale
+                  + R.U[BF] * want["dk"][0].abs()), "dk")
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 def test_attention_rows_whose_scores_are_all_minus_infinity(dtype):
     """Such a row has no largest score to subtract: zero, like one that sees nothing."""
