@@ -28,6 +28,8 @@
 // operand past the LDS in fragments (3.7), loads issued later in a stage (3 to 7 % slower).
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 #include "gmem.h"
 #include "tiles.h"
@@ -104,18 +106,27 @@ struct Stage {
   }
 
   // Rows c .. c + 31 at step ks of the stage: contraction 16ks + 8h + (0..7).
-  static __device__ __forceinline__ bf16x8 frag(const uint16_t* lds, uint32_t c, uint32_t ks,
-                                                uint32_t lane) {
+  static __device__ __forceinline__ void read(const uint16_t* lds, uint32_t c, uint32_t ks,
+                                              uint32_t lane, bf16x8* f) {
     const uint32_t h = lane / 32;
     if constexpr (TR) {
       const uint32_t m = lane % 16, r = 16 * ks + 8 * h + m / 4;
       const uint32_t col = c + (lane & 16) + 4 * (m % 4);
       const uint16_t* p = lds + r * T + (((col / 8) ^ swap(m / 4)) * 8 + 4 * (m % 2));
-      return join(read_tr(p), read_tr(p + 4 * T));
+      *f = join(read_tr(p), read_tr(p + 4 * T));
     } else {
       const uint32_t r = c + lane % 32;
-      return *reinterpret_cast<const bf16x8*>(lds + r * BK + (((2 * ks + h) ^ swap(lane % 32)) * 8));
+      *f = *reinterpret_cast<const bf16x8*>(lds + r * BK + (((2 * ks + h) ^ swap(lane % 32)) * 8));
     }
+  }
+  // The same of a stage of fp32 rows, two of its chunks.
+  static __device__ __forceinline__ void read(const uint16_t* lds, uint32_t c, uint32_t ks,
+                                              uint32_t lane, f32x8* f) {
+    const uint16_t* row = lds + (c + lane % 32) * BK;
+    const uint32_t at = 4 * ks + 2 * (lane / 32), by = swap(lane % 32);
+    *f = __builtin_shufflevector(*reinterpret_cast<const f32x4*>(row + (at ^ by) * 8),
+                                 *reinterpret_cast<const f32x4*>(row + ((at + 1) ^ by) * 8), 0, 1,
+                                 2, 3, 4, 5, 6, 7);
   }
 };
 
@@ -129,9 +140,13 @@ __device__ __forceinline__ uint16_t* lds_buffer() {
 
 // A block's TM x TN of A·Bᵀ over K (a multiple of BK), WM x WN waves of MB x NB products of 32.
 // NBUF stages in LDS: NBUF - 1 are on their way while one is multiplied.
+// F32: the operands are fp32, as stored, of twice the length and the distance in Mat's units, and go
+// through the fp32 matrix instructions.
 template <bool ATR, bool BTR, uint32_t TM_, uint32_t TN_, uint32_t WM_, uint32_t WN_,
-          uint32_t NBUF>
+          uint32_t NBUF, bool F32 = false>
 struct Tile {
+  static_assert(!F32 || (!ATR && !BTR), "no transposing reads of fp32");
+  typedef std::conditional_t<F32, f32x8, bf16x8> frag;
   static constexpr uint32_t TM = TM_, TN = TN_, WM = WM_, WN = WN_, NT = 64 * WM * WN;
   static constexpr uint32_t MB = TM / WM / 32, NB = TN / WN / 32;
   typedef Stage<ATR, TM, NT> SA;
@@ -141,12 +156,12 @@ struct Tile {
 
   __device__ __forceinline__ void step(const uint16_t* a, const uint16_t* b) {
 #pragma unroll
-    for (uint32_t ks = 0; ks < BK / 16; ks++) {
-      bf16x8 fa[MB], fb[NB];
+    for (uint32_t ks = 0; ks < BK / (F32 ? 32 : 16); ks++) {
+      frag fa[MB], fb[NB];
 #pragma unroll
-      for (uint32_t m = 0; m < MB; m++) fa[m] = SA::frag(a, wm + 32 * m, ks, lane);
+      for (uint32_t m = 0; m < MB; m++) SA::read(a, wm + 32 * m, ks, lane, &fa[m]);
 #pragma unroll
-      for (uint32_t n = 0; n < NB; n++) fb[n] = SB::frag(b, wn + 32 * n, ks, lane);
+      for (uint32_t n = 0; n < NB; n++) SB::read(b, wn + 32 * n, ks, lane, &fb[n]);
 #pragma unroll
       for (uint32_t m = 0; m < MB; m++)
 #pragma unroll
@@ -624,6 +639,9 @@ template <bool ATR, bool BTR>
 using Narrow = Tile<ATR, BTR, 256, 32, 8, 1, 4>;
 template <bool ATR, bool BTR>
 using NarrowX = Tile<ATR, BTR, 256, 32, 8, 1, 2>;  // beside Large in one kernel's LDS
+// fp32 rows as they are, through the fp32 matrix instructions: see kDirectRows
+using Direct = Tile<false, false, 256, 64, 8, 1, 2, true>;
+using NarrowDirect = Tile<false, false, 256, 32, 8, 1, 4, true>;
 enum Shape { kLarge, kTrimmed, kMedium, kNarrow };
 
 constexpr uint32_t kCus = 256;
@@ -640,7 +658,7 @@ struct Plan {
   uint32_t dp, terms, pairs, rows_pad, piece;
   Shape scores, products;
   uint32_t splits, per, wsplits, wper;  // shares of dx's and of dW's contractions
-  bool copy_w, copy_x, join_w;
+  bool copy_w, copy_x, join_w, direct;
   uint64_t w, x, part, hit, idx, pos, count, unit, weight, lse2, target, g, sums, wsums, bytes;
 };
 
@@ -652,10 +670,16 @@ uint64_t take(Plan* p, uint64_t bytes) {
 
 // Whether a matrix can be read where it lies: whole stages on 16-byte borders, and a tile of 256 of
 // its rows within 31 bits of offset.
-bool as_is(const pots_vocab_loss* a, const void* p, int64_t row) {
-  return a->dtype == POTS_OP_BF16 && a->dim % BK == 0 &&
-         reinterpret_cast<uint64_t>(p) % 16 == 0 && row % 8 == 0 && row >= 0 && row < 1 << 22;
+bool lies_well(const pots_vocab_loss* a, const void* p, int64_t row) {
+  const int64_t size = a->dtype == POTS_OP_BF16 ? 2 : 4;
+  return size * a->dim % (2 * BK) == 0 && reinterpret_cast<uint64_t>(p) % 16 == 0 &&
+         row * size % 16 == 0 && row >= 0 && row * size < 1 << 23;
 }
+bool as_is(const pots_vocab_loss* a, const void* p, int64_t row) {
+  return a->dtype == POTS_OP_BF16 && lies_well(a, p, row);
+}
+
+constexpr uint32_t kDirectRows = 768;
 
 Plan plan(const pots_vocab_loss* a, bool backward) {
   constexpr uint64_t kRoom = 512ull << 20;  // bytes of a piece of G, and of a copied one of W
@@ -664,8 +688,11 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
   p.pairs = a->dtype == POTS_OP_BF16 ? 1 : 6;
   p.dp = cdiv(a->dim, BK) * BK;
   p.rows_pad = cdiv(a->rows, 256) * 256;
-  p.copy_w = !as_is(a, a->w, a->w_row);
-  p.copy_x = backward || !as_is(a, a->x, a->x_row);
+  p.direct = !backward && a->dtype == POTS_OP_F32 && a->rows <= kDirectRows &&
+             lies_well(a, a->w, a->w_row) && lies_well(a, a->x, a->x_row);
+  if (p.direct) p.dp = 2 * a->dim, p.terms = p.pairs = 1;  // in units of two bytes
+  p.copy_w = !p.direct && !as_is(a, a->w, a->w_row);
+  p.copy_x = !p.direct && (backward || !as_is(a, a->x, a->x_row));
   const uint32_t all = cdiv(a->vocab, 256) * 256;
   uint64_t most = all;
   if (p.copy_w) most = min(most, kRoom / (2ull * p.terms * p.dp));
@@ -673,7 +700,7 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
   most = max(most, (uint64_t)2048);
   const uint32_t pieces = (uint32_t)((all + most - 1) / most);
   p.piece = cdiv(cdiv(all, pieces), 256) * 256;
-  p.scores = scores_shape(a->rows, p.piece);
+  p.scores = p.direct && a->rows > 32 ? kLarge : scores_shape(a->rows, p.piece);
   if (p.copy_w) p.w = take(&p, 2ull * p.terms * p.piece * p.dp);
   if (p.copy_x) p.x = take(&p, 2ull * p.terms * p.rows_pad * p.dp);
   if (!backward) {
@@ -744,7 +771,7 @@ int piece_of_w(const pots_vocab_loss* a, const Plan& p, char* work, uint32_t v0,
   const typename T::elem* src =
       reinterpret_cast<const typename T::elem*>(a->w) + (int64_t)v0 * a->w_row;
   if (!p.copy_w) {
-    *W = Mat{reinterpret_cast<const uint16_t*>(src), a->w_row, 0};
+    *W = Mat{reinterpret_cast<const uint16_t*>(src), a->w_row * (int64_t)(sizeof(*src) / 2), 0};
     return POTS_E_OK;
   }
   uint16_t* dst = reinterpret_cast<uint16_t*>(work + p.w);
@@ -766,7 +793,8 @@ int scores(const pots_vocab_loss* a, const Plan& p, const Mat& W, const Mat& X, 
 template <class T>
 int forward(const pots_vocab_loss* a, char* work, hipStream_t s) {
   const Plan p = plan(a, false);
-  Mat X = {reinterpret_cast<const uint16_t*>(a->x), a->x_row, 0};
+  Mat X = {reinterpret_cast<const uint16_t*>(a->x),
+           a->x_row * (int64_t)(sizeof(typename T::elem) / 2), 0};
   if (p.copy_x) {
     uint16_t* dst = reinterpret_cast<uint16_t*>(work + p.x);
     X = Mat{dst, (int64_t)p.dp, (int64_t)p.rows_pad * p.dp};
@@ -779,7 +807,9 @@ int forward(const pots_vocab_loss* a, char* work, hipStream_t s) {
     Mat W;
     int rc = piece_of_w<T>(a, p, work, v0, nv, &W, s);
     if (rc) return rc;
-    rc = p.scores == kLarge    ? scores<Large<false, false>>(a, p, W, X, v0, nv, work, s)
+    rc = p.direct              ? a->rows > 32 ? scores<Direct>(a, p, W, X, v0, nv, work, s)
+                                              : scores<NarrowDirect>(a, p, W, X, v0, nv, work, s)
+         : p.scores == kLarge  ? scores<Large<false, false>>(a, p, W, X, v0, nv, work, s)
          : p.scores == kMedium ? scores<Medium<false, false>>(a, p, W, X, v0, nv, work, s)
                                : scores<Narrow<false, false>>(a, p, W, X, v0, nv, work, s);
     if (rc) return rc;

@@ -271,6 +271,26 @@ def test_loss_of_several_pieces(dtype, rows):
     _loss_check(*_loss_inputs(21, dtype, rows, 64, 40003))
 
 
+@pytest.mark.parametrize("rows", [1, 32, 33, 64, 65, 210, 768, 769])
+@pytest.mark.parametrize("d, vocab", [(32, 90), (576, 257), (2048, 1300)])
+def test_loss_of_fp32_rows_read_where_they_lie(rows, d, vocab):
+    """Whole stages on 16-byte borders, rows apart from each other, and around the number of rows
+    from which operands are laid out instead."""
+    x, w, t, wt = _loss_inputs(rows + d, F32, rows, d, vocab)
+    far_x = torch.full((rows, d + 32), math.nan, device=DEV)[:, 32:].copy_(x)
+    far_w = torch.full((vocab, d + 4), math.nan, device=DEV)[:, 4:].copy_(w)
+    want = R.vocab_loss(x, w, t, wt)
+    for a, b in ((x, w), (far_x, far_w), (far_x[:, 1:], far_w[:, 1:])):
+        if a.shape[1] < d:
+            want = R.vocab_loss(a, b, t, wt)
+        loss, lse = ops.vocab_loss_forward(a, b, t)
+        R.within(loss, want["loss"], "loss")
+        R.within(lse, want["lse"], "lse")
+    w[vocab // 2, d - 1] = math.inf
+    loss, lse = ops.vocab_loss_forward(x.abs(), w, t)
+    assert bool((lse == math.inf).all() | lse.isnan().all())
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 def test_loss_strides(dtype):
     x, w, t, wt = _loss_inputs(22, dtype, 70, 64, 300)
