@@ -17,8 +17,9 @@
 // value is the exact sum of three bf16 terms (take_term), the second at most 2^-8 and the third 2^-16
 // of it. A product of two takes the six products of terms above 2^-24 of it; the three left out are
 // together below 2^-23. At six bf16 products' cost that is 1.3 times as fast as the library's
-// fp32 product (154 TFLOP/s). G is rounded to the inputs' type as an operand: half a step of
-// bf16, 2^-8, of each term of sums that are rounded to bf16 themselves.
+// fp32 product (154 TFLOP/s); few rows forward are multiplied as fp32. G is rounded to the inputs'
+// type as an operand: half a step of bf16, 2^-8, of each term of sums that are rounded to bf16
+// themselves.
 //
 // Bound by the matrix cores and what feeds them: a block's 256 x 256 tile needs 64 KiB a stage of 64,
 // and the loads alone (multiplications taken out, in a copy) take four fifths of the time;
@@ -639,8 +640,9 @@ template <bool ATR, bool BTR>
 using Narrow = Tile<ATR, BTR, 256, 32, 8, 1, 4>;
 template <bool ATR, bool BTR>
 using NarrowX = Tile<ATR, BTR, 256, 32, 8, 1, 2>;  // beside Large in one kernel's LDS
-// fp32 rows as they are, through the fp32 matrix instructions: see kDirectRows
-using Direct = Tile<false, false, 256, 64, 8, 1, 2, true>;
+// fp32 rows as they are, through the fp32 matrix instructions: see kDirectRows. Tiles of 128 rows
+// of w, three blocks to a compute unit, against 256 and one: 96 rows 226 us and 268, 512 753 and 763.
+using Direct = Tile<false, false, 128, 64, 4, 1, 2, true>;
 using NarrowDirect = Tile<false, false, 256, 32, 8, 1, 4, true>;
 enum Shape { kLarge, kTrimmed, kMedium, kNarrow };
 
@@ -679,6 +681,14 @@ bool as_is(const pots_vocab_loss* a, const void* p, int64_t row) {
   return a->dtype == POTS_OP_BF16 && lies_well(a, p, row);
 }
 
+// Up to so many fp32 rows the forward pass reads operands where they lie and multiplies with the
+// fp32 instructions: laying w out as three terms and reading them for six products costs more than
+// the slower multiplications. us at 2048 columns against 46432, laid out and where they lie: 40 rows
+// 604 and 148, 96 rows 596 and 226, 210 rows 634 and 412, 512 rows 925 and 753, 769 and
+// 768 rows 1345 and 1105; at 576 against 49152: 133 and 48, 135 and 69, 167 and 121, 243 and 222,
+// 349 and 325; 1024 rows laid out, 1374 and 357, are where the fp32 instructions would be slower.
+// Up to 32 rows bound by reading w (three rows 89 us, 4.3 TB/s), then by the fp32 instructions
+// (256 rows: 117 TFLOP/s).
 constexpr uint32_t kDirectRows = 768;
 
 Plan plan(const pots_vocab_loss* a, bool backward) {
@@ -700,7 +710,7 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
   most = max(most, (uint64_t)2048);
   const uint32_t pieces = (uint32_t)((all + most - 1) / most);
   p.piece = cdiv(cdiv(all, pieces), 256) * 256;
-  p.scores = p.direct && a->rows > 32 ? kLarge : scores_shape(a->rows, p.piece);
+  p.scores = p.direct && a->rows > 32 ? kMedium : scores_shape(a->rows, p.piece);
   if (p.copy_w) p.w = take(&p, 2ull * p.terms * p.piece * p.dp);
   if (p.copy_x) p.x = take(&p, 2ull * p.terms * p.rows_pad * p.dp);
   if (!backward) {
