@@ -747,7 +747,7 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
          k_dw * p.pairs / p.wsplits > 8)
     p.wsplits *= 2;
   p.wper = cdiv(max(k_dw, 1u), p.wsplits) * BK;
-  p.wsplits = max(cdiv(p.rows_pad, p.wper), 1u);
+  p.wsplits = max(cdiv(k_dw * BK, p.wper), 1u);
   const uint64_t esize = a->dtype == POTS_OP_BF16 ? 2 : 4;
   p.join_w = p.wsplits > 1 || a->dim % 4 || a->dw_row % 4 ||
              reinterpret_cast<uint64_t>(a->dw) % (4 * esize);
