@@ -291,6 +291,16 @@ def test_loss_of_fp32_rows_read_where_they_lie(rows, d, vocab):
     assert bool((lse == math.inf).all() | lse.isnan().all())
 
 
+@pytest.mark.parametrize("rows", [1, 32, 33, 70, 256, 257])
+@pytest.mark.parametrize("d, vocab", [(32, 90), (576, 257), (896, 1300)])
+def test_loss_gradients_of_few_fp32_rows(rows, d, vocab):
+    """One row, the ends of tiles of 32 and 256 rows, and rows apart from each other."""
+    _loss_check(*_loss_inputs(rows + d, F32, rows, d, vocab))
+    x, w, t, wt = _loss_inputs(rows, F32, rows, d, vocab)
+    _loss_check(torch.zeros(rows, d + 3, device=DEV)[:, 3:].copy_(x),
+                torch.zeros(vocab, d + 4, device=DEV)[:, 4:].copy_(w), t, wt)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 def test_loss_strides(dtype):
     x, w, t, wt = _loss_inputs(22, dtype, 70, 64, 300)
