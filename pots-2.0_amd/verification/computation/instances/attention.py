@@ -27,15 +27,11 @@ same computation.
 
 from __future__ import annotations
 
-import contextlib
-from collections.abc import Iterator
-
 import torch
 
-__all__ = ["ATTENTION", "FUSED", "register", "attention_forward", "fused_forward", "fused"]
+__all__ = ["ATTENTION", "register", "attention_forward", "uncaptured_mask"]
 
 ATTENTION = "pots_contiguous_bmm"
-FUSED = "pots_fused"
 
 
 def _check_right(b: torch.Tensor) -> None:
@@ -98,9 +94,12 @@ def attention_forward(module: torch.nn.Module, query: torch.Tensor, key: torch.T
                       scaling: float, dropout: float = 0.0, **kwargs):
     """transformers' attention-function signature: ``query [B, H, n, d_h]``, ``key`` and
     ``value [B, H_kv, n, d_h]``, an additive float mask ``[B, 1, n, n]`` or None; returns
-    ``(output [B, n, H, d_h], probabilities [B, H, n, n])``."""
+    ``(output [B, n, H, d_h], probabilities [B, H, n, n])``. With :func:`uncaptured_mask` as the
+    mask, the operator instead, which keeps no probabilities: ``(output, None)``."""
     if dropout:
         raise ValueError("attention dropout must be off: a step must be deterministic")
+    if attention_mask is not None and attention_mask.shape == _NO_TRANSCRIPT:
+        return _uncaptured(query, key, value, scaling, **kwargs)
     b, h, n, d = query.shape
     rep = module.num_key_value_groups
     # The products' format: autocast's when it is on (RoPE leaves Q and K in fp32 there, and
@@ -118,33 +117,28 @@ def attention_forward(module: torch.nn.Module, query: torch.Tensor, key: torch.T
     return out.view(b, h, n, d).transpose(1, 2).contiguous(), probs
 
 
-def fused_forward(module: torch.nn.Module, query: torch.Tensor, key: torch.Tensor,
-                  value: torch.Tensor, attention_mask: torch.Tensor | None, scaling: float,
-                  dropout: float = 0.0, **kwargs):
-    """The same attention for a pass that is not captured, without its probabilities
-    (``verification.computation.operators.attention``): causal, over whole sequences, so it
-    takes no mask. Returns ``(output [B, n, H, d_h], None)``."""
+# The shape that no batch of scores has: a layer's mask of it asks for the uncaptured attention.
+_NO_TRANSCRIPT = (0, 0, 0, 0)
+
+
+def uncaptured_mask(device: torch.device) -> torch.Tensor:
+    """The ``attention_mask`` of a model's call that is not captured: each of its layers then runs
+    ``verification.computation.operators.attention``, causal over whole sequences. The choice is an
+    argument like any other mask, so it goes with the call's layers wherever they run: in
+    another thread, beside captured calls of the same model, or a second time in the backward pass
+    of checkpointed layers."""
+    return torch.empty(_NO_TRANSCRIPT, device=device)
+
+
+def _uncaptured(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scaling: float, *,
+                sliding_window: int | None = None, **kwargs):
     from verification.computation import operators
-    if dropout:
-        raise ValueError("attention dropout must be off: a step must be deterministic")
-    if attention_mask is not None:
-        raise ValueError("the uncaptured attention is causal over whole sequences: no mask")
+    if sliding_window is not None:
+        raise ValueError("the uncaptured attention is over whole sequences: no sliding window")
     dev = query.device.type
     dt = torch.get_autocast_dtype(dev) if torch.is_autocast_enabled(dev) else query.dtype
     out = operators.attention(query.to(dt), key.to(dt), value.to(dt), scale=scaling)
     return out.transpose(1, 2), None
-
-
-@contextlib.contextmanager
-def fused(model: torch.nn.Module) -> Iterator[None]:
-    """``model`` with :func:`fused_forward` as its attention inside the block."""
-    register()
-    before = model.config._attn_implementation
-    model.config._attn_implementation = FUSED
-    try:
-        yield
-    finally:
-        model.config._attn_implementation = before
 
 
 _REGISTERED = False
@@ -152,15 +146,12 @@ _REGISTERED = False
 
 def register() -> str:
     """Register the core (and the eager causal mask it takes) with transformers under
-    :data:`ATTENTION`, and the uncaptured attention, which takes none, under :data:`FUSED`;
-    idempotent. Returns the core's name for a model config."""
+    :data:`ATTENTION`; idempotent. Returns the implementation name for a model config."""
     global _REGISTERED
     if not _REGISTERED:
         from transformers import AttentionInterface
         from transformers.masking_utils import AttentionMaskInterface, eager_mask
         AttentionInterface.register(ATTENTION, attention_forward)
         AttentionMaskInterface.register(ATTENTION, eager_mask)
-        AttentionInterface.register(FUSED, fused_forward)
-        AttentionMaskInterface.register(FUSED, lambda *args, **kwargs: None)
         _REGISTERED = True
     return ATTENTION

@@ -326,14 +326,20 @@ class DecoderComputation(DeclaredComputation):
         ``verification.computation.operators``, which keep no attention probability and no
         logit, and the loss's backward recomputes the logits a piece of the vocabulary at a
         time. The same mean over the masked tokens, and differentiable in the same weights; its
-        sums are taken in another order, so the bits are not the captured step's."""
+        sums are taken in another order, so the bits are not the captured step's. Heads are at
+        most ``operators.MAX_HEAD_DIM`` wide, and the model's attention is :meth:`build_model`'s
+        (``ValueError`` otherwise)."""
         from verification.computation import operators
-        from verification.computation.instances.attention import fused
+        from verification.computation.instances.attention import ATTENTION, uncaptured_mask
+        if model.config._attn_implementation != ATTENTION:
+            raise ValueError(f"the model's attention is {model.config._attn_implementation!r}, "
+                             f"not {ATTENTION!r}")
         dev = next(model.parameters()).device
         ids, targets, mask = self._batch(records, dev)
-        with fused(model), self.autocast(dev):
+        with self.autocast(dev):
             rows = operators.embedding(ids, model.get_input_embeddings().weight)
-            f = model.model(inputs_embeds=rows).last_hidden_state
+            f = model.model(inputs_embeds=rows,
+                            attention_mask=uncaptured_mask(dev)).last_hidden_state
         weights = mask.reshape(-1) / mask.sum()
         return operators.vocab_loss(f.reshape(-1, self.d).to(self.compute_dtype),
                                     model.get_output_embeddings().weight.to(self.compute_dtype),
