@@ -303,21 +303,27 @@ class _VocabLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, targets, weights):
         loss, lse = vocab_loss_forward(x, w, targets)
-        ctx.save_for_backward(x, w, targets, weights, lse)
+        ctx.save_for_backward(x, w, targets, weights, lse,
+                              loss if ctx.needs_input_grad[3] else None)
         return torch.where(weights != 0, loss * weights, 0.0).sum()
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        x, w, targets, weights, lse = ctx.saved_tensors
-        dx, dw = vocab_loss_backward(weights * g, x, w, targets, lse)
-        return dx, dw, None, None
+        x, w, targets, weights, lse, loss = ctx.saved_tensors
+        dx = dw = dweights = None
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+            dx, dw = vocab_loss_backward(weights * g, x, w, targets, lse)
+        if ctx.needs_input_grad[3]:
+            dweights = torch.where((weights != 0) | loss.isfinite(), loss * g, 0.0)
+        return dx, dw, None, dweights
 
 
 def vocab_loss(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
                weights: torch.Tensor) -> torch.Tensor:
     """``Σ_r weights_r · loss_r`` of :func:`vocab_loss_forward`'s losses, fp32, differentiable
-    in ``x`` and ``w``; rows of weight zero count for nothing, whatever their loss."""
+    in ``x``, ``w`` and ``weights``; rows of weight zero count for nothing, whatever their loss (the
+    gradient of such a weight is the row's loss, or zero where that is not finite)."""
     weights = _floats(weights, x.device, (x.shape[0],), "weights")
     return _VocabLoss.apply(x, w, targets, weights)
 

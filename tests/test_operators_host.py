@@ -162,3 +162,55 @@ def test_nothing_to_do_is_no_error(abi):
     assert abi.pots_attention_backward_work(_attention(n=0)) == 0
     assert abi.pots_vocab_loss_forward(_loss(rows=0), None, None) == 0
     assert abi.pots_embedding_forward(_embedding(tokens=0), None) == 0
+
+
+# ---- what autograd is given ---------------------------------------------------------------------
+
+@pytest.fixture
+def plain_loss(monkeypatch):
+    """The loss's two calls as plain formulas, on the CPU."""
+    calls = []
+
+    def forward(x, w, t):
+        calls.append("forward")
+        s = x @ w.T
+        lse = s.logsumexp(1)
+        return torch.where(t < 0, 0.0, lse - s.gather(1, t.clamp(min=0)[:, None])[:, 0]), lse
+
+    def backward(weights, x, w, t, lse):
+        calls.append("backward")
+        g = (x @ w.T - lse[:, None]).exp()
+        g[t >= 0, t[t >= 0]] -= 1
+        g = g * (weights * (t >= 0))[:, None]
+        return g @ w, g.T @ x
+
+    monkeypatch.setattr(ops, "vocab_loss_forward", forward)
+    monkeypatch.setattr(ops, "vocab_loss_backward", backward)
+    return calls
+
+
+def test_vocab_loss_weights_have_a_gradient(plain_loss):
+    """Each row's loss: the sum is linear in the weights. A row of weight zero has one too, unless it
+    holds what no loss comes of."""
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(6, 4, generator=g), torch.randn(9, 4, generator=g)
+    t = torch.tensor([3, 0, -100, 8, 5, 2])
+    weights = torch.tensor([0.5, 0.25, 1.0, 0.0, -1.0, 0.0])
+    x[5] = math.nan
+    want = ops.vocab_loss_forward(x, w, t)[0]
+    want[5] = 0.0
+    weights.requires_grad_()
+    (3 * ops.vocab_loss(x, w, t, weights)).backward()
+    assert torch.equal(weights.grad, 3 * want) and "backward" not in plain_loss
+    # by differences, of the weights that are not zero and of one that is
+    for i in (0, 1, 2, 3, 4):
+        step = torch.zeros(6)
+        step[i] = 0.25
+        up, down = (float(ops.vocab_loss(x, w, t, weights.detach() + s * step)) for s in (1, -1))
+        # (linear: six terms of a sum in fp32, each way)
+        assert abs((up - down) / 0.5 - float(want[i])) <= 4 * 12 * 2.0**-24 * (abs(up) + abs(down))
+    xg = x.nan_to_num().requires_grad_()
+    a, b = torch.autograd.grad(ops.vocab_loss(xg, w, t, weights), (xg, weights))
+    assert torch.equal(a, ops.vocab_loss_backward(weights.detach(), x.nan_to_num(), w, t,
+                                                  (x.nan_to_num() @ w.T).logsumexp(1))[0])
+    assert bool((b != 0)[[0, 1, 3, 4, 5]].all())
