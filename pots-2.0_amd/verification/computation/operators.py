@@ -299,13 +299,22 @@ def vocab_loss_backward(weights: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
     return dx, dw
 
 
+def _sum(t: torch.Tensor) -> torch.Tensor:
+    """The sum of a vector. torch's sum of many values clears its counters by a memset, which has no
+    place in a captured graph (recorded at 2^20 values, not at 2^16): such a vector is summed by
+    rows of 4096 first."""
+    if t.numel() > 1 << 16:
+        t = torch.nn.functional.pad(t, (0, -t.numel() % 4096)).view(-1, 4096).sum(1)
+    return t.sum()
+
+
 class _VocabLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, targets, weights):
         loss, lse = vocab_loss_forward(x, w, targets)
         ctx.save_for_backward(x, w, targets, weights, lse,
                               loss if ctx.needs_input_grad[3] else None)
-        return torch.where(weights != 0, loss * weights, 0.0).sum()
+        return _sum(torch.where(weights != 0, loss * weights, 0.0))
 
     @staticmethod
     @torch.autograd.function.once_differentiable

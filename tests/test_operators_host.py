@@ -214,3 +214,12 @@ def test_vocab_loss_weights_have_a_gradient(plain_loss):
     assert torch.equal(a, ops.vocab_loss_backward(weights.detach(), x.nan_to_num(), w, t,
                                                   (x.nan_to_num() @ w.T).logsumexp(1))[0])
     assert bool((b != 0)[[0, 1, 3, 4, 5]].all())
+
+
+@pytest.mark.parametrize("n", [0, 1, 5, 1 << 16, (1 << 16) + 1, 70000, 1 << 20])
+def test_the_sum_of_many_losses(n):
+    t = torch.randn(n, generator=torch.Generator().manual_seed(n))
+    got = ops._sum(t)
+    # (no order of adding up n values is further off)
+    assert got.shape == () and abs(float(got) - float(t.double().sum())) <= \
+        n * 2.0**-24 * float(t.double().abs().sum())
