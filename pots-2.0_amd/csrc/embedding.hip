@@ -406,10 +406,17 @@ Cut cut(const pots_embedding* a) {
 template <class T>
 int forward(const pots_embedding* a, hipStream_t s) {
   const uint32_t cpr = (a->dim + kPer<T> - 1) / kPer<T>;
-  const uint64_t nb = ((uint64_t)a->tokens * cpr + 255) / 256;
-  if (nb > 0x7FFFFFFFu) return POTS_E_ARG;
-  hipLaunchKernelGGL((embed_rows<T>), dim3((uint32_t)nb), dim3(256), 0, s, *a, cpr, chunked(a));
-  POTS_HIP(hipGetLastError());
+  const uint32_t most = (1u << 31) / cpr;  // tokens of a launch, which has less than 2^32 threads
+  const bool vec = chunked(a);
+  for (uint32_t t0 = 0; t0 < a->tokens; t0 += most) {
+    pots_embedding part = *a;
+    part.ids += t0;
+    part.rows = reinterpret_cast<typename T::elem*>(a->rows) + (int64_t)t0 * a->rows_row;
+    part.tokens = a->tokens - t0 < most ? a->tokens - t0 : most;
+    const uint32_t nb = (uint32_t)(((uint64_t)part.tokens * cpr + 255) / 256);
+    hipLaunchKernelGGL((embed_rows<T>), dim3(nb), dim3(256), 0, s, part, cpr, vec);
+    POTS_HIP(hipGetLastError());
+  }
   return POTS_E_OK;
 }
 

@@ -1,5 +1,5 @@
 // A driver for the sanitized CPU build of libpots_mi355x's host code (host_model.cpp stands in
-// for the HIP runtime). Three modes:
+// for the HIP runtime). Four modes:
 //
 //   host_check scan FILE...   pots_store_scan over the files (the untrusted prover files of an
 //                             on-disk transcript); one line per file with what the scan found,
@@ -12,6 +12,14 @@
 //                             refusals are checked against what the generator made.
 //   host_check pinned         pots_hash_leaves with and without pinned memory to be had, launches
 //                             succeeding and doing nothing: it does not fail.
+//   host_check launches CASE...
+//                             a training pass's operators, launches recorded and doing nothing. A
+//                             case is a name and its sizes, joined by commas:
+//                             attention_{forward,backward},BATCH,HEADS,KV_HEADS,N,HEAD_DIM,DTYPE;
+//                             vocab_loss_{forward,backward},ROWS,DIM,VOCAB,DTYPE;
+//                             embedding_{forward,backward},TOKENS,DIM,VOCAB,DTYPE,ADD. Each
+//                             gives a line "= CASE" with its return code and its scratch, after the
+//                             launches' lines: the kernel, its blocks and a block's threads.
 //
 // Exit status 0 when every result is as expected; the sanitizers abort on any finding.
 
@@ -20,8 +28,10 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <cxxabi.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <random>
 #include <string>
 #include <vector>
@@ -268,6 +278,7 @@ int plans(uint64_t seed, int count) {
 }  // namespace
 
 extern "C" void host_model_set(int pinned, int launches);
+extern "C" void host_model_on_launch(void (*f)(const char* kernel, dim3 grid, dim3 block));
 
 namespace {
 
@@ -290,13 +301,90 @@ int pinned() {
   return 0;
 }
 
+void print_launch(const char* kernel, dim3 grid, dim3 block) {
+  int status = 0;
+  char* plain = abi::__cxa_demangle(kernel, nullptr, nullptr, &status);
+  printf("%u %u %u %s\n", grid.x, grid.y, block.x, plain ? plain : kernel);
+  free(plain);
+}
+
+int launches(int argc, char** argv) {
+  host_model_set(1, 1);
+  host_model_on_launch(print_launch);
+  // (addresses for the launches' arguments; nothing reads them)
+  char* const p = reinterpret_cast<char*>(1ull << 44);
+  auto f32 = [&](int i) { return reinterpret_cast<float*>(p) + ((uint64_t)i << 40); };
+  for (int i = 2; i < argc; i++) {
+    std::string name;
+    uint32_t x[6] = {};
+    int n = -1;
+    const std::string text = argv[i];
+    for (size_t at = 0; at <= text.size();) {
+      const size_t end = std::min(text.find(',', at), text.size());
+      const std::string part = text.substr(at, end - at);
+      if (n < 0)
+        name = part;
+      else if (n < 6)
+        x[n] = (uint32_t)strtoull(part.c_str(), nullptr, 10);
+      n++;
+      at = end + 1;
+    }
+    int rc = 0;
+    uint64_t work = 0;
+    if (name == "attention_forward" || name == "attention_backward") {
+      pots_attention a = {};
+      a.batch = x[0], a.heads = x[1], a.kv_heads = x[2], a.n = x[3], a.head_dim = x[4];
+      a.dtype = x[5], a.causal = 1, a.scale = 1.f, a.lse = f32(8);
+      int k = 0;
+      for (pots_heads* h : {&a.q, &a.out, &a.dout, &a.dq, &a.k, &a.v, &a.dk, &a.dv}) {
+        const int64_t heads = k < 4 ? a.heads : a.kv_heads;
+        *h = pots_heads{f32(k++), heads * a.n * a.head_dim, (int64_t)a.n * a.head_dim,
+                        (int64_t)a.head_dim};
+      }
+      if (name == "attention_forward") {
+        rc = pots_attention_forward(&a, nullptr);
+      } else {
+        work = pots_attention_backward_work(&a);
+        rc = pots_attention_backward(&a, p, nullptr);
+      }
+    } else if (name == "vocab_loss_forward" || name == "vocab_loss_backward") {
+      pots_vocab_loss a = {};
+      a.rows = x[0], a.dim = x[1], a.vocab = x[2], a.dtype = x[3];
+      a.x = f32(1), a.w = f32(2), a.loss = f32(3), a.lse = f32(4), a.weights = f32(5);
+      a.dx = f32(6), a.dw = f32(7), a.targets = reinterpret_cast<const int64_t*>(f32(8));
+      a.x_row = a.w_row = a.dx_row = a.dw_row = a.dim;
+      const bool forward = name == "vocab_loss_forward";
+      work = (forward ? pots_vocab_loss_forward_work : pots_vocab_loss_backward_work)(&a);
+      rc = (forward ? pots_vocab_loss_forward : pots_vocab_loss_backward)(&a, p, nullptr);
+    } else if (name == "embedding_forward" || name == "embedding_backward") {
+      pots_embedding a = {};
+      a.tokens = x[0], a.dim = x[1], a.vocab = x[2], a.dtype = x[3], a.add = x[4], a.scale = 1.f;
+      a.ids = reinterpret_cast<const int64_t*>(f32(1)), a.table = f32(2), a.rows = f32(3);
+      a.table_row = a.rows_row = a.dim;
+      if (name == "embedding_forward") {
+        rc = pots_embedding_forward(&a, nullptr);
+      } else {
+        work = pots_embedding_backward_work(&a);
+        rc = pots_embedding_backward(&a, p, nullptr);
+      }
+    } else {
+      fprintf(stderr, "no operator %s\n", name.c_str());
+      return 1;
+    }
+    printf("= %s %d %llu\n", argv[i], rc, (unsigned long long)work);
+  }
+  return 0;
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
   if (argc == 2 && !strcmp(argv[1], "pinned")) return pinned();
   if (argc >= 2 && !strcmp(argv[1], "scan")) return scan(argc, argv);
+  if (argc >= 2 && !strcmp(argv[1], "launches")) return launches(argc, argv);
   if (argc == 4 && !strcmp(argv[1], "plans"))
     return plans(strtoull(argv[2], nullptr, 10), atoi(argv[3]));
-  fprintf(stderr, "usage: host_check scan FILE... | plans SEED COUNT | pinned\n");
+  fprintf(stderr, "usage: host_check scan FILE... | plans SEED COUNT | pinned | "
+          "launches CASE...\n");
   return 2;
 }

@@ -24,6 +24,7 @@ struct State {
   std::mutex mu;
   std::map<uintptr_t, size_t> device;     // base → bytes of each hipMalloc allocation
   std::map<const void*, void*> symbols;   // host shadow of a __device__ variable → its memory
+  std::map<const void*, const char*> kernels;  // host stub of a kernel → its (mangled) name
 };
 
 State& state() {
@@ -31,8 +32,16 @@ State& state() {
   return *s;
 }
 
+// What a launch's <<<...>>> hands to the kernel's stub.
+struct Call {
+  dim3 grid, block;
+  size_t shared;
+  hipStream_t stream;
+};
+thread_local Call g_call;
 thread_local hipError_t g_last = hipSuccess;
 bool g_pinned = true, g_launches = false;
+void (*g_on_launch)(const char* kernel, dim3 grid, dim3 block) = nullptr;
 int g_event_tag, g_stream_tag;
 
 hipError_t set(hipError_t e) {
@@ -86,6 +95,11 @@ hipError_t hipHostMalloc(void** ptr, size_t size, unsigned int) {
 void host_model_set(int pinned, int launches) {
   g_pinned = pinned != 0;
   g_launches = launches != 0;
+}
+
+// Called for every launch that HIP would take, with the kernel's name.
+void host_model_on_launch(void (*f)(const char* kernel, dim3 grid, dim3 block)) {
+  g_on_launch = f;
 }
 
 hipError_t hipHostFree(void* ptr) {
@@ -167,7 +181,21 @@ hipError_t hipEventRecord(hipEvent_t, hipStream_t) { return hipSuccess; }
 hipError_t hipEventSynchronize(hipEvent_t) { return hipSuccess; }
 hipError_t hipEventDestroy(hipEvent_t) { return hipSuccess; }
 
-hipError_t hipLaunchKernel(const void*, dim3, dim3, void**, size_t, hipStream_t) {
+// HIP takes less than 2^32 threads in a dimension of a launch, and no launch of none.
+hipError_t hipLaunchKernel(const void* f, dim3 grid, dim3 block, void**, size_t, hipStream_t) {
+  const uint64_t g[] = {grid.x, grid.y, grid.z}, b[] = {block.x, block.y, block.z};
+  for (int i = 0; i < 3; i++)
+    if (g[i] * b[i] == 0 || g[i] * b[i] >> 32) return set(hipErrorInvalidConfiguration);
+  if (g_on_launch) {
+    const char* name = "?";
+    State& st = state();
+    {
+      std::lock_guard<std::mutex> lock(st.mu);
+      auto it = st.kernels.find(f);
+      if (it != st.kernels.end()) name = it->second;
+    }
+    g_on_launch(name, grid, block);
+  }
   return g_launches ? hipSuccess : set(hipErrorNoDevice);
 }
 
@@ -189,8 +217,12 @@ void** __hipRegisterFatBinary(const void*) {
 
 void __hipUnregisterFatBinary(void**) {}
 
-void __hipRegisterFunction(void**, const void*, char*, const char*, unsigned int, uint3*,
-                           uint3*, dim3*, dim3*, int*) {}
+void __hipRegisterFunction(void**, const void* f, char*, const char* name, unsigned int, uint3*,
+                           uint3*, dim3*, dim3*, int*) {
+  State& st = state();
+  std::lock_guard<std::mutex> lock(st.mu);
+  st.kernels[f] = name;
+}
 
 void __hipRegisterVar(void**, void* var, char*, char*, int, size_t size, int, int) {
   void* mem = calloc(1, size ? size : 1);
@@ -201,14 +233,17 @@ void __hipRegisterVar(void**, void* var, char*, char*, int, size_t size, int, in
   st.symbols[var] = mem;
 }
 
-hipError_t __hipPushCallConfiguration(dim3, dim3, size_t, hipStream_t) { return hipSuccess; }
+hipError_t __hipPushCallConfiguration(dim3 grid, dim3 block, size_t shared, hipStream_t stream) {
+  g_call = Call{grid, block, shared, stream};
+  return hipSuccess;
+}
 
 hipError_t __hipPopCallConfiguration(dim3* grid, dim3* block, size_t* shared,
                                      hipStream_t* stream) {
-  if (grid) *grid = dim3(1, 1, 1);
-  if (block) *block = dim3(1, 1, 1);
-  if (shared) *shared = 0;
-  if (stream) *stream = nullptr;
+  if (grid) *grid = g_call.grid;
+  if (block) *block = g_call.block;
+  if (shared) *shared = g_call.shared;
+  if (stream) *stream = g_call.stream;
   return hipSuccess;
 }
 

@@ -1,0 +1,40 @@
+"""The operators' launches at sizes that no test could run, and those that the GPU tests of single
+paths rely on: the library's host code on the host model of the HIP runtime (``csrc/host_check``),
+which takes what HIP takes, at least one thread and less than 2^32 of them in a dimension."""
+
+from __future__ import annotations
+
+import pytest
+
+from test_host_sanitize import _run, driver  # noqa: F401  (a fixture)
+
+F32, BF16 = 0, 1
+E_ARG = -4
+
+
+def _launches(driver, *cases):  # noqa: F811
+    """For each case, its return code, its scratch and its launches: [(kernel, blocks, threads)]."""
+    out, now = [], []
+    for line in _run(driver, "launches", *cases).splitlines():
+        if line.startswith("= "):
+            _, _, rc, work = line.split()
+            out.append((int(rc), int(work), now))
+            now = []
+        else:
+            x, y, threads, name = line.split(" ", 3)
+            name = name.removeprefix("void ").split("(")[0].replace("pots::", "")
+            now.append((name, int(x) * int(y), int(threads)))
+    assert len(out) == len(cases)
+    return out
+
+
+@pytest.mark.parametrize("case", [
+    f"embedding_forward,{1 << 24},1024,1000,{F32}",    # 2^32 chunks of 16 bytes
+    f"embedding_forward,{1 << 24},1048576,1000,{F32}",
+])
+def test_looked_up_rows_past_a_launch(driver, case):  # noqa: F811
+    (rc, _, launches), = _launches(driver, case)
+    assert rc == 0
+    tokens, dim = (int(x) for x in case.split(",")[1:3])
+    threads = sum(x * t for _, x, t in launches)
+    assert threads >= tokens * dim // 4 and all(n == "embed_rows<Fp32>" for n, _, _ in launches)
