@@ -132,14 +132,21 @@ __device__ __forceinline__ void fill_rows_as(const pots_embedding& a, const uint
   }
 }
 
-// (two loops, since two stores of one loop that differ in this alone become one plain store)
+// The zeros of the blocks from `before` on, to rows r0 .. end; tables of 2^24 rows and more go round
+// (fill_blocks). (Two loops of stores, since two stores of one loop that differ in this alone become
+// one plain store.)
 template <class T, uint32_t NT>
 __device__ __forceinline__ void fill_rows(const pots_embedding& a, const uint64_t* keys,
-                                          uint32_t r0, uint32_t end, uint32_t cpr, bool vec) {
-  if ((uint64_t)a.vocab * cpr * 16 > kCache)
-    fill_rows_as<T, NT, true>(a, keys, r0, end, cpr, vec);
-  else
-    fill_rows_as<T, NT, false>(a, keys, r0, end, cpr, vec);
+                                          uint32_t before, uint32_t r0, uint32_t end,
+                                          uint32_t cpr, bool vec) {
+  const uint32_t step = (gridDim.x - before) * kFill;
+  for (uint32_t r = r0 + (blockIdx.x - before) * kFill; r < end; r += step) {
+    if ((uint64_t)a.vocab * cpr * 16 > kCache)
+      fill_rows_as<T, NT, true>(a, keys, r, end, cpr, vec);
+    else
+      fill_rows_as<T, NT, false>(a, keys, r, end, cpr, vec);
+    if (r + step < end) __syncthreads();  // every lane is done with what the block looked up
+  }
 }
 
 // Places 32 keys a block within their run, each of them in a lane of both halves of every wave:
@@ -155,7 +162,7 @@ __global__ __launch_bounds__(1024) void embed_order(pots_embedding a,
   __shared__ __attribute__((aligned(16))) uint32_t s_id[kOneRun];
   __shared__ uint32_t s_count[32][kOwn];
   if (blockIdx.x >= order) {
-    fill_rows<T, 1024>(a, nullptr, (blockIdx.x - order) * kFill, end, cpr, vec);
+    fill_rows<T, 1024>(a, nullptr, order, 0, end, cpr, vec);
     return;
   }
   const uint32_t t = threadIdx.x, lane = t % kOwn, part = t / kOwn;
@@ -254,7 +261,7 @@ __global__ __launch_bounds__(256) void embed_sum(pots_embedding a, uint64_t* __r
   }
   const uint64_t* const keys = FEW ? s_list : list;
   if (blockIdx.x >= blocks) {
-    fill_rows<T, 256>(a, keys, r0 + (blockIdx.x - blocks) * kFill, end, cpr, VEC);
+    fill_rows<T, 256>(a, keys, blocks, r0, end, cpr, VEC);
     return;
   }
   const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -322,7 +329,7 @@ __global__ __launch_bounds__(256) void embed_join(pots_embedding a,
   constexpr uint32_t P = kPer<T>;
   const uint32_t blocks = (sums + 3) / 4;
   if (blockIdx.x >= blocks) {
-    fill_rows<T, 256>(a, keys, r0 + (blockIdx.x - blocks) * kFill, a.vocab, cpr, vec);
+    fill_rows<T, 256>(a, keys, blocks, r0, a.vocab, cpr, vec);
     return;
   }
   const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -378,6 +385,13 @@ bool chunked(const pots_embedding* a) {
   return a->dim % per == 0 && a->table_row % per == 0 && a->rows_row % per == 0 &&
          reinterpret_cast<uint64_t>(a->table) % 16 == 0 &&
          reinterpret_cast<uint64_t>(a->rows) % 16 == 0;
+}
+
+// Blocks that write zeros to so many rows; no more than a launch has room for beside its others
+// (less than 2^32 threads).
+uint32_t fill_blocks(uint32_t rows) {
+  const uint32_t blocks = (rows + kFill - 1) / kFill;
+  return blocks < 1u << 20 ? blocks : 1u << 20;
 }
 
 struct Cut {
@@ -442,10 +456,9 @@ int backward(const pots_embedding* a, char* work, hipStream_t s) {
   const bool few = a->tokens <= kFew;
   const uint32_t r1 = a->add || few ? 0 : a->vocab / 12;
   const uint32_t r2 = a->add ? 0 : c.pieces > 1 ? a->vocab - r1 : a->vocab;
-  auto fills = [](uint32_t rows) { return (rows + kFill - 1) / kFill; };
   if (!few) {
-    hipLaunchKernelGGL((embed_order<T>), dim3(c.order + fills(r1)), dim3(1024), 0, s, *a, from,
-                       c.run, c.order, r1, c.cpr, vec);
+    hipLaunchKernelGGL((embed_order<T>), dim3(c.order + fill_blocks(r1)), dim3(1024), 0, s, *a,
+                       from, c.run, c.order, r1, c.cpr, vec);
     POTS_HIP(hipGetLastError());
   }
   for (uint64_t run = c.run; run < a->tokens; run *= kMerge) {
@@ -457,14 +470,14 @@ int backward(const pots_embedding* a, char* work, hipStream_t s) {
     to = t;
   }
   const uint32_t groups = (c.cpr + 63) / 64, sums = c.pieces * groups, blocks = (sums + 3) / 4;
-  if (blocks + fills(r2 - r1)) {
+  if (blocks + fill_blocks(r2 - r1)) {
     const auto kernel = sum_kernel<T>(few, a->add, vec);
-    hipLaunchKernelGGL(kernel, dim3(blocks + fills(r2 - r1)), dim3(256), 0, s, *a, from, c.piece,
-                       groups, sums, c.cpr, r1, r2, part);
+    hipLaunchKernelGGL(kernel, dim3(blocks + fill_blocks(r2 - r1)), dim3(256), 0, s, *a, from,
+                       c.piece, groups, sums, c.cpr, r1, r2, part);
     POTS_HIP(hipGetLastError());
   }
   if (c.pieces > 1) {
-    hipLaunchKernelGGL((embed_join<T>), dim3(blocks + (a->add ? 0 : fills(a->vocab - r2))),
+    hipLaunchKernelGGL((embed_join<T>), dim3(blocks + (a->add ? 0 : fill_blocks(a->vocab - r2))),
                        dim3(256), 0, s, *a, from, c.piece, groups, sums, c.cpr, r2, part, vec);
     POTS_HIP(hipGetLastError());
   }

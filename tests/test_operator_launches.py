@@ -38,3 +38,11 @@ def test_looked_up_rows_past_a_launch(driver, case):  # noqa: F811
     tokens, dim = (int(x) for x in case.split(",")[1:3])
     threads = sum(x * t for _, x, t in launches)
     assert threads >= tokens * dim // 4 and all(n == "embed_rows<Fp32>" for n, _, _ in launches)
+
+
+@pytest.mark.parametrize("tokens", [0, 1, 200, 257, 40000])
+@pytest.mark.parametrize("vocab", [(1 << 28) + 5, 1 << 30])
+def test_dense_gradients_of_tables_past_a_launch(driver, tokens, vocab):  # noqa: F811
+    """A block of zeros for every 16 rows of the table would be 2^32 threads."""
+    (rc, _, launches), = _launches(driver, f"embedding_backward,{tokens},8,{vocab},{BF16},0")
+    assert rc == 0 and "embed_sum" in " ".join(n for n, _, _ in launches)

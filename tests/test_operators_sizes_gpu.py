@@ -1,0 +1,50 @@
+"""The training pass's operators at sizes past one launch, one piece or one cache, and on the tiles
+that large products take. Which launches the sizes reach is asserted in test_operator_launches.py."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import operators_oracle as R
+from verification.computation import operators as ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- the embedding --------------------------------------------------------------------------
+
+def test_embedding_of_rows_past_a_launch():
+    """2^32 chunks of 16 bytes, 64 GiB."""
+    tokens, d, vocab = 1 << 24, 1024, 1000
+    g = torch.Generator(device=DEV).manual_seed(1)
+    table = torch.randn(vocab, d, generator=g, device=DEV)
+    ids = torch.randint(0, vocab, (tokens,), generator=g, device=DEV)
+    out = ops.embedding_forward(ids, table)
+    for part in (slice(i, i + (1 << 18)) for i in range(0, tokens, 1 << 18)):
+        assert torch.equal(out[part], table[ids[part]])
+
+
+@pytest.mark.parametrize("tokens", [3, 300])
+def test_embedding_gradient_of_a_table_past_a_launch(tokens):
+    """16 rows of zeros a block would be 2^32 threads."""
+    vocab, d = (1 << 28) + 5, 8
+    ids = torch.randint(0, vocab, (tokens,), generator=_gen(tokens))
+    ids[0], ids[1], ids[2] = vocab - 1, 0, 1 << 27
+    dout = torch.randn(tokens, d, generator=_gen(2)).to(BF)
+    torch.full((vocab, d), math.nan, dtype=BF, device=DEV)  # what the allocator hands out again
+    got = ops.embedding_backward(ids.to(DEV), dout.to(DEV), vocab)
+    rows, at = ids.unique(return_inverse=True)
+    want, bound = R.embedding(at, dout, len(rows), 1.0)
+    R.within(got[rows.to(DEV)], (want, bound), "rows with tokens")
+    got[rows.to(DEV)] = 0
+    for part in got.split(1 << 24):
+        assert not bool(part.any())  # (a NaN is not zero)
