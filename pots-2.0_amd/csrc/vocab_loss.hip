@@ -708,6 +708,8 @@ Plan plan(const pots_vocab_loss* a, bool backward) {
   if (p.copy_w) most = min(most, kRoom / (2ull * p.terms * p.dp));
   if (backward && a->rows) most = min(most, kRoom / (2ull * p.terms * p.rows_pad));
   most = max(most, (uint64_t)2048);
+  // (a launch has less than 2^32 threads: 2^22 large tiles are half of them)
+  most = min(most, 256ull * max((1u << 22) / max(p.rows_pad / 256, 1u), 1u));
   const uint32_t pieces = (uint32_t)((all + most - 1) / most);
   p.piece = cdiv(cdiv(all, pieces), 256) * 256;
   p.scores = p.direct && a->rows > 32 ? kMedium : scores_shape(a->rows, p.piece);

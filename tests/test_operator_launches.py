@@ -46,3 +46,18 @@ def test_dense_gradients_of_tables_past_a_launch(driver, tokens, vocab):  # noqa
     """A block of zeros for every 16 rows of the table would be 2^32 threads."""
     (rc, _, launches), = _launches(driver, f"embedding_backward,{tokens},8,{vocab},{BF16},0")
     assert rc == 0 and "embed_sum" in " ".join(n for n, _, _ in launches)
+
+
+@pytest.mark.parametrize("rows, vocab", [(1 << 20, 1 << 20), (1 << 24, 40000), (1 << 22, 1 << 18),
+                                         (129, 1 << 24), (5, 1 << 24)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_losses_of_more_tiles_than_a_launch(driver, rows, vocab, dtype):  # noqa: F811
+    """2^23 tiles of 512 threads and more: the vocabulary is taken in pieces. Every row meets every
+    vocabulary entry once."""
+    (rc, _, launches), = _launches(driver, f"vocab_loss_forward,{rows},64,{vocab},{dtype}")
+    assert rc == 0
+    area = {"256u, 256u": 1 << 16, "128u, 128u": 1 << 14, "256u, 32u": 1 << 13,
+            "128u, 64u": 1 << 13}
+    done = sum(x * next(v for k, v in area.items() if k in n)
+               for n, x, _ in launches if n.startswith("loss_scores"))
+    assert rows * vocab <= done <= 1.25 * (rows + 255) * (vocab + 255)

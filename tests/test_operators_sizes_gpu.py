@@ -48,3 +48,30 @@ def test_embedding_gradient_of_a_table_past_a_launch(tokens):
     got[rows.to(DEV)] = 0
     for part in got.split(1 << 24):
         assert not bool(part.any())  # (a NaN is not zero)
+
+
+# ---- the loss -------------------------------------------------------------------------------
+
+def _loss_inputs(seed, dtype, rows, d, vocab):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(rows, d, generator=g, device=DEV).to(dtype)
+    w = (torch.randn(vocab, d, generator=g, device=DEV) * (1.5 / d**0.5)).to(dtype)
+    t = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+    weights = torch.rand(rows, generator=g, device=DEV) / rows
+    weights[torch.rand(rows, generator=g, device=DEV) < 0.25] = 0
+    t[1], t[rows // 2], t[rows - 1] = -100, vocab - 1, vocab - 2
+    return x, w, t, weights
+
+
+def test_loss_of_more_tiles_than_a_launch():
+    """2^23 tiles of 512 threads: several pieces of the vocabulary, though w is read where it lies.
+    Some rows against the oracle."""
+    rows, d, vocab = (1 << 20) + 5, 64, (1 << 19) + 3
+    x, w, t, weights = _loss_inputs(3, BF, rows, d, vocab)
+    loss, lse = ops.vocab_loss_forward(x, w, t)
+    some = torch.cat([torch.arange(20), torch.arange(rows // 2 - 10, rows // 2 + 10),
+                      torch.arange(rows - 10, rows)]).to(DEV)
+    want = R.vocab_loss(x[some], w, t[some], weights[some])
+    R.within(loss[some], want["loss"], "loss")
+    R.within(lse[some], want["lse"], "lse")
+    assert bool(loss.isfinite().all()) and bool(lse.isfinite().all())
