@@ -602,25 +602,28 @@ __global__ __launch_bounds__(CX::NT) void loss_products(
   });
 }
 
-// Rows of dx or dW from the shares' sums, a block a row: row pos[r] of them (r without pos), zero
-// for the rows left out.
+// Rows of dx or dW from the shares' sums, a block a row (two where 2^24 rows would be 2^32 threads):
+// row pos[r] of them (r without pos), zero for the rows left out.
 template <class T>
 __global__ __launch_bounds__(256) void loss_join(const float* __restrict__ sums, uint32_t dp,
                                                  uint32_t splits, uint64_t slice,
                                                  const uint32_t* __restrict__ pos,
                                                  const float* __restrict__ unit, uint32_t d,
-                                                 typename T::elem* out, int64_t ld) {
-  const uint32_t row = blockIdx.x, at = pos ? pos[row] : row;
+                                                 typename T::elem* __restrict__ out, int64_t ld,
+                                                 uint32_t rows) {
   const float mul = *unit;
-  out += (int64_t)row * ld;
-  for (uint32_t c = threadIdx.x * 4; c < d; c += 1024) {
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    if (at != ~0u)
-      for (uint32_t s = 0; s < splits; s++)
-        y += gload<f32x4>(sums + s * slice + (uint64_t)at * dp + c);
+  for (uint32_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const uint32_t at = pos ? pos[row] : row;
+    typename T::elem* const to = out + (int64_t)row * ld;
+    for (uint32_t c = threadIdx.x * 4; c < d; c += 1024) {
+      f32x4 y = {0.f, 0.f, 0.f, 0.f};
+      if (at != ~0u)
+        for (uint32_t s = 0; s < splits; s++)
+          y += gload<f32x4>(sums + s * slice + (uint64_t)at * dp + c);
 #pragma unroll
-    for (uint32_t x = 0; x < 4; x++)
-      if (c + x < d) out[c + x] = T::put(y[x] * mul);
+      for (uint32_t x = 0; x < 4; x++)
+        if (c + x < d) to[c + x] = T::put(y[x] * mul);
+    }
   }
 }
 
@@ -647,6 +650,7 @@ using NarrowDirect = Tile<false, false, 256, 32, 8, 1, 4, true>;
 enum Shape { kLarge, kTrimmed, kMedium, kNarrow };
 
 constexpr uint32_t kCus = 256;
+constexpr uint32_t kMostJoined = 1u << 23;  // blocks of loss_join
 
 uint32_t cdiv(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
 
@@ -868,8 +872,9 @@ int piece_grads(const pots_vocab_loss* a, const Plan& p, const Mat& W, const Mat
                      (uint64_t)p.piece * p.dp, a->dim, dw, a->dw_row);
   POTS_HIP(hipGetLastError());
   if (p.join_w) {
-    hipLaunchKernelGGL((loss_join<T>), dim3(nv), dim3(256), 0, s, f32(p.wsums), p.dp, p.wsplits,
-                       (uint64_t)p.piece * p.dp, nullptr, f32(p.unit), a->dim, dw, a->dw_row);
+    hipLaunchKernelGGL((loss_join<T>), dim3(min(nv, kMostJoined)), dim3(256), 0, s, f32(p.wsums),
+                       p.dp, p.wsplits, (uint64_t)p.piece * p.dp, nullptr, f32(p.unit), a->dim,
+                       dw, a->dw_row, nv);
     POTS_HIP(hipGetLastError());
   }
   return POTS_E_OK;
@@ -905,9 +910,10 @@ int backward(const pots_vocab_loss* a, char* work, hipStream_t s) {
     if (rc) return rc;
   }
   if (a->rows == 0) return POTS_E_OK;
-  hipLaunchKernelGGL((loss_join<T>), dim3(a->rows), dim3(256), 0, s, f32(p.sums), p.dp,
-                     p.splits, (uint64_t)p.rows_pad * p.dp, u32(p.pos), f32(p.unit), a->dim,
-                     reinterpret_cast<typename T::elem*>(a->dx), a->dx_row);
+  hipLaunchKernelGGL((loss_join<T>), dim3(min(a->rows, kMostJoined)), dim3(256), 0, s,
+                     f32(p.sums), p.dp, p.splits, (uint64_t)p.rows_pad * p.dp, u32(p.pos),
+                     f32(p.unit), a->dim, reinterpret_cast<typename T::elem*>(a->dx), a->dx_row,
+                     a->rows);
   POTS_HIP(hipGetLastError());
   return POTS_E_OK;
 }

@@ -61,3 +61,9 @@ def test_losses_of_more_tiles_than_a_launch(driver, rows, vocab, dtype):  # noqa
     done = sum(x * next(v for k, v in area.items() if k in n)
                for n, x, _ in launches if n.startswith("loss_scores"))
     assert rows * vocab <= done <= 1.25 * (rows + 255) * (vocab + 255)
+
+
+@pytest.mark.parametrize("rows, vocab", [(1 << 24, 100), (1 << 20, 1 << 16), (1, 1 << 24)])
+def test_gradients_of_as_many_rows_as_the_loss_takes(driver, rows, vocab):  # noqa: F811
+    (rc, _, launches), = _launches(driver, f"vocab_loss_backward,{rows},64,{vocab},{BF16}")
+    assert rc == 0 and launches[-1][0] == "loss_join<Bf16>"

@@ -75,3 +75,19 @@ def test_loss_of_more_tiles_than_a_launch():
     R.within(loss[some], want["loss"], "loss")
     R.within(lse[some], want["lse"], "lse")
     assert bool(loss.isfinite().all()) and bool(lse.isfinite().all())
+
+
+def test_loss_gradients_of_as_many_rows_as_it_takes():
+    """2^24 rows, whose sums one launch of a block a row could not join."""
+    rows, d, vocab = 1 << 24, 8, 100
+    x, w, t, weights = _loss_inputs(4, BF, rows, d, vocab)
+    _, lse = ops.vocab_loss_forward(x, w, t)
+    dx = torch.full((rows, d), math.nan, dtype=BF, device=DEV)  # what the allocator hands out again
+    del dx
+    dx, dw = ops.vocab_loss_backward(weights, x, w, t, lse)
+    half = rows // 2
+    some = torch.cat([torch.arange(50), torch.arange(half - 50, half + 50),
+                      torch.arange(rows - 50, rows)]).to(DEV)
+    R.within(dx[some], R.vocab_loss(x[some], w, t[some], weights[some])["dx"], "dx")
+    assert bool(dw.isfinite().all()) and not bool(dx.isnan().any())
+    assert bool(((dx == 0).all(1) == ((weights == 0) | (t < 0))).all())
