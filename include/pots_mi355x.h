@@ -431,11 +431,12 @@ typedef struct pots_heads {
 
 /* Softmax attention of `batch` sequences of n positions over their own keys: `heads` query
  * heads, each `heads / kv_heads` consecutive ones sharing a key head, of a head_dim that is a
- * multiple of 8 (a narrower head is one with columns of zeros). Position i sees j where
- * j < length, i < length and (causal) j <= i; lengths is int32 [batch] (values past n count as
- * n, negative ones as 0), or null for n. A position that sees nothing has an output of zero,
- * lse -inf and gradients of zero; what lies past a sequence's length is not read. lse and delta
- * are fp32 [batch, heads, n], natural logarithms. */
+ * multiple of 8 (a narrower head is one with columns of zeros); batch * heads is at most 2^20,
+ * and there are less than 2^24 blocks of 128 rows of all heads (half of that backward for heads
+ * wider than 64). Position i sees j where j < length, i < length and (causal) j <= i; lengths is
+ * int32 [batch] (values past n count as n, negative ones as 0), or null for n. A position that
+ * sees nothing has an output of zero, lse -inf and gradients of zero; what lies past a sequence's
+ * length is not read. lse is fp32 [batch, heads, n], natural logarithms. */
 typedef struct pots_attention {
   pots_heads q, k, v, out;
   pots_heads dout, dq, dk, dv; /* backward only */

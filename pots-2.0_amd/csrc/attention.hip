@@ -756,6 +756,8 @@ bool aligned(const pots_attention* a, const pots_heads& x) {
 
 uint32_t cdiv(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
 
+constexpr uint64_t kMostBlocks = (1u << 24) - 1;  // of 256 threads: less than 2^32 in a launch
+
 // Whether blocks of 128 rows leave compute units without one: blocks of 32 then.
 bool few(uint64_t sequences, uint32_t n) { return sequences * cdiv(n, 128) < 256; }
 
@@ -792,7 +794,7 @@ int forward(const pots_attention* a, hipStream_t s) {
   typedef Shape<T, DP, SPLIT> S;
   const uint32_t tiles = cdiv(a->n, S::R);
   const uint64_t blocks = (uint64_t)a->batch * a->heads * tiles;
-  if (blocks > 0x7FFFFFFFu) return POTS_E_ARG;
+  if (blocks > kMostBlocks) return POTS_E_ARG;
   hipLaunchKernelGGL((attn_fwd<T, DP, SPLIT>), dim3((uint32_t)blocks), dim3(S::NT), 0, s, *a,
                      tiles);
   POTS_HIP(hipGetLastError());
@@ -806,7 +808,7 @@ int backward(const pots_attention* a, char* work, hipStream_t s) {
   const uint64_t qblocks = (uint64_t)a->batch * a->heads * c.tiles;
   const uint64_t kblocks =
       (uint64_t)a->batch * a->kv_heads * c.tiles * c.splits * (S::kApart ? 2 : 1);
-  if (qblocks > 0x7FFFFFFFu || kblocks > 0x7FFFFFFFu) return POTS_E_ARG;
+  if (qblocks > kMostBlocks || kblocks > kMostBlocks) return POTS_E_ARG;
   float* stat = reinterpret_cast<float*>(work);
   float* part = nullptr;
   if (c.splits > 1)

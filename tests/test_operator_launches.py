@@ -67,3 +67,16 @@ def test_losses_of_more_tiles_than_a_launch(driver, rows, vocab, dtype):  # noqa
 def test_gradients_of_as_many_rows_as_the_loss_takes(driver, rows, vocab):  # noqa: F811
     (rc, _, launches), = _launches(driver, f"vocab_loss_backward,{rows},64,{vocab},{BF16}")
     assert rc == 0 and launches[-1][0] == "loss_join<Bf16>"
+
+
+@pytest.mark.parametrize("case, most", [
+    (f"attention_forward,{1 << 20},1,1,{{}},8,{BF16}", 15 * 128),
+    (f"attention_backward,{1 << 20},1,1,{{}},8,{BF16}", 15 * 128),
+    (f"attention_forward,1,{1 << 20},{1 << 20},{{}},128,{F32}", 15 * 128),
+    (f"attention_backward,1,{1 << 20},{1 << 20},{{}},128,{F32}", 7 * 128)])
+def test_attention_of_more_rows_than_a_launch(driver, case, most):  # noqa: F811
+    """Below 2^24 blocks of 128 rows; from there on the sizes are out of range, and nothing is
+    enqueued."""
+    good, bad = _launches(driver, case.format(most), case.format(most + 1))
+    assert good[0] == 0 and good[2]
+    assert bad[0] == E_ARG and not bad[2]
