@@ -45,6 +45,7 @@ _ATTENTION = struct.Struct("<32q2q7If")
 _LOSS = struct.Struct("<12q4I")
 _EMBEDDING = struct.Struct("<5q5If")
 _NO_HEADS = (0, 0, 0, 0)
+_MOST, _LEAST = torch.finfo(torch.float32).max, 2.0**-149  # of fp32, above zero
 
 
 def _dtype(t: torch.Tensor, what: str) -> int:
@@ -72,6 +73,14 @@ def _floats(t: torch.Tensor, device: torch.device, shape: tuple[int, ...],
     if t.dtype != torch.float32 or t.device != device or t.shape != shape:
         raise ValueError(f"{what} must be float32 {tuple(shape)} on {device}")
     return t.contiguous()
+
+
+def _packed(block: struct.Struct, *values) -> bytes:
+    """An argument block. A size past its 32 bits is a size out of range like any other."""
+    try:
+        return block.pack(*values)
+    except struct.error as e:
+        raise ValueError(f"a size is out of range: {e}") from None
 
 
 def _indices(t: torch.Tensor, device: torch.device, what: str) -> torch.Tensor:
@@ -139,8 +148,8 @@ def _attention_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _like(v, q, (b, kv, n, d), "v")
     if scale is None:
         scale = 1.0 / math.sqrt(d)
-    elif not (scale > 0 and math.isfinite(scale)):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    elif not _LEAST <= scale <= _MOST:
+        raise ValueError(f"scale must be positive and finite in fp32, got {scale}")
     if lengths is not None:
         if lengths.dtype != torch.int32 or lengths.shape != (b,) or lengths.device != q.device:
             raise ValueError(f"lengths must be int32 [{b}] on {q.device}")
@@ -176,10 +185,10 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     lse = torch.empty(b, h, n, dtype=torch.float32, device=q.device)
 
     def pack(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bytes:
-        return _ATTENTION.pack(*_heads(q), *_heads(k), *_heads(v), *_heads(out), *_NO_HEADS,
-                               *_NO_HEADS, *_NO_HEADS, *_NO_HEADS, lse.data_ptr(),
-                               0 if lengths is None else lengths.data_ptr(), b, h, k.shape[1], n,
-                               d, code, causal, scale)
+        return _packed(_ATTENTION, *_heads(q), *_heads(k), *_heads(v), *_heads(out), *_NO_HEADS,
+                       *_NO_HEADS, *_NO_HEADS, *_NO_HEADS, lse.data_ptr(),
+                       0 if lengths is None else lengths.data_ptr(), b, h, k.shape[1], n, d, code,
+                       causal, scale)
 
     _call_attention("attention_forward", (q, k, v), d, pack)
     return out if d == own else out[..., :own], lse
@@ -206,10 +215,10 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
 
     def pack(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
              dout: torch.Tensor) -> bytes:
-        return _ATTENTION.pack(*_heads(q), *_heads(k), *_heads(v), *_heads(out), *_heads(dout),
-                               *_heads(dq), *_heads(dk), *_heads(dv), lse.data_ptr(),
-                               0 if lengths is None else lengths.data_ptr(), b, h, kv, n, d, code,
-                               causal, scale)
+        return _packed(_ATTENTION, *_heads(q), *_heads(k), *_heads(v), *_heads(out),
+                       *_heads(dout), *_heads(dq), *_heads(dk), *_heads(dv), lse.data_ptr(),
+                       0 if lengths is None else lengths.data_ptr(), b, h, kv, n, d, code, causal,
+                       scale)
 
     _call_attention("attention_backward", (q, k, v, out, dout), d, pack)
     if d != own:
@@ -273,9 +282,9 @@ def vocab_loss_forward(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     x, w = _matrix(x), _matrix(w)
     loss = torch.empty(rows, dtype=torch.float32, device=x.device)
     lse = torch.empty(rows, dtype=torch.float32, device=x.device)
-    args = _LOSS.pack(x.data_ptr(), w.data_ptr(), targets.data_ptr(), loss.data_ptr(),
-                      lse.data_ptr(), 0, 0, 0, x.stride(0), w.stride(0), 0, 0, rows, dim,
-                      w.shape[0], code)
+    args = _packed(_LOSS, x.data_ptr(), w.data_ptr(), targets.data_ptr(), loss.data_ptr(),
+                   lse.data_ptr(), 0, 0, 0, x.stride(0), w.stride(0), 0, 0, rows, dim, w.shape[0],
+                   code)
     native.get().operator("vocab_loss_forward", args, x.device)
     return loss, lse
 
@@ -292,9 +301,9 @@ def vocab_loss_backward(weights: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
     x, w = _matrix(x), _matrix(w)
     dx = torch.empty(rows, dim, dtype=x.dtype, device=x.device)
     dw = torch.empty(w.shape[0], dim, dtype=x.dtype, device=x.device)
-    args = _LOSS.pack(x.data_ptr(), w.data_ptr(), targets.data_ptr(), 0, lse.data_ptr(),
-                      weights.data_ptr(), dx.data_ptr(), dw.data_ptr(), x.stride(0), w.stride(0),
-                      dim, dim, rows, dim, w.shape[0], code)
+    args = _packed(_LOSS, x.data_ptr(), w.data_ptr(), targets.data_ptr(), 0, lse.data_ptr(),
+                   weights.data_ptr(), dx.data_ptr(), dw.data_ptr(), x.stride(0), w.stride(0),
+                   dim, dim, rows, dim, w.shape[0], code)
     native.get().operator("vocab_loss_backward", args, x.device)
     return dx, dw
 
@@ -333,11 +342,18 @@ def vocab_loss(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
     """``Σ_r weights_r · loss_r`` of :func:`vocab_loss_forward`'s losses, fp32, differentiable
     in ``x``, ``w`` and ``weights``; rows of weight zero count for nothing, whatever their loss (the
     gradient of such a weight is the row's loss, or zero where that is not finite)."""
+    if x.dim() != 2:
+        raise ValueError("x must be [rows, dim]")
     weights = _floats(weights, x.device, (x.shape[0],), "weights")
     return _VocabLoss.apply(x, w, targets, weights)
 
 
 # ---- the embedding --------------------------------------------------------------------------
+
+def _check_scale(scale: float) -> None:
+    if not -_MOST <= scale <= _MOST:
+        raise ValueError(f"scale must be finite in fp32, got {scale}")
+
 
 def embedding_forward(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0
                       ) -> torch.Tensor:
@@ -346,13 +362,14 @@ def embedding_forward(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError("table must be [vocab, dim], neither of them 0")
     code = _dtype(table, "table")
+    _check_scale(scale)
     ids = _indices(ids, table.device, "ids")
     _on_gpu(table)
     table = _matrix(table)
     out = torch.empty(*ids.shape, table.shape[1], dtype=table.dtype, device=table.device)
-    args = _EMBEDDING.pack(ids.data_ptr(), table.data_ptr(), out.data_ptr(), table.stride(0),
-                           table.shape[1], ids.numel(), table.shape[1], table.shape[0], code, 0,
-                           scale)
+    args = _packed(_EMBEDDING, ids.data_ptr(), table.data_ptr(), out.data_ptr(),
+                   table.stride(0), table.shape[1], ids.numel(), table.shape[1], table.shape[0],
+                   code, 0, scale)
     native.get().operator("embedding_forward", args, table.device)
     return out
 
@@ -364,12 +381,13 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, vocab: int, *,
     table already has) it is added there, touching only the rows that occur, and that tensor is
     returned. Ids outside the table add to nothing."""
     code = _dtype(dout, "dout")
+    _check_scale(scale)
     ids = _indices(ids, dout.device, "ids")
     dim = dout.shape[-1] if dout.dim() else 0
     if dim < 1 or dout.shape[:-1] != ids.shape:
         raise ValueError(f"dout must be {tuple(ids.shape)} rows, got {tuple(dout.shape)}")
-    if vocab < 1:
-        raise ValueError(f"vocab must be positive, got {vocab}")
+    if not 1 <= vocab <= 1 << 30:
+        raise ValueError(f"vocab must be in [1, 2^30], got {vocab}")
     if add_to is not None:
         _like(add_to, dout, (vocab, dim), "add_to")
         if add_to.stride(1) != 1 or add_to.stride(0) < dim:
@@ -379,9 +397,9 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, vocab: int, *,
     table = add_to
     if table is None:
         table = torch.empty(vocab, dim, dtype=dout.dtype, device=dout.device)
-    args = _EMBEDDING.pack(ids.data_ptr(), table.data_ptr(), rows.data_ptr(), table.stride(0),
-                           rows.stride(0), ids.numel(), dim, vocab, code, add_to is not None,
-                           scale)
+    args = _packed(_EMBEDDING, ids.data_ptr(), table.data_ptr(), rows.data_ptr(),
+                   table.stride(0), rows.stride(0), ids.numel(), dim, vocab, code,
+                   add_to is not None, scale)
     native.get().operator("embedding_backward", args, dout.device)
     return table
 

@@ -223,3 +223,66 @@ def test_the_sum_of_many_losses(n):
     # (no order of adding up n values is further off)
     assert got.shape == () and abs(float(got) - float(t.double().sum())) <= \
         n * 2.0**-24 * float(t.double().abs().sum())
+
+
+class _NoLibrary:
+    @staticmethod
+    def get():
+        return _NoLibrary
+
+    @staticmethod
+    def operator(name, args, device):
+        raise AssertionError("out-of-range sizes reached the library")
+
+
+@pytest.fixture
+def without_gpu(monkeypatch):
+    """The calls' own checks on tensors without memory."""
+    monkeypatch.setattr(ops, "_on_gpu", lambda t: None)
+    monkeypatch.setattr(ops, "native", _NoLibrary)
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+BIG = 1 << 32
+
+
+@pytest.mark.parametrize("scale", [1e39, 3.5e38, 1e-60])
+def test_attention_refuses_scales_that_fp32_does_not_hold(without_gpu, scale):
+    q, k = _meta(*Q), _meta(*KV)
+    with pytest.raises(ValueError, match="scale"):
+        ops.attention_forward(q, k, k, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        ops.attention_backward(q, q, k, k, q, _meta(2, 4, 5, dtype=torch.float32), scale=scale)
+
+
+@pytest.mark.parametrize("scale", [1e39, -3.5e38, math.inf, math.nan])
+def test_embedding_refuses_scales_that_fp32_does_not_hold(without_gpu, scale):
+    ids = _meta(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="scale"):
+        ops.embedding_forward(ids, _meta(5, 4), scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        ops.embedding_backward(ids, _meta(3, 4), 5, scale=scale)
+
+
+def test_sizes_past_32_bits_are_refused(without_gpu):
+    ids, x = _meta(BIG, dtype=torch.int64), _meta(BIG, 1)
+    q, f = _meta(1, 1, BIG, 8), _meta(BIG, dtype=torch.float32)
+    for call in (lambda: ops.attention_forward(q, q, q),
+                 lambda: ops.attention_forward(q[..., :3], q[..., :3], q[..., :3]),
+                 lambda: ops.attention_backward(q, q, q, q, q, f.view(1, 1, BIG)),
+                 lambda: ops.vocab_loss_forward(x, _meta(5, 1), ids),
+                 lambda: ops.vocab_loss_forward(_meta(3, 1), x, _meta(3, dtype=torch.int64)),
+                 lambda: ops.vocab_loss_backward(f, x, _meta(5, 1), ids, f),
+                 lambda: ops.embedding_forward(ids, _meta(5, 1)),
+                 lambda: ops.embedding_backward(ids, x, 5),
+                 lambda: ops.embedding_backward(ids[:3], x[:3], BIG)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_a_loss_of_no_matrix_is_refused():
+    with pytest.raises(ValueError):
+        ops.vocab_loss(torch.tensor(1.0), _t(5, 4), _t(3, dtype=torch.int64), _t(3))
