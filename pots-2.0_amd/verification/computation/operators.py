@@ -390,7 +390,7 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, vocab: int, *,
         raise ValueError(f"vocab must be in [1, 2^30], got {vocab}")
     if add_to is not None:
         _like(add_to, dout, (vocab, dim), "add_to")
-        if add_to.stride(1) != 1 or add_to.stride(0) < dim:
+        if dim > 1 and add_to.stride(1) != 1 or vocab > 1 and add_to.stride(0) < dim:
             raise ValueError("add_to must have rows of consecutive values, each its own")
     _on_gpu(dout)
     rows = _matrix(dout.reshape(-1, dim))

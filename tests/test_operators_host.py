@@ -286,3 +286,19 @@ def test_sizes_past_32_bits_are_refused(without_gpu):
 def test_a_loss_of_no_matrix_is_refused():
     with pytest.raises(ValueError):
         ops.vocab_loss(torch.tensor(1.0), _t(5, 4), _t(3, dtype=torch.int64), _t(3))
+
+
+def test_added_gradients_of_single_values_and_single_rows(monkeypatch, without_gpu):
+    """One value a row has no distance to the next one, and one row none to another row."""
+    calls = []
+    monkeypatch.setattr(_NoLibrary, "operator",
+                        staticmethod(lambda name, args, device: calls.append(name)))
+    ids = _meta(3, dtype=torch.int64)
+    for dim, into in ((1, _meta(1, 5).t()), (4, _meta(5, 4)), (4, _meta(4).as_strided((1, 4), (0, 1))),
+                      (1, _meta(8)[:1, None].as_strided((1, 1), (0, 0)))):
+        got = ops.embedding_backward(ids, _meta(3, dim), into.shape[0], add_to=into)
+        assert got is into
+    assert calls == ["embedding_backward"] * 4
+    for into in (_meta(4, 5).t(), _meta(4).expand(5, 4), _meta(8).as_strided((5, 1), (0, 1))):
+        with pytest.raises(ValueError):
+            ops.embedding_backward(ids, _meta(3, into.shape[1]), 5, add_to=into)

@@ -50,6 +50,22 @@ def test_embedding_gradient_of_a_table_past_a_launch(tokens):
         assert not bool(part.any())  # (a NaN is not zero)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_embedding_added_to_single_values_and_to_a_single_row(dtype):
+    g = _gen(5)
+    ids = torch.randint(-1, 301, (700,), generator=g)
+    one = torch.randn(700, 1, generator=g).to(dtype)
+    into = torch.randn(1, 300, generator=g).to(dtype).to(DEV).t()
+    want = R.embedding(ids, one, 300, 1.0, into)
+    assert ops.embedding_backward(ids.to(DEV), one.to(DEV), 300, add_to=into) is into
+    R.within(into, want, "single values")
+    rows = torch.randn(700, 40, generator=g).to(dtype)
+    into = torch.randn(40, generator=g).to(dtype).to(DEV).as_strided((1, 40), (0, 1))
+    want = R.embedding(ids, rows, 1, 1.0, into)
+    ops.embedding_backward(ids.to(DEV), rows.to(DEV), 1, add_to=into)
+    R.within(into, want, "a single row")
+
+
 # ---- the loss -------------------------------------------------------------------------------
 
 def _loss_inputs(seed, dtype, rows, d, vocab):
