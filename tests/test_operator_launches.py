@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import pytest
 
+import test_operators_sizes_gpu as sizes
 from test_host_sanitize import _run, driver  # noqa: F401  (a fixture)
 
 F32, BF16 = 0, 1
@@ -80,3 +81,35 @@ def test_attention_of_more_rows_than_a_launch(driver, case, most):  # noqa: F811
     good, bad = _launches(driver, case.format(most), case.format(most + 1))
     assert good[0] == 0 and good[2]
     assert bad[0] == E_ARG and not bad[2]
+
+
+@pytest.mark.parametrize("case", sizes.LOSSES)
+def test_what_the_sizes_of_the_loss_reach(driver, case):  # noqa: F811
+    dtype, rows, d, vocab, scores, dx, dw, forward, backward = case
+    what = f"{rows},{d},{vocab},{BF16 if dtype == sizes.BF else F32}"
+    a, b = (x[2] for x in _launches(driver, f"vocab_loss_forward,{what}",
+                                    f"vocab_loss_backward,{what}"))
+    tiles = [n for n, _, _ in a if n.startswith("loss_scores")]
+    assert len(tiles) == forward and all(f"Tile<false, false, {scores}" in n for n in tiles)
+    tiles = [n for n, _, _ in b if n.startswith("loss_products")]
+    assert len(tiles) == backward
+    assert all(f"Tile<true, false, {dx}" in n and f"Tile<true, true, {dw}" in n for n in tiles)
+
+
+def test_the_sizes_of_the_loss_reach_every_tile():
+    assert {c[4] for c in sizes.LOSSES} == {sizes.DIRECT, sizes.NARROW_DIRECT, sizes.LARGE,
+                                            sizes.MEDIUM, sizes.NARROW}
+    assert {c[5] for c in sizes.LOSSES} == {sizes.LARGE, sizes.TRIMMED, sizes.MEDIUM,
+                                            sizes.NARROW_X}
+    for tile in (sizes.LARGE, sizes.TRIMMED):  # those of whole batches, in both types
+        assert {c[0] for c in sizes.LOSSES if c[5] == tile} == {sizes.BF, sizes.F32}
+
+
+@pytest.mark.parametrize("tokens, d, vocab", sizes.TABLES)
+def test_what_the_sizes_of_the_tables_reach(driver, tokens, d, vocab):  # noqa: F811
+    (_, _, launches), = _launches(driver, f"embedding_backward,{tokens},{d},{vocab},{F32},0")
+    assert vocab * d * 4 > 256 << 20
+    by = {n.split("<")[0]: x for n, x, _ in launches}
+    # blocks beyond those of the tokens, 32 to one that orders: zeros are written there
+    assert by["embed_order"] > -(-tokens // 32) and "embed_join" in by
+    assert ("embed_merge" in by) == (tokens > 16384)

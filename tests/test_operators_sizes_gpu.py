@@ -50,6 +50,22 @@ def test_embedding_gradient_of_a_table_past_a_launch(tokens):
         assert not bool(part.any())  # (a NaN is not zero)
 
 
+# tokens, dim, vocab of fp32 tables past the last cache, whose zeros are written beside the ordering
+# (and the merge), the sums and the joins
+TABLES = [(300, 1024, 70001), (5000, 1024, 70001), (20000, 700, 110003)]
+
+
+@pytest.mark.parametrize("tokens, d, vocab", TABLES)
+def test_embedding_gradient_of_large_tables_beside_the_ordering(tokens, d, vocab):
+    g = _gen(tokens)
+    ids = (torch.rand(tokens, generator=g, dtype=torch.float64) ** 3 * vocab).long()
+    ids[0], ids[1], ids[2], ids[3] = vocab - 1, 0, vocab, -1
+    dout = torch.randn(tokens, d, generator=g)
+    torch.full((vocab, d), math.nan, device=DEV)  # what the allocator hands out again
+    got = ops.embedding_backward(ids.to(DEV), dout.to(DEV), vocab, scale=0.5)
+    R.within(got, R.embedding(ids, dout, vocab, 0.5), "gradient")
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 def test_embedding_added_to_single_values_and_to_a_single_row(dtype):
     g = _gen(5)
@@ -77,6 +93,39 @@ def _loss_inputs(seed, dtype, rows, d, vocab):
     weights[torch.rand(rows, generator=g, device=DEV) < 0.25] = 0
     t[1], t[rows // 2], t[rows - 1] = -100, vocab - 1, vocab - 2
     return x, w, t, weights
+
+
+# dtype, rows, dim, vocab; then what they reach: the tiles of the forward pass, of the backward
+# pass's two products, and the pieces of the vocabulary each way.
+DIRECT, NARROW_DIRECT = "128u, 64u, 4u, 1u, 2u, true", "256u, 32u, 8u, 1u, 4u, true"
+LARGE, MEDIUM, NARROW = "256u, 256u", "128u, 128u", "256u, 32u, 8u, 1u, 4u, false"
+TRIMMED, NARROW_X = "192u, 256u", "256u, 32u, 8u, 1u, 2u"
+LOSSES = [
+    (BF, 300, 64, 32769, LARGE, TRIMMED, TRIMMED, 1, 1),
+    (F32, 300, 64, 32769, DIRECT, TRIMMED, TRIMMED, 1, 1),
+    (BF, 300, 256, 32769, LARGE, LARGE, LARGE, 1, 1),
+    (F32, 300, 256, 32769, DIRECT, LARGE, LARGE, 1, 1),
+    (BF, 1100, 1536, 17001, LARGE, LARGE, LARGE, 1, 1),
+    (F32, 1024, 576, 49152, LARGE, TRIMMED, TRIMMED, 1, 1),
+    (F32, 900, 1001, 20003, LARGE, LARGE, LARGE, 1, 1),
+    # several pieces, the last one odd
+    (F32, 2049, 64, 90001, LARGE, TRIMMED, TRIMMED, 1, 3),
+    (BF, 4097, 200, 66001, LARGE, LARGE, LARGE, 1, 2),
+    (F32, 33, 2001, 46001, MEDIUM, MEDIUM, MEDIUM, 2, 2),
+    (F32, 7, 64, 360001, NARROW_DIRECT, NARROW_X, LARGE, 1, 2),
+    (F32, 7, 2001, 46001, NARROW, NARROW_X, LARGE, 2, 2),
+    (BF, 100, 64, 1200001, MEDIUM, MEDIUM, MEDIUM, 1, 2),
+]
+
+
+@pytest.mark.parametrize("dtype, rows, d, vocab", [case[:4] for case in LOSSES])
+def test_loss_on_every_tile_and_over_pieces(dtype, rows, d, vocab):
+    x, w, t, weights = _loss_inputs(rows + d, dtype, rows, d, vocab)
+    loss, lse = ops.vocab_loss_forward(x, w, t)
+    dx, dw = ops.vocab_loss_backward(weights, x, w, t, lse)
+    want = R.vocab_loss(x, w, t, weights)
+    for name, got in (("loss", loss), ("lse", lse), ("dx", dx), ("dw", dw)):
+        R.within(got, want[name], name)
 
 
 def test_loss_of_more_tiles_than_a_launch():
