@@ -544,3 +544,46 @@ def test_refusals_on_the_gpu(shape):
             ops.attention_forward(q, k[..., :8], v)
         else:
             ops.attention_forward(q, k.cpu(), v)
+
+
+# ---- what else autograd and strides do ---------------------------------------------------------
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_only_the_tensor_that_wants_a_gradient_gets_one(which):
+    q, k, v, g, x, w, t, wt, ids, rows = _pass_inputs(48, F32)
+    out, lse = ops.attention_forward(q, k, v)
+    want = ops.attention_backward(g, q, k, v, out, lse)[which]
+    (q, k, v)[which].requires_grad_()
+    (ops.attention(q, k, v) * g).sum().backward()
+    for i, a in enumerate((q, k, v)):
+        assert (a.grad is None) == (i != which)
+    assert torch.equal((q, k, v)[which].grad, want)
+    _, lse = ops.vocab_loss_forward(x, w, t)
+    want = (*ops.vocab_loss_backward(wt, x, w, t, lse), ops.vocab_loss_forward(x, w, t)[0])[which]
+    (x, w, wt)[which].requires_grad_()
+    ops.vocab_loss(x, w, t, wt).backward()
+    for i, a in enumerate((x, w, wt)):
+        assert (a.grad is None) == (i != which)
+    assert torch.equal((x, w, wt)[which].grad, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_embedding_of_a_transposed_table(dtype):
+    g = _gen(49)
+    table = _rand(g, 41, 50, dtype=dtype).t()
+    ids = torch.randint(-2, 60, (3, 40), generator=g).to(DEV)
+    inside = (ids >= 0) & (ids < 50)
+    out = ops.embedding_forward(ids, table)
+    assert table.shape == (50, 41) and 0 < int(inside.sum()) < 120
+    assert torch.equal(out[inside], table[ids[inside]]) and bool(out[~inside].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_loss_weights_gradient_against_the_formula(dtype):
+    x, w, t, wt = _loss_inputs(50, dtype, 70, 64, 300)
+    x[69], wt[69] = math.nan, 0.0
+    wt.requires_grad_()
+    (0.5 * ops.vocab_loss(x, w, t, wt)).backward()
+    want, bound = R.vocab_loss(x[:69], w, t[:69], wt[:69].detach())["loss"]
+    R.within(wt.grad[:69], (0.5 * want, 0.5 * bound), "the weights' gradient")
+    assert float(wt.grad[69]) == 0.0 and int((wt[:69] == 0).sum()) > 0
