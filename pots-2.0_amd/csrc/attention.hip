@@ -586,57 +586,45 @@ __device__ __forceinline__ void dkv_block(
   const float c = a.scale * kLog2e;
   uint32_t q0 = first;
   auto step = [&](const elem* s_q, const elem* s_g, const float* s_stat) {
-    constexpr uint32_t C = 1;
 #pragma unroll
-    for (uint32_t y = 0; y < U; y += C) {
-      const uint32_t u0 = SPLIT ? wave : y, qu = q0 + 32 * u0;
-      if (qu >= len || kw >= len || (a.causal && qu + 32 * C - 1 < kw)) continue;
-      f32x16 s[C], dp[C];
+    for (uint32_t y = 0; y < U; y++) {
+      const uint32_t u = SPLIT ? wave : y, qu = q0 + 32 * u;
+      if (qu >= len || kw >= len || (a.causal && qu + 31 < kw)) continue;
+      f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-      for (uint32_t u = 0; u < C; u++) {
-        s[u] = zero16();
-        dp[u] = zero16();
+      for (uint32_t ks = 0; ks < KS; ks++) {
+        s = mma(R::row(s_q, 32 * u + i, 16 * ks + 8 * h), kf[ks], s);
+        if (kDk) dp = mma(R::row(s_g, 32 * u + i, 16 * ks + 8 * h), vf[ks], dp);
+      }
 #pragma unroll
-        for (uint32_t ks = 0; ks < KS; ks++) {
-          s[u] = mma(R::row(s_q, 32 * (u0 + u) + i, 16 * ks + 8 * h), kf[ks], s[u]);
-          if (kDk) dp[u] = mma(R::row(s_g, 32 * (u0 + u) + i, 16 * ks + 8 * h), vf[ks], dp[u]);
+      for (uint32_t g = 0; g < 4; g++) {
+        const float* st = s_stat + 32 * u + 8 * g + 4 * h;
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(st);
+        const f32x4 dl = *reinterpret_cast<const f32x4*>(st + kStat);
+#pragma unroll
+        for (uint32_t x = 0; x < 4; x++) {
+          const uint32_t r = 4 * g + x;
+          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ls[x]));
+          if (kDk) dp[r] = s[r] * (dp[r] - dl[x]);
+        }
+      }
+      if (kw + 32 > len || qu + 32 > len || (a.causal && qu < kw + 31)) {
+#pragma unroll
+        for (uint32_t r = 0; r < 16; r++) {
+          const uint32_t q = qu + d_row(r, h);
+          if (key >= len || q >= len || (a.causal && q < key)) s[r] = dp[r] = 0.f;
         }
       }
 #pragma unroll
-      for (uint32_t u = 0; u < C; u++)
+      for (uint32_t t = 0; t < 2; t++) {
+        const frag p = T::pack(kDv ? s : dp, 8 * t), ds = T::pack(dp, 8 * t);
 #pragma unroll
-        for (uint32_t g = 0; g < 4; g++) {
-          const float* st = s_stat + 32 * (u0 + u) + 8 * g + 4 * h;
-          const f32x4 ls = *reinterpret_cast<const f32x4*>(st);
-          const f32x4 dl = *reinterpret_cast<const f32x4*>(st + kStat);
-#pragma unroll
-          for (uint32_t x = 0; x < 4; x++) {
-            const uint32_t r = 4 * g + x;
-            s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], c, -ls[x]));
-            if (kDk) dp[u][r] = s[u][r] * (dp[u][r] - dl[x]);
-          }
+        for (uint32_t db = 0; db < NB; db++) {
+          const uint32_t r0 = 32 * u + 16 * t;
+          if (kDv) dv[db] = mma(R::col(s_g, r0, 32 * db, lane), p, dv[db]);
+          if (kDk) dk[db] = mma(R::col(s_q, r0, 32 * db, lane), ds, dk[db]);
         }
-      if (kw + 32 > len || qu + 32 * C > len || (a.causal && qu < kw + 31)) {
-#pragma unroll
-        for (uint32_t u = 0; u < C; u++)
-#pragma unroll
-          for (uint32_t r = 0; r < 16; r++) {
-            const uint32_t q = qu + 32 * u + d_row(r, h);
-            if (key >= len || q >= len || (a.causal && q < key)) s[u][r] = dp[u][r] = 0.f;
-          }
       }
-#pragma unroll
-      for (uint32_t u = 0; u < C; u++)
-#pragma unroll
-        for (uint32_t t = 0; t < 2; t++) {
-          const frag p = T::pack(kDv ? s[u] : dp[u], 8 * t), ds = T::pack(dp[u], 8 * t);
-#pragma unroll
-          for (uint32_t db = 0; db < NB; db++) {
-            const uint32_t r0 = 32 * (u0 + u) + 16 * t;
-            if (kDv) dv[db] = mma(R::col(s_g, r0, 32 * db, lane), p, dv[db]);
-            if (kDk) dk[db] = mma(R::col(s_q, r0, 32 * db, lane), ds, dk[db]);
-          }
-        }
     }
     q0 = q0 + QT < len ? q0 + QT : first;
   };
