@@ -452,10 +452,10 @@ uint64_t pots_attention_backward_work(const pots_attention *a);
 int pots_attention_backward(const pots_attention *a, void *work, void *stream);
 
 /* Softmax cross entropy of feature rows x [rows, dim] against a vocabulary matrix w
- * [vocab, dim]: loss_r = lse_r - x_r.w_t, fp32, with t the row's int64 target; 0 where t < 0, NaN where
- * t >= vocab. Backward: dx and dw of sum_r weights_r loss_r; a row of weight zero or without a
+ * [vocab, dim]: loss_r = lse_r - x_r.w_t, fp32, with t the row's int64 target; 0 where t < 0, NaN
+ * where t >= vocab. Backward: dx and dw of sum_r weights_r loss_r; a row of weight zero or without a
  * target counts for nothing, whatever its features. Rows of x, w, dx and dw are `*_row`
- * elements apart. */
+ * elements apart. Up to 2^24 rows and vocabulary entries and 2^16 columns. */
 typedef struct pots_vocab_loss {
   const void *x, *w;
   const int64_t *targets;
@@ -472,9 +472,10 @@ uint64_t pots_vocab_loss_backward_work(const pots_vocab_loss *a);
 int pots_vocab_loss_backward(const pots_vocab_loss *a, void *work, void *stream);
 
 /* Rows of a table [vocab, dim] by token, times scale: out_i = scale * table[ids_i] (NaN where
- * ids_i is outside the table). Backward: table_v (+)= scale * the sum of rows_i over ids_i = v,
- * taken in the order of i in fp32; with `add` it is added to what the table holds, without it
- * every row is written. An id outside the table adds to nothing. */
+ * ids_i is outside the table). Backward: table_v (+)= scale * the sum of rows_i over ids_i = v, in
+ * fp32, added up in runs of consecutive i and the runs in order; with `add` it is added to what the
+ * table holds, without it every row is written. An id outside the table adds to nothing. Up to 2^24
+ * tokens, 2^30 rows and 2^20 columns. */
 typedef struct pots_embedding {
   const int64_t *ids;
   void *table;

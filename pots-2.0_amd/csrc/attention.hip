@@ -20,17 +20,25 @@
 // heads leave attn_dkv with few blocks: then the query heads of a group are split over blocks, each
 // with fp32 sums of its own that attn_fold adds in order.
 //
-// Bound, for long sequences in bf16, by the exponentials and the other vector work beside the
-// products (two waves a SIMD take turns), and by LDS reads, one fragment for each product. The 1.5B
-// shape (48 sequences of 2048 x 128, causal; products of the half that is seen): attn_fwd 74 us, 0.70
-// PFLOP/s; attn_dq 95 us, 0.81; attn_dkv 190 us, 0.68; the 0.5B shape (112 of 1024 x 64): 29, 39
-// and 57 us. fp32 is bound by its matrix instructions, a sixteenth of bf16's rate. Tiles that went
-// through registers into padded LDS, with no tile on its way, took 159, 207 and 467 us.
+// Bound, for long sequences in bf16, by no unit alone: the 1.5B shape (48 sequences of 2048 x 128,
+// causal; products of the half that is seen) keeps the matrix cores busy for 0.31 of the cycles in
+// attn_fwd, 0.38 in attn_dq and 0.32 in attn_dkv, issues vector instructions for about 0.43, 0.31
+// and 0.24 (an exponential as four; in attn_fwd the maximum and its rescale too), and reads LDS
+// for 0.16 to 0.21, without bank conflicts. Two waves a SIMD take turns at them, and in attn_dkv
+// they wait for a tile or for each other for half of their time. attn_fwd 74 us, 0.70 PFLOP/s; attn_dq 95 us,
+// 0.81; attn_dkv 190 us, 0.68; the 0.5B shape (112 of 1024 x 64): 29, 39 and 57 us. fp32 is bound by
+// its matrix instructions, a sixteenth of bf16's rate, and small steps by how few blocks they have.
+// Tiles that went through registers into padded LDS, with no tile on its way, took 159, 207 and
+// 467 us.
 //
-// Roundings: bf16 p and ds (the right operands of the second products) are rounded to bf16, off by
-// at most 2^-8 of each term of a sum whose result is rounded the same, and D is taken from out as
-// it was rounded, but where a row sees few keys (attn_dq); scores, statistics and sums are fp32. A value that is not finite, inside its sequence's length, may reach every row of
-// its tile (zero times infinity); what lies past a length is never read.
+// Roundings: bf16 p and ds (the right operands of the second products) are rounded to bf16, since the
+// matrix cores take no product of bf16 and fp32: off by at most 2^-8 of each term of a sum whose
+// result is rounded the same. The gradients of the 1.5B shape are off by 2.4e-3 of their norm, 1.7e-3
+// with that last rounding alone, its output by 2.0e-3 and 1.6e-3. D is taken from out as it was
+// rounded, but where a row sees few keys (attn_dq). Scores, statistics and sums are fp32.
+//
+// A value that is not finite, inside its sequence's length, may reach every row of its tile (zero
+// times infinity); what lies past a length is never read.
 #include <math.h>
 
 #include "common.h"
@@ -190,10 +198,12 @@ __device__ __forceinline__ void unit_of(uint32_t seqs, uint32_t* seq, uint32_t* 
 // through the other side's tiles of 64 (32 in fp32) together. Split: where that leaves compute
 // units without a block, a block has 32 rows and each wave takes its own 32 of a tile's 128; the
 // waves' sums are joined at the end, in order. A split block loads a tile when it has done with the
-// one before: its sequences are short, and two blocks to a compute unit cover for each other. The
-// 135M decoder's layer (fp32, 36 query heads' sequences of 256), us:
-// blocks of one wave 24 (attn_fwd), 32 (attn_dq) and 47 (attn_dkv), split ones 14, 21 and 22;
-// two sequences of 675 x 128 in fp32 56, 78 and 80 with two waves and a tile ahead, 37, 51 and 49.
+// one before: its sequences are short, and where two blocks fit a compute unit (bf16, but attn_dkv
+// of heads past 96; fp32 heads to 64, in attn_dkv to 32) they cover for each other. Elsewhere the loads
+// show, but a second tile would leave no room for four waves. The 135M decoder's layer (fp32, 36
+// query heads' sequences of 256), us: blocks of one wave 24 (attn_fwd), 32 (attn_dq) and 47 (attn_dkv),
+// split ones 14, 21 and 22; two sequences of 675 x 128 in fp32 56, 78 and 80 with two waves and a tile
+// ahead, 37, 51 and 49.
 template <class T, uint32_t DP, bool SPLIT>
 struct Shape {
   static constexpr uint32_t kWide = DP * sizeof(typename T::elem);  // bytes of a row

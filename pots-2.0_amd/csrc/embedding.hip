@@ -6,11 +6,12 @@
 // TB/s, part of it out of the last cache), the dense gradient of the same 185 us (983 MB, 5.3 TB/s,
 // which a copy does not exceed). Few tokens are bound by the launches, 5 us each.
 //
-// The gradient's sums are taken in the order of the positions, so no result depends on atomics: the
-// tokens are sorted by (id, position), the sorted list is cut into equal pieces whatever the ids'
-// frequencies, and each piece adds up its rows in registers. A row whose tokens lie within one
-// piece is written right away; one that crosses pieces leaves fp32 sums that embed_join adds in
-// order.
+// No result depends on atomics: the tokens are sorted by (id, position), the sorted list is cut into
+// equal pieces whatever the ids' frequencies, and each piece adds up its rows in registers, in the
+// order of the positions. A row whose tokens lie within one piece is written right away; one that
+// crosses pieces leaves fp32 sums that embed_join adds in order. (A dense gradient's pieces may be
+// longer than those of one that is added to a table: cut. The same tokens' sums may then differ in
+// their last bits.)
 //
 // Sorting: the keys (id above position, so all differ) are placed by counting. A block holds 32 of
 // them and counts the smaller ones of their run, two instructions a pair: up to 16384 tokens are

@@ -376,10 +376,11 @@ def embedding_forward(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 
 
 def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, vocab: int, *,
                        scale: float = 1.0, add_to: torch.Tensor | None = None) -> torch.Tensor:
-    """The table's gradient ``[vocab, dim]``: row v is ``scale`` times the sum, in fp32 and in
-    the order of the positions, of ``dout``'s rows whose id is v. With ``add_to`` (a gradient the
-    table already has) it is added there, touching only the rows that occur, and that tensor is
-    returned. Ids outside the table add to nothing."""
+    """The table's gradient ``[vocab, dim]``: row v is ``scale`` times the sum in fp32 of
+    ``dout``'s rows whose id is v, added up in runs of consecutive positions and the runs in order
+    (whose length is the call's: a dense and an added gradient of the same tokens may differ in their
+    last bits). With ``add_to`` (a gradient the table already has) it is added there, touching only
+    the rows that occur, and that tensor is returned. Ids outside the table add to nothing."""
     code = _dtype(dout, "dout")
     _check_scale(scale)
     ids = _indices(ids, dout.device, "ids")
