@@ -17,7 +17,8 @@
 // value is the exact sum of three bf16 terms (take_term), the second at most 2^-8 and the third 2^-16
 // of it. A product of two takes the six products of terms above 2^-24 of it; the three left out are
 // together below 2^-23. At six bf16 products' cost that is 1.3 times as fast as the library's
-// fp32 product (154 TFLOP/s); few rows forward are multiplied as fp32. G is rounded to the inputs'
+// fp32 product (154 TFLOP/s); few rows forward are multiplied as fp32. (An infinite value meets zero
+// terms: its rows' scores are NaN, not infinite, where they are made of terms.) G is rounded to the inputs'
 // type as an operand: half a step of bf16, 2^-8, of each term of sums that are rounded to bf16
 // themselves.
 //

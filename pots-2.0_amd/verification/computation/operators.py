@@ -14,7 +14,7 @@ either to memory. These calls run such a pass on the same model, with the kernel
 Tensors are on the GPU, in fp32 or bf16; sums, softmax statistics and losses are fp32. Calls
 enqueue on the current stream and never wait for the GPU; outputs and scratch come from torch's
 allocator on that stream, so a tensor made on another stream needs the usual
-``wait_stream``. Results are the same bits on every run. Wrong shapes, types and devices raise
+``wait_stream``. Results are the same bits on every run. Wrong shapes, types, sizes and devices raise
 ``ValueError``; ids and targets are not read on the host, so those outside the vocabulary show
 in the result instead (NaN; a negative target is a row without a loss).
 ``verification.computation.instances.decoder.DecoderComputation.uncaptured_loss`` runs all three.

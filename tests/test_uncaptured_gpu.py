@@ -68,3 +68,20 @@ def test_a_step_of_training_lowers_the_loss():
         for p in model.parameters():
             p -= 0.5 * p.grad
         assert float(c.uncaptured_loss(model, records)) < float(first.detach())
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_checkpointed_layers_give_the_same_gradients(dtype, reentrant):
+    """The layers run again in the backward pass, with the same operators: the same bits."""
+    c, model, records = _step(True, True, dtype)
+    loss = c.uncaptured_loss(model, records)
+    want = _grads(model, loss)
+    model.train()
+    model.gradient_checkpointing_enable(
+        gradient_checkpointing_kwargs={"use_reentrant": reentrant})
+    again = c.uncaptured_loss(model, records)
+    assert torch.equal(again.detach(), loss.detach())
+    got = _grads(model, again)
+    for name, g in want.items():
+        assert torch.equal(got[name], g), name
