@@ -3,9 +3,9 @@ transposed right operand.
 
 transformers' eager attention (the reference's choice, decoder.py:568-598) forms
 ``Q̃·K̃ᵀ`` with ``K̃ᵀ`` as a transposed view, and autograd's backward of every batched product
-``A·B`` forms ``δC·Bᵀ`` with ``Bᵀ`` a transposed view. On this pool's MI355X boxes the platform
-guidance is that bf16 batched products (``torch.bmm`` and what calls it) have faulted the GPU
-when their right operand was a transposed view, so the bf16 prover cannot run them. This core
+``A·B`` forms ``δC·Bᵀ`` with ``Bᵀ`` a transposed view. Batched products in bf16 (``torch.bmm``
+and what calls it) have faulted MI355X GPUs when their right operand was a transposed view, so the
+bf16 prover cannot run them. This core
 computes the same six products of the reference's inventory (``S``, ``O``, ``dA``, ``dV``,
 ``dQ``, ``dK``; reference decoder.py:416-471) with every right operand contiguous:
 
