@@ -490,6 +490,106 @@ int pots_embedding_forward(const pots_embedding *a, void *stream);
 uint64_t pots_embedding_backward_work(const pots_embedding *a);
 int pots_embedding_backward(const pots_embedding *a, void *work, void *stream);
 
+/* ---- What a training step does between its products, and after them -----------------------
+ *
+ * The residual's addition with the root-mean-square norm, rotary turns of queries and keys, the
+ * gated activation, and the clipped update of the weights; as above: device memory, calls that
+ * enqueue and allocate nothing, `work` of the *_work call's size, results that do not depend on
+ * the order of blocks. Rows start anywhere that an element may: `*_row` elements apart, the values
+ * of a row consecutive. */
+
+#define POTS_OP_E4M3 2 /* outputs of pots_rms_norm_quantized alone */
+#define POTS_OP_INT8 3
+#define POTS_OP_F64 4 /* the frequencies of pots_rotary alone */
+
+/* t = x + residual (rounded to total_type; x itself where residual is null, and total is then not
+ * written); s = 1 / sqrt(mean of t^2 over the row + eps); y = t s weight. rstd receives s; the
+ * rows of y and total follow each other. Up to 2^14 columns and 2^31 - 1 rows.
+ * Quantized: y / scale in e4m3 or int8, to nearest (ties to even), with a scale for each `block`
+ * columns (32, 64, 128 or 256; 0: the whole row): the largest size of y there over 448 or 127, at
+ * least 2^-126. Where y holds a NaN the block's scale is NaN; where it holds an infinity the scale is
+ * infinite.
+ * Backward, h = t s and g = dy weight: dt = dtotal + s (g - h mean(g h)), to dresidual in
+ * total_type and to dx in x_type (each may be null, and so may dtotal), their rows following each
+ * other; dweight (may be null) is the rows' sum of dy h, in weight_type. x, residual and y are not
+ * read. */
+typedef struct pots_rms_norm {
+  const void *x, *residual, *weight;
+  void *total; /* forward: written; backward: read */
+  void *y;
+  float *rstd;   /* [rows]; forward: written; backward: read */
+  float *scales; /* [rows][blocks], quantized only */
+  const void *dy, *dtotal;
+  void *dx, *dresidual, *dweight;
+  int64_t x_row, residual_row, total_row, dy_row, dtotal_row; /* total_row: backward only */
+  uint32_t rows, dim, block;
+  uint32_t x_type, total_type, weight_type, y_type; /* y_type: of y and dy */
+  float eps;
+} pots_rms_norm;
+
+int pots_rms_norm_forward(const pots_rms_norm *a, void *stream);
+int pots_rms_norm_quantized(const pots_rms_norm *a, void *stream);
+uint64_t pots_rms_norm_backward_work(const pots_rms_norm *a);
+int pots_rms_norm_backward(const pots_rms_norm *a, void *work, void *stream);
+
+/* Pairs (u, v) of each head of q [batch, heads, n, head_dim] and k [batch, kv_heads, ...], turned to
+ * (u cos - v sin, u sin + v cos) by the angle position * frequency of the pair (`inverse`: by its
+ * negative, which is the gradient). Pair i is (i, i + pairs), or (2i, 2i + 1) where `adjacent`;
+ * columns from 2 * pairs on are copied. Its position is that of the axis a with
+ * ends[a - 1] <= i < ends[a]: int32 or int64 at positions + a * position_axis + batch *
+ * position_batch + token * position_token (elements). Angles are taken in 64 bits. Strides and
+ * pointers of heads are any that an element may have. Up to 2^10 columns, 4 axes, 2^31 - 1 tokens and
+ * 2^16 heads. q_out and k_out are not the inputs' memory. */
+typedef struct pots_rotary {
+  pots_heads q, k, q_out, k_out;
+  const void *positions, *frequencies;
+  int64_t position_axis, position_batch, position_token;
+  uint32_t batch, heads, kv_heads, n, head_dim, pairs, axes;
+  uint32_t ends[4];
+  uint32_t dtype, frequency_type, position_bits; /* frequencies: POTS_OP_F32 or POTS_OP_F64 */
+  uint32_t adjacent, inverse;
+} pots_rotary;
+
+int pots_rotary_turn(const pots_rotary *a, void *stream);
+
+/* out = silu(gate) * up, silu(g) = g / (1 + e^-g); backward: dgate and dup of it. The rows of out,
+ * dgate and dup follow each other. rows * columns is at most 2^40. */
+typedef struct pots_gated_silu {
+  const void *gate, *up, *dout;
+  void *out, *dgate, *dup;
+  int64_t gate_row, up_row, dout_row;
+  uint32_t rows, columns, dtype;
+} pots_gated_silu;
+
+int pots_gated_silu_forward(const pots_gated_silu *a, void *stream);
+int pots_gated_silu_backward(const pots_gated_silu *a, void *stream);
+
+/* The 2-norm of many tensors' values together, from a sum of squares in 64 bits, to norm; and with
+ * factor = max_norm / norm where the norm exceeds max_norm and 1 elsewhere (a NaN norm has a NaN
+ * factor): clip, out = factor * gradient in gradient_type; step, out = weight - eta * factor *
+ * gradient in weight_type. The `tensors` entries (1 to 2^16) follow the block in memory. Values of a
+ * tensor are consecutive, from where an element may start. An out may be its own gradient or
+ * weight; two outs that overlap, or an out over another input or shifted over its own, are refused. */
+typedef struct pots_gradients {
+  float *norm;
+  float max_norm, eta;
+  uint32_t tensors, pad;
+} pots_gradients;
+
+typedef struct pots_gradient {
+  const void *gradient, *weight; /* weight: step only */
+  void *out;
+  uint64_t count;
+  uint32_t gradient_type, weight_type;
+} pots_gradient;
+
+uint64_t pots_gradient_norm_work(const pots_gradients *a);
+int pots_gradient_norm(const pots_gradients *a, void *work, void *stream);
+uint64_t pots_clip_gradients_work(const pots_gradients *a);
+int pots_clip_gradients(const pots_gradients *a, void *work, void *stream);
+uint64_t pots_sgd_step_work(const pots_gradients *a);
+int pots_sgd_step(const pots_gradients *a, void *work, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,133 @@
+// The gated activation of a decoder's MLP, with its gradient.
+//
+//   out = silu(g)·u,  silu(g) = g·σ(g),  σ(g) = 1 / (1 + e^−g)
+//   dg = dout·u·σ(g)(1 + g·(1 − σ(g))),  du = dout·silu(g)
+//
+// Bound by memory: three tensors forward, five backward, each once, 16 bytes a lane. The arithmetic
+// is fp32, rounded once. e^−g overflows to infinity for g < −88, where σ is then 0, as it is in
+// fp32; 1 − σ is e^−g·σ, taken from whichever of e^−g and e^g is at most 1.
+#include <math.h>
+
+#include "common.h"
+#include "gmem.h"
+#include "tiles.h"
+#include "values.h"
+
+namespace pots {
+
+template <class T>
+constexpr uint32_t kValues = 16 / sizeof(typename T::elem);
+
+// Quotients by a number that is the same for the launch, of numbers below 2^31.
+struct Divisor {
+  uint32_t by, factor, shift;
+
+  explicit Divisor(uint32_t d) : by(d), shift(0) {
+    while (shift < 31 && (1u << shift) < d) shift++;
+    factor = (uint32_t)(((1ull << (31 + shift)) + d - 1) / d);  // (2^31 for d = 1)
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t n) const {
+    return (uint32_t)((uint64_t)n * factor >> 31 >> shift);
+  }
+};
+
+struct Sigma {
+  float one, rest;  // σ(g) and 1 − σ(g)
+};
+__device__ __forceinline__ Sigma sigma(float g) {
+  const float e = expf(-fabsf(g)), q = 1.f / (1.f + e);
+  return g >= 0.f ? Sigma{q, e * q} : Sigma{e * q, q};
+}
+
+template <class T, bool GRAD>
+__global__ __launch_bounds__(256) void gated(pots_gated_silu a, Divisor runs, uint32_t all) {
+  typedef typename T::elem elem;
+  constexpr uint32_t N = kValues<T>;
+  const uint32_t e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= all) return;
+  const uint32_t row = runs.of(e), c = (e - row * runs.by) * N;
+  Run<T, N> g[1], u[1], d[1];
+  load_runs<T, N, 1>(reinterpret_cast<const elem*>(a.gate) + row * a.gate_row, c, 0, a.columns, g);
+  load_runs<T, N, 1>(reinterpret_cast<const elem*>(a.up) + row * a.up_row, c, 0, a.columns, u);
+  if (GRAD)
+    load_runs<T, N, 1>(reinterpret_cast<const elem*>(a.dout) + row * a.dout_row, c, 0, a.columns, d);
+  float y[N], z[N];
+#pragma unroll
+  for (uint32_t j = 0; j < N; j++) {
+    const float x = T::get(g[0][j]), v = T::get(u[0][j]);
+    const Sigma s = sigma(x);
+    if (GRAD) {
+      const float dy = T::get(d[0][j]);
+      y[j] = dy * v * (s.one * (1.f + x * s.rest));
+      z[j] = dy * (x * s.one);
+    } else {
+      y[j] = x * s.one * v;
+    }
+  }
+  const int64_t at = (int64_t)row * a.columns + c;
+  store_run<T, N>(reinterpret_cast<elem*>(GRAD ? a.dgate : a.out) + at, a.columns - c, y);
+  if (GRAD) store_run<T, N>(reinterpret_cast<elem*>(a.dup) + at, a.columns - c, z);
+}
+
+namespace {
+
+bool bad(const pots_gated_silu* a) {
+  return !a || a->dtype > POTS_OP_BF16 || a->columns > 1u << 30 ||
+         (uint64_t)a->rows * a->columns > 1ull << 40;
+}
+
+template <class T, bool GRAD>
+int run(const pots_gated_silu* call, hipStream_t s) {
+  typedef typename T::elem elem;
+  pots_gated_silu a = *call;
+  // Rows that follow each other everywhere are one row, as long as it is one.
+  const int64_t c = a.columns;
+  if ((uint64_t)a.rows * a.columns <= 1u << 30 && a.gate_row == c && a.up_row == c &&
+      (!GRAD || a.dout_row == c)) {
+    a.columns *= a.rows;
+    a.rows = 1;
+  }
+  const uint32_t per = (a.columns + kValues<T> - 1) / kValues<T>;
+  const uint32_t most = (1u << 30) / per;  // rows of a launch
+  for (uint64_t r0 = 0; r0 < a.rows; r0 += most) {
+    pots_gated_silu part = a;
+    part.rows = (uint32_t)(a.rows - r0 < most ? a.rows - r0 : most);
+    part.gate = reinterpret_cast<const elem*>(a.gate) + (int64_t)r0 * a.gate_row;
+    part.up = reinterpret_cast<const elem*>(a.up) + (int64_t)r0 * a.up_row;
+    const int64_t at = (int64_t)r0 * a.columns;
+    if (GRAD) {
+      part.dout = reinterpret_cast<const elem*>(a.dout) + (int64_t)r0 * a.dout_row;
+      part.dgate = reinterpret_cast<elem*>(a.dgate) + at;
+      part.dup = reinterpret_cast<elem*>(a.dup) + at;
+    } else {
+      part.out = reinterpret_cast<elem*>(a.out) + at;
+    }
+    const uint32_t all = part.rows * per;
+    hipLaunchKernelGGL((gated<T, GRAD>), dim3((all + 255) / 256), dim3(256), 0, s, part, Divisor(per),
+                       all);
+    POTS_HIP(hipGetLastError());
+  }
+  return POTS_E_OK;
+}
+
+}  // namespace
+
+}  // namespace pots
+
+using namespace pots;
+
+extern "C" int pots_gated_silu_forward(const pots_gated_silu* a, void* stream) {
+  if (bad(a)) return POTS_E_ARG;
+  if (a->rows == 0 || a->columns == 0) return POTS_E_OK;
+  if (!a->gate || !a->up || !a->out) return POTS_E_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return a->dtype == POTS_OP_BF16 ? run<Bf16, false>(a, s) : run<Fp32, false>(a, s);
+}
+
+extern "C" int pots_gated_silu_backward(const pots_gated_silu* a, void* stream) {
+  if (bad(a)) return POTS_E_ARG;
+  if (a->rows == 0 || a->columns == 0) return POTS_E_OK;
+  if (!a->gate || !a->up || !a->dout || !a->dgate || !a->dup) return POTS_E_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return a->dtype == POTS_OP_BF16 ? run<Bf16, true>(a, s) : run<Fp32, true>(a, s);
+}

@@ -1,0 +1,356 @@
+// The 2-norm of a whole model's gradient, and what a step does with it: the gradient scaled by the
+// clip's factor, or the weights updated by it.
+//
+//   norm = √Σ g²,  f = min(1, max_norm / norm),  out = f·g  or  out = w − (η f)·g
+//
+// Bound by memory, and the gradient is read twice: the factor needs all of it first. The second pass
+// goes backwards, so that what the first read last is still in the last cache. Squares are added in
+// fp64, which no fp32 gradient leaves: 3.4e38² is 1e77, and the smallest one's square 2e-90.
+//
+// The tensors' addresses travel as kernel arguments, kNormed or kUpdated tensors a launch: a captured
+// graph keeps them, and no copy to the device precedes the work. Tensors are cut into chunks; block b of
+// g takes the chunks b, b + g, ... and leaves one sum, and the blocks of the second pass each add up all
+// sums in the same order.
+#include <math.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "common.h"
+#include "gmem.h"
+#include "tiles.h"
+#include "values.h"
+
+namespace pots {
+
+constexpr uint32_t kChunk = 4096;  // values of a chunk: four runs of four to each of 256 lanes
+constexpr uint32_t kRunsOf = kChunk / 1024;
+constexpr uint32_t kNormed = 160, kUpdated = 96;  // tensors of a launch: below 4 KiB of arguments
+constexpr uint32_t kBlocks = 2048;  // eight to a compute unit
+constexpr uint32_t kMostTensors = 1u << 16;
+
+struct Normed {
+  const void* g[kNormed];
+  uint64_t count[kNormed];
+  uint32_t first[kNormed];  // chunk; those from kNormed's own on
+  uint8_t type[kNormed];
+  uint32_t tensors, chunks;
+};
+
+struct Updated {
+  const void *g[kUpdated], *w[kUpdated];
+  void* out[kUpdated];
+  uint64_t count[kUpdated];
+  uint32_t first[kUpdated];
+  uint8_t type[kUpdated], weight_type[kUpdated];
+  uint32_t tensors, chunks;
+};
+
+__device__ __forceinline__ double sum_block(double v, double* s) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+  if (threadIdx.x % 64 == 0) s[threadIdx.x / 64] = v;
+  __syncthreads();
+  return s[0] + s[1] + s[2] + s[3];
+}
+
+// A lane's four runs of the chunk that starts at value `at` of a tensor of `count`.
+template <class T>
+__device__ __forceinline__ void chunk_of(const void* p, uint64_t at, uint64_t count,
+                                         float (&v)[kRunsOf][4]) {
+  const typename T::elem* q = reinterpret_cast<const typename T::elem*>(p) + at;
+  Run<T, 4> x[kRunsOf];
+  if (count - at >= kChunk) {
+#pragma unroll
+    for (uint32_t i = 0; i < kRunsOf; i++) x[i] = load_any<Run<T, 4>>(q + 4 * threadIdx.x + 1024 * i);
+  } else {
+    load_runs<T, 4, kRunsOf>(q, 4 * threadIdx.x, 1024, (uint32_t)(count - at), x);
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < kRunsOf; i++)
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) v[i][j] = T::get(x[i][j]);
+}
+
+__global__ __launch_bounds__(256) void norm_sums(Normed t, double* __restrict__ part) {
+  __shared__ double s_sum[4];
+  double sum[4] = {};
+  uint32_t i = 0;
+  for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    while (i + 1 < t.tensors && c >= t.first[i + 1]) i++;
+    const uint64_t at = (uint64_t)(c - t.first[i]) * kChunk;
+    float v[kRunsOf][4];
+    if (t.type[i] == POTS_OP_BF16)
+      chunk_of<Bf16>(t.g[i], at, t.count[i], v);
+    else
+      chunk_of<Fp32>(t.g[i], at, t.count[i], v);
+#pragma unroll
+    for (uint32_t r = 0; r < kRunsOf; r++)
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) sum[j] = fma((double)v[r][j], (double)v[r][j], sum[j]);
+  }
+  const double all = sum_block((sum[0] + sum[1]) + (sum[2] + sum[3]), s_sum);
+  if (threadIdx.x == 0) part[blockIdx.x] = all;
+}
+
+__device__ __forceinline__ double norm_of(const double* part, uint32_t parts, double* s) {
+  double v = 0.;
+  for (uint32_t i = threadIdx.x; i < parts; i += 256) v += part[i];
+  return sqrt(sum_block(v, s));
+}
+
+__global__ __launch_bounds__(256) void norm_write(const double* __restrict__ part, uint32_t parts,
+                                                  float* norm) {
+  __shared__ double s_sum[4];
+  const double n = norm_of(part, parts, s_sum);
+  if (threadIdx.x == 0) *norm = (float)n;
+}
+
+// STEP: w - eta·f·g, else f·g. The launch that writes the norm has its address.
+template <bool STEP>
+__global__ __launch_bounds__(256) void update(Updated t, const double* __restrict__ part,
+                                              uint32_t parts, float max_norm, float eta, float* norm) {
+  __shared__ double s_sum[4];
+  const double n = norm_of(part, parts, s_sum);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+  const double factor = n <= (double)max_norm ? 1. : (double)max_norm / n;
+  const float f = (float)(STEP ? -(double)eta * factor : factor);
+  if (blockIdx.x >= t.chunks) return;
+  uint32_t i = t.tensors - 1;
+  const uint32_t last = (t.chunks - 1 - blockIdx.x) / gridDim.x * gridDim.x + blockIdx.x;
+  for (uint32_t k = 0; k <= last / gridDim.x; k++) {
+    const uint32_t c = last - k * gridDim.x;
+    while (c < t.first[i]) i--;
+    const uint64_t at = (uint64_t)(c - t.first[i]) * kChunk, count = t.count[i];
+    float g[kRunsOf][4], w[kRunsOf][4];
+    if (t.type[i] == POTS_OP_BF16)
+      chunk_of<Bf16>(t.g[i], at, count, g);
+    else
+      chunk_of<Fp32>(t.g[i], at, count, g);
+    if (STEP) {
+      if (t.weight_type[i] == POTS_OP_BF16)
+        chunk_of<Bf16>(t.w[i], at, count, w);
+      else
+        chunk_of<Fp32>(t.w[i], at, count, w);
+    }
+    const uint32_t left = count - at < kChunk ? (uint32_t)(count - at) : kChunk;
+    const uint32_t type = STEP ? t.weight_type[i] : t.type[i];
+#pragma unroll
+    for (uint32_t r = 0; r < kRunsOf; r++) {
+      const uint32_t at_r = 4 * threadIdx.x + 1024 * r;
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) g[r][j] = STEP ? fmaf(f, g[r][j], w[r][j]) : f * g[r][j];
+      put_run<4>(t.out[i], type, (int64_t)at + at_r, left > at_r ? left - at_r : 0, g[r]);
+    }
+  }
+}
+
+namespace {
+
+const pots_gradient* entries(const pots_gradients* a) {
+  return reinterpret_cast<const pots_gradient*>(a + 1);
+}
+
+uint64_t chunks_of(const pots_gradient& e) { return (e.count + kChunk - 1) / kChunk; }
+
+bool bad(const pots_gradients* a, bool clips, bool steps) {
+  if (!a || a->tensors == 0 || a->tensors > kMostTensors) return true;
+  if (clips && !(a->max_norm > 0.f)) return true;
+  if (steps && !isfinite(a->eta)) return true;
+  uint64_t chunks = 0;
+  for (uint32_t i = 0; i < a->tensors; i++) {
+    const pots_gradient& e = entries(a)[i];
+    if (e.gradient_type > POTS_OP_BF16 || (steps && e.weight_type > POTS_OP_BF16) ||
+        e.count > 1ull << 42)
+      return true;
+    chunks += chunks_of(e);
+  }
+  return chunks > 0x7fffffffu;
+}
+
+// Launches over the tensors that hold something, N of them each: f(table, its first entry).
+template <uint32_t N, class F>
+int each_launch(const pots_gradients* a, F&& f) {
+  std::vector<uint32_t> some;
+  some.reserve(a->tensors);
+  for (uint32_t i = 0; i < a->tensors; i++)
+    if (entries(a)[i].count) some.push_back(i);
+  for (size_t at = 0; at < some.size(); at += N) {
+    const uint32_t n = (uint32_t)std::min<size_t>(N, some.size() - at);
+    const int rc = f(some.data() + at, n);
+    if (rc != POTS_E_OK) return rc;
+  }
+  return POTS_E_OK;
+}
+
+uint32_t blocks_of(uint64_t chunks) { return (uint32_t)std::min<uint64_t>(chunks, kBlocks); }
+
+uint32_t parts_of(const pots_gradients* a) {
+  uint32_t parts = 0;
+  (void)each_launch<kNormed>(a, [&](const uint32_t* some, uint32_t n) {
+    uint64_t chunks = 0;
+    for (uint32_t i = 0; i < n; i++) chunks += chunks_of(entries(a)[some[i]]);
+    parts += blocks_of(chunks);
+    return POTS_E_OK;
+  });
+  return parts;
+}
+
+int sums(const pots_gradients* a, double* part, uint32_t* parts, hipStream_t s) {
+  *parts = 0;
+  return each_launch<kNormed>(a, [&](const uint32_t* some, uint32_t n) {
+    Normed t = {};
+    for (uint32_t i = 0; i < n; i++) {
+      const pots_gradient& e = entries(a)[some[i]];
+      t.g[i] = e.gradient;
+      t.count[i] = e.count;
+      t.first[i] = t.chunks;
+      t.type[i] = (uint8_t)e.gradient_type;
+      t.chunks += (uint32_t)chunks_of(e);
+    }
+    t.tensors = n;
+    const uint32_t blocks = blocks_of(t.chunks);
+    hipLaunchKernelGGL(norm_sums, dim3(blocks), dim3(256), 0, s, t, part + *parts);
+    POTS_HIP(hipGetLastError());
+    *parts += blocks;
+    return POTS_E_OK;
+  });
+}
+
+template <bool STEP>
+int updates(const pots_gradients* a, const double* part, uint32_t parts, hipStream_t s) {
+  std::vector<Updated> launches;
+  (void)each_launch<kUpdated>(a, [&](const uint32_t* some, uint32_t n) {
+    launches.emplace_back();
+    Updated& t = launches.back();
+    t.tensors = n;
+    t.chunks = 0;
+    for (uint32_t i = 0; i < n; i++) {
+      const pots_gradient& e = entries(a)[some[i]];
+      t.g[i] = e.gradient;
+      t.w[i] = e.weight;
+      t.out[i] = e.out;
+      t.count[i] = e.count;
+      t.first[i] = t.chunks;
+      t.type[i] = (uint8_t)e.gradient_type;
+      t.weight_type[i] = (uint8_t)e.weight_type;
+      t.chunks += (uint32_t)chunks_of(e);
+    }
+    return POTS_E_OK;
+  });
+  if (launches.empty()) launches.emplace_back(Updated{});  // the norm of nothing
+  float* norm = a->norm;
+  for (size_t i = launches.size(); i-- > 0;) {
+    const uint32_t blocks = std::max(1u, blocks_of(launches[i].chunks));
+    hipLaunchKernelGGL((update<STEP>), dim3(blocks), dim3(256), 0, s, launches[i], part, parts,
+                       a->max_norm, a->eta, norm);
+    POTS_HIP(hipGetLastError());
+    norm = nullptr;
+  }
+  return POTS_E_OK;
+}
+
+// Whether what is written lies apart from everything else: each out from the others, and from every
+// input but its own entry's, which it may be exactly.
+struct Range {
+  uint64_t from, to;
+  uint32_t entry, size;
+};
+
+bool overlaps(const pots_gradients* a, bool steps) {
+  std::vector<Range> outs;
+  const uint32_t sizes[] = {4, 2};
+  for (uint32_t i = 0; i < a->tensors; i++) {
+    const pots_gradient& e = entries(a)[i];
+    const uint32_t size = sizes[steps ? e.weight_type : e.gradient_type];
+    const uint64_t p = reinterpret_cast<uint64_t>(e.out);
+    if (e.count) outs.push_back({p, p + e.count * size, i, size});
+  }
+  std::sort(outs.begin(), outs.end(), [](const Range& x, const Range& y) { return x.from < y.from; });
+  for (size_t i = 1; i < outs.size(); i++)
+    if (outs[i].from < outs[i - 1].to) return true;
+  for (uint32_t i = 0; i < a->tensors; i++) {
+    const pots_gradient& e = entries(a)[i];
+    if (!e.count) continue;
+    const void* const ins[] = {e.gradient, e.weight};
+    const uint32_t types[] = {e.gradient_type, e.weight_type};
+    for (uint32_t k = 0; k < (steps ? 2u : 1u); k++) {
+      const uint64_t from = reinterpret_cast<uint64_t>(ins[k]);
+      const uint64_t to = from + e.count * sizes[types[k]];
+      auto o = std::upper_bound(outs.begin(), outs.end(), from,
+                                [](uint64_t p, const Range& r) { return p < r.to; });
+      for (; o != outs.end() && o->from < to; ++o)
+        if (o->entry != i || o->from != from || o->size != sizes[types[k]]) return true;
+    }
+  }
+  return false;
+}
+
+bool missing(const pots_gradients* a, bool writes, bool steps) {
+  if (!a->norm) return true;
+  for (uint32_t i = 0; i < a->tensors; i++) {
+    const pots_gradient& e = entries(a)[i];
+    if (e.count && (!e.gradient || (writes && !e.out) || (steps && !e.weight))) return true;
+  }
+  return false;
+}
+
+template <bool STEP>
+int change(const pots_gradients* a, void* work, void* stream) {
+  if (bad(a, true, STEP) || missing(a, true, STEP) || overlaps(a, STEP)) return POTS_E_ARG;
+  if (parts_of(a) && !work) return POTS_E_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  double* const part = static_cast<double*>(work);
+  uint32_t parts = 0;
+  const int rc = sums(a, part, &parts, s);
+  return rc != POTS_E_OK ? rc : updates<STEP>(a, part, parts, s);
+}
+
+}  // namespace
+
+}  // namespace pots
+
+using namespace pots;
+
+// (the lists that the entry points make may find no memory)
+template <class R, class F>
+static R guarded(R failed, F&& f) noexcept {
+  try {
+    return f();
+  } catch (...) {
+    return failed;
+  }
+}
+
+extern "C" uint64_t pots_gradient_norm_work(const pots_gradients* a) {
+  return guarded<uint64_t>(0, [&] { return bad(a, false, false) ? 0 : 8ull * parts_of(a); });
+}
+
+extern "C" int pots_gradient_norm(const pots_gradients* a, void* work, void* stream) {
+  return guarded<int>(POTS_E_NOMEM, [&] {
+    if (bad(a, false, false) || missing(a, false, false)) return POTS_E_ARG;
+    if (parts_of(a) && !work) return POTS_E_ARG;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    double* const part = static_cast<double*>(work);
+    uint32_t parts = 0;
+    const int rc = sums(a, part, &parts, s);
+    if (rc != POTS_E_OK) return rc;
+    hipLaunchKernelGGL(norm_write, dim3(1), dim3(256), 0, s, part, parts, a->norm);
+    POTS_HIP(hipGetLastError());
+    return POTS_E_OK;
+  });
+}
+
+extern "C" uint64_t pots_clip_gradients_work(const pots_gradients* a) {
+  return pots_gradient_norm_work(a);
+}
+
+extern "C" int pots_clip_gradients(const pots_gradients* a, void* work, void* stream) {
+  return guarded<int>(POTS_E_NOMEM, [&] { return change<false>(a, work, stream); });
+}
+
+extern "C" uint64_t pots_sgd_step_work(const pots_gradients* a) { return pots_gradient_norm_work(a); }
+
+extern "C" int pots_sgd_step(const pots_gradients* a, void* work, void* stream) {
+  return guarded<int>(POTS_E_NOMEM, [&] { return change<true>(a, work, stream); });
+}

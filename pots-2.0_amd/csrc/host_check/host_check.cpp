@@ -316,7 +316,7 @@ int launches(int argc, char** argv) {
   auto f32 = [&](int i) { return reinterpret_cast<float*>(p) + ((uint64_t)i << 40); };
   for (int i = 2; i < argc; i++) {
     std::string name;
-    uint32_t x[6] = {};
+    uint32_t x[8] = {};
     int n = -1;
     const std::string text = argv[i];
     for (size_t at = 0; at <= text.size();) {
@@ -324,7 +324,7 @@ int launches(int argc, char** argv) {
       const std::string part = text.substr(at, end - at);
       if (n < 0)
         name = part;
-      else if (n < 6)
+      else if (n < 8)
         x[n] = (uint32_t)strtoull(part.c_str(), nullptr, 10);
       n++;
       at = end + 1;
@@ -367,6 +367,62 @@ int launches(int argc, char** argv) {
         work = pots_embedding_backward_work(&a);
         rc = pots_embedding_backward(&a, p, nullptr);
       }
+    } else if (name == "rms_norm_forward" || name == "rms_norm_quantized" ||
+               name == "rms_norm_backward") {
+      pots_rms_norm a = {};
+      a.rows = x[0], a.dim = x[1], a.block = x[2], a.x_type = x[3], a.total_type = x[4];
+      a.weight_type = x[5], a.y_type = x[6], a.eps = 1e-6f;
+      a.x = f32(1), a.residual = f32(2), a.weight = f32(3), a.total = f32(4), a.y = f32(5);
+      a.rstd = f32(6), a.scales = f32(7), a.dy = f32(8), a.dx = f32(9), a.dweight = f32(10);
+      a.x_row = a.residual_row = a.total_row = a.dy_row = a.dim;
+      if (name == "rms_norm_backward") {
+        work = pots_rms_norm_backward_work(&a);
+        rc = pots_rms_norm_backward(&a, p, nullptr);
+      } else {
+        rc = (name == "rms_norm_forward" ? pots_rms_norm_forward : pots_rms_norm_quantized)(&a,
+                                                                                           nullptr);
+      }
+    } else if (name == "rotary_turn") {
+      pots_rotary a = {};
+      a.batch = x[0], a.heads = x[1], a.kv_heads = x[2], a.n = x[3], a.head_dim = x[4];
+      a.pairs = x[5], a.dtype = x[6], a.axes = 1, a.ends[0] = a.pairs, a.position_bits = 64;
+      a.positions = f32(5), a.frequencies = f32(6), a.position_token = 1;
+      int k = 0;
+      for (pots_heads* h : {&a.q, &a.q_out, &a.k, &a.k_out})
+        *h = pots_heads{f32(1 + k++), (int64_t)a.n * a.heads * a.head_dim, a.head_dim,
+                        (int64_t)a.heads * a.head_dim};
+      rc = pots_rotary_turn(&a, nullptr);
+    } else if (name == "gated_silu_forward" || name == "gated_silu_backward") {
+      pots_gated_silu a = {};
+      a.rows = x[0], a.columns = x[1], a.dtype = x[2];
+      a.gate = f32(1), a.up = f32(2), a.dout = f32(3), a.out = f32(4), a.dgate = f32(5);
+      a.dup = f32(6), a.gate_row = a.up_row = (int64_t)a.columns * (1 + x[3]), a.dout_row = a.columns;
+      rc = (name == "gated_silu_forward" ? pots_gated_silu_forward : pots_gated_silu_backward)(
+          &a, nullptr);
+    } else if (name == "gradient_norm" || name == "clip_gradients" || name == "sgd_step") {
+      // x[0] tensors of x[1] values, of which every third is one value longer; x[2]: in place; x[3]:
+      // how far the outs lie behind the inputs otherwise
+      std::vector<char> block(sizeof(pots_gradients) + x[0] * sizeof(pots_gradient));
+      pots_gradients a = {};
+      a.norm = f32(9), a.max_norm = 1.f, a.eta = 0.1f, a.tensors = x[0];
+      memcpy(block.data(), &a, sizeof a);
+      uint64_t at = 0;
+      for (uint32_t i = 0; i < x[0]; i++) {
+        pots_gradient e = {};
+        e.count = x[1] + (i % 3 == 0);
+        e.gradient = reinterpret_cast<char*>(f32(1)) + at;
+        e.weight = reinterpret_cast<char*>(f32(2)) + at;
+        const void* in = name == "sgd_step" ? e.weight : e.gradient;
+        e.out = x[2] ? const_cast<char*>(static_cast<const char*>(in)) + x[3]
+                     : reinterpret_cast<char*>(f32(3)) + at;
+        at += 4 * e.count;
+        memcpy(block.data() + sizeof a + i * sizeof e, &e, sizeof e);
+      }
+      const pots_gradients* g = reinterpret_cast<const pots_gradients*>(block.data());
+      work = pots_gradient_norm_work(g);
+      rc = (name == "gradient_norm" ? pots_gradient_norm
+            : name == "sgd_step"    ? pots_sgd_step
+                                    : pots_clip_gradients)(g, p, nullptr);
     } else {
       fprintf(stderr, "no operator %s\n", name.c_str());
       return 1;

@@ -1,0 +1,400 @@
+// The residual's addition and the root-mean-square norm of the sum, with its gradient and with an
+// output in 8 bits.
+//
+//   t = x + r,  s = 1 / √(mean t² + ε),  y = t·s·w
+//   h = t·s, g = dy·w:  dt = dtotal + s (g − h·mean(g·h)),  dw = Σ_rows dy·h
+//   8 bits: a = the largest |y| of a group, scale = a / 448 (e4m3) or a / 127 (int8), q = y / scale
+//
+// Bound by memory: a row is read once into registers, four consecutive values of each 256 to a lane
+// (any width of type then fills whole lines), and everything follows from there. Sums, the norm and
+// y before its rounding are fp32; t is rounded to the residual's type first, since the next layer
+// reads that t, and so does the gradient.
+//
+// dw: every wave adds up its own rows in registers, a block's waves join in LDS, and norm_join adds
+// the blocks' sums in their order, so that no atomics are needed.
+#include <math.h>
+
+#include "common.h"
+#include "gmem.h"
+#include "tiles.h"
+#include "values.h"
+
+namespace pots {
+
+constexpr uint32_t kMaxDim = 1u << 14;
+constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126, the smallest normal number
+
+// A row's W waves: each of its lanes holds G runs of four, the columns 4 (64 (W·i + wave) + lane)
+// on; W·G·256 columns.
+template <uint32_t G, uint32_t W>
+struct Row {
+  static constexpr uint32_t kRuns = G, kWaves = W;
+  // waves of one row to a block, or four rows to a block
+  static constexpr uint32_t kThreads = W == 1 ? 256 : 64 * W;
+  static constexpr uint32_t kRows = kThreads / (64 * W);
+
+  // The sum over a row, in every lane of it; s: W floats of LDS, used in turn by two calls.
+  static __device__ __forceinline__ float sum(float v, float (*s)[W], uint32_t& turn) {
+    v = sum_wave(v);
+    if constexpr (W > 1) {
+      if (threadIdx.x % 64 == 0) s[turn][threadIdx.x / 64] = v;
+      __syncthreads();
+      v = 0.f;
+#pragma unroll
+      for (uint32_t w = 0; w < W; w++) v += s[turn][w];
+      turn ^= 1;
+    }
+    return v;
+  }
+  static __device__ __forceinline__ uint32_t most(uint32_t v, uint32_t (*s)[W], uint32_t& turn) {
+#pragma unroll
+    for (int m = 32; m; m >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, m));
+    if constexpr (W > 1) {
+      if (threadIdx.x % 64 == 0) s[turn][threadIdx.x / 64] = v;
+      __syncthreads();
+#pragma unroll
+      for (uint32_t w = 0; w < W; w++) v = max(v, s[turn][w]);
+      turn ^= 1;
+    }
+    return v;
+  }
+};
+
+// How many columns of the row are left from c on.
+__device__ __forceinline__ uint32_t left_of(uint32_t c, uint32_t dim) { return c < dim ? dim - c : 0; }
+
+template <class X, class T, bool RES, bool Q, class R>
+__global__ __launch_bounds__(R::kThreads) void norm_rows(pots_rms_norm a) {
+  constexpr uint32_t G = R::kRuns, W = R::kWaves;
+  __shared__ float s_sum[2][W];
+  __shared__ uint32_t s_most[2][W];
+  uint32_t turn = 0, turn_most = 0;
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t first = 4 * ((W == 1 ? 0 : wave * 64) + lane);
+  const float over = 1.f / (float)a.dim;
+  AnyRuns<G> gain;
+  gain.load(a.weight, a.weight_type, first, 256 * W, a.dim);
+  const uint32_t step = gridDim.x * R::kRows;
+  for (uint64_t row = blockIdx.x * R::kRows + (W == 1 ? wave : 0); row < a.rows; row += step) {
+    float t[G][4];
+    Run<X, 4> x[G];
+    Run<T, 4> r[G];
+    load_runs<X, 4, G>(reinterpret_cast<const typename X::elem*>(a.x) + (int64_t)row * a.x_row, first,
+                       256 * W, a.dim, x);
+    if (RES)
+      load_runs<T, 4, G>(
+          reinterpret_cast<const typename T::elem*>(a.residual) + (int64_t)row * a.residual_row, first,
+          256 * W, a.dim, r);
+    float sum = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < G; i++) {
+      const uint32_t c = first + 256 * W * i;
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) {
+        t[i][j] = X::get(x[i][j]);
+        if (RES) t[i][j] = T::get(T::put(t[i][j] + T::get(r[i][j])));
+        sum += t[i][j] * t[i][j];
+      }
+      if (RES)
+        store_run<T, 4>(reinterpret_cast<typename T::elem*>(a.total) + row * a.dim + c,
+                        left_of(c, a.dim), t[i]);
+    }
+    const float s = 1.f / sqrtf(R::sum(sum, s_sum, turn) * over + a.eps);
+    if (!Q && lane == 0 && (W == 1 || wave == 0)) gstore<float>(a.rstd + row, s);
+    uint32_t most = 0;  // sizes as bits, whose order puts NaN above infinity
+#pragma unroll
+    for (uint32_t i = 0; i < G; i++) {
+      float w[4];
+      gain.get(a.weight_type, i, w);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) {
+        t[i][j] = t[i][j] * s * w[j];
+        if (Q) most = max(most, __float_as_uint(t[i][j]) & 0x7fffffffu);
+      }
+    }
+    if constexpr (!Q) {
+#pragma unroll
+      for (uint32_t i = 0; i < G; i++) {
+        const uint32_t c = first + 256 * W * i;
+        put_run<4>(a.y, a.y_type, (int64_t)(row * a.dim) + c, left_of(c, a.dim), t[i]);
+      }
+    } else {
+      const float top = a.y_type == POTS_OP_E4M3 ? 448.f : 127.f;
+      const uint32_t lanes = a.block / 4;  // of a group; 0: the row
+      const uint32_t groups = a.block ? (a.dim + a.block - 1) / a.block : 1;
+      if (!a.block) most = R::most(most, s_most, turn_most);
+#pragma unroll
+      for (uint32_t i = 0; i < G; i++) {
+        const uint32_t c = first + 256 * W * i, left = left_of(c, a.dim);
+        if (a.block) {
+          most = 0;
+#pragma unroll
+          for (uint32_t j = 0; j < 4; j++)
+            most = max(most, __float_as_uint(t[i][j]) & 0x7fffffffu);
+          for (uint32_t m = 1; m < lanes; m *= 2)
+            most = max(most, (uint32_t)__shfl_xor((int)most, (int)m));
+        }
+        float scale = __uint_as_float(most) / top;
+        scale = scale < kLeastScale ? kLeastScale : scale;
+        if (a.block ? left && lane % lanes == 0 : c == 0)
+          gstore<float>(a.scales + row * groups + (a.block ? c / a.block : 0), scale);
+        uint8_t* const q = reinterpret_cast<uint8_t*>(a.y) + row * a.dim + c;
+        uint32_t b;
+        float v[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) v[j] = t[i][j] / scale;
+        if (a.y_type == POTS_OP_E4M3) {  // (v is at most 448 and a rounding: no overflow but NaN's)
+          b = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+          b = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], (int)b, true);
+        } else {
+          b = 0;
+#pragma unroll
+          for (uint32_t j = 0; j < 4; j++) {
+            const float e = rintf(v[j]);
+            b |= ((uint32_t)(e == e ? (int)e : 0) & 0xff) << 8 * j;
+          }
+        }
+        if (left >= 4) {
+          store_any(q, b);
+        } else {
+#pragma unroll
+          for (uint32_t j = 0; j < 3; j++)
+            if (j < left) gstore<uint8_t>(q + j, (uint8_t)(b >> 8 * j));
+        }
+      }
+    }
+  }
+}
+
+// part: [block][dim] sums of dy·h, where a.dweight is there.
+template <class Y, class T, class R>
+__global__ __launch_bounds__(R::kThreads) void norm_grad(pots_rms_norm a, float* __restrict__ part) {
+  constexpr uint32_t G = R::kRuns, W = R::kWaves;
+  __shared__ float s_sum[2][W];
+  __shared__ float s_dw[W == 1 ? 4 * 256 * G : 1];
+  uint32_t turn = 0;
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t first = 4 * ((W == 1 ? 0 : wave * 64) + lane);
+  const float over = 1.f / (float)a.dim;
+  float dw[G][4] = {};
+  AnyRuns<G> gain;
+  gain.load(a.weight, a.weight_type, first, 256 * W, a.dim);
+  const uint32_t step = gridDim.x * R::kRows;
+  for (uint64_t row = blockIdx.x * R::kRows + (W == 1 ? wave : 0); row < a.rows; row += step) {
+    Run<Y, 4> y[G];
+    Run<T, 4> r[G], d[G];
+    const typename T::elem* const dt =
+        reinterpret_cast<const typename T::elem*>(a.dtotal) + (int64_t)row * a.dtotal_row;
+    const float s = gload<float>(a.rstd + row);
+    load_runs<Y, 4, G>(reinterpret_cast<const typename Y::elem*>(a.dy) + (int64_t)row * a.dy_row, first,
+                       256 * W, a.dim, y);
+    load_runs<T, 4, G>(
+        reinterpret_cast<const typename T::elem*>(a.total) + (int64_t)row * a.total_row, first,
+        256 * W, a.dim, r);
+    // (sixteen waves have no registers for it before the sum)
+    if (W < 16 && a.dtotal) load_runs<T, 4, G>(dt, first, 256 * W, a.dim, d);
+    float sum = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < G; i++) {
+      float w[4];
+      gain.get(a.weight_type, i, w);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) {
+        const float h = T::get(r[i][j]) * s, dy = Y::get(y[i][j]);
+        sum += dy * w[j] * h;
+        dw[i][j] += dy * h;
+      }
+    }
+    const float mean = R::sum(sum, s_sum, turn) * over;
+    if (W == 16 && a.dtotal) load_runs<T, 4, G>(dt, first, 256 * W, a.dim, d);
+#pragma unroll
+    for (uint32_t i = 0; i < G; i++) {
+      const uint32_t c = first + 256 * W * i, left = left_of(c, a.dim);
+      const int64_t at = (int64_t)(row * a.dim) + c;
+      float v[4], w[4];
+      gain.get(a.weight_type, i, w);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) {
+        const float h = T::get(r[i][j]) * s;
+        v[j] = s * (Y::get(y[i][j]) * w[j] - h * mean);
+        if (a.dtotal) v[j] += T::get(d[i][j]);
+      }
+      if (a.dresidual)
+        store_run<T, 4>(reinterpret_cast<typename T::elem*>(a.dresidual) + at, left, v);
+      if (a.dx) put_run<4>(a.dx, a.x_type, at, left, v);
+    }
+  }
+  if (!a.dweight) return;
+  float* const own = part + (uint64_t)blockIdx.x * a.dim;
+  if constexpr (W == 1) {
+#pragma unroll
+    for (uint32_t i = 0; i < G; i++)
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) s_dw[wave * 256 * G + 256 * i + 4 * lane + j] = dw[i][j];
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < a.dim; c += 256)
+      own[c] = s_dw[c] + s_dw[c + 256 * G] + s_dw[c + 512 * G] + s_dw[c + 768 * G];
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < G; i++) {
+      const uint32_t c = first + 256 * W * i;
+      put_run<4>(own, POTS_OP_F32, c, left_of(c, a.dim), dw[i]);
+    }
+  }
+}
+
+// dweight from `parts` rows of sums: 32 columns a block, a 32nd of the rows to each group of lanes.
+__global__ __launch_bounds__(1024) void norm_join(const float* __restrict__ part, void* dweight,
+                                                  uint32_t parts, uint32_t dim, uint32_t type) {
+  __shared__ float s_sum[32][33];
+  const uint32_t x = threadIdx.x % 32, g = threadIdx.x / 32, c = blockIdx.x * 32 + x;
+  float sum = 0.f;
+  if (c < dim) {
+    for (uint32_t p = g; p < parts; p += 256) {
+      float v[8];
+#pragma unroll
+      for (uint32_t u = 0; u < 8; u++) {
+        const uint32_t at = p + 32 * u;
+        v[u] = at < parts ? gload<float>(part + (uint64_t)at * dim + c) : 0.f;
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < 8; u++) sum += v[u];
+    }
+  }
+  s_sum[g][x] = sum;
+  __syncthreads();
+  if (g != 0 || c >= dim) return;
+  for (uint32_t i = 1; i < 32; i++) sum += s_sum[i][x];
+  if (type == POTS_OP_BF16)
+    gstore<uint16_t>(reinterpret_cast<uint16_t*>(dweight) + c, f32_to_bf16(sum));
+  else
+    gstore<float>(reinterpret_cast<float*>(dweight) + c, sum);
+}
+
+namespace {
+
+bool bad(const pots_rms_norm* a) {
+  return !a || a->dim == 0 || a->dim > kMaxDim || a->rows > 0x7fffffffu ||
+         a->x_type > POTS_OP_BF16 || a->total_type > POTS_OP_BF16 ||
+         a->weight_type > POTS_OP_BF16 || !(a->eps > 0.f) || !isfinite(a->eps);
+}
+
+// Rows of up to 2048 columns are a wave's: the sum over a row then needs no barrier. Wider ones are
+// shared by four or sixteen waves, so that a lane holds 32 values at most.
+template <class F>
+int by_width(uint32_t dim, F&& f) {
+  if (dim <= 256) return f(Row<1, 1>{});
+  if (dim <= 512) return f(Row<2, 1>{});
+  if (dim <= 1024) return f(Row<4, 1>{});
+  if (dim <= 1536) return f(Row<6, 1>{});
+  if (dim <= 2048) return f(Row<8, 1>{});
+  if (dim <= 4096) return f(Row<4, 4>{});
+  if (dim <= 8192) return f(Row<8, 4>{});
+  return f(Row<4, 16>{});
+}
+
+template <class F>
+int by_type(uint32_t type, F&& f) {
+  return type == POTS_OP_BF16 ? f(Bf16{}) : f(Fp32{});
+}
+
+template <bool Q>
+int forward(const pots_rms_norm* a, hipStream_t s) {
+  return by_width(a->dim, [&](auto r) {
+    typedef decltype(r) R;
+    const uint32_t want = (uint32_t)(((uint64_t)a->rows + R::kRows - 1) / R::kRows);
+    const uint32_t nb = want < 8192 ? want : 8192;
+    return by_type(a->x_type, [&](auto x) {
+      return by_type(a->total_type, [&](auto t) {
+        typedef decltype(x) X;
+        typedef decltype(t) T;
+        if (a->residual) {
+          hipLaunchKernelGGL((norm_rows<X, T, true, Q, R>), dim3(nb), dim3(R::kThreads), 0, s, *a);
+        } else {
+          hipLaunchKernelGGL((norm_rows<X, X, false, Q, R>), dim3(nb), dim3(R::kThreads), 0, s, *a);
+        }
+        POTS_HIP(hipGetLastError());
+        return POTS_E_OK;
+      });
+    });
+  });
+}
+
+// Blocks of the gradient's kernel: two to a compute unit, whose sums of dw are the bytes that
+// norm_join reads.
+template <class R>
+uint32_t grad_blocks(const pots_rms_norm* a) {
+  const uint64_t want = ((uint64_t)a->rows + R::kRows - 1) / R::kRows;
+  return (uint32_t)(want < 512 ? want : 512);
+}
+
+bool bad_back(const pots_rms_norm* a) { return bad(a) || a->y_type > POTS_OP_BF16; }
+
+}  // namespace
+
+}  // namespace pots
+
+using namespace pots;
+
+static int forward_checked(const pots_rms_norm* a, bool quantized, void* stream) {
+  if (bad(a)) return POTS_E_ARG;
+  if (quantized) {
+    if (a->y_type != POTS_OP_E4M3 && a->y_type != POTS_OP_INT8) return POTS_E_ARG;
+    if (a->block != 0 && a->block != 32 && a->block != 64 && a->block != 128 && a->block != 256)
+      return POTS_E_ARG;
+  } else if (a->y_type > POTS_OP_BF16) {
+    return POTS_E_ARG;
+  }
+  if (a->rows == 0) return POTS_E_OK;
+  if (!a->x || !a->weight || !a->y || (quantized ? !a->scales : !a->rstd) ||
+      (a->residual && !a->total))
+    return POTS_E_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return quantized ? forward<true>(a, s) : forward<false>(a, s);
+}
+
+extern "C" int pots_rms_norm_forward(const pots_rms_norm* a, void* stream) {
+  return forward_checked(a, false, stream);
+}
+
+extern "C" int pots_rms_norm_quantized(const pots_rms_norm* a, void* stream) {
+  return forward_checked(a, true, stream);
+}
+
+extern "C" uint64_t pots_rms_norm_backward_work(const pots_rms_norm* a) {
+  if (bad_back(a) || !a->dweight) return 0;
+  uint64_t blocks = 0;
+  (void)by_width(a->dim, [&](auto r) {
+    blocks = grad_blocks<decltype(r)>(a);
+    return POTS_E_OK;
+  });
+  return blocks * a->dim * 4;
+}
+
+extern "C" int pots_rms_norm_backward(const pots_rms_norm* a, void* work, void* stream) {
+  if (bad_back(a)) return POTS_E_ARG;
+  if (a->rows && (!a->dy || !a->total || !a->weight || !a->rstd)) return POTS_E_ARG;
+  if (a->rows && a->dweight && !work) return POTS_E_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  float* const part = static_cast<float*>(work);
+  uint32_t blocks = 0;
+  const int rc = by_width(a->dim, [&](auto r) {
+    typedef decltype(r) R;
+    blocks = grad_blocks<R>(a);
+    if (!blocks) return POTS_E_OK;
+    return by_type(a->y_type, [&](auto y) {
+      return by_type(a->total_type, [&](auto t) {
+        typedef decltype(y) Y;
+        typedef decltype(t) T;
+        hipLaunchKernelGGL((norm_grad<Y, T, R>), dim3(blocks), dim3(R::kThreads), 0, s, *a, part);
+        POTS_HIP(hipGetLastError());
+        return POTS_E_OK;
+      });
+    });
+  });
+  if (rc != POTS_E_OK || !a->dweight) return rc;
+  hipLaunchKernelGGL(norm_join, dim3((a->dim + 31) / 32), dim3(1024), 0, s, part, a->dweight,
+                     blocks, a->dim, a->weight_type);
+  POTS_HIP(hipGetLastError());
+  return POTS_E_OK;
+}

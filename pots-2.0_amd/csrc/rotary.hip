@@ -1,0 +1,226 @@
+// Rotary positions of queries and keys, on one axis or several.
+//
+//   (u, v) -> (u cos θ − v sin θ, u sin θ + v cos θ),  θ = position · frequency of the pair
+//
+// The gradient is the turn by −θ. Bound by memory: q and k are read and written once, in one
+// launch. θ is taken in whole turns and their fraction in 64 bits, so that far positions lose
+// nothing (below 2^-45 of a turn up to position 2^20); the sine and cosine of the fraction, less than
+// an eighth of a turn, are fp32. A block computes them for a few tokens into LDS, once for all heads; its
+// lanes then go over the tokens' heads, 16 bytes of u and 16 of v at a time. Where the pairs are no
+// multiple of such a run, the last run overlaps the one before it and writes the same values.
+#include <math.h>
+
+#include "common.h"
+#include "gmem.h"
+#include "tiles.h"
+#include "values.h"
+
+namespace pots {
+
+constexpr uint32_t kMaxWidth = 1024, kMaxHeads = 1u << 16;
+constexpr uint32_t kAngles = 1024, kTokens = 64;  // of a block, at the most
+constexpr uint32_t kAhead = 4;  // runs that a lane has on their way
+
+template <class T>
+constexpr uint32_t kPairs = 16 / sizeof(typename T::elem);  // pairs that a lane turns at a time
+
+struct Turn {
+  float c, s;
+};
+
+__device__ __forceinline__ Turn turn_of(double position, double frequency, bool inverse) {
+  const double f = frequency * 0.15915494309189535;  // 1 / 2π
+  const double r = fma(position, f, -rint(position * f));
+  const double quarter = rint(4.0 * r);
+  float s, c;
+  sincospif((float)(2.0 * fma(quarter, -0.25, r)), &s, &c);
+  const int q = (int)quarter & 3;  // a quarter turn: (c, s) to (-s, c)
+  Turn t;
+  t.c = q == 0 ? c : q == 1 ? -s : q == 2 ? -c : s;
+  t.s = q == 0 ? s : q == 1 ? c : q == 2 ? -s : -c;
+  if (inverse) t.s = -t.s;
+  return t;
+}
+
+// Elements of a lane's run: the pairs from i0 on, of the two halves or beside each other; or columns
+// that are copied.
+template <class T, bool ADJACENT>
+struct Piece {
+  static constexpr uint32_t P = kPairs<T>;
+  Run<T, P> lo, hi;
+
+  __device__ __forceinline__ void load(const typename T::elem* p, uint32_t at, uint32_t apart) {
+    lo = load_any<Run<T, P>>(p + at);
+    hi = load_any<Run<T, P>>(p + at + apart);
+  }
+  __device__ __forceinline__ void store(typename T::elem* p, uint32_t at, uint32_t apart) const {
+    store_any(p + at, lo);
+    store_any(p + at + apart, hi);
+  }
+  __device__ __forceinline__ void turn(const Turn* t) {
+#pragma unroll
+    for (uint32_t j = 0; j < P; j++) {
+      const Turn x = t[j];
+      if (ADJACENT) {
+        Run<T, P>& r = j < P / 2 ? lo : hi;
+        const uint32_t at = 2 * j % P;
+        const float u = T::get(r[at]), v = T::get(r[at + 1]);
+        r[at] = T::put(u * x.c - v * x.s);
+        r[at + 1] = T::put(u * x.s + v * x.c);
+      } else {
+        const float u = T::get(lo[j]), v = T::get(hi[j]);
+        lo[j] = T::put(u * x.c - v * x.s);
+        hi[j] = T::put(u * x.s + v * x.c);
+      }
+    }
+  }
+};
+
+// A head whose pairs (or whose copied columns) are fewer than a run: value by value.
+template <class T, bool ADJACENT>
+__device__ __forceinline__ void turn_few(const typename T::elem* in, typename T::elem* out,
+                                         uint32_t pairs, const Turn* t) {
+  for (uint32_t i = 0; i < pairs; i++) {
+    const uint32_t a = ADJACENT ? 2 * i : i, b = ADJACENT ? 2 * i + 1 : i + pairs;
+    const float u = T::get(gload<typename T::elem>(in + a));
+    const float v = T::get(gload<typename T::elem>(in + b));
+    gstore<typename T::elem>(out + a, T::put(u * t[i].c - v * t[i].s));
+    gstore<typename T::elem>(out + b, T::put(u * t[i].s + v * t[i].c));
+  }
+}
+
+template <class T, bool ADJACENT>
+__global__ __launch_bounds__(256) void rotary_turn(pots_rotary a, uint32_t tokens, uint64_t from) {
+  typedef typename T::elem elem;
+  constexpr uint32_t P = kPairs<T>;
+  __shared__ Turn s_turn[kAngles];
+  __shared__ int64_t s_at[4][kTokens];  // where the block's tokens lie in q, k and the outputs
+  const uint64_t all = (uint64_t)a.batch * a.n, t0 = from + (uint64_t)blockIdx.x * tokens;
+  const uint32_t here = (uint32_t)(all - t0 < tokens ? all - t0 : tokens);
+  const uint32_t heads = a.heads + a.kv_heads;
+  for (uint32_t t = threadIdx.x; t < here; t += 256) {
+    const uint32_t b = (uint32_t)((t0 + t) / a.n), n = (uint32_t)(t0 + t - (uint64_t)b * a.n);
+    s_at[0][t] = b * a.q.batch + n * a.q.row;
+    s_at[1][t] = b * a.k.batch + n * a.k.row;
+    s_at[2][t] = b * a.q_out.batch + n * a.q_out.row;
+    s_at[3][t] = b * a.k_out.batch + n * a.k_out.row;
+  }
+  for (uint32_t e = threadIdx.x; e < here * a.pairs; e += 256) {
+    const uint32_t t = e / a.pairs, i = e - t * a.pairs;
+    const uint32_t b = (uint32_t)((t0 + t) / a.n), n = (uint32_t)(t0 + t - (uint64_t)b * a.n);
+    uint32_t axis = 0;
+    for (uint32_t x = 0; x + 1 < a.axes; x++) axis += i >= a.ends[x];
+    const int64_t at = axis * a.position_axis + b * a.position_batch + n * a.position_token;
+    const double position =
+        a.position_bits == 64
+            ? (double)gload<int64_t>(reinterpret_cast<const int64_t*>(a.positions) + at)
+            : (double)gload<int32_t>(reinterpret_cast<const int32_t*>(a.positions) + at);
+    const double f = a.frequency_type == POTS_OP_F64
+                         ? gload<double>(reinterpret_cast<const double*>(a.frequencies) + i)
+                         : (double)gload<float>(reinterpret_cast<const float*>(a.frequencies) + i);
+    s_turn[e] = turn_of(position, f, a.inverse);
+  }
+  __syncthreads();
+  // A head's runs: those of its pairs, then those of the columns that are copied.
+  const uint32_t turned = a.pairs < P ? 1 : (a.pairs + P - 1) / P;
+  const uint32_t rest = a.head_dim - 2 * a.pairs;
+  const uint32_t runs = turned + (rest < 2 * P ? rest != 0 : (rest + 2 * P - 1) / (2 * P));
+  const uint32_t slots = 256 / runs, slot = threadIdx.x / runs, run = threadIdx.x - slot * runs;
+  if (slot >= slots) return;
+  const bool turns = run < turned, whole = turns ? a.pairs >= P : rest >= 2 * P;
+  const uint32_t i0 = min(run * P, a.pairs - P);
+  const uint32_t at = !turns ? 2 * a.pairs + min((run - turned) * 2 * P, rest - 2 * P)
+                      : ADJACENT ? 2 * i0 : i0;
+  const uint32_t apart = turns && !ADJACENT ? a.pairs : P;
+  const uint32_t items = here * heads;
+  auto place = [&](uint32_t item, uint32_t& t, const elem*& in, elem*& out) {
+    t = item / heads;
+    const uint32_t h = item - t * heads;
+    if (h < a.heads) {
+      in = reinterpret_cast<const elem*>(a.q.ptr) + s_at[0][t] + h * a.q.head;
+      out = reinterpret_cast<elem*>(a.q_out.ptr) + s_at[2][t] + h * a.q_out.head;
+    } else {
+      const uint32_t g = h - a.heads;
+      in = reinterpret_cast<const elem*>(a.k.ptr) + s_at[1][t] + g * a.k.head;
+      out = reinterpret_cast<elem*>(a.k_out.ptr) + s_at[3][t] + g * a.k_out.head;
+    }
+  };
+  if (whole) {
+    for (uint32_t item = slot; item < items; item += kAhead * slots) {
+      Piece<T, ADJACENT> x[kAhead];
+      elem* out[kAhead];
+      uint32_t t[kAhead];
+#pragma unroll
+      for (uint32_t j = 0; j < kAhead; j++) {
+        const elem* in;  // (past the last item: that one again, and nothing is stored)
+        place(min(item + j * slots, items - 1), t[j], in, out[j]);
+        x[j].load(in, at, apart);
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < kAhead; j++) {
+        if (turns) x[j].turn(s_turn + t[j] * a.pairs + i0);
+        if (item + j * slots < items) x[j].store(out[j], at, apart);
+      }
+    }
+  } else {
+    for (uint32_t item = slot; item < items; item += slots) {
+      uint32_t t;
+      const elem* in;
+      elem* out;
+      place(item, t, in, out);
+      if (turns)
+        turn_few<T, ADJACENT>(in, out, a.pairs, s_turn + t * a.pairs);
+      else
+        for (uint32_t c = 2 * a.pairs; c < a.head_dim; c++)
+          gstore<elem>(out + c, gload<elem>(in + c));
+    }
+  }
+}
+
+namespace {
+
+bool bad(const pots_rotary* a) {
+  if (!a || a->dtype > POTS_OP_BF16 || a->head_dim == 0 || a->head_dim > kMaxWidth ||
+      a->pairs == 0 || 2 * a->pairs > a->head_dim || a->pairs > kMaxWidth || a->axes == 0 ||
+      a->axes > 4 || a->heads == 0 || a->kv_heads == 0 || a->heads > kMaxHeads ||
+      a->kv_heads > kMaxHeads || (uint64_t)a->batch * a->n > 0x7fffffffu)
+    return true;
+  if (a->frequency_type != POTS_OP_F32 && a->frequency_type != POTS_OP_F64) return true;
+  if (a->position_bits != 32 && a->position_bits != 64) return true;
+  for (uint32_t x = 1; x < a->axes; x++)
+    if (a->ends[x] < a->ends[x - 1]) return true;
+  return a->ends[a->axes - 1] != a->pairs;
+}
+
+template <class T>
+int turn(const pots_rotary* a, hipStream_t s) {
+  // Tokens of a block: few enough for four blocks to a compute unit, as many as their angles allow.
+  const uint64_t all = (uint64_t)a->batch * a->n;
+  uint64_t tokens = all / 1024;
+  const uint32_t most = kAngles / a->pairs < kTokens ? kAngles / a->pairs : kTokens;
+  tokens = tokens < 1 ? 1 : tokens > most ? most : tokens;
+  const auto kernel = a->adjacent ? rotary_turn<T, true> : rotary_turn<T, false>;
+  constexpr uint64_t kLaunch = 1u << 23;  // blocks: a launch has less than 2^32 threads
+  for (uint64_t from = 0; from < all; from += kLaunch * tokens) {
+    const uint64_t blocks = (all - from + tokens - 1) / tokens;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(blocks < kLaunch ? blocks : kLaunch)), dim3(256), 0, s,
+                       *a, (uint32_t)tokens, from);
+    POTS_HIP(hipGetLastError());
+  }
+  return POTS_E_OK;
+}
+
+}  // namespace
+
+}  // namespace pots
+
+using namespace pots;
+
+extern "C" int pots_rotary_turn(const pots_rotary* a, void* stream) {
+  if (bad(a)) return POTS_E_ARG;
+  if (a->batch == 0 || a->n == 0) return POTS_E_OK;
+  if (!a->q.ptr || !a->k.ptr || !a->q_out.ptr || !a->k_out.ptr || !a->positions || !a->frequencies)
+    return POTS_E_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return a->dtype == POTS_OP_BF16 ? turn<Bf16>(a, s) : turn<Fp32>(a, s);
+}

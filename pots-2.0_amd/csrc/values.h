@@ -1,0 +1,146 @@
+// Runs of values of rows that start anywhere, as the memory-bound operators read and write them.
+//
+// The GPU's global loads and stores take 16 bytes at any address of an element, so a row of odd width
+// or offset is read and written as wide as an aligned one, but for the run that crosses its end.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "gmem.h"
+#include "tiles.h"
+
+namespace pots {
+
+// N values of a row, one lane's share.
+template <class T, uint32_t N>
+using Run = typename T::elem __attribute__((ext_vector_type(N)));
+
+// Loads and stores of a V that is aligned as an E alone.
+template <class V, class E>
+struct __attribute__((packed, aligned(alignof(E)))) Loose {
+  V v;
+};
+template <class V, class E>
+__device__ __forceinline__ V load_any(const E* p) {
+  return ((const POTS_GLOBAL Loose<V, E>*)p)->v;
+}
+template <class V, class E>
+__device__ __forceinline__ void store_any(E* p, V v) {
+  ((POTS_GLOBAL Loose<V, E>*)p)->v = v;
+}
+
+// A run's values from the one numbered `by` (0 to N - 1) on, zeros behind them.
+template <class T, uint32_t N>
+__device__ __forceinline__ Run<T, N> shifted(Run<T, N> x, uint32_t by) {
+#pragma unroll
+  for (uint32_t m = 1; m < N; m *= 2) {
+    Run<T, N> y = {};
+#pragma unroll
+    for (uint32_t j = 0; j + m < N; j++) y[j] = x[j + m];
+    x = by & m ? y : x;
+  }
+  return x;
+}
+
+// A lane's G runs of a row of `dim` values: those from first + i·step on, zeros past the row's end. A
+// run that crosses the end is read as the row's last N values and shifted, so that all loads are on
+// their way before the first is waited for. (dim is the same for all lanes, and one of the three ways
+// is taken.)
+template <class T, uint32_t N, uint32_t G>
+__device__ __forceinline__ void load_runs(const typename T::elem* row, uint32_t first, uint32_t step,
+                                          uint32_t dim, Run<T, N> (&x)[G]) {
+  if (dim % N == 0) {
+#pragma unroll
+    for (uint32_t i = 0; i < G; i++) {
+      x[i] = Run<T, N>{};
+      if (first + i * step < dim) x[i] = load_any<Run<T, N>>(row + first + i * step);
+    }
+  } else if (dim > N) {
+#pragma unroll
+    for (uint32_t i = 0; i < G; i++) {
+      x[i] = Run<T, N>{};
+      if (first + i * step < dim) x[i] = load_any<Run<T, N>>(row + min(first + i * step, dim - N));
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < G; i++) {
+      const uint32_t c = first + i * step;
+      x[i] = shifted<T, N>(x[i], c < dim ? c - min(c, dim - N) : 0);
+    }
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < G; i++) {
+      x[i] = Run<T, N>{};
+#pragma unroll
+      for (uint32_t j = 0; j < N; j++)
+        if (first + i * step + j < dim) x[i][j] = gload<typename T::elem>(row + first + i * step + j);
+    }
+  }
+}
+
+// N values from p on, of which the row has `left`.
+template <class T, uint32_t N>
+__device__ __forceinline__ void store_run(typename T::elem* p, uint32_t left,
+                                          const float (&v)[N]) {
+  if (left >= N) {
+    Run<T, N> x;
+#pragma unroll
+    for (uint32_t j = 0; j < N; j++) x[j] = T::put(v[j]);
+    store_any(p, x);
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j + 1 < N; j++)
+      if (j < left) gstore<typename T::elem>(p + j, T::put(v[j]));
+  }
+}
+
+// The same for a type that is the call's.
+template <uint32_t N>
+__device__ __forceinline__ void put_run(void* p, uint32_t type, int64_t at, uint32_t left,
+                                        const float (&v)[N]) {
+  if (type == POTS_OP_BF16)
+    store_run<Bf16, N>(reinterpret_cast<uint16_t*>(p) + at, left, v);
+  else
+    store_run<Fp32, N>(reinterpret_cast<float*>(p) + at, left, v);
+}
+
+// Runs of four whose type is the call's: held as they lie in memory, made fp32 where they are used.
+template <uint32_t G>
+struct AnyRuns {
+  Run<Fp32, 4> raw[G];
+
+  __device__ __forceinline__ void load(const void* p, uint32_t type, uint32_t first, uint32_t step,
+                                       uint32_t dim) {
+    if (type == POTS_OP_BF16) {
+      Run<Bf16, 4> x[G];
+      load_runs<Bf16, 4, G>(reinterpret_cast<const uint16_t*>(p), first, step, dim, x);
+#pragma unroll
+      for (uint32_t i = 0; i < G; i++) {
+        const u32x2v bits = __builtin_bit_cast(u32x2v, x[i]);
+        raw[i][0] = __uint_as_float(bits[0]);
+        raw[i][1] = __uint_as_float(bits[1]);
+      }
+    } else {
+      load_runs<Fp32, 4, G>(reinterpret_cast<const float*>(p), first, step, dim, raw);
+    }
+  }
+  __device__ __forceinline__ void get(uint32_t type, uint32_t i, float (&v)[4]) const {
+    float x[4] = {raw[i][0], raw[i][1], raw[i][2], raw[i][3]};
+    // (here and not where they were loaded: the conversion would wait for them there)
+    asm volatile("" : "+v"(x[0]), "+v"(x[1]));
+    const uint32_t lo = __float_as_uint(x[0]), hi = __float_as_uint(x[1]);
+    const bool halves = type == POTS_OP_BF16;
+    v[0] = halves ? __uint_as_float(lo << 16) : x[0];
+    v[1] = halves ? __uint_as_float(lo & 0xffff0000u) : x[1];
+    v[2] = halves ? __uint_as_float(hi << 16) : x[2];
+    v[3] = halves ? __uint_as_float(hi & 0xffff0000u) : x[3];
+  }
+};
+
+__device__ __forceinline__ float sum_wave(float v) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+}  // namespace pots

@@ -164,6 +164,19 @@ class Native:
             "pots_embedding_forward": ([ctypes.c_char_p, _vp], _int),
             "pots_embedding_backward_work": ([ctypes.c_char_p], _u64),
             "pots_embedding_backward": ([ctypes.c_char_p, _vp, _vp], _int),
+            "pots_rms_norm_forward": ([ctypes.c_char_p, _vp], _int),
+            "pots_rms_norm_quantized": ([ctypes.c_char_p, _vp], _int),
+            "pots_rms_norm_backward_work": ([ctypes.c_char_p], _u64),
+            "pots_rms_norm_backward": ([ctypes.c_char_p, _vp, _vp], _int),
+            "pots_rotary_turn": ([ctypes.c_char_p, _vp], _int),
+            "pots_gated_silu_forward": ([ctypes.c_char_p, _vp], _int),
+            "pots_gated_silu_backward": ([ctypes.c_char_p, _vp], _int),
+            "pots_gradient_norm_work": ([ctypes.c_char_p], _u64),
+            "pots_gradient_norm": ([ctypes.c_char_p, _vp, _vp], _int),
+            "pots_clip_gradients_work": ([ctypes.c_char_p], _u64),
+            "pots_clip_gradients": ([ctypes.c_char_p, _vp, _vp], _int),
+            "pots_sgd_step_work": ([ctypes.c_char_p], _u64),
+            "pots_sgd_step": ([ctypes.c_char_p, _vp, _vp], _int),
         }
         for name, (args, res) in sigs.items():
             fn = getattr(lib, name)
@@ -172,10 +185,13 @@ class Native:
         self._lib = lib
         # name: its entry point, and the one that says how much scratch it wants
         self._operators = {
-            f"{op}_{way}": (getattr(lib, f"pots_{op}_{way}"),
-                            getattr(lib, f"pots_{op}_{way}_work", None)
-                            if f"pots_{op}_{way}_work" in sigs else None)
-            for op in ("attention", "vocab_loss", "embedding") for way in ("forward", "backward")}
+            name: (getattr(lib, f"pots_{name}"),
+                   getattr(lib, f"pots_{name}_work", None) if f"pots_{name}_work" in sigs else None)
+            for name in ("attention_forward", "attention_backward", "vocab_loss_forward",
+                         "vocab_loss_backward", "embedding_forward", "embedding_backward",
+                         "rms_norm_forward", "rms_norm_quantized", "rms_norm_backward",
+                         "rotary_turn", "gated_silu_forward", "gated_silu_backward",
+                         "gradient_norm", "clip_gradients", "sgd_step")}
         self.version = lib.pots_mi355x_version().decode()
         self.blake3_version = lib.pots_blake3_version().decode()
         self.simd_degree = int(lib.pots_simd_degree())

@@ -320,7 +320,8 @@ class DecoderComputation(DeclaredComputation):
             logits = model(input_ids=ids).logits
         return self._block_loss(logits, targets, mask, mask.sum())
 
-    def uncaptured_loss(self, model: torch.nn.Module, records) -> torch.Tensor:
+    def uncaptured_loss(self, model: torch.nn.Module, records, *, fused: bool = False
+                        ) -> torch.Tensor:
         """:meth:`loss` for a pass that leaves no transcript (a held-out batch, a step between
         audits), on the GPU: the embedding, the attention and the loss run as the operators of
         ``verification.computation.operators``, which keep no attention probability and no
@@ -328,7 +329,11 @@ class DecoderComputation(DeclaredComputation):
         time. The same mean over the masked tokens, and differentiable in the same weights; its
         sums are taken in another order, so the bits are not the captured step's. Heads are at
         most ``operators.MAX_HEAD_DIM`` wide, and the model's attention is :meth:`build_model`'s
-        (``ValueError`` otherwise)."""
+        (``ValueError`` otherwise).
+
+        With ``fused`` the rest of a layer runs as operators too: the residual's additions with
+        the norms after them, the rotary positions and the gated activation
+        (:meth:`_fused_features`)."""
         from verification.computation import operators
         from verification.computation.instances.attention import ATTENTION, uncaptured_mask
         if model.config._attn_implementation != ATTENTION:
@@ -338,12 +343,58 @@ class DecoderComputation(DeclaredComputation):
         ids, targets, mask = self._batch(records, dev)
         with self.autocast(dev):
             rows = operators.embedding(ids, model.get_input_embeddings().weight)
-            f = model.model(inputs_embeds=rows,
+            f = self._fused_features(model, rows) if fused else \
+                model.model(inputs_embeds=rows,
                             attention_mask=uncaptured_mask(dev)).last_hidden_state
         weights = mask.reshape(-1) / mask.sum()
         return operators.vocab_loss(f.reshape(-1, self.d).to(self.compute_dtype),
                                     model.get_output_embeddings().weight.to(self.compute_dtype),
                                     targets.reshape(-1), weights)
+
+    def _fused_features(self, model: torch.nn.Module, rows: torch.Tensor) -> torch.Tensor:
+        """The model's features ``F`` from its embedded tokens ``[n_s, n, d]``: each layer's linear
+        modules called as they are, and between them operators. The residual stream keeps the
+        rows' type (the masters' fp32); norms read the branch in the products' type and write what
+        the next products read. Layers that are checkpointed, an activation other than silu, a
+        sliding window and frequencies that a call would rescale are refused."""
+        from verification.computation import operators
+        body, cfg = model.model, model.config
+        rope = body.rotary_emb
+        if getattr(body, "gradient_checkpointing", False) and body.training:
+            raise ValueError("fused layers are not checkpointed")
+        if cfg.hidden_act != "silu":
+            raise ValueError(f"the model's activation is {cfg.hidden_act!r}, not 'silu'")
+        if getattr(rope, "attention_scaling", 1.0) != 1.0 or \
+                "dynamic" in rope.rope_type or rope.rope_type == "longrope":
+            raise ValueError(f"rotary positions of type {rope.rope_type!r} are not fused")
+        dev, dt = rows.device, self.compute_dtype
+        n_s, n = rows.shape[:2]
+        positions = torch.arange(n, device=dev)
+
+        def heads(x: torch.Tensor, width: int) -> torch.Tensor:
+            return x.view(n_s, n, -1, width).transpose(1, 2)
+
+        def normed(module: torch.nn.Module, stream: torch.Tensor, branch: torch.Tensor | None):
+            eps = module.variance_epsilon
+            if branch is None:
+                return operators.rms_norm(stream, module.weight, eps=eps, out_dtype=dt), stream
+            return operators.rms_norm(branch, module.weight, eps=eps, residual=stream,
+                                      out_dtype=dt)
+
+        stream, branch = rows, None
+        for layer in body.layers:
+            att, mlp = layer.self_attn, layer.mlp
+            if getattr(att, "sliding_window", None) is not None:
+                raise ValueError("the uncaptured attention is over whole sequences: no sliding "
+                                 "window")
+            y, stream = normed(layer.input_layernorm, stream, branch)
+            q, k = operators.rotary(heads(att.q_proj(y), att.head_dim),
+                                    heads(att.k_proj(y), att.head_dim), positions, rope.inv_freq)
+            o = operators.attention(q, k, heads(att.v_proj(y), att.head_dim), scale=att.scaling)
+            branch = att.o_proj(o.transpose(1, 2).reshape(n_s, n, -1))
+            y, stream = normed(layer.post_attention_layernorm, stream, branch)
+            branch = mlp.down_proj(operators.gated_silu(mlp.gate_proj(y), mlp.up_proj(y)))
+        return normed(body.norm, stream, branch)[0]
 
     def forward_backward(self, model: torch.nn.Module, records, stage) -> torch.Tensor:
         """One training pass. With one head block, the loss over the whole batch and its

@@ -1,15 +1,21 @@
-"""The operators of a training pass that nobody audits: attention, the loss over a vocabulary
-and the embedding, each with its gradient.
+"""The operators of a training step that nobody audits: attention, the loss over a vocabulary
+and the embedding, each with its gradient; what lies between a layer's products (norms, rotary
+positions, the gated activation); and the clipped update.
 
 A captured step (``verification.prover``) keeps every product of the inventory, the attention
 probabilities and the logits among them, because a verifier will ask for them. A step that
 leaves no transcript (a warm-up, a held-out loss, the steps between audits) need not write
 either to memory. These calls run such a pass on the same model, with the kernels of
-``libpots_mi355x`` (``pots_attention_*``, ``pots_vocab_loss_*``, ``pots_embedding_*``):
+``libpots_mi355x`` (``pots_attention_*``, ``pots_vocab_loss_*``, ``pots_embedding_*``,
+``pots_rms_norm_*``, ``pots_rotary_turn``, ``pots_gated_silu_*``, ``pots_gradient_norm``,
+``pots_clip_gradients``, ``pots_sgd_step``):
 
-- :func:`attention`, :func:`vocab_loss` and :func:`embedding` are differentiable;
+- :func:`attention`, :func:`vocab_loss`, :func:`embedding`, :func:`rms_norm`, :func:`rotary` and
+  :func:`gated_silu` are differentiable;
 - the ``*_forward`` and ``*_backward`` functions under them are the kernels' own calls, for
-  programs that keep their own tape or only evaluate.
+  programs that keep their own tape or only evaluate;
+- :func:`rms_norm_quantized` gives a norm's output in 8 bits;
+- :func:`gradient_norm`, :func:`clip_gradients` and :func:`sgd_step` take a model's whole gradient.
 
 Tensors are on the GPU, in fp32 or bf16; sums, softmax statistics and losses are fp32. Calls
 enqueue on the current stream and never wait for the GPU; outputs and scratch come from torch's
@@ -17,7 +23,8 @@ allocator on that stream, so a tensor made on another stream needs the usual
 ``wait_stream``. Results are the same bits on every run. Wrong shapes, types, sizes and devices raise
 ``ValueError``; ids and targets are not read on the host, so those outside the vocabulary show
 in the result instead (NaN; a negative target is a row without a loss).
-``verification.computation.instances.decoder.DecoderComputation.uncaptured_loss`` runs all three.
+``verification.computation.instances.decoder.DecoderComputation.uncaptured_loss`` and
+``verification.prover.step.uncaptured_step`` run them.
 
 A differentiable call saves its inputs by reference. A backward pass that is captured into a
 graph wants leaves that no other live tape has used on another stream, as with any torch
@@ -28,6 +35,7 @@ from __future__ import annotations
 
 import math
 import struct
+from collections.abc import Sequence
 
 import torch
 
@@ -35,15 +43,28 @@ from verification.commitment import native
 
 __all__ = ["attention", "attention_forward", "attention_backward", "vocab_loss",
            "vocab_loss_forward", "vocab_loss_backward", "embedding", "embedding_forward",
-           "embedding_backward", "MAX_HEAD_DIM"]
+           "embedding_backward", "rms_norm", "rms_norm_forward", "rms_norm_backward",
+           "rms_norm_quantized", "rotary", "rotary_forward", "rotary_backward",
+           "rotary_frequencies", "gated_silu", "gated_silu_forward", "gated_silu_backward",
+           "gradient_norm", "clip_gradients", "sgd_step", "MAX_HEAD_DIM", "MAX_NORM_DIM",
+           "MAX_ROTARY_DIM"]
 
 MAX_HEAD_DIM = 128
+MAX_NORM_DIM = 1 << 14
+MAX_ROTARY_DIM = 1024
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
-# pots_attention, pots_vocab_loss and pots_embedding (include/pots_mi355x.h)
+_EIGHT_BITS = {torch.float8_e4m3fn: 2, torch.int8: 3}
+_F64 = 4
+# the argument blocks of include/pots_mi355x.h
 _ATTENTION = struct.Struct("<32q2q7If")
 _LOSS = struct.Struct("<12q4I")
 _EMBEDDING = struct.Struct("<5q5If")
+_NORM = struct.Struct("<17q7If")
+_ROTARY = struct.Struct("<21q16I")
+_GATED = struct.Struct("<9q3I4x")
+_GRADIENTS = struct.Struct("<q2f2I")
+_GRADIENT = struct.Struct("<3qQ2I")
 _NO_HEADS = (0, 0, 0, 0)
 _MOST, _LEAST = torch.finfo(torch.float32).max, 2.0**-149  # of fp32, above zero
 
@@ -422,3 +443,408 @@ class _Embedding(torch.autograd.Function):
 def embedding(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
     """:func:`embedding_forward`, differentiable in ``table``."""
     return _Embedding.apply(ids, table, scale)
+
+
+# ---- the norm -------------------------------------------------------------------------------
+
+def _as_rows(t: torch.Tensor) -> torch.Tensor:
+    """``[..., d]`` as rows of consecutive values, wherever they start."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _norm_args(x: torch.Tensor, weight: torch.Tensor, eps: float, what: str) -> int:
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_NORM_DIM:
+        raise ValueError(f"{what} must be [..., dim] with dim in [1, {MAX_NORM_DIM}], got "
+                         f"{tuple(x.shape)}")
+    if weight.shape != x.shape[-1:] or weight.device != x.device:
+        raise ValueError(f"weight must be [{x.shape[-1]}] on {x.device}")
+    if not _LEAST <= eps <= _MOST:
+        raise ValueError(f"eps must be positive and finite in fp32, got {eps}")
+    return _dtype(weight, "weight")
+
+
+def _summands(x: torch.Tensor, residual: torch.Tensor | None) -> None:
+    _dtype(x, "x")
+    if residual is None:
+        return
+    if residual.shape != x.shape or residual.device != x.device:
+        raise ValueError(f"residual must be {tuple(x.shape)} on {x.device}")
+    _dtype(residual, "residual")
+
+
+def _run_norm(name: str, x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None,
+              y: torch.Tensor, y_type: int, rstd: torch.Tensor | None,
+              scales: torch.Tensor | None, block: int, eps: float) -> torch.Tensor:
+    """The forward calls; the sum that was normed."""
+    _on_gpu(x)
+    total = x if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    rows, own = _as_rows(x), weight.contiguous()
+    other = None if residual is None else _as_rows(residual)
+    args = _packed(_NORM, rows.data_ptr(), 0 if other is None else other.data_ptr(), own.data_ptr(),
+                   0 if other is None else total.data_ptr(), y.data_ptr(),
+                   0 if rstd is None else rstd.data_ptr(),
+                   0 if scales is None else scales.data_ptr(), 0, 0, 0, 0, 0, rows.stride(0),
+                   0 if other is None else other.stride(0), 0, 0, 0, rows.shape[0], rows.shape[1],
+                   block, _DTYPES[x.dtype], _DTYPES[total.dtype], _DTYPES[weight.dtype], y_type, eps)
+    native.get().operator(name, args, x.device)
+    return total
+
+
+def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6,
+                     residual: torch.Tensor | None = None, out_dtype: torch.dtype | None = None
+                     ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``y = t · s · weight`` over rows ``[..., dim]`` with ``t = x + residual`` and
+    ``s = 1/√(mean t² + eps)``: ``(y, t, s)``. Each tensor has its own type, fp32 or bf16: ``t``
+    the residual's (rounded to it once, and that is what is normed), ``y`` ``out_dtype``
+    (``x``'s unless given), ``s`` fp32 ``[...]``. Without a residual ``t`` is ``x`` itself. Squares
+    are added in fp32: rows of sizes above 1e18 overflow."""
+    _norm_args(x, weight, eps, "x")
+    _summands(x, residual)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _DTYPES:
+        raise ValueError(f"out_dtype must be float32 or bfloat16, not {out_dtype}")
+    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    total = _run_norm("rms_norm_forward", x, weight, residual, y, _DTYPES[out_dtype], rstd, None, 0,
+                      eps)
+    return y, total, rstd
+
+
+def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6,
+                       residual: torch.Tensor | None = None,
+                       dtype: torch.dtype = torch.float8_e4m3fn, block: int | None = None
+                       ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """:func:`rms_norm_forward`'s ``y`` in 8 bits, ``float8_e4m3fn`` or ``int8``: ``(q, scales,
+    t)`` with ``y ≈ q · scale``, rounded to nearest from fp32. A scale (fp32 ``[..., blocks]``) is
+    the largest size of a row (``block`` None), or of each ``block`` columns (32, 64, 128 or 256;
+    the last may be fewer), over 448 or 127, and at least 2^-126. A block that holds a NaN has the
+    scale NaN; one that holds an infinity an infinite scale."""
+    _norm_args(x, weight, eps, "x")
+    _summands(x, residual)
+    if dtype not in _EIGHT_BITS:
+        raise ValueError(f"dtype must be float8_e4m3fn or int8, not {dtype}")
+    if block not in (None, 32, 64, 128, 256):
+        raise ValueError(f"block must be 32, 64, 128 or 256, or None for a row, not {block}")
+    blocks = 1 if block is None else -(-x.shape[-1] // block)
+    q = torch.empty(x.shape, dtype=dtype, device=x.device)
+    scales = torch.empty(*x.shape[:-1], blocks, dtype=torch.float32, device=x.device)
+    total = _run_norm("rms_norm_quantized", x, weight, residual, q, _EIGHT_BITS[dtype], None,
+                      scales, block or 0, eps)
+    return q, scales, total
+
+
+def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, weight: torch.Tensor,
+                      rstd: torch.Tensor, *, dtotal: torch.Tensor | None = None,
+                      x_dtype: torch.dtype | None = None
+                      ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(dx, dresidual, dweight)`` of :func:`rms_norm_forward` with its ``t`` and ``s``, for the
+    gradients ``dy`` of ``y`` and ``dtotal`` (of ``t``'s type, or None) of ``t``. ``x`` and the
+    residual have the same gradient: ``dresidual`` in ``t``'s type, ``dx`` in ``x_dtype`` (``t``'s
+    unless given; the same tensor where they are one type). ``dweight`` is summed in fp32 over all
+    rows, in ``weight``'s type."""
+    code = _norm_args(total, weight, 1.0, "total")
+    _dtype(total, "total")
+    if dy.shape != total.shape or dy.device != total.device:
+        raise ValueError(f"dy must be {tuple(total.shape)} on {total.device}")
+    dy_type = _dtype(dy, "dy")
+    if dtotal is not None:
+        _like(dtotal, total, total.shape, "dtotal")
+    rstd = _floats(rstd, total.device, total.shape[:-1], "rstd")
+    x_dtype = total.dtype if x_dtype is None else x_dtype
+    if x_dtype not in _DTYPES:
+        raise ValueError(f"x_dtype must be float32 or bfloat16, not {x_dtype}")
+    _on_gpu(total)
+    dresidual = torch.empty(total.shape, dtype=total.dtype, device=total.device)
+    dx = dresidual
+    if x_dtype != total.dtype:
+        dx = torch.empty(total.shape, dtype=x_dtype, device=total.device)
+    dweight = torch.empty(weight.shape, dtype=weight.dtype, device=total.device)
+    g, t, own = _as_rows(dy), _as_rows(total), weight.contiguous()
+    other = None if dtotal is None else _as_rows(dtotal)
+    args = _packed(_NORM, 0, 0, own.data_ptr(), t.data_ptr(), 0, rstd.data_ptr(), 0, g.data_ptr(),
+                   0 if other is None else other.data_ptr(),
+                   0 if dx is dresidual else dx.data_ptr(), dresidual.data_ptr(),
+                   dweight.data_ptr(), 0, 0, t.stride(0), g.stride(0),
+                   0 if other is None else other.stride(0), t.shape[0], t.shape[1], 0,
+                   _DTYPES[x_dtype], _DTYPES[total.dtype], code, dy_type, 1.0)
+    native.get().operator("rms_norm_backward", args, total.device)
+    return dx, dresidual, dweight
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps, out_dtype):
+        y, total, rstd = rms_norm_forward(x, weight, eps=eps, residual=residual,
+                                          out_dtype=out_dtype)
+        ctx.save_for_backward(total, weight, rstd)
+        ctx.x_dtype, ctx.added = x.dtype, residual is not None
+        ctx.set_materialize_grads(False)
+        return (y, total) if ctx.added else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dtotal=None):
+        total, weight, rstd = ctx.saved_tensors
+        if dy is None and dtotal is None:
+            return None, None, None, None, None
+        if dy is None:  # nobody read the norm
+            return dtotal.to(ctx.x_dtype), None, dtotal, None, None
+        dx, dresidual, dweight = rms_norm_backward(dy, total, weight, rstd, dtotal=dtotal,
+                                                   x_dtype=ctx.x_dtype)
+        return dx, dweight, dresidual if ctx.added else None, None, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6,
+             residual: torch.Tensor | None = None, out_dtype: torch.dtype | None = None
+             ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """:func:`rms_norm_forward`'s ``y``, and with a residual ``(y, t)``, differentiable in ``x``,
+    ``weight`` and ``residual``."""
+    return _RmsNorm.apply(x, weight, residual, eps, out_dtype)
+
+
+# ---- rotary positions -----------------------------------------------------------------------
+
+def rotary_frequencies(width: int, *, base: float = 10000.0,
+                       device: torch.device | str = "cuda") -> torch.Tensor:
+    """``base^(−2i/width)`` for the ``width/2`` pairs i of a head, fp64."""
+    if width < 2 or width % 2:
+        raise ValueError(f"width must be even and positive, got {width}")
+    i = torch.arange(0, width, 2, dtype=torch.float64)
+    return (base ** (-i / width)).to(device)
+
+
+def _turned(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
+            frequencies: torch.Tensor, sections: Sequence[int] | None, adjacent: bool,
+            inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q and k must be [batch, heads, n, head_dim]")
+    b, h, n, d = q.shape
+    kv = k.shape[1]
+    code = _dtype(q, "q")
+    if not 1 <= d <= MAX_ROTARY_DIM or h < 1 or kv < 1:
+        raise ValueError(f"head_dim must be in [1, {MAX_ROTARY_DIM}] and there must be heads, got "
+                         f"{tuple(q.shape)}")
+    _like(k, q, (b, kv, n, d), "k")
+    pairs = frequencies.numel()
+    if (frequencies.dtype not in (torch.float32, torch.float64) or frequencies.dim() != 1
+            or frequencies.device != q.device or not 2 <= 2 * pairs <= d):
+        raise ValueError(f"frequencies must be float32 or float64 [pairs] on {q.device}, one for "
+                         f"each pair of a head of {d}")
+    counts = (pairs,) if sections is None else tuple(sections)
+    if not 1 <= len(counts) <= 4 or min(counts) < 0 or sum(counts) != pairs:
+        raise ValueError(f"sections must be up to 4 counts whose sum is {pairs}, got {counts}")
+    axes = len(counts)
+    at = positions[None] if sections is None else positions
+    if at.dtype not in (torch.int64, torch.int32) or at.device != q.device:
+        raise ValueError(f"positions must be int64 or int32 on {q.device}")
+    if at.dim() == 2:
+        at = at[:, None]
+    if at.dim() != 3 or at.shape[0] != axes or at.shape[1] not in (1, b) or at.shape[2] != n:
+        raise ValueError(f"positions must be {'' if sections is None else f'{axes} times '}"
+                         f"[{n}] or [{b}, {n}], got {tuple(positions.shape)}")
+    _on_gpu(q)
+    at = at.expand(axes, b, n)
+    q, k = (t if d == 1 or t.stride(3) == 1 else t.contiguous() for t in (q, k))
+    frequencies = frequencies.contiguous()
+    to_q, to_k = _new_heads(b, h, n, d, q), _new_heads(b, kv, n, d, q)
+    ends = [sum(counts[:i + 1]) for i in range(axes)] + [pairs] * (4 - axes)
+    args = _packed(_ROTARY, *_places(q), *_places(k), *_places(to_q), *_places(to_k),
+                   at.data_ptr(), frequencies.data_ptr(), *at.stride(), b, h, kv, n, d, pairs, axes,
+                   *ends, code, 0 if frequencies.dtype == torch.float32 else _F64,
+                   64 if at.dtype == torch.int64 else 32, adjacent, inverse)
+    native.get().operator("rotary_turn", args, q.device)
+    return to_q, to_k
+
+
+def _places(t: torch.Tensor) -> tuple[int, int, int, int]:
+    return t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)
+
+
+def rotary_forward(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
+                   frequencies: torch.Tensor, *, sections: Sequence[int] | None = None,
+                   adjacent: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """``q [b, h, n, d]`` and ``k [b, kv, n, d]`` with their pairs turned by the angles
+    ``position · frequency``, any strides, fp32 or bf16, ``d`` up to 1024. ``frequencies`` (fp32
+    or fp64 ``[pairs]``, :func:`rotary_frequencies`): pair i is the columns ``(i, i + pairs)``, or
+    ``(2i, 2i + 1)`` with ``adjacent``; columns from ``2 · pairs`` on are copied. ``positions``
+    (int64 or int32) are ``[n]`` or ``[b, n]``. With ``sections``, counts of consecutive pairs for
+    each of up to 4 axes (time, height, width), they are ``[axes, n]`` or ``[axes, b, n]``. Angles
+    are taken in 64 bits. The results lie in memory as ``[b, n, heads, d]``."""
+    return _turned(q, k, positions, frequencies, sections, adjacent, False)
+
+
+def rotary_backward(dq: torch.Tensor, dk: torch.Tensor, positions: torch.Tensor,
+                    frequencies: torch.Tensor, *, sections: Sequence[int] | None = None,
+                    adjacent: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gradients of :func:`rotary_forward`'s ``q`` and ``k`` from those of its results: the
+    turns back."""
+    return _turned(dq, dk, positions, frequencies, sections, adjacent, True)
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, frequencies, sections, adjacent):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.kw = {"sections": sections, "adjacent": adjacent}
+        return rotary_forward(q, k, positions, frequencies, **ctx.kw)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        return *rotary_backward(dq, dk, *ctx.saved_tensors, **ctx.kw), None, None, None, None
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor,
+           *, sections: Sequence[int] | None = None, adjacent: bool = False
+           ) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`rotary_forward`, differentiable in ``q`` and ``k``."""
+    return _Rotary.apply(q, k, positions, frequencies, sections, adjacent)
+
+
+# ---- the gated activation -------------------------------------------------------------------
+
+def _gated_args(gate: torch.Tensor, up: torch.Tensor) -> int:
+    code = _dtype(gate, "gate")
+    if gate.dim() < 1:
+        raise ValueError("gate must be [..., columns]")
+    _like(up, gate, gate.shape, "up")
+    return code
+
+
+def gated_silu_forward(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """``silu(gate) · up``, ``silu(g) = g / (1 + e^−g)``, of two tensors ``[..., columns]`` of one
+    shape and type, each anywhere (the halves of one product, for instance)."""
+    code = _gated_args(gate, up)
+    _on_gpu(gate)
+    out = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    if out.numel():
+        g, u = _as_rows(gate), _as_rows(up)
+        args = _packed(_GATED, g.data_ptr(), u.data_ptr(), 0, out.data_ptr(), 0, 0, g.stride(0),
+                       u.stride(0), 0, *g.shape, code)
+        native.get().operator("gated_silu_forward", args, gate.device)
+    return out
+
+
+def gated_silu_backward(dout: torch.Tensor, gate: torch.Tensor, up: torch.Tensor
+                        ) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(dgate, dup)`` of :func:`gated_silu_forward`."""
+    code = _gated_args(gate, up)
+    _like(dout, gate, gate.shape, "dout")
+    _on_gpu(gate)
+    dgate = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    dup = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    if dgate.numel():
+        g, u, d = _as_rows(gate), _as_rows(up), _as_rows(dout)
+        args = _packed(_GATED, g.data_ptr(), u.data_ptr(), d.data_ptr(), 0, dgate.data_ptr(),
+                       dup.data_ptr(), g.stride(0), u.stride(0), d.stride(0), *g.shape, code)
+        native.get().operator("gated_silu_backward", args, gate.device)
+    return dgate, dup
+
+
+class _GatedSilu(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, up):
+        ctx.save_for_backward(gate, up)
+        return gated_silu_forward(gate, up)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        return gated_silu_backward(g, *ctx.saved_tensors)
+
+
+def gated_silu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """:func:`gated_silu_forward`, differentiable in ``gate`` and ``up``."""
+    return _GatedSilu.apply(gate, up)
+
+
+# ---- the whole gradient ---------------------------------------------------------------------
+
+def _tensors(of: Sequence[torch.Tensor], what: str, device: torch.device | None = None
+             ) -> tuple[list[torch.Tensor], list[int], torch.device]:
+    """A list of tensors of one device, and their types."""
+    of = list(of)
+    if not of or not all([isinstance(t, torch.Tensor) for t in of]):
+        raise ValueError(f"{what} must be tensors, at least one")
+    device = of[0].device if device is None else device
+    if any([t.device != device for t in of]):
+        raise ValueError(f"{what} must be on {device}")
+    codes = [_DTYPES.get(t.dtype) if t.layout is torch.strided else None for t in of]
+    if None in codes:
+        raise ValueError(f"{what} must be dense, float32 or bfloat16")
+    return of, codes, device
+
+
+def _written(of: Sequence[torch.Tensor], like: list[torch.Tensor], what: str
+             ) -> list[torch.Tensor]:
+    of = list(of)
+    if ([t.shape for t in of] != [t.shape for t in like]
+            or [t.dtype for t in of] != [t.dtype for t in like]
+            or any([t.device != u.device for t, u in zip(of, like)])):
+        raise ValueError(f"{what} must have the shapes, types and device of what goes there")
+    if not all([t.is_contiguous() for t in of]):
+        raise ValueError(f"{what} must be contiguous, since they are written")
+    return of
+
+
+def _change(name: str, gradients: list[torch.Tensor], codes: list[int],
+            weights: list[torch.Tensor] | None, weight_codes: list[int],
+            out: list[torch.Tensor] | None, max_norm: float, eta: float) -> torch.Tensor:
+    """The calls over lists; the norm."""
+    device = gradients[0].device
+    _on_gpu(gradients[0])
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    g = [t if t.is_contiguous() else t.contiguous() for t in gradients]
+    w = None if weights is None else [t if t.is_contiguous() else t.contiguous() for t in weights]
+    zeros = [0] * len(g)
+    entries = map(_GRADIENT.pack, [t.data_ptr() for t in g],
+                  zeros if w is None else [t.data_ptr() for t in w],
+                  zeros if out is None else [t.data_ptr() for t in out], [t.numel() for t in g],
+                  codes, weight_codes)
+    args = _packed(_GRADIENTS, norm.data_ptr(), max_norm, eta, len(g), 0) + b"".join(entries)
+    native.get().operator(name, args, device)
+    if out is not None:  # autograd is told, as it is of any write
+        torch.autograd.graph.increment_version(out)
+    return norm
+
+
+def _max_norm(max_norm: float) -> float:
+    if not max_norm >= _LEAST:
+        raise ValueError(f"max_norm must be positive in fp32, got {max_norm}")
+    return max_norm if max_norm <= _MOST else math.inf
+
+
+def gradient_norm(gradients: Sequence[torch.Tensor]) -> torch.Tensor:
+    """The 2-norm of the values of all ``gradients`` (fp32 or bf16, of any shapes) together, fp32
+    ``[]``. Squares are added in fp64, so nothing overflows on the way."""
+    g, codes, _ = _tensors(gradients, "gradients")
+    return _change("gradient_norm", g, codes, None, [0] * len(g), None, 0.0, 0.0)
+
+
+def clip_gradients(gradients: Sequence[torch.Tensor], max_norm: float, *,
+                   out: Sequence[torch.Tensor] | None = None) -> torch.Tensor:
+    """Scale ``gradients`` by ``min(1, max_norm / norm)``, in place or into ``out``; returns their
+    :func:`gradient_norm`. A norm that is NaN makes every value NaN, and an infinite one zero but
+    for the infinities (NaN). What is written must be contiguous, and overlap nothing but the
+    gradient that it replaces."""
+    g, codes, _ = _tensors(gradients, "gradients")
+    to = _written(g if out is None else out, g, "gradients" if out is None else "out")
+    return _change("clip_gradients", g, codes, None, [0] * len(g), to, _max_norm(max_norm), 0.0)
+
+
+def sgd_step(weights: Sequence[torch.Tensor], gradients: Sequence[torch.Tensor], eta: float, *,
+             max_norm: float = math.inf, out: Sequence[torch.Tensor] | None = None
+             ) -> torch.Tensor:
+    """``W ← W − eta · min(1, max_norm / norm) · G`` over a model's weights and their gradients, in
+    place or into ``out``, the gradients left as they are; returns their :func:`gradient_norm`.
+    Weights and gradients are fp32 or bf16 each; the update is one fp32 multiplication and addition,
+    rounded once. Norms that are not finite and what is written: :func:`clip_gradients`."""
+    g, codes, device = _tensors(gradients, "gradients")
+    w, weight_codes, _ = _tensors(weights, "weights", device)
+    if [t.shape for t in w] != [t.shape for t in g]:
+        raise ValueError("weights and gradients must have the same shapes")
+    if not -_MOST <= eta <= _MOST:
+        raise ValueError(f"eta must be finite in fp32, got {eta}")
+    to = _written(w if out is None else out, w, "weights" if out is None else "out")
+    return _change("sgd_step", g, codes, w, weight_codes, to, _max_norm(max_norm), eta)

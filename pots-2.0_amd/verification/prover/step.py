@@ -17,6 +17,7 @@ PCIe.
 
 from __future__ import annotations
 
+import math
 from collections.abc import Callable, Iterator, Mapping, Sequence
 from contextlib import contextmanager
 from dataclasses import dataclass, field
@@ -29,7 +30,7 @@ from verification.computation.interface import (DeclaredComputation, load_weight
 from verification.computation.matmul_ops import param_storage_map
 from verification.prover.capture import MatmulCapture, MutatedCaptureError
 
-__all__ = ["StepOutput", "prove_step", "commit"]
+__all__ = ["StepOutput", "prove_step", "uncaptured_step", "commit"]
 
 Perturbation = Callable[[torch.Tensor], torch.Tensor]
 
@@ -164,6 +165,27 @@ def prove_step(c: DeclaredComputation, model: torch.nn.Module, w_t: Mapping[str,
         versions=(record_versions + w_t_versions + tuple(product_versions)
                   + _versions(list(w_next.values()))),
         capture=summary, operands=operands)
+
+
+def uncaptured_step(c: DeclaredComputation, model: torch.nn.Module, records: Sequence[Any], *,
+                    max_norm: float = math.inf) -> tuple[torch.Tensor, torch.Tensor]:
+    """One step that leaves no transcript, on the GPU: the gradient of the computation's
+    ``uncaptured_loss`` over fused layers, clipped to ``max_norm``, and plain SGD at the declared
+    ``eta``, in place. Returns the loss and the gradient's norm before the clip, both on the GPU.
+    ``model`` is left holding the new weights with its gradients cleared; a weight without a
+    gradient stays as it is."""
+    from verification.computation import operators
+    if not hasattr(c, "uncaptured_loss"):
+        raise ValueError(f"{type(c).__name__} has no uncaptured pass")
+    if not torch.is_grad_enabled():
+        raise RuntimeError("uncaptured_step needs grad mode on")
+    model.zero_grad(set_to_none=True)
+    loss = c.uncaptured_loss(model, records, fused=True)
+    loss.backward()
+    weights = [p for p in model.parameters() if p.grad is not None]
+    norm = operators.sgd_step(weights, [p.grad for p in weights], c.eta, max_norm=max_norm)
+    model.zero_grad(set_to_none=True)
+    return loss.detach(), norm
 
 
 def commit(c: DeclaredComputation, step: StepOutput):
