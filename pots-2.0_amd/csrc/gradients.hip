@@ -26,7 +26,13 @@ namespace pots {
 constexpr uint32_t kChunk = 4096;  // values of a chunk: four runs of four to each of 256 lanes
 constexpr uint32_t kRunsOf = kChunk / 1024;
 constexpr uint32_t kNormed = 160, kUpdated = 96;  // tensors of a launch: below 4 KiB of arguments
-constexpr uint32_t kBlocks = 2048;  // eight to a compute unit
+// Four to a compute unit: the update of 1.54e9 fp32 weights takes 4.30 ms, with eight 4.43.
+constexpr uint32_t kBlocks = 1024;
+// The last cache is left to the chunks that the second pass begins with, 192 MiB of fp32: what comes
+// before them is read past it, and so is all that the second pass reads and writes if there is more
+// than that (1.54e9 weights: 4.68 ms all through it, 4.30 so; a clip of 1.35e8 gradients 335 and 276
+// us). A smaller gradient's results stay there for whoever reads them next.
+constexpr uint64_t kKept = 12288;
 constexpr uint32_t kMostTensors = 1u << 16;
 
 struct Normed {
@@ -34,7 +40,7 @@ struct Normed {
   uint64_t count[kNormed];
   uint32_t first[kNormed];  // chunk; those from kNormed's own on
   uint8_t type[kNormed];
-  uint32_t tensors, chunks;
+  uint32_t tensors, chunks, kept;
 };
 
 struct Updated {
@@ -43,7 +49,7 @@ struct Updated {
   uint64_t count[kUpdated];
   uint32_t first[kUpdated];
   uint8_t type[kUpdated], weight_type[kUpdated];
-  uint32_t tensors, chunks;
+  uint32_t tensors, chunks, past;
 };
 
 __device__ __forceinline__ double sum_block(double v, double* s) {
@@ -55,14 +61,17 @@ __device__ __forceinline__ double sum_block(double v, double* s) {
 }
 
 // A lane's four runs of the chunk that starts at value `at` of a tensor of `count`.
-template <class T>
+template <class T, bool PAST>
 __device__ __forceinline__ void chunk_of(const void* p, uint64_t at, uint64_t count,
                                          float (&v)[kRunsOf][4]) {
   const typename T::elem* q = reinterpret_cast<const typename T::elem*>(p) + at;
   Run<T, 4> x[kRunsOf];
   if (count - at >= kChunk) {
 #pragma unroll
-    for (uint32_t i = 0; i < kRunsOf; i++) x[i] = load_any<Run<T, 4>>(q + 4 * threadIdx.x + 1024 * i);
+    for (uint32_t i = 0; i < kRunsOf; i++) {
+      const typename T::elem* const r = q + 4 * threadIdx.x + 1024 * i;
+      x[i] = PAST ? load_past<Run<T, 4>>(r) : load_any<Run<T, 4>>(r);
+    }
   } else {
     load_runs<T, 4, kRunsOf>(q, 4 * threadIdx.x, 1024, (uint32_t)(count - at), x);
   }
@@ -70,6 +79,15 @@ __device__ __forceinline__ void chunk_of(const void* p, uint64_t at, uint64_t co
   for (uint32_t i = 0; i < kRunsOf; i++)
 #pragma unroll
     for (uint32_t j = 0; j < 4; j++) v[i][j] = T::get(x[i][j]);
+}
+
+template <bool PAST>
+__device__ __forceinline__ void chunk_of(const void* p, uint32_t type, uint64_t at, uint64_t count,
+                                         float (&v)[kRunsOf][4]) {
+  if (type == POTS_OP_BF16)
+    chunk_of<Bf16, PAST>(p, at, count, v);
+  else
+    chunk_of<Fp32, PAST>(p, at, count, v);
 }
 
 __global__ __launch_bounds__(256) void norm_sums(Normed t, double* __restrict__ part) {
@@ -80,10 +98,10 @@ __global__ __launch_bounds__(256) void norm_sums(Normed t, double* __restrict__ 
     while (i + 1 < t.tensors && c >= t.first[i + 1]) i++;
     const uint64_t at = (uint64_t)(c - t.first[i]) * kChunk;
     float v[kRunsOf][4];
-    if (t.type[i] == POTS_OP_BF16)
-      chunk_of<Bf16>(t.g[i], at, t.count[i], v);
+    if (c < t.kept)
+      chunk_of<true>(t.g[i], t.type[i], at, t.count[i], v);
     else
-      chunk_of<Fp32>(t.g[i], at, t.count[i], v);
+      chunk_of<false>(t.g[i], t.type[i], at, t.count[i], v);
 #pragma unroll
     for (uint32_t r = 0; r < kRunsOf; r++)
 #pragma unroll
@@ -106,6 +124,23 @@ __global__ __launch_bounds__(256) void norm_write(const double* __restrict__ par
   if (threadIdx.x == 0) *norm = (float)n;
 }
 
+template <bool STEP, bool PAST>
+__device__ __forceinline__ void update_chunk(const Updated& t, uint32_t i, uint64_t at, float f) {
+  const uint64_t count = t.count[i];
+  float g[kRunsOf][4], w[kRunsOf][4];
+  chunk_of<PAST>(t.g[i], t.type[i], at, count, g);
+  if (STEP) chunk_of<PAST>(t.w[i], t.weight_type[i], at, count, w);
+  const uint32_t left = count - at < kChunk ? (uint32_t)(count - at) : kChunk;
+  const uint32_t type = STEP ? t.weight_type[i] : t.type[i];
+#pragma unroll
+  for (uint32_t r = 0; r < kRunsOf; r++) {
+    const uint32_t c = 4 * threadIdx.x + 1024 * r;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) g[r][j] = STEP ? fmaf(f, g[r][j], w[r][j]) : f * g[r][j];
+    put_run<4, PAST>(t.out[i], type, (int64_t)at + c, left > c ? left - c : 0, g[r]);
+  }
+}
+
 // STEP: w - eta·f·g, else f·g. The launch that writes the norm has its address.
 template <bool STEP>
 __global__ __launch_bounds__(256) void update(Updated t, const double* __restrict__ part,
@@ -121,27 +156,11 @@ __global__ __launch_bounds__(256) void update(Updated t, const double* __restric
   for (uint32_t k = 0; k <= last / gridDim.x; k++) {
     const uint32_t c = last - k * gridDim.x;
     while (c < t.first[i]) i--;
-    const uint64_t at = (uint64_t)(c - t.first[i]) * kChunk, count = t.count[i];
-    float g[kRunsOf][4], w[kRunsOf][4];
-    if (t.type[i] == POTS_OP_BF16)
-      chunk_of<Bf16>(t.g[i], at, count, g);
+    const uint64_t at = (uint64_t)(c - t.first[i]) * kChunk;
+    if (t.past)
+      update_chunk<STEP, true>(t, i, at, f);
     else
-      chunk_of<Fp32>(t.g[i], at, count, g);
-    if (STEP) {
-      if (t.weight_type[i] == POTS_OP_BF16)
-        chunk_of<Bf16>(t.w[i], at, count, w);
-      else
-        chunk_of<Fp32>(t.w[i], at, count, w);
-    }
-    const uint32_t left = count - at < kChunk ? (uint32_t)(count - at) : kChunk;
-    const uint32_t type = STEP ? t.weight_type[i] : t.type[i];
-#pragma unroll
-    for (uint32_t r = 0; r < kRunsOf; r++) {
-      const uint32_t at_r = 4 * threadIdx.x + 1024 * r;
-#pragma unroll
-      for (uint32_t j = 0; j < 4; j++) g[r][j] = STEP ? fmaf(f, g[r][j], w[r][j]) : f * g[r][j];
-      put_run<4>(t.out[i], type, (int64_t)at + at_r, left > at_r ? left - at_r : 0, g[r]);
-    }
+      update_chunk<STEP, false>(t, i, at, f);
   }
 }
 
@@ -153,19 +172,23 @@ const pots_gradient* entries(const pots_gradients* a) {
 
 uint64_t chunks_of(const pots_gradient& e) { return (e.count + kChunk - 1) / kChunk; }
 
+uint64_t chunks_of(const pots_gradients* a) {
+  uint64_t chunks = 0;
+  for (uint32_t i = 0; i < a->tensors; i++) chunks += chunks_of(entries(a)[i]);
+  return chunks;
+}
+
 bool bad(const pots_gradients* a, bool clips, bool steps) {
   if (!a || a->tensors == 0 || a->tensors > kMostTensors) return true;
   if (clips && !(a->max_norm > 0.f)) return true;
   if (steps && !isfinite(a->eta)) return true;
-  uint64_t chunks = 0;
   for (uint32_t i = 0; i < a->tensors; i++) {
     const pots_gradient& e = entries(a)[i];
     if (e.gradient_type > POTS_OP_BF16 || (steps && e.weight_type > POTS_OP_BF16) ||
         e.count > 1ull << 42)
       return true;
-    chunks += chunks_of(e);
   }
-  return chunks > 0x7fffffffu;
+  return chunks_of(a) > 0x7fffffffu;
 }
 
 // Launches over the tensors that hold something, N of them each: f(table, its first entry).
@@ -198,6 +221,7 @@ uint32_t parts_of(const pots_gradients* a) {
 
 int sums(const pots_gradients* a, double* part, uint32_t* parts, hipStream_t s) {
   *parts = 0;
+  uint64_t left = chunks_of(a);  // from the launch's first one to the list's last
   return each_launch<kNormed>(a, [&](const uint32_t* some, uint32_t n) {
     Normed t = {};
     for (uint32_t i = 0; i < n; i++) {
@@ -209,6 +233,8 @@ int sums(const pots_gradients* a, double* part, uint32_t* parts, hipStream_t s) 
       t.chunks += (uint32_t)chunks_of(e);
     }
     t.tensors = n;
+    t.kept = left > kKept ? (uint32_t)std::min<uint64_t>(left - kKept, t.chunks) : 0;
+    left -= t.chunks;
     const uint32_t blocks = blocks_of(t.chunks);
     hipLaunchKernelGGL(norm_sums, dim3(blocks), dim3(256), 0, s, t, part + *parts);
     POTS_HIP(hipGetLastError());
@@ -220,11 +246,13 @@ int sums(const pots_gradients* a, double* part, uint32_t* parts, hipStream_t s) 
 template <bool STEP>
 int updates(const pots_gradients* a, const double* part, uint32_t parts, hipStream_t s) {
   std::vector<Updated> launches;
+  const bool past = chunks_of(a) > kKept;
   (void)each_launch<kUpdated>(a, [&](const uint32_t* some, uint32_t n) {
     launches.emplace_back();
     Updated& t = launches.back();
     t.tensors = n;
     t.chunks = 0;
+    t.past = past;
     for (uint32_t i = 0; i < n; i++) {
       const pots_gradient& e = entries(a)[some[i]];
       t.g[i] = e.gradient;

@@ -24,18 +24,19 @@ namespace pots {
 constexpr uint32_t kMaxDim = 1u << 14;
 constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126, the smallest normal number
 
-// A row's W waves: each of its lanes holds G runs of four, the columns 4 (64 (W·i + wave) + lane)
-// on; W·G·256 columns.
-template <uint32_t G, uint32_t W>
+// How a row lies in a block: L lanes of a wave, or W whole waves, and G runs of four values to each
+// lane, the columns 4·(L·W·i + lane of the row) on; 4·L·W·G columns at the most.
+template <uint32_t G, uint32_t W, uint32_t L = 64>
 struct Row {
-  static constexpr uint32_t kRuns = G, kWaves = W;
-  // waves of one row to a block, or four rows to a block
+  static constexpr uint32_t kRuns = G, kWaves = W, kLanes = L, kStep = 4 * L * W;
   static constexpr uint32_t kThreads = W == 1 ? 256 : 64 * W;
-  static constexpr uint32_t kRows = kThreads / (64 * W);
+  static constexpr uint32_t kRows = kThreads / (L * W);  // of a block
+  static_assert(L == 64 || W == 1, "a row is a part of one wave or all of some");
 
   // The sum over a row, in every lane of it; s: W floats of LDS, used in turn by two calls.
   static __device__ __forceinline__ float sum(float v, float (*s)[W], uint32_t& turn) {
-    v = sum_wave(v);
+#pragma unroll
+    for (int m = L / 2; m; m >>= 1) v += __shfl_xor(v, m);
     if constexpr (W > 1) {
       if (threadIdx.x % 64 == 0) s[turn][threadIdx.x / 64] = v;
       __syncthreads();
@@ -48,7 +49,7 @@ struct Row {
   }
   static __device__ __forceinline__ uint32_t most(uint32_t v, uint32_t (*s)[W], uint32_t& turn) {
 #pragma unroll
-    for (int m = 32; m; m >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, m));
+    for (int m = L / 2; m; m >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, m));
     if constexpr (W > 1) {
       if (threadIdx.x % 64 == 0) s[turn][threadIdx.x / 64] = v;
       __syncthreads();
@@ -65,30 +66,29 @@ __device__ __forceinline__ uint32_t left_of(uint32_t c, uint32_t dim) { return c
 
 template <class X, class T, bool RES, bool Q, class R>
 __global__ __launch_bounds__(R::kThreads) void norm_rows(pots_rms_norm a) {
-  constexpr uint32_t G = R::kRuns, W = R::kWaves;
+  constexpr uint32_t G = R::kRuns, W = R::kWaves, L = R::kLanes, S = R::kStep;
   __shared__ float s_sum[2][W];
   __shared__ uint32_t s_most[2][W];
   uint32_t turn = 0, turn_most = 0;
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const uint32_t first = 4 * ((W == 1 ? 0 : wave * 64) + lane);
+  const uint32_t lane = threadIdx.x % (L * W), own = threadIdx.x / (L * W), first = 4 * lane;
   const float over = 1.f / (float)a.dim;
   AnyRuns<G> gain;
-  gain.load(a.weight, a.weight_type, first, 256 * W, a.dim);
+  gain.load(a.weight, a.weight_type, first, S, a.dim);
   const uint32_t step = gridDim.x * R::kRows;
-  for (uint64_t row = blockIdx.x * R::kRows + (W == 1 ? wave : 0); row < a.rows; row += step) {
+  for (uint64_t row = blockIdx.x * R::kRows + own; row < a.rows; row += step) {
     float t[G][4];
     Run<X, 4> x[G];
     Run<T, 4> r[G];
     load_runs<X, 4, G>(reinterpret_cast<const typename X::elem*>(a.x) + (int64_t)row * a.x_row, first,
-                       256 * W, a.dim, x);
+                       S, a.dim, x);
     if (RES)
       load_runs<T, 4, G>(
           reinterpret_cast<const typename T::elem*>(a.residual) + (int64_t)row * a.residual_row, first,
-          256 * W, a.dim, r);
+          S, a.dim, r);
     float sum = 0.f;
 #pragma unroll
     for (uint32_t i = 0; i < G; i++) {
-      const uint32_t c = first + 256 * W * i;
+      const uint32_t c = first + S * i;
 #pragma unroll
       for (uint32_t j = 0; j < 4; j++) {
         t[i][j] = X::get(x[i][j]);
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(R::kThreads) void norm_rows(pots_rms_norm a) {
                         left_of(c, a.dim), t[i]);
     }
     const float s = 1.f / sqrtf(R::sum(sum, s_sum, turn) * over + a.eps);
-    if (!Q && lane == 0 && (W == 1 || wave == 0)) gstore<float>(a.rstd + row, s);
+    if (!Q && lane == 0) gstore<float>(a.rstd + row, s);
     uint32_t most = 0;  // sizes as bits, whose order puts NaN above infinity
 #pragma unroll
     for (uint32_t i = 0; i < G; i++) {
@@ -115,17 +115,17 @@ __global__ __launch_bounds__(R::kThreads) void norm_rows(pots_rms_norm a) {
     if constexpr (!Q) {
 #pragma unroll
       for (uint32_t i = 0; i < G; i++) {
-        const uint32_t c = first + 256 * W * i;
+        const uint32_t c = first + S * i;
         put_run<4>(a.y, a.y_type, (int64_t)(row * a.dim) + c, left_of(c, a.dim), t[i]);
       }
     } else {
       const float top = a.y_type == POTS_OP_E4M3 ? 448.f : 127.f;
-      const uint32_t lanes = a.block / 4;  // of a group; 0: the row
+      const uint32_t lanes = min(a.block / 4, L);  // of a group
       const uint32_t groups = a.block ? (a.dim + a.block - 1) / a.block : 1;
       if (!a.block) most = R::most(most, s_most, turn_most);
 #pragma unroll
       for (uint32_t i = 0; i < G; i++) {
-        const uint32_t c = first + 256 * W * i, left = left_of(c, a.dim);
+        const uint32_t c = first + S * i, left = left_of(c, a.dim);
         if (a.block) {
           most = 0;
 #pragma unroll
@@ -169,30 +169,29 @@ __global__ __launch_bounds__(R::kThreads) void norm_rows(pots_rms_norm a) {
 // part: [block][dim] sums of dy·h, where a.dweight is there.
 template <class Y, class T, class R>
 __global__ __launch_bounds__(R::kThreads) void norm_grad(pots_rms_norm a, float* __restrict__ part) {
-  constexpr uint32_t G = R::kRuns, W = R::kWaves;
+  constexpr uint32_t G = R::kRuns, W = R::kWaves, L = R::kLanes, S = R::kStep;
   __shared__ float s_sum[2][W];
-  __shared__ float s_dw[W == 1 ? 4 * 256 * G : 1];
+  __shared__ float s_dw[W == 1 ? R::kRows * S * G : 1];
   uint32_t turn = 0;
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const uint32_t first = 4 * ((W == 1 ? 0 : wave * 64) + lane);
+  const uint32_t lane = threadIdx.x % (L * W), own = threadIdx.x / (L * W), first = 4 * lane;
   const float over = 1.f / (float)a.dim;
   float dw[G][4] = {};
   AnyRuns<G> gain;
-  gain.load(a.weight, a.weight_type, first, 256 * W, a.dim);
+  gain.load(a.weight, a.weight_type, first, S, a.dim);
   const uint32_t step = gridDim.x * R::kRows;
-  for (uint64_t row = blockIdx.x * R::kRows + (W == 1 ? wave : 0); row < a.rows; row += step) {
+  for (uint64_t row = blockIdx.x * R::kRows + own; row < a.rows; row += step) {
     Run<Y, 4> y[G];
     Run<T, 4> r[G], d[G];
     const typename T::elem* const dt =
         reinterpret_cast<const typename T::elem*>(a.dtotal) + (int64_t)row * a.dtotal_row;
     const float s = gload<float>(a.rstd + row);
     load_runs<Y, 4, G>(reinterpret_cast<const typename Y::elem*>(a.dy) + (int64_t)row * a.dy_row, first,
-                       256 * W, a.dim, y);
+                       S, a.dim, y);
     load_runs<T, 4, G>(
         reinterpret_cast<const typename T::elem*>(a.total) + (int64_t)row * a.total_row, first,
-        256 * W, a.dim, r);
+        S, a.dim, r);
     // (sixteen waves have no registers for it before the sum)
-    if (W < 16 && a.dtotal) load_runs<T, 4, G>(dt, first, 256 * W, a.dim, d);
+    if (W < 16 && a.dtotal) load_runs<T, 4, G>(dt, first, S, a.dim, d);
     float sum = 0.f;
 #pragma unroll
     for (uint32_t i = 0; i < G; i++) {
@@ -206,10 +205,10 @@ __global__ __launch_bounds__(R::kThreads) void norm_grad(pots_rms_norm a, float*
       }
     }
     const float mean = R::sum(sum, s_sum, turn) * over;
-    if (W == 16 && a.dtotal) load_runs<T, 4, G>(dt, first, 256 * W, a.dim, d);
+    if (W == 16 && a.dtotal) load_runs<T, 4, G>(dt, first, S, a.dim, d);
 #pragma unroll
     for (uint32_t i = 0; i < G; i++) {
-      const uint32_t c = first + 256 * W * i, left = left_of(c, a.dim);
+      const uint32_t c = first + S * i, left = left_of(c, a.dim);
       const int64_t at = (int64_t)(row * a.dim) + c;
       float v[4], w[4];
       gain.get(a.weight_type, i, w);
@@ -225,20 +224,24 @@ __global__ __launch_bounds__(R::kThreads) void norm_grad(pots_rms_norm a, float*
     }
   }
   if (!a.dweight) return;
-  float* const own = part + (uint64_t)blockIdx.x * a.dim;
-  if constexpr (W == 1) {
+  float* const sums = part + (uint64_t)blockIdx.x * a.dim;
+  if constexpr (W == 1) {  // (each of the block's rows has had sums of its own)
 #pragma unroll
     for (uint32_t i = 0; i < G; i++)
 #pragma unroll
-      for (uint32_t j = 0; j < 4; j++) s_dw[wave * 256 * G + 256 * i + 4 * lane + j] = dw[i][j];
+      for (uint32_t j = 0; j < 4; j++) s_dw[own * S * G + S * i + first + j] = dw[i][j];
     __syncthreads();
-    for (uint32_t c = threadIdx.x; c < a.dim; c += 256)
-      own[c] = s_dw[c] + s_dw[c + 256 * G] + s_dw[c + 512 * G] + s_dw[c + 768 * G];
+    for (uint32_t c = threadIdx.x; c < a.dim; c += 256) {
+      float v = 0.f;
+#pragma unroll
+      for (uint32_t r = 0; r < R::kRows; r++) v += s_dw[r * S * G + c];
+      sums[c] = v;
+    }
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < G; i++) {
-      const uint32_t c = first + 256 * W * i;
-      put_run<4>(own, POTS_OP_F32, c, left_of(c, a.dim), dw[i]);
+      const uint32_t c = first + S * i;
+      put_run<4>(sums, POTS_OP_F32, c, left_of(c, a.dim), dw[i]);
     }
   }
 }
@@ -279,17 +282,22 @@ bool bad(const pots_rms_norm* a) {
          a->weight_type > POTS_OP_BF16 || !(a->eps > 0.f) || !isfinite(a->eps);
 }
 
-// Rows of up to 2048 columns are a wave's: the sum over a row then needs no barrier. Wider ones are
-// shared by four or sixteen waves, so that a lane holds 32 values at most.
+// Rows of up to 1024 columns are a wave's or a part of one: the sum over a row then needs no barrier.
+// Wider ones are shared by four to sixteen waves, so that a lane holds 16 values at most: in a wave of
+// its own a row of 2048 leaves room for few waves, and forward and backward of 6144 such rows took 84 us
+// where four waves to a row take 71. (8192 columns: 80 us with eight waves, 90 with four. 65536 rows of
+// 64: 85 us in a wave each, 32 in a quarter of one.)
 template <class F>
 int by_width(uint32_t dim, F&& f) {
+  if (dim <= 64) return f(Row<1, 1, 16>{});
+  if (dim <= 128) return f(Row<1, 1, 32>{});
   if (dim <= 256) return f(Row<1, 1>{});
   if (dim <= 512) return f(Row<2, 1>{});
+  if (dim <= 768) return f(Row<3, 1>{});
   if (dim <= 1024) return f(Row<4, 1>{});
-  if (dim <= 1536) return f(Row<6, 1>{});
-  if (dim <= 2048) return f(Row<8, 1>{});
+  if (dim <= 2048) return f(Row<2, 4>{});
   if (dim <= 4096) return f(Row<4, 4>{});
-  if (dim <= 8192) return f(Row<8, 4>{});
+  if (dim <= 8192) return f(Row<4, 8>{});
   return f(Row<4, 16>{});
 }
 
@@ -303,7 +311,7 @@ int forward(const pots_rms_norm* a, hipStream_t s) {
   return by_width(a->dim, [&](auto r) {
     typedef decltype(r) R;
     const uint32_t want = (uint32_t)(((uint64_t)a->rows + R::kRows - 1) / R::kRows);
-    const uint32_t nb = want < 8192 ? want : 8192;
+    const uint32_t nb = want < 4096 ? want : 4096;
     return by_type(a->x_type, [&](auto x) {
       return by_type(a->total_type, [&](auto t) {
         typedef decltype(x) X;
@@ -320,12 +328,20 @@ int forward(const pots_rms_norm* a, hipStream_t s) {
   });
 }
 
-// Blocks of the gradient's kernel: two to a compute unit, whose sums of dw are the bytes that
-// norm_join reads.
+// Blocks of the gradient's kernel. Each leaves a row of sums of dw for norm_join, so they are few, two to a
+// compute unit; more where a lane has few runs on their way (49152 rows of 256 columns, both
+// directions: 92 us with 512 blocks, 69 with 1536, 77 with 4096; 8192 rows of 1536: 71 with 1024, 78
+// with 2048).
 template <class R>
 uint32_t grad_blocks(const pots_rms_norm* a) {
+  constexpr uint32_t most = R::kWaves == 1 ? (R::kRuns == 1   ? 1536
+                                              : R::kRuns == 2 ? 1024
+                                              : R::kRuns == 3 ? 768
+                                                              : 512)
+                            : R::kRuns == 2  ? 1024
+                                             : 512;
   const uint64_t want = ((uint64_t)a->rows + R::kRows - 1) / R::kRows;
-  return (uint32_t)(want < 512 ? want : 512);
+  return (uint32_t)(want < most ? want : most);
 }
 
 bool bad_back(const pots_rms_norm* a) { return bad(a) || a->y_type > POTS_OP_BF16; }

@@ -19,7 +19,7 @@ namespace pots {
 
 constexpr uint32_t kMaxWidth = 1024, kMaxHeads = 1u << 16;
 constexpr uint32_t kAngles = 1024, kTokens = 64;  // of a block, at the most
-constexpr uint32_t kAhead = 4;  // runs that a lane has on their way
+constexpr uint32_t kAhead = 2;  // runs that a lane has on their way
 
 template <class T>
 constexpr uint32_t kPairs = 16 / sizeof(typename T::elem);  // pairs that a lane turns at a time
@@ -94,21 +94,56 @@ __global__ __launch_bounds__(256) void rotary_turn(pots_rotary a, uint32_t token
   typedef typename T::elem elem;
   constexpr uint32_t P = kPairs<T>;
   __shared__ Turn s_turn[kAngles];
-  __shared__ int64_t s_at[4][kTokens];  // where the block's tokens lie in q, k and the outputs
   const uint64_t all = (uint64_t)a.batch * a.n, t0 = from + (uint64_t)blockIdx.x * tokens;
   const uint32_t here = (uint32_t)(all - t0 < tokens ? all - t0 : tokens);
-  const uint32_t heads = a.heads + a.kv_heads;
-  for (uint32_t t = threadIdx.x; t < here; t += 256) {
-    const uint32_t b = (uint32_t)((t0 + t) / a.n), n = (uint32_t)(t0 + t - (uint64_t)b * a.n);
-    s_at[0][t] = b * a.q.batch + n * a.q.row;
-    s_at[1][t] = b * a.k.batch + n * a.k.row;
-    s_at[2][t] = b * a.q_out.batch + n * a.q_out.row;
-    s_at[3][t] = b * a.k_out.batch + n * a.k_out.row;
-  }
+  const uint32_t heads = a.heads + a.kv_heads, items = here * heads;
+  const uint32_t b0 = (uint32_t)(t0 / a.n), n0 = (uint32_t)(t0 - (uint64_t)b0 * a.n);
+  // The block's token t: its sequence and its place there. (One division less where all are of one.)
+  auto token = [&](uint32_t t, uint32_t& b, uint32_t& n) {
+    b = b0, n = n0 + t;
+    if (n >= a.n) {
+      b += n / a.n;
+      n %= a.n;
+    }
+  };
+  auto place = [&](uint32_t item, uint32_t& t, const elem*& in, elem*& out) {
+    t = item / heads;
+    uint32_t h = item - t * heads, b, n;
+    token(t, b, n);
+    const bool key = h >= a.heads;
+    if (key) h -= a.heads;
+    const pots_heads& i = key ? a.k : a.q;
+    const pots_heads& o = key ? a.k_out : a.q_out;
+    in = reinterpret_cast<const elem*>(i.ptr) + b * i.batch + n * i.row + h * i.head;
+    out = reinterpret_cast<elem*>(o.ptr) + b * o.batch + n * o.row + h * o.head;
+  };
+  // A head's runs: those of its pairs, then those of the columns that are copied.
+  const uint32_t turned = a.pairs < P ? 1 : (a.pairs + P - 1) / P;
+  const uint32_t rest = a.head_dim - 2 * a.pairs;
+  const uint32_t runs = turned + (rest < 2 * P ? rest != 0 : (rest + 2 * P - 1) / (2 * P));
+  const uint32_t slots = 256 / runs, slot = threadIdx.x / runs, run = threadIdx.x - slot * runs;
+  const bool turns = run < turned, whole = turns ? a.pairs >= P : rest >= 2 * P;
+  const uint32_t i0 = min(run * P, a.pairs - P);
+  const uint32_t at = !turns ? 2 * a.pairs + min((run - turned) * 2 * P, rest - 2 * P)
+                      : ADJACENT ? 2 * i0 : i0;
+  const uint32_t apart = turns && !ADJACENT ? a.pairs : P;
+  const uint32_t first = slot < slots ? slot : items;  // (lanes past the last slot have no item)
+  Piece<T, ADJACENT> x[kAhead];
+  elem* out[kAhead];
+  uint32_t t[kAhead];
+  auto load = [&](uint32_t item) {
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; j++) {
+      const elem* in;  // (past the last item: that one again, and nothing is stored)
+      place(min(item + j * slots, items - 1), t[j], in, out[j]);
+      x[j].load(in, at, apart);
+    }
+  };
+  if (whole && first < items) load(first);  // on their way while the angles are taken
   for (uint32_t e = threadIdx.x; e < here * a.pairs; e += 256) {
     const uint32_t t = e / a.pairs, i = e - t * a.pairs;
-    const uint32_t b = (uint32_t)((t0 + t) / a.n), n = (uint32_t)(t0 + t - (uint64_t)b * a.n);
-    uint32_t axis = 0;
+    uint32_t b, n, axis = 0;
+    token(t, b, n);
     for (uint32_t x = 0; x + 1 < a.axes; x++) axis += i >= a.ends[x];
     const int64_t at = axis * a.position_axis + b * a.position_batch + n * a.position_token;
     const double position =
@@ -121,41 +156,9 @@ __global__ __launch_bounds__(256) void rotary_turn(pots_rotary a, uint32_t token
     s_turn[e] = turn_of(position, f, a.inverse);
   }
   __syncthreads();
-  // A head's runs: those of its pairs, then those of the columns that are copied.
-  const uint32_t turned = a.pairs < P ? 1 : (a.pairs + P - 1) / P;
-  const uint32_t rest = a.head_dim - 2 * a.pairs;
-  const uint32_t runs = turned + (rest < 2 * P ? rest != 0 : (rest + 2 * P - 1) / (2 * P));
-  const uint32_t slots = 256 / runs, slot = threadIdx.x / runs, run = threadIdx.x - slot * runs;
-  if (slot >= slots) return;
-  const bool turns = run < turned, whole = turns ? a.pairs >= P : rest >= 2 * P;
-  const uint32_t i0 = min(run * P, a.pairs - P);
-  const uint32_t at = !turns ? 2 * a.pairs + min((run - turned) * 2 * P, rest - 2 * P)
-                      : ADJACENT ? 2 * i0 : i0;
-  const uint32_t apart = turns && !ADJACENT ? a.pairs : P;
-  const uint32_t items = here * heads;
-  auto place = [&](uint32_t item, uint32_t& t, const elem*& in, elem*& out) {
-    t = item / heads;
-    const uint32_t h = item - t * heads;
-    if (h < a.heads) {
-      in = reinterpret_cast<const elem*>(a.q.ptr) + s_at[0][t] + h * a.q.head;
-      out = reinterpret_cast<elem*>(a.q_out.ptr) + s_at[2][t] + h * a.q_out.head;
-    } else {
-      const uint32_t g = h - a.heads;
-      in = reinterpret_cast<const elem*>(a.k.ptr) + s_at[1][t] + g * a.k.head;
-      out = reinterpret_cast<elem*>(a.k_out.ptr) + s_at[3][t] + g * a.k_out.head;
-    }
-  };
   if (whole) {
-    for (uint32_t item = slot; item < items; item += kAhead * slots) {
-      Piece<T, ADJACENT> x[kAhead];
-      elem* out[kAhead];
-      uint32_t t[kAhead];
-#pragma unroll
-      for (uint32_t j = 0; j < kAhead; j++) {
-        const elem* in;  // (past the last item: that one again, and nothing is stored)
-        place(min(item + j * slots, items - 1), t[j], in, out[j]);
-        x[j].load(in, at, apart);
-      }
+    for (uint32_t item = first; item < items; item += kAhead * slots) {
+      if (item != first) load(item);
 #pragma unroll
       for (uint32_t j = 0; j < kAhead; j++) {
         if (turns) x[j].turn(s_turn + t[j] * a.pairs + i0);
@@ -163,7 +166,7 @@ __global__ __launch_bounds__(256) void rotary_turn(pots_rotary a, uint32_t token
       }
     }
   } else {
-    for (uint32_t item = slot; item < items; item += slots) {
+    for (uint32_t item = first; item < items; item += slots) {
       uint32_t t;
       const elem* in;
       elem* out;
@@ -194,9 +197,10 @@ bool bad(const pots_rotary* a) {
 
 template <class T>
 int turn(const pots_rotary* a, hipStream_t s) {
-  // Tokens of a block: few enough for four blocks to a compute unit, as many as their angles allow.
+  // Tokens of a block: few enough for eight blocks to a compute unit (8192 tokens of 14 heads of 128: 15.3
+  // us, with four 16.4, with sixteen 17), as many as their angles allow.
   const uint64_t all = (uint64_t)a->batch * a->n;
-  uint64_t tokens = all / 1024;
+  uint64_t tokens = all / 2048;
   const uint32_t most = kAngles / a->pairs < kTokens ? kAngles / a->pairs : kTokens;
   tokens = tokens < 1 ? 1 : tokens > most ? most : tokens;
   const auto kernel = a->adjacent ? rotary_turn<T, true> : rotary_turn<T, false>;

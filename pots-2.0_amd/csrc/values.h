@@ -30,6 +30,16 @@ __device__ __forceinline__ void store_any(E* p, V v) {
   ((POTS_GLOBAL Loose<V, E>*)p)->v = v;
 }
 
+// The same past the caches: for what nobody reads soon, or again.
+template <class V, class E>
+__device__ __forceinline__ V load_past(const E* p) {
+  return __builtin_nontemporal_load(&((const POTS_GLOBAL Loose<V, E>*)p)->v);
+}
+template <class V, class E>
+__device__ __forceinline__ void store_past(E* p, V v) {
+  __builtin_nontemporal_store(v, &((POTS_GLOBAL Loose<V, E>*)p)->v);
+}
+
 // A run's values from the one numbered `by` (0 to N - 1) on, zeros behind them.
 template <class T, uint32_t N>
 __device__ __forceinline__ Run<T, N> shifted(Run<T, N> x, uint32_t by) {
@@ -47,14 +57,16 @@ __device__ __forceinline__ Run<T, N> shifted(Run<T, N> x, uint32_t by) {
 // run that crosses the end is read as the row's last N values and shifted, so that all loads are on
 // their way before the first is waited for. (dim is the same for all lanes, and one of the three ways
 // is taken.)
-template <class T, uint32_t N, uint32_t G>
+template <class T, uint32_t N, uint32_t G, bool PAST = false>
 __device__ __forceinline__ void load_runs(const typename T::elem* row, uint32_t first, uint32_t step,
                                           uint32_t dim, Run<T, N> (&x)[G]) {
   if (dim % N == 0) {
 #pragma unroll
     for (uint32_t i = 0; i < G; i++) {
       x[i] = Run<T, N>{};
-      if (first + i * step < dim) x[i] = load_any<Run<T, N>>(row + first + i * step);
+      if (first + i * step < dim)
+        x[i] = PAST ? load_past<Run<T, N>>(row + first + i * step)
+                    : load_any<Run<T, N>>(row + first + i * step);
     }
   } else if (dim > N) {
 #pragma unroll
@@ -79,14 +91,17 @@ __device__ __forceinline__ void load_runs(const typename T::elem* row, uint32_t 
 }
 
 // N values from p on, of which the row has `left`.
-template <class T, uint32_t N>
+template <class T, uint32_t N, bool PAST = false>
 __device__ __forceinline__ void store_run(typename T::elem* p, uint32_t left,
                                           const float (&v)[N]) {
   if (left >= N) {
     Run<T, N> x;
 #pragma unroll
     for (uint32_t j = 0; j < N; j++) x[j] = T::put(v[j]);
-    store_any(p, x);
+    if (PAST)
+      store_past(p, x);
+    else
+      store_any(p, x);
   } else {
 #pragma unroll
     for (uint32_t j = 0; j + 1 < N; j++)
@@ -95,13 +110,13 @@ __device__ __forceinline__ void store_run(typename T::elem* p, uint32_t left,
 }
 
 // The same for a type that is the call's.
-template <uint32_t N>
+template <uint32_t N, bool PAST = false>
 __device__ __forceinline__ void put_run(void* p, uint32_t type, int64_t at, uint32_t left,
                                         const float (&v)[N]) {
   if (type == POTS_OP_BF16)
-    store_run<Bf16, N>(reinterpret_cast<uint16_t*>(p) + at, left, v);
+    store_run<Bf16, N, PAST>(reinterpret_cast<uint16_t*>(p) + at, left, v);
   else
-    store_run<Fp32, N>(reinterpret_cast<float*>(p) + at, left, v);
+    store_run<Fp32, N, PAST>(reinterpret_cast<float*>(p) + at, left, v);
 }
 
 // Runs of four whose type is the call's: held as they lie in memory, made fp32 where they are used.
@@ -136,11 +151,5 @@ struct AnyRuns {
     v[3] = halves ? __uint_as_float(hi & 0xffff0000u) : x[3];
   }
 };
-
-__device__ __forceinline__ float sum_wave(float v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-  return v;
-}
 
 }  // namespace pots

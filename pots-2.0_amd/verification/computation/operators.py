@@ -33,7 +33,9 @@ function.
 
 from __future__ import annotations
 
+import itertools
 import math
+import operator
 import struct
 from collections.abc import Sequence
 
@@ -447,10 +449,23 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0) -> 
 
 # ---- the norm -------------------------------------------------------------------------------
 
-def _as_rows(t: torch.Tensor) -> torch.Tensor:
-    """``[..., d]`` as rows of consecutive values, wherever they start."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``[..., d]`` as rows of consecutive values, and how far apart they start."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _new(shape: Sequence[int], dtype: torch.dtype, *near: torch.Tensor | None) -> torch.Tensor:
+    """An uninitialised tensor on the device of ``near``, of which one of the type makes it."""
+    for t in near:
+        if t is not None and t.dtype == dtype:  # (half the host time of torch.empty)
+            return t.new_empty(shape)
+    return torch.empty(shape, dtype=dtype, device=near[0].device)
 
 
 def _norm_args(x: torch.Tensor, weight: torch.Tensor, eps: float, what: str) -> int:
@@ -477,16 +492,18 @@ def _run_norm(name: str, x: torch.Tensor, weight: torch.Tensor, residual: torch.
               y: torch.Tensor, y_type: int, rstd: torch.Tensor | None,
               scales: torch.Tensor | None, block: int, eps: float) -> torch.Tensor:
     """The forward calls; the sum that was normed."""
-    _on_gpu(x)
-    total = x if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    rows, own = _as_rows(x), weight.contiguous()
-    other = None if residual is None else _as_rows(residual)
-    args = _packed(_NORM, rows.data_ptr(), 0 if other is None else other.data_ptr(), own.data_ptr(),
-                   0 if other is None else total.data_ptr(), y.data_ptr(),
+    total, to, other, other_ptr, other_row = x, 0, None, 0, 0
+    if residual is not None:
+        total = residual.new_empty(x.shape)
+        other, other_row = _rows(residual)
+        to, other_ptr = total.data_ptr(), other.data_ptr()
+    rows, row = _rows(x)
+    own, dim = weight.contiguous(), x.shape[-1]
+    args = _packed(_NORM, rows.data_ptr(), other_ptr, own.data_ptr(), to, y.data_ptr(),
                    0 if rstd is None else rstd.data_ptr(),
-                   0 if scales is None else scales.data_ptr(), 0, 0, 0, 0, 0, rows.stride(0),
-                   0 if other is None else other.stride(0), 0, 0, 0, rows.shape[0], rows.shape[1],
-                   block, _DTYPES[x.dtype], _DTYPES[total.dtype], _DTYPES[weight.dtype], y_type, eps)
+                   0 if scales is None else scales.data_ptr(), 0, 0, 0, 0, 0, row, other_row, 0, 0, 0,
+                   x.numel() // dim, dim, block, _DTYPES[x.dtype], _DTYPES[total.dtype],
+                   _DTYPES[weight.dtype], y_type, eps)
     native.get().operator(name, args, x.device)
     return total
 
@@ -504,8 +521,9 @@ def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in _DTYPES:
         raise ValueError(f"out_dtype must be float32 or bfloat16, not {out_dtype}")
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _on_gpu(x)
+    y = _new(x.shape, out_dtype, x, residual)
+    rstd = _new(x.shape[:-1], torch.float32, weight, residual)
     total = _run_norm("rms_norm_forward", x, weight, residual, y, _DTYPES[out_dtype], rstd, None, 0,
                       eps)
     return y, total, rstd
@@ -527,8 +545,9 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e
     if block not in (None, 32, 64, 128, 256):
         raise ValueError(f"block must be 32, 64, 128 or 256, or None for a row, not {block}")
     blocks = 1 if block is None else -(-x.shape[-1] // block)
+    _on_gpu(x)
     q = torch.empty(x.shape, dtype=dtype, device=x.device)
-    scales = torch.empty(*x.shape[:-1], blocks, dtype=torch.float32, device=x.device)
+    scales = _new((*x.shape[:-1], blocks), torch.float32, weight, residual)
     total = _run_norm("rms_norm_quantized", x, weight, residual, q, _EIGHT_BITS[dtype], None,
                       scales, block or 0, eps)
     return q, scales, total
@@ -555,18 +574,19 @@ def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, weight: torch.Tenso
     if x_dtype not in _DTYPES:
         raise ValueError(f"x_dtype must be float32 or bfloat16, not {x_dtype}")
     _on_gpu(total)
-    dresidual = torch.empty(total.shape, dtype=total.dtype, device=total.device)
-    dx = dresidual
+    dresidual = dx = total.new_empty(total.shape)
     if x_dtype != total.dtype:
-        dx = torch.empty(total.shape, dtype=x_dtype, device=total.device)
-    dweight = torch.empty(weight.shape, dtype=weight.dtype, device=total.device)
-    g, t, own = _as_rows(dy), _as_rows(total), weight.contiguous()
-    other = None if dtotal is None else _as_rows(dtotal)
+        dx = _new(total.shape, x_dtype, dy, weight)
+    dweight = weight.new_empty(weight.shape)
+    (g, g_row), (t, t_row), own = _rows(dy), _rows(total), weight.contiguous()
+    other, other_ptr, other_row = None, 0, 0
+    if dtotal is not None:
+        other, other_row = _rows(dtotal)
+        other_ptr = other.data_ptr()
+    dim = total.shape[-1]
     args = _packed(_NORM, 0, 0, own.data_ptr(), t.data_ptr(), 0, rstd.data_ptr(), 0, g.data_ptr(),
-                   0 if other is None else other.data_ptr(),
-                   0 if dx is dresidual else dx.data_ptr(), dresidual.data_ptr(),
-                   dweight.data_ptr(), 0, 0, t.stride(0), g.stride(0),
-                   0 if other is None else other.stride(0), t.shape[0], t.shape[1], 0,
+                   other_ptr, 0 if dx is dresidual else dx.data_ptr(), dresidual.data_ptr(),
+                   dweight.data_ptr(), 0, 0, t_row, g_row, other_row, total.numel() // dim, dim, 0,
                    _DTYPES[x_dtype], _DTYPES[total.dtype], code, dy_type, 1.0)
     native.get().operator("rms_norm_backward", args, total.device)
     return dx, dresidual, dweight
@@ -634,23 +654,27 @@ def _turned(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     counts = (pairs,) if sections is None else tuple(sections)
     if not 1 <= len(counts) <= 4 or min(counts) < 0 or sum(counts) != pairs:
         raise ValueError(f"sections must be up to 4 counts whose sum is {pairs}, got {counts}")
-    axes = len(counts)
-    at = positions[None] if sections is None else positions
+    axes, at = len(counts), positions
     if at.dtype not in (torch.int64, torch.int32) or at.device != q.device:
         raise ValueError(f"positions must be int64 or int32 on {q.device}")
-    if at.dim() == 2:
-        at = at[:, None]
-    if at.dim() != 3 or at.shape[0] != axes or at.shape[1] not in (1, b) or at.shape[2] != n:
+    # (strides as they are: views of small tensors cost more than the launch)
+    shape, strides = at.shape, at.stride()
+    if sections is None:
+        shape, strides = (1, *shape), (0, *strides)
+    if len(shape) == 2:
+        shape, strides = (shape[0], 1, shape[1]), (strides[0], 0, strides[1])
+    if len(shape) != 3 or shape[0] != axes or shape[1] not in (1, b) or shape[2] != n:
         raise ValueError(f"positions must be {'' if sections is None else f'{axes} times '}"
                          f"[{n}] or [{b}, {n}], got {tuple(positions.shape)}")
+    if shape[1] == 1:
+        strides = (strides[0], 0, strides[2])
     _on_gpu(q)
-    at = at.expand(axes, b, n)
-    q, k = (t if d == 1 or t.stride(3) == 1 else t.contiguous() for t in (q, k))
+    q, k = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k))
     frequencies = frequencies.contiguous()
     to_q, to_k = _new_heads(b, h, n, d, q), _new_heads(b, kv, n, d, q)
-    ends = [sum(counts[:i + 1]) for i in range(axes)] + [pairs] * (4 - axes)
+    ends = list(itertools.accumulate(counts)) + [pairs] * (4 - axes)
     args = _packed(_ROTARY, *_places(q), *_places(k), *_places(to_q), *_places(to_k),
-                   at.data_ptr(), frequencies.data_ptr(), *at.stride(), b, h, kv, n, d, pairs, axes,
+                   at.data_ptr(), frequencies.data_ptr(), *strides, b, h, kv, n, d, pairs, axes,
                    *ends, code, 0 if frequencies.dtype == torch.float32 else _F64,
                    64 if at.dtype == torch.int64 else 32, adjacent, inverse)
     native.get().operator("rotary_turn", args, q.device)
@@ -717,11 +741,11 @@ def gated_silu_forward(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     shape and type, each anywhere (the halves of one product, for instance)."""
     code = _gated_args(gate, up)
     _on_gpu(gate)
-    out = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    out = gate.new_empty(gate.shape)
     if out.numel():
-        g, u = _as_rows(gate), _as_rows(up)
-        args = _packed(_GATED, g.data_ptr(), u.data_ptr(), 0, out.data_ptr(), 0, 0, g.stride(0),
-                       u.stride(0), 0, *g.shape, code)
+        (g, g_row), (u, u_row), columns = _rows(gate), _rows(up), gate.shape[-1]
+        args = _packed(_GATED, g.data_ptr(), u.data_ptr(), 0, out.data_ptr(), 0, 0, g_row, u_row, 0,
+                       out.numel() // columns, columns, code)
         native.get().operator("gated_silu_forward", args, gate.device)
     return out
 
@@ -732,12 +756,12 @@ def gated_silu_backward(dout: torch.Tensor, gate: torch.Tensor, up: torch.Tensor
     code = _gated_args(gate, up)
     _like(dout, gate, gate.shape, "dout")
     _on_gpu(gate)
-    dgate = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
-    dup = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    dgate, dup = gate.new_empty(gate.shape), gate.new_empty(gate.shape)
     if dgate.numel():
-        g, u, d = _as_rows(gate), _as_rows(up), _as_rows(dout)
+        (g, g_row), (u, u_row), (d, d_row) = _rows(gate), _rows(up), _rows(dout)
+        columns = gate.shape[-1]
         args = _packed(_GATED, g.data_ptr(), u.data_ptr(), d.data_ptr(), 0, dgate.data_ptr(),
-                       dup.data_ptr(), g.stride(0), u.stride(0), d.stride(0), *g.shape, code)
+                       dup.data_ptr(), g_row, u_row, d_row, dgate.numel() // columns, columns, code)
         native.get().operator("gated_silu_backward", args, gate.device)
     return dgate, dup
 
@@ -761,51 +785,75 @@ def gated_silu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 # ---- the whole gradient ---------------------------------------------------------------------
 
-def _tensors(of: Sequence[torch.Tensor], what: str, device: torch.device | None = None
-             ) -> tuple[list[torch.Tensor], list[int], torch.device]:
-    """A list of tensors of one device, and their types."""
-    of = list(of)
-    if not of or not all([isinstance(t, torch.Tensor) for t in of]):
-        raise ValueError(f"{what} must be tensors, at least one")
-    device = of[0].device if device is None else device
-    if any([t.device != device for t in of]):
-        raise ValueError(f"{what} must be on {device}")
-    codes = [_DTYPES.get(t.dtype) if t.layout is torch.strided else None for t in of]
-    if None in codes:
-        raise ValueError(f"{what} must be dense, float32 or bfloat16")
-    return of, codes, device
+# what a list's checks read of every tensor, as functions that map() calls without a frame
+_TYPE_OF, _SHAPE_OF = operator.attrgetter("dtype"), operator.attrgetter("shape")
+_DEVICE_OF, _POINTER, _COUNT = torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.numel
+_CONTIGUOUS = torch.Tensor.is_contiguous
 
 
-def _written(of: Sequence[torch.Tensor], like: list[torch.Tensor], what: str
-             ) -> list[torch.Tensor]:
-    of = list(of)
-    if ([t.shape for t in of] != [t.shape for t in like]
-            or [t.dtype for t in of] != [t.dtype for t in like]
-            or any([t.device != u.device for t, u in zip(of, like)])):
-        raise ValueError(f"{what} must have the shapes, types and device of what goes there")
-    if not all([t.is_contiguous() for t in of]):
-        raise ValueError(f"{what} must be contiguous, since they are written")
-    return of
+class _List:
+    """Tensors of one device: their types, and whether all are contiguous."""
+
+    def __init__(self, of: Sequence[torch.Tensor], what: str) -> None:
+        self.tensors, self.what = list(of), what
+        if not self.tensors:
+            raise ValueError(f"{what} must be tensors, at least one")
+        try:
+            self.devices = set(map(_DEVICE_OF, self.tensors))
+            self.types = list(map(_DTYPES.get, map(_TYPE_OF, self.tensors)))
+            self.whole = all(map(_CONTIGUOUS, self.tensors))
+        except TypeError:
+            raise ValueError(f"{what} must be tensors, at least one") from None
+        if None in self.types or not self.whole and any(
+                [t.layout is not torch.strided for t in self.tensors]):
+            raise ValueError(f"{what} must be dense, float32 or bfloat16")
+        if len(self.devices) > 1:
+            raise ValueError(f"{what} must be on one device")
+
+    def like(self, other: "_List", types: bool) -> None:
+        if self.devices != other.devices:
+            raise ValueError(f"{self.what} and {other.what} must be on one device")
+        if list(map(_SHAPE_OF, self.tensors)) != list(map(_SHAPE_OF, other.tensors)):
+            raise ValueError(f"{self.what} and {other.what} must have the same shapes")
+        if types and self.types != other.types:
+            raise ValueError(f"{self.what} and {other.what} must have the same types")
+
+    def read(self) -> list[torch.Tensor]:
+        return self.tensors if self.whole else [t.contiguous() for t in self.tensors]
 
 
-def _change(name: str, gradients: list[torch.Tensor], codes: list[int],
-            weights: list[torch.Tensor] | None, weight_codes: list[int],
-            out: list[torch.Tensor] | None, max_norm: float, eta: float) -> torch.Tensor:
+def _written(out: Sequence[torch.Tensor] | None, of: _List) -> _List:
+    """Where the results go that stand for ``of``: there, unless there is an ``out``."""
+    to = of
+    if out is not None:
+        to = _List(out, "out")
+        to.like(of, types=True)
+    if not to.whole:
+        raise ValueError(f"{to.what} must be contiguous, since they are written")
+    return to
+
+
+def _change(name: str, gradients: _List, weights: _List | None, out: _List | None,
+            max_norm: float, eta: float) -> torch.Tensor:
     """The calls over lists; the norm."""
-    device = gradients[0].device
-    _on_gpu(gradients[0])
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    g = [t if t.is_contiguous() else t.contiguous() for t in gradients]
-    w = None if weights is None else [t if t.is_contiguous() else t.contiguous() for t in weights]
+    first = gradients.tensors[0]
+    _on_gpu(first)
+    norm = torch.empty((), dtype=torch.float32, device=first.device)
+    g = gradients.read()
+    pointers = list(map(_POINTER, g))
     zeros = [0] * len(g)
-    entries = map(_GRADIENT.pack, [t.data_ptr() for t in g],
-                  zeros if w is None else [t.data_ptr() for t in w],
-                  zeros if out is None else [t.data_ptr() for t in out], [t.numel() for t in g],
-                  codes, weight_codes)
+    w_pointers, w_types, to = zeros, zeros, pointers
+    if weights is not None:
+        w = weights.read()
+        to = w_pointers = list(map(_POINTER, w))
+        w_types = weights.types
+    if out is not None and out is not gradients and out is not weights:
+        to = list(map(_POINTER, out.tensors))
+    entries = map(_GRADIENT.pack, pointers, w_pointers, to, map(_COUNT, g), gradients.types, w_types)
     args = _packed(_GRADIENTS, norm.data_ptr(), max_norm, eta, len(g), 0) + b"".join(entries)
-    native.get().operator(name, args, device)
+    native.get().operator(name, args, first.device)
     if out is not None:  # autograd is told, as it is of any write
-        torch.autograd.graph.increment_version(out)
+        torch.autograd.graph.increment_version(out.tensors)
     return norm
 
 
@@ -818,8 +866,7 @@ def _max_norm(max_norm: float) -> float:
 def gradient_norm(gradients: Sequence[torch.Tensor]) -> torch.Tensor:
     """The 2-norm of the values of all ``gradients`` (fp32 or bf16, of any shapes) together, fp32
     ``[]``. Squares are added in fp64, so nothing overflows on the way."""
-    g, codes, _ = _tensors(gradients, "gradients")
-    return _change("gradient_norm", g, codes, None, [0] * len(g), None, 0.0, 0.0)
+    return _change("gradient_norm", _List(gradients, "gradients"), None, None, 0.0, 0.0)
 
 
 def clip_gradients(gradients: Sequence[torch.Tensor], max_norm: float, *,
@@ -828,9 +875,8 @@ def clip_gradients(gradients: Sequence[torch.Tensor], max_norm: float, *,
     :func:`gradient_norm`. A norm that is NaN makes every value NaN, and an infinite one zero but
     for the infinities (NaN). What is written must be contiguous, and overlap nothing but the
     gradient that it replaces."""
-    g, codes, _ = _tensors(gradients, "gradients")
-    to = _written(g if out is None else out, g, "gradients" if out is None else "out")
-    return _change("clip_gradients", g, codes, None, [0] * len(g), to, _max_norm(max_norm), 0.0)
+    g = _List(gradients, "gradients")
+    return _change("clip_gradients", g, None, _written(out, g), _max_norm(max_norm), 0.0)
 
 
 def sgd_step(weights: Sequence[torch.Tensor], gradients: Sequence[torch.Tensor], eta: float, *,
@@ -840,11 +886,8 @@ def sgd_step(weights: Sequence[torch.Tensor], gradients: Sequence[torch.Tensor],
     place or into ``out``, the gradients left as they are; returns their :func:`gradient_norm`.
     Weights and gradients are fp32 or bf16 each; the update is one fp32 multiplication and addition,
     rounded once. Norms that are not finite and what is written: :func:`clip_gradients`."""
-    g, codes, device = _tensors(gradients, "gradients")
-    w, weight_codes, _ = _tensors(weights, "weights", device)
-    if [t.shape for t in w] != [t.shape for t in g]:
-        raise ValueError("weights and gradients must have the same shapes")
+    g, w = _List(gradients, "gradients"), _List(weights, "weights")
+    w.like(g, types=False)
     if not -_MOST <= eta <= _MOST:
         raise ValueError(f"eta must be finite in fp32, got {eta}")
-    to = _written(w if out is None else out, w, "weights" if out is None else "out")
-    return _change("sgd_step", g, codes, w, weight_codes, to, _max_norm(max_norm), eta)
+    return _change("sgd_step", g, w, _written(out, w), _max_norm(max_norm), eta)

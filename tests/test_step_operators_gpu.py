@@ -648,6 +648,17 @@ def test_what_overlaps_is_refused():
     assert bool((t == 0.5).all())
 
 
+def test_tensors_of_two_devices_are_refused():
+    a, b = torch.ones(4, device=DEV), torch.ones(4)
+    for call in (lambda: ops.gradient_norm([a, b]), lambda: ops.clip_gradients([a], 1.0, out=[b]),
+                 lambda: ops.sgd_step([a], [b], 1.0), lambda: ops.sgd_step([b], [a], 1.0),
+                 lambda: ops.rms_norm_forward(a, b), lambda: ops.rms_norm_forward(a, a, residual=b),
+                 lambda: ops.gated_silu_forward(a, b),
+                 lambda: ops.rotary_forward(a.view(1, 1, 1, 4), a.view(1, 1, 1, 4), b[:1].long(), a[:2])):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_autograd_sees_the_writes():
     w = torch.ones(8, device=DEV, requires_grad=True)
     g = torch.ones(8, device=DEV)
