@@ -23,19 +23,23 @@
 
 namespace pots {
 
-constexpr uint32_t kChunk = 4096;  // values of a chunk: four runs of four to each of 256 lanes
-constexpr uint32_t kRunsOf = kChunk / 1024;
+// Values of a chunk: 16 KiB of the gradient, four or eight runs of four to each of 256 lanes, which are all
+// on their way at once.
+constexpr uint32_t kRuns32 = 4, kRuns16 = 8;
+__host__ __device__ constexpr uint32_t chunk_values(uint32_t type) {
+  return 1024 * (type == POTS_OP_BF16 ? kRuns16 : kRuns32);
+}
 constexpr uint32_t kNormed = 160, kUpdated = 96;  // tensors of a launch: below 4 KiB of arguments
 // Four to a compute unit: the update of 1.54e9 fp32 weights takes 4.30 ms, with eight 4.43.
 constexpr uint32_t kBlocks = 1024;
-// The last cache is left to the chunks that the second pass begins with, 192 MiB of fp32: what comes
+// The last cache is left to the chunks that the second pass begins with, 192 MiB: what comes
 // before them is read past it, and so is all that the second pass reads and writes if there is more
 // than that (1.54e9 weights: 4.68 ms all through it, 4.30 so; a clip of 1.35e8 gradients 335 and 276
 // us). A smaller gradient's results stay there for whoever reads them next.
 constexpr uint64_t kKept = 12288;
 constexpr uint32_t kMostTensors = 1u << 16;
 
-struct Normed {
+struct alignas(16) Normed {
   const void* g[kNormed];
   uint64_t count[kNormed];
   uint32_t first[kNormed];  // chunk; those from kNormed's own on
@@ -43,7 +47,7 @@ struct Normed {
   uint32_t tensors, chunks, kept;
 };
 
-struct Updated {
+struct alignas(16) Updated {
   const void *g[kUpdated], *w[kUpdated];
   void* out[kUpdated];
   uint64_t count[kUpdated];
@@ -60,52 +64,89 @@ __device__ __forceinline__ double sum_block(double v, double* s) {
   return s[0] + s[1] + s[2] + s[3];
 }
 
-// A lane's four runs of the chunk that starts at value `at` of a tensor of `count`.
-template <class T, bool PAST>
+// A launch's table, from its arguments to LDS: the look-ups in it are one after the other, and each from
+// the arguments would wait for memory.
+template <class TABLE>
+__device__ __forceinline__ void table_to_lds(const TABLE& t, TABLE& to) {
+  static_assert(sizeof(TABLE) % 16 == 0 && sizeof(TABLE) <= 4096, "a run of 16 bytes to each lane");
+  const u32x4v* const from = reinterpret_cast<const u32x4v*>(&t);
+  if (threadIdx.x < sizeof(TABLE) / 16)
+    reinterpret_cast<u32x4v*>(&to)[threadIdx.x] = from[threadIdx.x];
+  __syncthreads();
+}
+
+// The tensor that chunk c lies in, of those that start at the chunks first[0 .. n).
+__device__ __forceinline__ uint32_t tensor_of(const uint32_t* first, uint32_t n, uint32_t c) {
+  uint32_t lo = 0;
+  while (n > 1) {
+    const uint32_t half = n / 2;
+    if (first[lo + half] <= c) lo += half;
+    n -= half;
+  }
+  return lo;
+}
+
+// A lane's R runs of the chunk that starts at value `at` of a tensor of `count`.
+template <class T, uint32_t R, bool PAST>
 __device__ __forceinline__ void chunk_of(const void* p, uint64_t at, uint64_t count,
-                                         float (&v)[kRunsOf][4]) {
+                                         float (&v)[R][4]) {
   const typename T::elem* q = reinterpret_cast<const typename T::elem*>(p) + at;
-  Run<T, 4> x[kRunsOf];
-  if (count - at >= kChunk) {
+  Run<T, 4> x[R];
+  if (count - at >= 1024 * R) {
 #pragma unroll
-    for (uint32_t i = 0; i < kRunsOf; i++) {
+    for (uint32_t i = 0; i < R; i++) {
       const typename T::elem* const r = q + 4 * threadIdx.x + 1024 * i;
       x[i] = PAST ? load_past<Run<T, 4>>(r) : load_any<Run<T, 4>>(r);
     }
   } else {
-    load_runs<T, 4, kRunsOf>(q, 4 * threadIdx.x, 1024, (uint32_t)(count - at), x);
+    load_runs<T, 4, R>(q, 4 * threadIdx.x, 1024, (uint32_t)(count - at), x);
   }
 #pragma unroll
-  for (uint32_t i = 0; i < kRunsOf; i++)
+  for (uint32_t i = 0; i < R; i++)
 #pragma unroll
     for (uint32_t j = 0; j < 4; j++) v[i][j] = T::get(x[i][j]);
 }
 
-template <bool PAST>
+template <uint32_t R, bool PAST>
 __device__ __forceinline__ void chunk_of(const void* p, uint32_t type, uint64_t at, uint64_t count,
-                                         float (&v)[kRunsOf][4]) {
+                                         float (&v)[R][4]) {
   if (type == POTS_OP_BF16)
-    chunk_of<Bf16, PAST>(p, at, count, v);
+    chunk_of<Bf16, R, PAST>(p, at, count, v);
   else
-    chunk_of<Fp32, PAST>(p, at, count, v);
+    chunk_of<Fp32, R, PAST>(p, at, count, v);
 }
 
-__global__ __launch_bounds__(256) void norm_sums(Normed t, double* __restrict__ part) {
+template <class T, uint32_t R, bool PAST>
+__device__ __forceinline__ void add_squares(const Normed& t, uint32_t i, uint64_t at,
+                                            double (&sum)[4]) {
+  float v[R][4];
+  chunk_of<T, R, PAST>(t.g[i], at, t.count[i], v);
+#pragma unroll
+  for (uint32_t r = 0; r < R; r++)
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) sum[j] = fma((double)v[r][j], (double)v[r][j], sum[j]);
+}
+
+__global__ __launch_bounds__(256) void norm_sums(Normed args, double* __restrict__ part) {
   __shared__ double s_sum[4];
+  __shared__ Normed t;
+  table_to_lds(args, t);
   double sum[4] = {};
-  uint32_t i = 0;
+  uint32_t i = tensor_of(t.first, t.tensors, blockIdx.x);
   for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
     while (i + 1 < t.tensors && c >= t.first[i + 1]) i++;
-    const uint64_t at = (uint64_t)(c - t.first[i]) * kChunk;
-    float v[kRunsOf][4];
-    if (c < t.kept)
-      chunk_of<true>(t.g[i], t.type[i], at, t.count[i], v);
-    else
-      chunk_of<false>(t.g[i], t.type[i], at, t.count[i], v);
-#pragma unroll
-    for (uint32_t r = 0; r < kRunsOf; r++)
-#pragma unroll
-      for (uint32_t j = 0; j < 4; j++) sum[j] = fma((double)v[r][j], (double)v[r][j], sum[j]);
+    const uint64_t at = (uint64_t)(c - t.first[i]) * chunk_values(t.type[i]);
+    if (t.type[i] == POTS_OP_BF16) {
+      if (c < t.kept)
+        add_squares<Bf16, kRuns16, true>(t, i, at, sum);
+      else
+        add_squares<Bf16, kRuns16, false>(t, i, at, sum);
+    } else {
+      if (c < t.kept)
+        add_squares<Fp32, kRuns32, true>(t, i, at, sum);
+      else
+        add_squares<Fp32, kRuns32, false>(t, i, at, sum);
+    }
   }
   const double all = sum_block((sum[0] + sum[1]) + (sum[2] + sum[3]), s_sum);
   if (threadIdx.x == 0) part[blockIdx.x] = all;
@@ -113,7 +154,13 @@ __global__ __launch_bounds__(256) void norm_sums(Normed t, double* __restrict__ 
 
 __device__ __forceinline__ double norm_of(const double* part, uint32_t parts, double* s) {
   double v = 0.;
-  for (uint32_t i = threadIdx.x; i < parts; i += 256) v += part[i];
+  for (uint32_t i = threadIdx.x; i < parts; i += 1024) {
+    double x[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++)
+      x[j] = i + 256 * j < parts ? gload<double>(part + i + 256 * j) : 0.;
+    v += (x[0] + x[1]) + (x[2] + x[3]);
+  }
   return sqrt(sum_block(v, s));
 }
 
@@ -124,16 +171,16 @@ __global__ __launch_bounds__(256) void norm_write(const double* __restrict__ par
   if (threadIdx.x == 0) *norm = (float)n;
 }
 
-template <bool STEP, bool PAST>
+template <bool STEP, uint32_t R, bool PAST>
 __device__ __forceinline__ void update_chunk(const Updated& t, uint32_t i, uint64_t at, float f) {
   const uint64_t count = t.count[i];
-  float g[kRunsOf][4], w[kRunsOf][4];
-  chunk_of<PAST>(t.g[i], t.type[i], at, count, g);
-  if (STEP) chunk_of<PAST>(t.w[i], t.weight_type[i], at, count, w);
-  const uint32_t left = count - at < kChunk ? (uint32_t)(count - at) : kChunk;
+  float g[R][4], w[R][4];
+  chunk_of<R, PAST>(t.g[i], t.type[i], at, count, g);
+  if (STEP) chunk_of<R, PAST>(t.w[i], t.weight_type[i], at, count, w);
+  const uint32_t left = count - at < 1024 * R ? (uint32_t)(count - at) : 1024 * R;
   const uint32_t type = STEP ? t.weight_type[i] : t.type[i];
 #pragma unroll
-  for (uint32_t r = 0; r < kRunsOf; r++) {
+  for (uint32_t r = 0; r < R; r++) {
     const uint32_t c = 4 * threadIdx.x + 1024 * r;
 #pragma unroll
     for (uint32_t j = 0; j < 4; j++) g[r][j] = STEP ? fmaf(f, g[r][j], w[r][j]) : f * g[r][j];
@@ -143,24 +190,33 @@ __device__ __forceinline__ void update_chunk(const Updated& t, uint32_t i, uint6
 
 // STEP: w - eta·f·g, else f·g. The launch that writes the norm has its address.
 template <bool STEP>
-__global__ __launch_bounds__(256) void update(Updated t, const double* __restrict__ part,
+__global__ __launch_bounds__(256) void update(Updated args, const double* __restrict__ part,
                                               uint32_t parts, float max_norm, float eta, float* norm) {
   __shared__ double s_sum[4];
+  __shared__ Updated t;
+  table_to_lds(args, t);
   const double n = norm_of(part, parts, s_sum);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
   const double factor = n <= (double)max_norm ? 1. : (double)max_norm / n;
   const float f = (float)(STEP ? -(double)eta * factor : factor);
   if (blockIdx.x >= t.chunks) return;
-  uint32_t i = t.tensors - 1;
   const uint32_t last = (t.chunks - 1 - blockIdx.x) / gridDim.x * gridDim.x + blockIdx.x;
+  uint32_t i = tensor_of(t.first, t.tensors, last);
   for (uint32_t k = 0; k <= last / gridDim.x; k++) {
     const uint32_t c = last - k * gridDim.x;
     while (c < t.first[i]) i--;
-    const uint64_t at = (uint64_t)(c - t.first[i]) * kChunk;
-    if (t.past)
-      update_chunk<STEP, true>(t, i, at, f);
-    else
-      update_chunk<STEP, false>(t, i, at, f);
+    const uint64_t at = (uint64_t)(c - t.first[i]) * chunk_values(t.type[i]);
+    if (t.type[i] == POTS_OP_BF16) {
+      if (t.past)
+        update_chunk<STEP, kRuns16, true>(t, i, at, f);
+      else
+        update_chunk<STEP, kRuns16, false>(t, i, at, f);
+    } else {
+      if (t.past)
+        update_chunk<STEP, kRuns32, true>(t, i, at, f);
+      else
+        update_chunk<STEP, kRuns32, false>(t, i, at, f);
+    }
   }
 }
 
@@ -170,7 +226,10 @@ const pots_gradient* entries(const pots_gradients* a) {
   return reinterpret_cast<const pots_gradient*>(a + 1);
 }
 
-uint64_t chunks_of(const pots_gradient& e) { return (e.count + kChunk - 1) / kChunk; }
+uint64_t chunks_of(const pots_gradient& e) {
+  const uint32_t values = chunk_values(e.gradient_type);
+  return (e.count + values - 1) / values;
+}
 
 uint64_t chunks_of(const pots_gradients* a) {
   uint64_t chunks = 0;

@@ -93,7 +93,7 @@ __global__ __launch_bounds__(R::kThreads) void norm_rows(pots_rms_norm a) {
       for (uint32_t j = 0; j < 4; j++) {
         t[i][j] = X::get(x[i][j]);
         if (RES) t[i][j] = T::get(T::put(t[i][j] + T::get(r[i][j])));
-        sum += t[i][j] * t[i][j];
+        sum = fmaf(t[i][j], t[i][j], sum);
       }
       if (RES)
         store_run<T, 4>(reinterpret_cast<typename T::elem*>(a.total) + row * a.dim + c,
@@ -136,13 +136,19 @@ __global__ __launch_bounds__(R::kThreads) void norm_rows(pots_rms_norm a) {
         }
         float scale = __uint_as_float(most) / top;
         scale = scale < kLeastScale ? kLeastScale : scale;
+        // y / scale, as a division rounds it, from the reciprocal that the group shares: a product and
+        // its remainder's. Where the scale is infinite or NaN there is no remainder: 0·y.
+        const float inv = 1.f / scale, divisor = scale < INFINITY ? scale : 0.f;
         if (a.block ? left && lane % lanes == 0 : c == 0)
           gstore<float>(a.scales + row * groups + (a.block ? c / a.block : 0), scale);
         uint8_t* const q = reinterpret_cast<uint8_t*>(a.y) + row * a.dim + c;
         uint32_t b;
         float v[4];
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++) v[j] = t[i][j] / scale;
+        for (uint32_t j = 0; j < 4; j++) {
+          const float first = t[i][j] * inv;
+          v[j] = fmaf(fmaf(-first, divisor, t[i][j]), inv, first);
+        }
         if (a.y_type == POTS_OP_E4M3) {  // (v is at most 448 and a rounding: no overflow but NaN's)
           b = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
           b = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], (int)b, true);
@@ -200,8 +206,8 @@ __global__ __launch_bounds__(R::kThreads) void norm_grad(pots_rms_norm a, float*
 #pragma unroll
       for (uint32_t j = 0; j < 4; j++) {
         const float h = T::get(r[i][j]) * s, dy = Y::get(y[i][j]);
-        sum += dy * w[j] * h;
-        dw[i][j] += dy * h;
+        sum = fmaf(dy * w[j], h, sum);
+        dw[i][j] = fmaf(dy, h, dw[i][j]);
       }
     }
     const float mean = R::sum(sum, s_sum, turn) * over;
@@ -215,7 +221,7 @@ __global__ __launch_bounds__(R::kThreads) void norm_grad(pots_rms_norm a, float*
 #pragma unroll
       for (uint32_t j = 0; j < 4; j++) {
         const float h = T::get(r[i][j]) * s;
-        v[j] = s * (Y::get(y[i][j]) * w[j] - h * mean);
+        v[j] = s * fmaf(-h, mean, Y::get(y[i][j]) * w[j]);
         if (a.dtotal) v[j] += T::get(d[i][j]);
       }
       if (a.dresidual)

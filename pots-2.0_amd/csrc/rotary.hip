@@ -6,8 +6,9 @@
 // launch. θ is taken in whole turns and their fraction in 64 bits, so that far positions lose
 // nothing (below 2^-45 of a turn up to position 2^20); the sine and cosine of the fraction, less than
 // an eighth of a turn, are fp32. A block computes them for a few tokens into LDS, once for all heads; its
-// lanes then go over the tokens' heads, 16 bytes of u and 16 of v at a time. Where the pairs are no
-// multiple of such a run, the last run overlaps the one before it and writes the same values.
+// lanes then go over the tokens' heads, 16 bytes of u and 16 of v at a time, the first of them on their
+// way meanwhile. Where the pairs are no multiple of such a run, the last run overlaps the one before it
+// and writes the same values.
 #include <math.h>
 
 #include "common.h"
@@ -20,9 +21,6 @@ namespace pots {
 constexpr uint32_t kMaxWidth = 1024, kMaxHeads = 1u << 16;
 constexpr uint32_t kAngles = 1024, kTokens = 64;  // of a block, at the most
 constexpr uint32_t kAhead = 2;  // runs that a lane has on their way
-
-template <class T>
-constexpr uint32_t kPairs = 16 / sizeof(typename T::elem);  // pairs that a lane turns at a time
 
 struct Turn {
   float c, s;
@@ -42,11 +40,10 @@ __device__ __forceinline__ Turn turn_of(double position, double frequency, bool 
   return t;
 }
 
-// Elements of a lane's run: the pairs from i0 on, of the two halves or beside each other; or columns
-// that are copied.
-template <class T, bool ADJACENT>
+// A lane's part of a head: P pairs, of the two halves or beside each other, or 2P columns that are
+// copied. lo and hi lie `apart`.
+template <class T, uint32_t P, bool ADJACENT>
 struct Piece {
-  static constexpr uint32_t P = kPairs<T>;
   Run<T, P> lo, hi;
 
   __device__ __forceinline__ void load(const typename T::elem* p, uint32_t at, uint32_t apart) {
@@ -56,6 +53,57 @@ struct Piece {
   __device__ __forceinline__ void store(typename T::elem* p, uint32_t at, uint32_t apart) const {
     store_any(p + at, lo);
     store_any(p + at + apart, hi);
+  }
+  // Fewer pairs than P, value by value.
+  __device__ __forceinline__ void load_pairs(const typename T::elem* p, uint32_t apart,
+                                             uint32_t pairs) {
+#pragma unroll
+    for (uint32_t j = 0; j + 1 < P; j++) {
+      if (j >= pairs) break;
+      if (ADJACENT) {
+        Run<T, P>& r = j < P / 2 ? lo : hi;
+        r[2 * j % P] = gload<typename T::elem>(p + 2 * j);
+        r[2 * j % P + 1] = gload<typename T::elem>(p + 2 * j + 1);
+      } else {
+        lo[j] = gload<typename T::elem>(p + j);
+        hi[j] = gload<typename T::elem>(p + apart + j);
+      }
+    }
+  }
+  __device__ __forceinline__ void store_pairs(typename T::elem* p, uint32_t apart,
+                                              uint32_t pairs) const {
+#pragma unroll
+    for (uint32_t j = 0; j + 1 < P; j++) {
+      if (j >= pairs) break;
+      if (ADJACENT) {
+        const Run<T, P>& r = j < P / 2 ? lo : hi;
+        gstore<typename T::elem>(p + 2 * j, r[2 * j % P]);
+        gstore<typename T::elem>(p + 2 * j + 1, r[2 * j % P + 1]);
+      } else {
+        gstore<typename T::elem>(p + j, lo[j]);
+        gstore<typename T::elem>(p + apart + j, hi[j]);
+      }
+    }
+  }
+  // Fewer columns than 2P, in pieces of P, P / 2, ... 1 of them, as their count has them.
+  template <uint32_t N, bool LOAD, class E>
+  __device__ __forceinline__ void columns(E* p, uint32_t rest) {
+    Run<T, P>& r = N == P ? lo : hi;
+    constexpr uint32_t at = N == P ? 0 : P - 2 * N;
+    if (rest & N) {
+      E* const q = p + (rest & ~(2 * N - 1));
+      Run<T, N> x;
+      if constexpr (LOAD) {
+        x = load_any<Run<T, N>>(q);
+#pragma unroll
+        for (uint32_t j = 0; j < N; j++) r[at + j] = x[j];
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < N; j++) x[j] = r[at + j];
+        store_any(q, x);
+      }
+    }
+    if constexpr (N > 1) columns<N / 2, LOAD>(p, rest);
   }
   __device__ __forceinline__ void turn(const Turn* t) {
 #pragma unroll
@@ -76,24 +124,11 @@ struct Piece {
   }
 };
 
-// A head whose pairs (or whose copied columns) are fewer than a run: value by value.
-template <class T, bool ADJACENT>
-__device__ __forceinline__ void turn_few(const typename T::elem* in, typename T::elem* out,
-                                         uint32_t pairs, const Turn* t) {
-  for (uint32_t i = 0; i < pairs; i++) {
-    const uint32_t a = ADJACENT ? 2 * i : i, b = ADJACENT ? 2 * i + 1 : i + pairs;
-    const float u = T::get(gload<typename T::elem>(in + a));
-    const float v = T::get(gload<typename T::elem>(in + b));
-    gstore<typename T::elem>(out + a, T::put(u * t[i].c - v * t[i].s));
-    gstore<typename T::elem>(out + b, T::put(u * t[i].s + v * t[i].c));
-  }
-}
-
-template <class T, bool ADJACENT>
+// FEW: a head has fewer pairs than P, or fewer other columns than 2P.
+template <class T, uint32_t P, bool ADJACENT, bool FEW>
 __global__ __launch_bounds__(256) void rotary_turn(pots_rotary a, uint32_t tokens, uint64_t from) {
   typedef typename T::elem elem;
-  constexpr uint32_t P = kPairs<T>;
-  __shared__ Turn s_turn[kAngles];
+  __shared__ Turn s_turn[kAngles + P];  // (a head of fewer pairs than P reads past its last one)
   const uint64_t all = (uint64_t)a.batch * a.n, t0 = from + (uint64_t)blockIdx.x * tokens;
   const uint32_t here = (uint32_t)(all - t0 < tokens ? all - t0 : tokens);
   const uint32_t heads = a.heads + a.kv_heads, items = here * heads;
@@ -122,13 +157,15 @@ __global__ __launch_bounds__(256) void rotary_turn(pots_rotary a, uint32_t token
   const uint32_t rest = a.head_dim - 2 * a.pairs;
   const uint32_t runs = turned + (rest < 2 * P ? rest != 0 : (rest + 2 * P - 1) / (2 * P));
   const uint32_t slots = 256 / runs, slot = threadIdx.x / runs, run = threadIdx.x - slot * runs;
-  const bool turns = run < turned, whole = turns ? a.pairs >= P : rest >= 2 * P;
-  const uint32_t i0 = min(run * P, a.pairs - P);
-  const uint32_t at = !turns ? 2 * a.pairs + min((run - turned) * 2 * P, rest - 2 * P)
-                      : ADJACENT ? 2 * i0 : i0;
+  const bool turns = run < turned, whole = !FEW || (turns ? a.pairs >= P : rest >= 2 * P);
+  const uint32_t i0 = a.pairs >= P ? min(run * P, a.pairs - P) : 0;
+  const uint32_t c0 = rest >= 2 * P ? min((run - turned) * 2 * P, rest - 2 * P) : 0;
+  const uint32_t at = !turns ? 2 * a.pairs + c0 : ADJACENT ? 2 * i0 : i0;
   const uint32_t apart = turns && !ADJACENT ? a.pairs : P;
   const uint32_t first = slot < slots ? slot : items;  // (lanes past the last slot have no item)
-  Piece<T, ADJACENT> x[kAhead];
+  Piece<T, P, ADJACENT> x[kAhead];
+  if (FEW)
+    for (uint32_t j = 0; j < kAhead; j++) x[j] = {};
   elem* out[kAhead];
   uint32_t t[kAhead];
   auto load = [&](uint32_t item) {
@@ -136,10 +173,15 @@ __global__ __launch_bounds__(256) void rotary_turn(pots_rotary a, uint32_t token
     for (uint32_t j = 0; j < kAhead; j++) {
       const elem* in;  // (past the last item: that one again, and nothing is stored)
       place(min(item + j * slots, items - 1), t[j], in, out[j]);
-      x[j].load(in, at, apart);
+      if (whole)
+        x[j].load(in, at, apart);
+      else if (turns)
+        x[j].load_pairs(in, apart, a.pairs);
+      else
+        x[j].template columns<P, true>(in + at, rest);
     }
   };
-  if (whole && first < items) load(first);  // on their way while the angles are taken
+  if (first < items) load(first);  // on their way while the angles are taken
   for (uint32_t e = threadIdx.x; e < here * a.pairs; e += 256) {
     const uint32_t t = e / a.pairs, i = e - t * a.pairs;
     uint32_t b, n, axis = 0;
@@ -156,26 +198,18 @@ __global__ __launch_bounds__(256) void rotary_turn(pots_rotary a, uint32_t token
     s_turn[e] = turn_of(position, f, a.inverse);
   }
   __syncthreads();
-  if (whole) {
-    for (uint32_t item = first; item < items; item += kAhead * slots) {
-      if (item != first) load(item);
+  for (uint32_t item = first; item < items; item += kAhead * slots) {
+    if (item != first) load(item);
 #pragma unroll
-      for (uint32_t j = 0; j < kAhead; j++) {
-        if (turns) x[j].turn(s_turn + t[j] * a.pairs + i0);
-        if (item + j * slots < items) x[j].store(out[j], at, apart);
-      }
-    }
-  } else {
-    for (uint32_t item = first; item < items; item += slots) {
-      uint32_t t;
-      const elem* in;
-      elem* out;
-      place(item, t, in, out);
-      if (turns)
-        turn_few<T, ADJACENT>(in, out, a.pairs, s_turn + t * a.pairs);
+    for (uint32_t j = 0; j < kAhead; j++) {
+      if (turns) x[j].turn(s_turn + t[j] * a.pairs + i0);
+      if (item + j * slots >= items) continue;
+      if (whole)
+        x[j].store(out[j], at, apart);
+      else if (turns)
+        x[j].store_pairs(out[j], apart, a.pairs);
       else
-        for (uint32_t c = 2 * a.pairs; c < a.head_dim; c++)
-          gstore<elem>(out + c, gload<elem>(in + c));
+        x[j].template columns<P, false>(out[j] + at, rest);
     }
   }
 }
@@ -195,7 +229,7 @@ bool bad(const pots_rotary* a) {
   return a->ends[a->axes - 1] != a->pairs;
 }
 
-template <class T>
+template <class T, uint32_t P>
 int turn(const pots_rotary* a, hipStream_t s) {
   // Tokens of a block: few enough for eight blocks to a compute unit (8192 tokens of 14 heads of 128: 15.3
   // us, with four 16.4, with sixteen 17), as many as their angles allow.
@@ -203,7 +237,11 @@ int turn(const pots_rotary* a, hipStream_t s) {
   uint64_t tokens = all / 2048;
   const uint32_t most = kAngles / a->pairs < kTokens ? kAngles / a->pairs : kTokens;
   tokens = tokens < 1 ? 1 : tokens > most ? most : tokens;
-  const auto kernel = a->adjacent ? rotary_turn<T, true> : rotary_turn<T, false>;
+  const uint32_t rest = a->head_dim - 2 * a->pairs;
+  const bool few = a->pairs < P || (rest && rest < 2 * P);
+  const auto kernel =
+      few ? (a->adjacent ? rotary_turn<T, P, true, true> : rotary_turn<T, P, false, true>)
+          : (a->adjacent ? rotary_turn<T, P, true, false> : rotary_turn<T, P, false, false>);
   constexpr uint64_t kLaunch = 1u << 23;  // blocks: a launch has less than 2^32 threads
   for (uint64_t from = 0; from < all; from += kLaunch * tokens) {
     const uint64_t blocks = (all - from + tokens - 1) / tokens;
@@ -226,5 +264,6 @@ extern "C" int pots_rotary_turn(const pots_rotary* a, void* stream) {
   if (!a->q.ptr || !a->k.ptr || !a->q_out.ptr || !a->k_out.ptr || !a->positions || !a->frequencies)
     return POTS_E_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return a->dtype == POTS_OP_BF16 ? turn<Bf16>(a, s) : turn<Fp32>(a, s);
+  if (a->dtype != POTS_OP_BF16) return turn<Fp32, 4>(a, s);
+  return a->pairs >= 8 ? turn<Bf16, 8>(a, s) : turn<Bf16, 4>(a, s);
 }

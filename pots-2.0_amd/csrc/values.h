@@ -43,14 +43,21 @@ __device__ __forceinline__ void store_past(E* p, V v) {
 // A run's values from the one numbered `by` (0 to N - 1) on, zeros behind them.
 template <class T, uint32_t N>
 __device__ __forceinline__ Run<T, N> shifted(Run<T, N> x, uint32_t by) {
+  if constexpr (sizeof(x) == 8) {
+    return __builtin_bit_cast(Run<T, N>, __builtin_bit_cast(uint64_t, x) >> 8 * sizeof(x[0]) * by);
+  } else if constexpr (sizeof(x) == 16) {
+    return __builtin_bit_cast(
+        Run<T, N>, __builtin_bit_cast(unsigned __int128, x) >> 8 * (uint32_t)sizeof(x[0]) * by);
+  } else {
 #pragma unroll
-  for (uint32_t m = 1; m < N; m *= 2) {
-    Run<T, N> y = {};
+    for (uint32_t m = 1; m < N; m *= 2) {
+      Run<T, N> y = {};
 #pragma unroll
-    for (uint32_t j = 0; j + m < N; j++) y[j] = x[j + m];
-    x = by & m ? y : x;
+      for (uint32_t j = 0; j + m < N; j++) y[j] = x[j + m];
+      x = by & m ? y : x;
+    }
+    return x;
   }
-  return x;
 }
 
 // A lane's G runs of a row of `dim` values: those from first + i·step on, zeros past the row's end. A
@@ -139,16 +146,22 @@ struct AnyRuns {
       load_runs<Fp32, 4, G>(reinterpret_cast<const float*>(p), first, step, dim, raw);
     }
   }
+  // (The empty statements keep the conversion here, where it does not wait for other loads, and in a
+  // branch, which is the same for all lanes.)
   __device__ __forceinline__ void get(uint32_t type, uint32_t i, float (&v)[4]) const {
-    float x[4] = {raw[i][0], raw[i][1], raw[i][2], raw[i][3]};
-    // (here and not where they were loaded: the conversion would wait for them there)
-    asm volatile("" : "+v"(x[0]), "+v"(x[1]));
-    const uint32_t lo = __float_as_uint(x[0]), hi = __float_as_uint(x[1]);
-    const bool halves = type == POTS_OP_BF16;
-    v[0] = halves ? __uint_as_float(lo << 16) : x[0];
-    v[1] = halves ? __uint_as_float(lo & 0xffff0000u) : x[1];
-    v[2] = halves ? __uint_as_float(hi << 16) : x[2];
-    v[3] = halves ? __uint_as_float(hi & 0xffff0000u) : x[3];
+    float lo = raw[i][0], hi = raw[i][1];
+    asm volatile("" : "+v"(lo), "+v"(hi));
+    v[0] = lo;
+    v[1] = hi;
+    v[2] = raw[i][2];
+    v[3] = raw[i][3];
+    if (type == POTS_OP_BF16) {
+      asm volatile("");
+      v[0] = __uint_as_float(__float_as_uint(lo) << 16);
+      v[1] = __uint_as_float(__float_as_uint(lo) & 0xffff0000u);
+      v[2] = __uint_as_float(__float_as_uint(hi) << 16);
+      v[3] = __uint_as_float(__float_as_uint(hi) & 0xffff0000u);
+    }
   }
 };
 
