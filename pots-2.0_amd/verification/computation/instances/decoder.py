@@ -387,6 +387,8 @@ class DecoderComputation(DeclaredComputation):
             if getattr(att, "sliding_window", None) is not None:
                 raise ValueError("the uncaptured attention is over whole sequences: no sliding "
                                  "window")
+            if att.training and att.attention_dropout:
+                raise ValueError("attention dropout must be off: a step must be deterministic")
             y, stream = normed(layer.input_layernorm, stream, branch)
             q, k = operators.rotary(heads(att.q_proj(y), att.head_dim),
                                     heads(att.k_proj(y), att.head_dim), positions, rope.inv_freq)

@@ -460,12 +460,20 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     return t, t.stride(0)
 
 
-def _new(shape: Sequence[int], dtype: torch.dtype, *near: torch.Tensor | None) -> torch.Tensor:
-    """An uninitialised tensor on the device of ``near``, of which one of the type makes it."""
+# (torch.empty takes twice the host time of these)
+def _new_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A contiguous tensor of ``t``'s shape."""
+    if t.is_contiguous():
+        return torch.empty_like(t, dtype=dtype)
+    return torch.empty(t.shape, dtype=dtype, device=t.device)
+
+
+def _new_floats(shape: Sequence[int], *near: torch.Tensor | None) -> torch.Tensor:
+    """An fp32 tensor on the device of ``near``."""
     for t in near:
-        if t is not None and t.dtype == dtype:  # (half the host time of torch.empty)
+        if t is not None and t.dtype == torch.float32:
             return t.new_empty(shape)
-    return torch.empty(shape, dtype=dtype, device=near[0].device)
+    return torch.empty(shape, dtype=torch.float32, device=near[0].device)
 
 
 def _norm_args(x: torch.Tensor, weight: torch.Tensor, eps: float, what: str) -> int:
@@ -494,7 +502,7 @@ def _run_norm(name: str, x: torch.Tensor, weight: torch.Tensor, residual: torch.
     """The forward calls; the sum that was normed."""
     total, to, other, other_ptr, other_row = x, 0, None, 0, 0
     if residual is not None:
-        total = residual.new_empty(x.shape)
+        total = _new_like(residual, residual.dtype)
         other, other_row = _rows(residual)
         to, other_ptr = total.data_ptr(), other.data_ptr()
     rows, row = _rows(x)
@@ -522,8 +530,8 @@ def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6
     if out_dtype not in _DTYPES:
         raise ValueError(f"out_dtype must be float32 or bfloat16, not {out_dtype}")
     _on_gpu(x)
-    y = _new(x.shape, out_dtype, x, residual)
-    rstd = _new(x.shape[:-1], torch.float32, weight, residual)
+    y = _new_like(x, out_dtype)
+    rstd = _new_floats(x.shape[:-1], weight, residual)
     total = _run_norm("rms_norm_forward", x, weight, residual, y, _DTYPES[out_dtype], rstd, None, 0,
                       eps)
     return y, total, rstd
@@ -546,8 +554,8 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e
         raise ValueError(f"block must be 32, 64, 128 or 256, or None for a row, not {block}")
     blocks = 1 if block is None else -(-x.shape[-1] // block)
     _on_gpu(x)
-    q = torch.empty(x.shape, dtype=dtype, device=x.device)
-    scales = _new((*x.shape[:-1], blocks), torch.float32, weight, residual)
+    q = _new_like(x, dtype)
+    scales = _new_floats((*x.shape[:-1], blocks), weight, residual)
     total = _run_norm("rms_norm_quantized", x, weight, residual, q, _EIGHT_BITS[dtype], None,
                       scales, block or 0, eps)
     return q, scales, total
@@ -574,10 +582,10 @@ def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, weight: torch.Tenso
     if x_dtype not in _DTYPES:
         raise ValueError(f"x_dtype must be float32 or bfloat16, not {x_dtype}")
     _on_gpu(total)
-    dresidual = dx = total.new_empty(total.shape)
+    dresidual = dx = _new_like(total, total.dtype)
     if x_dtype != total.dtype:
-        dx = _new(total.shape, x_dtype, dy, weight)
-    dweight = weight.new_empty(weight.shape)
+        dx = _new_like(total, x_dtype)
+    dweight = _new_like(weight, weight.dtype)
     (g, g_row), (t, t_row), own = _rows(dy), _rows(total), weight.contiguous()
     other, other_ptr, other_row = None, 0, 0
     if dtotal is not None:
@@ -651,9 +659,12 @@ def _turned(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
             or frequencies.device != q.device or not 2 <= 2 * pairs <= d):
         raise ValueError(f"frequencies must be float32 or float64 [pairs] on {q.device}, one for "
                          f"each pair of a head of {d}")
-    counts = (pairs,) if sections is None else tuple(sections)
-    if not 1 <= len(counts) <= 4 or min(counts) < 0 or sum(counts) != pairs:
-        raise ValueError(f"sections must be up to 4 counts whose sum is {pairs}, got {counts}")
+    counts = ends = (pairs,)
+    if sections is not None:
+        counts = tuple(sections)
+        if not 1 <= len(counts) <= 4 or min(counts) < 0 or sum(counts) != pairs:
+            raise ValueError(f"sections must be up to 4 counts whose sum is {pairs}, got {counts}")
+        ends = tuple(itertools.accumulate(counts))
     axes, at = len(counts), positions
     if at.dtype not in (torch.int64, torch.int32) or at.device != q.device:
         raise ValueError(f"positions must be int64 or int32 on {q.device}")
@@ -669,20 +680,20 @@ def _turned(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     if shape[1] == 1:
         strides = (strides[0], 0, strides[2])
     _on_gpu(q)
-    q, k = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k))
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if k.stride(3) != 1:
+        k = k.contiguous()
     frequencies = frequencies.contiguous()
-    to_q, to_k = _new_heads(b, h, n, d, q), _new_heads(b, kv, n, d, q)
-    ends = list(itertools.accumulate(counts)) + [pairs] * (4 - axes)
-    args = _packed(_ROTARY, *_places(q), *_places(k), *_places(to_q), *_places(to_k),
-                   at.data_ptr(), frequencies.data_ptr(), *strides, b, h, kv, n, d, pairs, axes,
-                   *ends, code, 0 if frequencies.dtype == torch.float32 else _F64,
+    of_q, of_k = (n * h * d, d, h * d), (n * kv * d, d, kv * d)  # as _new_heads has them
+    to_q, to_k = q.new_empty_strided(q.shape, (*of_q, 1)), q.new_empty_strided(k.shape, (*of_k, 1))
+    args = _packed(_ROTARY, q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
+                   to_q.data_ptr(), *of_q, to_k.data_ptr(), *of_k, at.data_ptr(),
+                   frequencies.data_ptr(), *strides, b, h, kv, n, d, pairs, axes, *ends,
+                   *(pairs,) * (4 - axes), code, 0 if frequencies.dtype == torch.float32 else _F64,
                    64 if at.dtype == torch.int64 else 32, adjacent, inverse)
     native.get().operator("rotary_turn", args, q.device)
     return to_q, to_k
-
-
-def _places(t: torch.Tensor) -> tuple[int, int, int, int]:
-    return t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)
 
 
 def rotary_forward(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
@@ -741,7 +752,7 @@ def gated_silu_forward(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     shape and type, each anywhere (the halves of one product, for instance)."""
     code = _gated_args(gate, up)
     _on_gpu(gate)
-    out = gate.new_empty(gate.shape)
+    out = _new_like(gate, gate.dtype)
     if out.numel():
         (g, g_row), (u, u_row), columns = _rows(gate), _rows(up), gate.shape[-1]
         args = _packed(_GATED, g.data_ptr(), u.data_ptr(), 0, out.data_ptr(), 0, 0, g_row, u_row, 0,
@@ -756,7 +767,7 @@ def gated_silu_backward(dout: torch.Tensor, gate: torch.Tensor, up: torch.Tensor
     code = _gated_args(gate, up)
     _like(dout, gate, gate.shape, "dout")
     _on_gpu(gate)
-    dgate, dup = gate.new_empty(gate.shape), gate.new_empty(gate.shape)
+    dgate, dup = _new_like(gate, gate.dtype), _new_like(gate, gate.dtype)
     if dgate.numel():
         (g, g_row), (u, u_row), (d, d_row) = _rows(gate), _rows(up), _rows(dout)
         columns = gate.shape[-1]
@@ -852,8 +863,11 @@ def _change(name: str, gradients: _List, weights: _List | None, out: _List | Non
     entries = map(_GRADIENT.pack, pointers, w_pointers, to, map(_COUNT, g), gradients.types, w_types)
     args = _packed(_GRADIENTS, norm.data_ptr(), max_norm, eta, len(g), 0) + b"".join(entries)
     native.get().operator(name, args, first.device)
-    if out is not None:  # autograd is told, as it is of any write
-        torch.autograd.graph.increment_version(out.tensors)
+    if out is not None:  # autograd is told, as it is of any write (it counts none of inference's)
+        try:
+            torch.autograd.graph.increment_version(out.tensors)
+        except RuntimeError:
+            torch.autograd.graph.increment_version([t for t in out.tensors if not t.is_inference()])
     return norm
 
 

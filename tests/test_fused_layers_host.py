@@ -82,6 +82,11 @@ def test_what_fused_layers_refuse():
     with pytest.raises(ValueError, match="sliding"):
         c.uncaptured_loss(model, records, fused=True)
     c, model, records = _step(True)
+    model.train()
+    model.model.layers[1].self_attn.attention_dropout = 0.1
+    with pytest.raises(ValueError, match="dropout"):
+        c.uncaptured_loss(model, records, fused=True)
+    c, model, records = _step(True)
     model.model.rotary_emb.rope_type = "dynamic"
     with pytest.raises(ValueError, match="rotary"):
         c.uncaptured_loss(model, records, fused=True)

@@ -671,6 +671,20 @@ def test_autograd_sees_the_writes():
         y.backward()
 
 
+def test_inference_tensors():
+    """They have no version to count, and are written like others."""
+    with torch.inference_mode():
+        w, g = torch.ones(8, device=DEV), torch.full((8,), 2.0, device=DEV)
+        x = torch.randn(3, 8, device=DEV)
+        ops.sgd_step([w], [g], 0.25)
+        y, total = ops.rms_norm(x, w, residual=x)
+        ops.gated_silu(y, total)
+    v = torch.ones(8, device=DEV)
+    version = v._version
+    ops.sgd_step([w, v], [g, g], 0.25)
+    assert bool((w == 0).all()) and bool((v == 0.5).all()) and v._version > version
+
+
 # ---- streams, repetition and graphs ---------------------------------------------------------
 
 def _pass(x, w, res, dy, q, k, at, f, gate, up, grads, weights, out):
