@@ -3,9 +3,9 @@
 //   out = silu(g)·u,  silu(g) = g·σ(g),  σ(g) = 1 / (1 + e^−g)
 //   dg = dout·u·σ(g)(1 + g·(1 − σ(g))),  du = dout·silu(g)
 //
-// Bound by memory: three tensors forward, five backward, each once, 16 bytes a lane. The arithmetic
-// is fp32, rounded once. e^−g overflows to infinity for g < −88, where σ is then 0, as it is in
-// fp32; 1 − σ is e^−g·σ, taken from whichever of e^−g and e^g is at most 1.
+// Bound by memory: three tensors forward, five backward, each once, 16 bytes a lane (8192 x 8960 in bf16
+// 75 us and 106, 5.9 and 6.9 TB/s). The arithmetic is fp32, rounded once. σ and 1 − σ come from e^−|g|,
+// which is at most 1, so that neither loses its last bits to the other.
 #include <math.h>
 
 #include "common.h"
@@ -34,8 +34,17 @@ struct Divisor {
 struct Sigma {
   float one, rest;  // σ(g) and 1 − σ(g)
 };
+// From e^−|g| = 2^n·2^f, n + f = −|g|·log2 e in two parts, and a reciprocal between 1/2 and 1 improved once
+// by Newton's step. (With the library's exponential and an exact division the vector units are busy for
+// 0.87 of a large call, so for 0.62, and a call that the cache holds takes a tenth longer: 1024 x 4864 in
+// bf16 forward 9.9 us, so 9.0.) |g| past 200 is 200, since e^−200 is zero; a NaN comes back with g, by which all is
+// multiplied.
 __device__ __forceinline__ Sigma sigma(float g) {
-  const float e = expf(-fabsf(g)), q = 1.f / (1.f + e);
+  constexpr float kLog2e = 1.44269502f, kRest = 1.92596299e-8f;  // log2 e in fp32, and what is left
+  const float a = fminf(fabsf(g), 200.f), hi = -a * kLog2e;
+  const float lo = fmaf(-a, kRest, fmaf(-a, kLog2e, -hi)), n = rintf(hi);
+  const float e = __builtin_ldexpf(__builtin_amdgcn_exp2f(hi - n + lo), (int)n);
+  const float d = 1.f + e, r = __builtin_amdgcn_rcpf(d), q = fmaf(fmaf(-d, r, 1.f), r, r);
   return g >= 0.f ? Sigma{q, e * q} : Sigma{e * q, q};
 }
 
@@ -64,7 +73,7 @@ __global__ __launch_bounds__(256) void gated(pots_gated_silu a, Divisor runs, ui
     const Sigma s = sigma(x);
     if (GRAD) {
       const float dy = T::get(d[0][j]);
-      y[j] = dy * v * (s.one * (1.f + x * s.rest));
+      y[j] = dy * v * (s.one * fmaf(x, s.rest, 1.f));
       z[j] = dy * (x * s.one);
     } else {
       y[j] = x * s.one * v;

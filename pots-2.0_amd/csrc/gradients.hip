@@ -29,7 +29,9 @@ constexpr uint32_t kRuns32 = 4, kRuns16 = 8;
 __host__ __device__ constexpr uint32_t chunk_values(uint32_t type) {
   return 1024 * (type == POTS_OP_BF16 ? kRuns16 : kRuns32);
 }
-constexpr uint32_t kNormed = 160, kUpdated = 96;  // tensors of a launch: below 4 KiB of arguments
+// Tensors of a launch: below 4 KiB of arguments, or a third of that for few (each KiB of arguments
+// takes the host half a microsecond).
+constexpr uint32_t kNormed = 160, kUpdated = 96, kFewTensors = 32;
 // Four to a compute unit: the update of 1.54e9 fp32 weights takes 4.30 ms, with eight 4.43.
 constexpr uint32_t kBlocks = 1024;
 // The last cache is left to the chunks that the second pass begins with, 192 MiB: what comes
@@ -39,20 +41,24 @@ constexpr uint32_t kBlocks = 1024;
 constexpr uint64_t kKept = 12288;
 constexpr uint32_t kMostTensors = 1u << 16;
 
+template <uint32_t N>
 struct alignas(16) Normed {
-  const void* g[kNormed];
-  uint64_t count[kNormed];
-  uint32_t first[kNormed];  // chunk; those from kNormed's own on
-  uint8_t type[kNormed];
-  uint32_t tensors, chunks, kept;
+  static constexpr uint32_t kMost = N;
+  const void* g[N];
+  uint64_t count[N];
+  uint32_t first[N];  // chunk
+  uint8_t type[N];
+  uint32_t tensors, chunks, kept;  // the chunks from `kept` on stay in the cache
 };
 
+template <uint32_t N>
 struct alignas(16) Updated {
-  const void *g[kUpdated], *w[kUpdated];
-  void* out[kUpdated];
-  uint64_t count[kUpdated];
-  uint32_t first[kUpdated];
-  uint8_t type[kUpdated], weight_type[kUpdated];
+  static constexpr uint32_t kMost = N;
+  const void *g[N], *w[N];
+  void* out[N];
+  uint64_t count[N];
+  uint32_t first[N];
+  uint8_t type[N], weight_type[N];
   uint32_t tensors, chunks, past;
 };
 
@@ -116,8 +122,8 @@ __device__ __forceinline__ void chunk_of(const void* p, uint32_t type, uint64_t 
     chunk_of<Fp32, R, PAST>(p, at, count, v);
 }
 
-template <class T, uint32_t R, bool PAST>
-__device__ __forceinline__ void add_squares(const Normed& t, uint32_t i, uint64_t at,
+template <class T, uint32_t R, bool PAST, class TABLE>
+__device__ __forceinline__ void add_squares(const TABLE& t, uint32_t i, uint64_t at,
                                             double (&sum)[4]) {
   float v[R][4];
   chunk_of<T, R, PAST>(t.g[i], at, t.count[i], v);
@@ -127,9 +133,10 @@ __device__ __forceinline__ void add_squares(const Normed& t, uint32_t i, uint64_
     for (uint32_t j = 0; j < 4; j++) sum[j] = fma((double)v[r][j], (double)v[r][j], sum[j]);
 }
 
-__global__ __launch_bounds__(256) void norm_sums(Normed args, double* __restrict__ part) {
+template <class TABLE>
+__global__ __launch_bounds__(256) void norm_sums(TABLE args, double* __restrict__ part) {
   __shared__ double s_sum[4];
-  __shared__ Normed t;
+  __shared__ TABLE t;
   table_to_lds(args, t);
   double sum[4] = {};
   uint32_t i = tensor_of(t.first, t.tensors, blockIdx.x);
@@ -171,8 +178,8 @@ __global__ __launch_bounds__(256) void norm_write(const double* __restrict__ par
   if (threadIdx.x == 0) *norm = (float)n;
 }
 
-template <bool STEP, uint32_t R, bool PAST>
-__device__ __forceinline__ void update_chunk(const Updated& t, uint32_t i, uint64_t at, float f) {
+template <bool STEP, uint32_t R, bool PAST, class TABLE>
+__device__ __forceinline__ void update_chunk(const TABLE& t, uint32_t i, uint64_t at, float f) {
   const uint64_t count = t.count[i];
   float g[R][4], w[R][4];
   chunk_of<R, PAST>(t.g[i], t.type[i], at, count, g);
@@ -189,11 +196,11 @@ __device__ __forceinline__ void update_chunk(const Updated& t, uint32_t i, uint6
 }
 
 // STEP: w - eta·f·g, else f·g. The launch that writes the norm has its address.
-template <bool STEP>
-__global__ __launch_bounds__(256) void update(Updated args, const double* __restrict__ part,
+template <bool STEP, class TABLE>
+__global__ __launch_bounds__(256) void update(TABLE args, const double* __restrict__ part,
                                               uint32_t parts, float max_norm, float eta, float* norm) {
   __shared__ double s_sum[4];
-  __shared__ Updated t;
+  __shared__ TABLE t;
   table_to_lds(args, t);
   const double n = norm_of(part, parts, s_sum);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
@@ -250,15 +257,15 @@ bool bad(const pots_gradients* a, bool clips, bool steps) {
   return chunks_of(a) > 0x7fffffffu;
 }
 
-// Launches over the tensors that hold something, N of them each: f(table, its first entry).
-template <uint32_t N, class F>
-int each_launch(const pots_gradients* a, F&& f) {
+// The entries that hold something, `most` of them at a time: f(their indices, how many).
+template <class F>
+int each_launch(const pots_gradients* a, uint32_t most, F&& f) {
   std::vector<uint32_t> some;
   some.reserve(a->tensors);
   for (uint32_t i = 0; i < a->tensors; i++)
     if (entries(a)[i].count) some.push_back(i);
-  for (size_t at = 0; at < some.size(); at += N) {
-    const uint32_t n = (uint32_t)std::min<size_t>(N, some.size() - at);
+  for (size_t at = 0; at < some.size(); at += most) {
+    const uint32_t n = (uint32_t)std::min<size_t>(most, some.size() - at);
     const int rc = f(some.data() + at, n);
     if (rc != POTS_E_OK) return rc;
   }
@@ -269,7 +276,7 @@ uint32_t blocks_of(uint64_t chunks) { return (uint32_t)std::min<uint64_t>(chunks
 
 uint32_t parts_of(const pots_gradients* a) {
   uint32_t parts = 0;
-  (void)each_launch<kNormed>(a, [&](const uint32_t* some, uint32_t n) {
+  (void)each_launch(a, kNormed, [&](const uint32_t* some, uint32_t n) {
     uint64_t chunks = 0;
     for (uint32_t i = 0; i < n; i++) chunks += chunks_of(entries(a)[some[i]]);
     parts += blocks_of(chunks);
@@ -278,11 +285,12 @@ uint32_t parts_of(const pots_gradients* a) {
   return parts;
 }
 
-int sums(const pots_gradients* a, double* part, uint32_t* parts, hipStream_t s) {
+template <class TABLE>
+int sums_by(const pots_gradients* a, double* part, uint32_t* parts, hipStream_t s) {
   *parts = 0;
   uint64_t left = chunks_of(a);  // from the launch's first one to the list's last
-  return each_launch<kNormed>(a, [&](const uint32_t* some, uint32_t n) {
-    Normed t = {};
+  return each_launch(a, TABLE::kMost, [&](const uint32_t* some, uint32_t n) {
+    TABLE t = {};
     for (uint32_t i = 0; i < n; i++) {
       const pots_gradient& e = entries(a)[some[i]];
       t.g[i] = e.gradient;
@@ -295,20 +303,25 @@ int sums(const pots_gradients* a, double* part, uint32_t* parts, hipStream_t s) 
     t.kept = left > kKept ? (uint32_t)std::min<uint64_t>(left - kKept, t.chunks) : 0;
     left -= t.chunks;
     const uint32_t blocks = blocks_of(t.chunks);
-    hipLaunchKernelGGL(norm_sums, dim3(blocks), dim3(256), 0, s, t, part + *parts);
+    hipLaunchKernelGGL(norm_sums<TABLE>, dim3(blocks), dim3(256), 0, s, t, part + *parts);
     POTS_HIP(hipGetLastError());
     *parts += blocks;
     return POTS_E_OK;
   });
 }
 
-template <bool STEP>
-int updates(const pots_gradients* a, const double* part, uint32_t parts, hipStream_t s) {
-  std::vector<Updated> launches;
+int sums(const pots_gradients* a, double* part, uint32_t* parts, hipStream_t s) {
+  return a->tensors <= kFewTensors ? sums_by<Normed<kFewTensors>>(a, part, parts, s)
+                                   : sums_by<Normed<kNormed>>(a, part, parts, s);
+}
+
+template <bool STEP, class TABLE>
+int updates_by(const pots_gradients* a, const double* part, uint32_t parts, hipStream_t s) {
+  std::vector<TABLE> launches;
   const bool past = chunks_of(a) > kKept;
-  (void)each_launch<kUpdated>(a, [&](const uint32_t* some, uint32_t n) {
+  (void)each_launch(a, TABLE::kMost, [&](const uint32_t* some, uint32_t n) {
     launches.emplace_back();
-    Updated& t = launches.back();
+    TABLE& t = launches.back();
     t.tensors = n;
     t.chunks = 0;
     t.past = past;
@@ -325,16 +338,22 @@ int updates(const pots_gradients* a, const double* part, uint32_t parts, hipStre
     }
     return POTS_E_OK;
   });
-  if (launches.empty()) launches.emplace_back(Updated{});  // the norm of nothing
+  if (launches.empty()) launches.emplace_back(TABLE{});  // the norm of nothing
   float* norm = a->norm;
   for (size_t i = launches.size(); i-- > 0;) {
     const uint32_t blocks = std::max(1u, blocks_of(launches[i].chunks));
-    hipLaunchKernelGGL((update<STEP>), dim3(blocks), dim3(256), 0, s, launches[i], part, parts,
+    hipLaunchKernelGGL((update<STEP, TABLE>), dim3(blocks), dim3(256), 0, s, launches[i], part, parts,
                        a->max_norm, a->eta, norm);
     POTS_HIP(hipGetLastError());
     norm = nullptr;
   }
   return POTS_E_OK;
+}
+
+template <bool STEP>
+int updates(const pots_gradients* a, const double* part, uint32_t parts, hipStream_t s) {
+  return a->tensors <= kFewTensors ? updates_by<STEP, Updated<kFewTensors>>(a, part, parts, s)
+                                   : updates_by<STEP, Updated<kUpdated>>(a, part, parts, s);
 }
 
 // Whether what is written lies apart from everything else: each out from the others, and from every

@@ -849,7 +849,7 @@ def _change(name: str, gradients: _List, weights: _List | None, out: _List | Non
     """The calls over lists; the norm."""
     first = gradients.tensors[0]
     _on_gpu(first)
-    norm = torch.empty((), dtype=torch.float32, device=first.device)
+    norm = _new_floats((), first)
     g = gradients.read()
     pointers = list(map(_POINTER, g))
     zeros = [0] * len(g)
