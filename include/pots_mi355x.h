@@ -503,7 +503,7 @@ int pots_embedding_backward(const pots_embedding *a, void *work, void *stream);
 #define POTS_OP_F64 4 /* the frequencies of pots_rotary alone */
 
 /* t = x + residual (rounded to total_type; x itself where residual is null, and total is then not
- * written); s = 1 / sqrt(mean of t^2 over the row + eps); y = t s weight. rstd receives s; the
+ * written); s = 1 / sqrt(mean of t^2 over the row + eps), eps at least 2^-126; y = t s weight. rstd receives s; the
  * rows of y and total follow each other. Up to 2^14 columns and 2^31 - 1 rows.
  * Quantized: y / scale in e4m3 or int8, to nearest (ties to even), with a scale for each `block`
  * columns (32, 64, 128 or 256; 0: the whole row): the largest size of y there over 448 or 127, at

@@ -482,8 +482,8 @@ def _norm_args(x: torch.Tensor, weight: torch.Tensor, eps: float, what: str) -> 
                          f"{tuple(x.shape)}")
     if weight.shape != x.shape[-1:] or weight.device != x.device:
         raise ValueError(f"weight must be [{x.shape[-1]}] on {x.device}")
-    if not _LEAST <= eps <= _MOST:
-        raise ValueError(f"eps must be positive and finite in fp32, got {eps}")
+    if not 2.0**-126 <= eps <= _MOST:
+        raise ValueError(f"eps must be a normal positive number of fp32, got {eps}")
     return _dtype(weight, "weight")
 
 

@@ -48,7 +48,7 @@ H, BF, I64 = torch.float16, torch.bfloat16, torch.int64
     (X, W, {"residual": _t(2, 8)}, "residual"),
     (X, W, {"residual": _t(3, 8, dtype=H)}, "float32 or bfloat16"),
     (X, W, {"eps": 0.0}, "eps"), (X, W, {"eps": -1e-6}, "eps"), (X, W, {"eps": math.nan}, "eps"),
-    (X, W, {"eps": math.inf}, "eps"), (X, W, {"eps": 1e39}, "eps"), (X, W, {}, "GPU"),
+    (X, W, {"eps": math.inf}, "eps"), (X, W, {"eps": 1e39}, "eps"), (X, W, {"eps": 1e-39}, "eps"), (X, W, {}, "GPU"),
 ])
 def test_norms_refuse(x, w, kw, message):
     for call in (ops.rms_norm_forward, ops.rms_norm_quantized, ops.rms_norm):
@@ -168,7 +168,7 @@ def _norm(**kw):
 
 
 @pytest.mark.parametrize("kw", [dict(dim=0), dict(dim=(1 << 14) + 1), dict(rows=1 << 31), dict(x=2),
-                                dict(total=2), dict(weight=4), dict(eps=0.0), dict(eps=-1.0),
+                                dict(total=2), dict(weight=4), dict(eps=0.0), dict(eps=1e-39), dict(eps=-1.0),
                                 dict(eps=math.nan), dict(eps=math.inf), {}])
 def test_norm_entry_points_refuse(abi, kw):
     """Sizes, types and numbers out of range; with none, null pointers."""
