@@ -7,7 +7,7 @@
 //
 // Bound by memory: a row is read once into registers, four consecutive values of each 256 to a lane
 // (any width of type then fills whole lines), and everything follows from there. 8192 rows of 1536, x
-// and y bf16, r and t fp32: 27 us, 5.6 TB/s; the gradient 35 and 4 for dw, 4.0. (A copy of that size
+// and y bf16, r and t fp32: 27 us, 5.6 TB/s; the gradient 34, 4.6, and 4 for dw. (A copy of that size
 // reaches 5.0; the gradient finds part of t in the last cache, so stores past it lost 5 %.) In 8 bits, where a
 // value is one to three bytes, instructions count as well: the root, the scales and the divisions by
 // them are the hardware's approximations improved once (8192 x 1536 from bf16 to e4m3 in blocks of 128:
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(R::kThreads) void norm_rows(pots_rms_norm a) {
         } else {
           b = 0;
 #pragma unroll
-          for (uint32_t j = 0; j < 4; j++)  // 1 to 255 for -127 to 127; a NaN is taken as 0
+          for (uint32_t j = 0; j < 4; j++)  // 1 to 255 for -127 to 127 (and 0, -128, for a NaN)
             b = __builtin_amdgcn_cvt_pk_u8_f32(rintf(v[j]) + 128.f, j, b);
           b ^= 0x80808080u;
         }
