@@ -18,19 +18,6 @@ namespace pots {
 template <class T>
 constexpr uint32_t kValues = 16 / sizeof(typename T::elem);
 
-// Quotients by a number that is the same for the launch, of numbers below 2^31.
-struct Divisor {
-  uint32_t by, factor, shift;
-
-  explicit Divisor(uint32_t d) : by(d), shift(0) {
-    while (shift < 31 && (1u << shift) < d) shift++;
-    factor = (uint32_t)(((1ull << (31 + shift)) + d - 1) / d);  // (2^31 for d = 1)
-  }
-  __device__ __forceinline__ uint32_t of(uint32_t n) const {
-    return (uint32_t)((uint64_t)n * factor >> 31 >> shift);
-  }
-};
-
 struct Sigma {
   float one, rest;  // σ(g) and 1 − σ(g)
 };

@@ -12,6 +12,19 @@
 
 namespace pots {
 
+// Quotients by a number that is the same for the launch, of numbers below 2^31.
+struct Divisor {
+  uint32_t by, factor, shift;
+
+  explicit Divisor(uint32_t d) : by(d), shift(0) {
+    while (shift < 31 && (1u << shift) < d) shift++;
+    factor = (uint32_t)(((1ull << (31 + shift)) + d - 1) / d);  // (2^31 for d = 1)
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t n) const {
+    return (uint32_t)((uint64_t)n * factor >> 31 >> shift);
+  }
+};
+
 // N values of a row, one lane's share.
 template <class T, uint32_t N>
 using Run = typename T::elem __attribute__((ext_vector_type(N)));
