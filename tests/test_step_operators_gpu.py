@@ -186,6 +186,28 @@ def test_norm_gradients_by_differences(rt):
         assert abs(got - want) <= off * size + 1e-6, i
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_norm_gradients_of_broadcast_inputs(dtype):
+    """One row for all of a batch, one weight for two norms, and one tensor as branch and residual."""
+    g = _gen(13)
+    rows, d = 50, 70
+    row, w = _rand(g, 1, d, dtype=dtype).requires_grad_(), _rand(g, d).requires_grad_()
+    res = _rand(g, rows, d)
+    o = [_rand(g, rows, d, dtype=dtype), _rand(g, 1, d, dtype=dtype)]
+    y, total = ops.rms_norm(row.expand(rows, d), w, residual=res)
+    z, double = ops.rms_norm(row, w, residual=row)
+    torch.autograd.backward([y, z], o)
+    first = R.norm_backward(o[0], total.detach(), w.detach(), 1e-6, None, dtype)
+    other = R.norm_backward(o[1], double.detach(), w.detach(), 1e-6, None, dtype)
+    R.within(w.grad, tuple(a + b for a, b in zip(first["dweight"], other["dweight"])), "dw")
+    # torch adds up the rows' gradients and the three shares, in fp32 or rounding each sum to the type
+    shares = [(first["dx"][0], first["dx"][1]), (2 * other["dx"][0], 2 * other["dx"][1])]
+    value = sum(v.sum(0, keepdim=True) for v, _ in shares)
+    size = sum(v.abs().sum(0, keepdim=True) for v, _ in shares)
+    bound = sum(b.sum(0, keepdim=True) for _, b in shares)
+    R.within(row.grad, (value, bound + (rows * R.E32 + 3 * R.U[dtype]) * size), "dx")
+
+
 def test_norm_gradients_where_one_output_is_unused():
     g = _gen(4)
     x, r = _rand(g, 3, 40, dtype=BF).requires_grad_(), _rand(g, 3, 40).requires_grad_()
