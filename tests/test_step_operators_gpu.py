@@ -707,6 +707,86 @@ def test_inference_tensors():
     assert bool((w == 0).all()) and bool((v == 0.5).all()) and v._version > version
 
 
+# ---- more than 2^31 values ------------------------------------------------------------------
+
+LAST = slice(-3, None)
+
+
+def _large(rows, d, seed):
+    """bf16 rows beyond 2^31 values, of which the first and last few differ from the others."""
+    t = torch.zeros(rows, d, dtype=BF, device=DEV)
+    g = _gen(seed)
+    t[:3], t[LAST] = _rand(g, 3, d, dtype=BF), _rand(g, 3, d, dtype=BF)
+    return t
+
+
+def test_large_norms():
+    rows, d = (1 << 31) // 2050 + 9, 2050
+    x, w = _large(rows, d, 1), _rand(_gen(2), d)
+    y, total, rstd = ops.rms_norm_forward(x, w, residual=x)
+    dx, _, dw = ops.rms_norm_backward(x, total, w, rstd)
+    want, sums = [], []
+    for part in (slice(0, 3), LAST):
+        n = R.norm(x[part], w, x[part], 1e-6, BF)
+        for name, t in (("y", y), ("total", total), ("rstd", rstd)):
+            R.within(t[part], n[name], name)
+        b = R.norm_backward(x[part], total[part], w, 1e-6, None, BF)
+        R.within(dx[part], b["dx"], "dx")
+        sums.append(b["dweight"])
+    assert not bool(y[3:-3].any()) and not bool(dx[3:-3].any())
+    R.within(dw, tuple(a + b for a, b in zip(*sums)), "dw")
+    del y, total, dx
+    for dtype in (E4M3, I8):
+        q, scales, _ = ops.rms_norm_quantized(x, w, dtype=dtype, block=128)
+        for part in (slice(0, 3), LAST):
+            n = R.quantized(x[part], w, None, 1e-6, dtype, 128)
+            R.within(q[part].float(), n["q"], "q")
+            R.within(scales[part], n["scales"], "scales")
+        assert bool((scales[3:-3] == 2.0**-126).all())
+
+
+@pytest.mark.parametrize("rows", [1, (1 << 31) // 2049 + 7])
+def test_large_activations(rows):
+    d = 2049 if rows > 1 else (1 << 30) - 1  # (one row is as long as it may be)
+    x = _large(max(rows, 6), d, 3) if rows > 1 else torch.zeros(1, d, dtype=BF, device=DEV)
+    if rows == 1:
+        x[0, -5:] = 1.5
+    out = ops.gated_silu_forward(x, x)
+    dg, du = ops.gated_silu_backward(x, x, x)
+    for part in ((slice(0, 3), LAST) if rows > 1 else ((0, slice(-9, None)),)):
+        want = R.gated(x[part], x[part], x[part])
+        for name, t in (("out", out), ("dgate", dg), ("dup", du)):
+            R.within(t[part], want[name], name)
+
+
+def test_large_turns():
+    b, h, n, d = 2, 9, 1 << 20, 128
+    q = torch.zeros(b, n, h, d, dtype=BF, device=DEV).transpose(1, 2)
+    g = _gen(4)
+    q[:, :, :2], q[:, :, LAST] = _rand(g, b, h, 2, d), _rand(g, b, h, 3, d)
+    f, at = R.by_frequency(d).to(DEV), torch.arange(n, device=DEV)
+    got = ops.rotary_forward(q, q[:, :1], at, f)
+    for part in (slice(0, 2), LAST):
+        for t, x in zip(got, (q, q[:, :1])):
+            want = R.rotary(x[:, :, part], at[part].expand(1, b, -1), f, (d // 2,), False, False)
+            R.within(t[:, :, part], want, "turned")
+
+
+def test_large_gradients():
+    """A tensor of more than 2^31 values in front of a small one."""
+    n = (1 << 31) + 12345
+    big, small = torch.zeros(n, dtype=BF, device=DEV), _rand(_gen(5), 1000)
+    big[:3], big[-3:] = 2.0, -4.0
+    w = torch.zeros(n, dtype=BF, device=DEV)
+    ends = torch.cat([big[:3], big[-3:]])
+    norm, bound = R.total_norm([ends, small])
+    R.within(ops.gradient_norm([big, small]), (norm, bound), "norm")
+    ops.sgd_step([w, torch.zeros_like(small)], [big, small], 0.5, max_norm=1.0)
+    want = R.changed([ends, small], 1.0, [torch.zeros_like(ends), torch.zeros_like(small)], 0.5)
+    R.within(torch.cat([w[:3], w[-3:]]), want[0], "w")
+    assert not bool(w[3:-3].any())
+
+
 # ---- streams, repetition and graphs ---------------------------------------------------------
 
 def _pass(x, w, res, dy, q, k, at, f, gate, up, grads, weights, out):
