@@ -566,7 +566,7 @@ int pots_gated_silu_backward(const pots_gated_silu *a, void *stream);
 
 /* The 2-norm of many tensors' values together, from a sum of squares in 64 bits, to norm; and with
  * factor = max_norm / norm where the norm exceeds max_norm and 1 elsewhere (a NaN norm has a NaN
- * factor): clip, out = factor * gradient in gradient_type; step, out = weight - eta * factor *
+ * factor; an infinite max_norm is no bound, and the factor is 1 whatever the norm): clip, out = factor * gradient in gradient_type; step, out = weight - eta * factor *
  * gradient in weight_type. The `tensors` entries (1 to 2^16) follow the block in memory. Values of a
  * tensor are consecutive, from where an element may start. An out may be its own gradient or
  * weight; two outs that overlap, or an out over another input or shifted over its own, are refused. */

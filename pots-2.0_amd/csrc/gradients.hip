@@ -3,6 +3,9 @@
 //
 //   norm = √Σ g²,  f = min(1, max_norm / norm),  out = f·g  or  out = w − (η f)·g
 //
+// An infinite max_norm is no bound: f is 1 whatever the norm, so that a value that is not finite stays its
+// own weight's affair.
+//
 // Bound by memory, and the gradient is read twice: the factor needs all of it first. The second pass
 // goes backwards, so that what the first read last is still in the last cache. Squares are added in
 // fp64, which no fp32 gradient leaves: 3.4e38² is 1e77, and the smallest one's square 2e-90.
@@ -204,7 +207,8 @@ __global__ __launch_bounds__(256) void update(TABLE args, const double* __restri
   table_to_lds(args, t);
   const double n = norm_of(part, parts, s_sum);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-  const double factor = n <= (double)max_norm ? 1. : (double)max_norm / n;
+  const double factor =
+      n <= (double)max_norm || max_norm == INFINITY ? 1. : (double)max_norm / n;
   const float f = (float)(STEP ? -(double)eta * factor : factor);
   if (blockIdx.x >= t.chunks) return;
   const uint32_t last = (t.chunks - 1 - blockIdx.x) / gridDim.x * gridDim.x + blockIdx.x;

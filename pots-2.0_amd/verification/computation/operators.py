@@ -887,8 +887,8 @@ def clip_gradients(gradients: Sequence[torch.Tensor], max_norm: float, *,
                    out: Sequence[torch.Tensor] | None = None) -> torch.Tensor:
     """Scale ``gradients`` by ``min(1, max_norm / norm)``, in place or into ``out``; returns their
     :func:`gradient_norm`. A norm that is NaN makes every value NaN, and an infinite one zero but
-    for the infinities (NaN). What is written must be contiguous, and overlap nothing but the
-    gradient that it replaces."""
+    for the infinities (NaN); with an infinite ``max_norm`` nothing is scaled, whatever the norm. What
+    is written must be contiguous, and overlap nothing but the gradient that it replaces."""
     g = _List(gradients, "gradients")
     return _change("clip_gradients", g, None, _written(out, g), _max_norm(max_norm), 0.0)
 
@@ -899,7 +899,8 @@ def sgd_step(weights: Sequence[torch.Tensor], gradients: Sequence[torch.Tensor],
     """``W ← W − eta · min(1, max_norm / norm) · G`` over a model's weights and their gradients, in
     place or into ``out``, the gradients left as they are; returns their :func:`gradient_norm`.
     Weights and gradients are fp32 or bf16 each; the update is one fp32 multiplication and addition,
-    rounded once. Norms that are not finite and what is written: :func:`clip_gradients`."""
+    rounded once. Without a bound (``max_norm`` infinite) it is ``W − eta · G`` value by value; norms that
+    are not finite otherwise, and what is written: :func:`clip_gradients`."""
     g, w = _List(gradients, "gradients"), _List(weights, "weights")
     w.like(g, types=False)
     if not -_MOST <= eta <= _MOST:

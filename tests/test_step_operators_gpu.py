@@ -628,6 +628,32 @@ def test_norms_that_are_not_finite():
     assert bool(w.isnan().all())
 
 
+@pytest.mark.parametrize("types", [(F32, F32), (BF, F32), (BF, BF)])
+def test_without_a_bound_values_are_their_own(types):
+    """No clip: what is not finite in one gradient is in its own weight alone, in place or not."""
+    for bad in (math.nan, math.inf, -math.inf):
+        g = [torch.tensor([1.0, bad, -2.0], device=DEV).to(types[0]),
+             torch.ones(5000, device=DEV, dtype=types[0])]
+        w = [torch.full(t.shape, 3.0, device=DEV, dtype=types[1]) for t in g]
+        want = [a.double() - 0.5 * b.double() for a, b in zip(w, g)]  # exact where it is finite
+        out = [torch.empty_like(t) for t in w]
+        norms = [ops.sgd_step(w, g, 0.5, out=out), ops.sgd_step(w, g, 0.5, max_norm=1e39),
+                 ops.clip_gradients(g, math.inf), ops.gradient_norm(g)]
+        for to in (out, w):
+            assert all(torch.equal(a.double().nan_to_num(7e9, 8e9, 9e9), b.nan_to_num(7e9, 8e9, 9e9))
+                       for a, b in zip(to, want))
+        for n in norms:
+            assert math.isnan(float(n)) if math.isnan(bad) else float(n) == math.inf
+        assert bool((g[1] == 1).all()) and g[0][::2].tolist() == [1.0, -2.0]
+        assert g[0][1].isnan() if math.isnan(bad) else float(g[0][1]) == bad
+        # with a bound, however large, the norm's factor is everyone's
+        ops.sgd_step(w, g, 0.5, max_norm=3e38, out=out)
+        if math.isnan(bad):
+            assert all(bool(t.isnan().all()) for t in out)
+        else:
+            assert torch.equal(out[1], w[1]) and out[0][1].isnan()
+
+
 def test_gradients_of_nothing():
     empty = torch.zeros(0, 3, device=DEV)
     assert float(ops.gradient_norm([empty])) == 0.0
