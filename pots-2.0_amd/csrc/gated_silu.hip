@@ -1,7 +1,7 @@
 // The gated activation of a decoder's MLP, with its gradient.
 //
 //   out = silu(g)·u,  silu(g) = g·σ(g),  σ(g) = 1 / (1 + e^−g)
-//   dg = dout·u·σ(g)(1 + g·(1 − σ(g))),  du = dout·silu(g)
+//   dg = dout·u·(σ(g) + g·(1 − σ(g))·σ(g)),  du = dout·silu(g)
 //
 // Bound by memory: three tensors forward, five backward, each once, 16 bytes a lane (8192 x 8960 in bf16
 // 75 us and 106, 5.9 and 6.9 TB/s). The arithmetic is fp32, rounded once. σ and 1 − σ come from e^−|g|,
@@ -60,7 +60,8 @@ __global__ __launch_bounds__(256) void gated(pots_gated_silu a, Divisor runs, ui
     const Sigma s = sigma(x);
     if (GRAD) {
       const float dy = T::get(d[0][j]);
-      y[j] = dy * v * (s.one * fmaf(x, s.rest, 1.f));
+      // (one rounding fewer than σ(1 + g(1 − σ)) has: of normal values the error is 6.4e-8 of dg's size, so 6.9)
+      y[j] = dy * v * fmaf(x * s.rest, s.one, s.one);
       z[j] = dy * (x * s.one);
     } else {
       y[j] = x * s.one * v;

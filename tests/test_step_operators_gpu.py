@@ -490,6 +490,22 @@ def test_gated_of_nothing_and_rows_past_32_bits():
     _gated_check(gate, up, dout)
 
 
+def test_gated_gradients_round_no_more_than_their_formula():
+    """By their RMS, counted in roundings of 2^-24 · 0.425 each (half a step at most, mantissas as they
+    come). d gate is the product of dout and up, the sum of sigma and its product with g(1 - sigma), and the
+    product of those two: three roundings. A rounding of 1 + e^-|g| or of its reciprocal is in sigma and in
+    1 - sigma and so counts up to one and a half times, or up to 2.25 in the square: 3.4 for both, since most count
+    less. The exponential's counts where it is not small: half a rounding. 6.9 in all."""
+    n, g = 1 << 20, torch.Generator(device=DEV).manual_seed(21)
+    gate, up = (1.5 * torch.randn(n, generator=g, device=DEV) for _ in range(2))
+    dout = torch.randn(n, generator=g, device=DEV)
+    dgate, _ = ops.gated_silu_backward(dout, gate, up)
+    x, v, dy = gate.double(), up.double(), dout.double()
+    want = dy * v * torch.sigmoid(x) * (1 + x * torch.sigmoid(-x))
+    off = float((dgate.double() - want).norm() / want.norm())
+    assert off <= 0.425 * R.E32 * math.sqrt(6.9), off
+
+
 def test_gated_gradients():
     g = _gen(12)
     leaves = [_rand(g, 4, 13).requires_grad_(), _rand(g, 1, 13).requires_grad_()]
