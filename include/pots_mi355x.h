@@ -553,7 +553,7 @@ typedef struct pots_rotary {
 int pots_rotary_turn(const pots_rotary *a, void *stream);
 
 /* out = silu(gate) * up, silu(g) = g / (1 + e^-g); backward: dgate and dup of it. The rows of out,
- * dgate and dup follow each other. rows * columns is at most 2^40. */
+ * dgate and dup follow each other. rows * columns is at most 2^40; any count of columns. */
 typedef struct pots_gated_silu {
   const void *gate, *up, *dout;
   void *out, *dgate, *dup;

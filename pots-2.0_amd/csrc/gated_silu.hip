@@ -75,9 +75,11 @@ __global__ __launch_bounds__(256) void gated(pots_gated_silu a, Divisor runs, ui
 namespace {
 
 bool bad(const pots_gated_silu* a) {
-  return !a || a->dtype > POTS_OP_BF16 || a->columns > 1u << 30 ||
-         (uint64_t)a->rows * a->columns > 1ull << 40;
+  return !a || a->dtype > POTS_OP_BF16 || (uint64_t)a->rows * a->columns > 1ull << 40;
 }
+
+// Values of a launch, at the most: below 2^32 threads, and 32 bits hold a column.
+constexpr uint32_t kLaunch = 1u << 30;
 
 template <class T, bool GRAD>
 int run(const pots_gated_silu* call, hipStream_t s) {
@@ -85,32 +87,35 @@ int run(const pots_gated_silu* call, hipStream_t s) {
   pots_gated_silu a = *call;
   // Rows that follow each other everywhere are one row, as long as it is one.
   const int64_t c = a.columns;
-  if ((uint64_t)a.rows * a.columns <= 1u << 30 && a.gate_row == c && a.up_row == c &&
+  if ((uint64_t)a.rows * a.columns <= kLaunch && a.gate_row == c && a.up_row == c &&
       (!GRAD || a.dout_row == c)) {
     a.columns *= a.rows;
     a.rows = 1;
   }
-  const uint32_t per = (a.columns + kValues<T> - 1) / kValues<T>;
-  const uint32_t most = (1u << 30) / per;  // rows of a launch
   const uint64_t bytes = (uint64_t)a.rows * a.columns * sizeof(elem) * (GRAD ? 5 : 3);
   const auto kernel = bytes > kCache ? gated<T, GRAD, true> : gated<T, GRAD, false>;
+  // Some rows a launch, or of longer rows a piece of one.
+  const uint32_t wide = a.columns < kLaunch ? a.columns : kLaunch;
+  const uint32_t most = a.columns > kLaunch ? 1 : kLaunch / ((wide + kValues<T> - 1) / kValues<T>);
   for (uint64_t r0 = 0; r0 < a.rows; r0 += most) {
-    pots_gated_silu part = a;
-    part.rows = (uint32_t)(a.rows - r0 < most ? a.rows - r0 : most);
-    part.gate = reinterpret_cast<const elem*>(a.gate) + (int64_t)r0 * a.gate_row;
-    part.up = reinterpret_cast<const elem*>(a.up) + (int64_t)r0 * a.up_row;
-    const int64_t at = (int64_t)r0 * a.columns;
-    if (GRAD) {
-      part.dout = reinterpret_cast<const elem*>(a.dout) + (int64_t)r0 * a.dout_row;
-      part.dgate = reinterpret_cast<elem*>(a.dgate) + at;
-      part.dup = reinterpret_cast<elem*>(a.dup) + at;
-    } else {
-      part.out = reinterpret_cast<elem*>(a.out) + at;
+    for (uint64_t c0 = 0; c0 < a.columns; c0 += wide) {
+      pots_gated_silu part = a;
+      part.rows = (uint32_t)(a.rows - r0 < most ? a.rows - r0 : most);
+      part.columns = (uint32_t)(a.columns - c0 < wide ? a.columns - c0 : wide);
+      part.gate = reinterpret_cast<const elem*>(a.gate) + (int64_t)r0 * a.gate_row + c0;
+      part.up = reinterpret_cast<const elem*>(a.up) + (int64_t)r0 * a.up_row + c0;
+      const uint64_t at = r0 * a.columns + c0;
+      if (GRAD) {
+        part.dout = reinterpret_cast<const elem*>(a.dout) + (int64_t)r0 * a.dout_row + c0;
+        part.dgate = reinterpret_cast<elem*>(a.dgate) + at;
+        part.dup = reinterpret_cast<elem*>(a.dup) + at;
+      } else {
+        part.out = reinterpret_cast<elem*>(a.out) + at;
+      }
+      const uint32_t per = (part.columns + kValues<T> - 1) / kValues<T>, all = part.rows * per;
+      hipLaunchKernelGGL(kernel, dim3((all + 255) / 256), dim3(256), 0, s, part, Divisor(per), all);
+      POTS_HIP(hipGetLastError());
     }
-    const uint32_t all = part.rows * per;
-    hipLaunchKernelGGL(kernel, dim3((all + 255) / 256), dim3(256), 0, s, part, Divisor(per),
-                       all);
-    POTS_HIP(hipGetLastError());
   }
   return POTS_E_OK;
 }

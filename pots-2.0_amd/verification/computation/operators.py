@@ -749,7 +749,8 @@ def _gated_args(gate: torch.Tensor, up: torch.Tensor) -> int:
 
 def gated_silu_forward(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     """``silu(gate) · up``, ``silu(g) = g / (1 + e^−g)``, of two tensors ``[..., columns]`` of one
-    shape and type, each anywhere (the halves of one product, for instance)."""
+    shape and type, each anywhere (the halves of one product, for instance): up to 2^32 − 1 rows
+    of up to 2^32 − 1 values, and 2^40 values in all."""
     code = _gated_args(gate, up)
     _on_gpu(gate)
     out = _new_like(gate, gate.dtype)

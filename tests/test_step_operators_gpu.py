@@ -506,6 +506,25 @@ def test_gated_gradients_round_no_more_than_their_formula():
     assert off <= 0.425 * R.E32 * math.sqrt(6.9), off
 
 
+def test_gated_rows_of_more_than_2_30_values():
+    """One tensor without rows, as long as it likes, and rows of such a length."""
+    n = (1 << 30) + 11
+    x = torch.zeros(2, n, dtype=BF, device=DEV)
+    for at in ((1 << 30) - 5, n - 3):  # on both sides of 2^30, and at the end
+        x[:, at:at + 8] = _rand(_gen(at % 7), 2, min(8, n - at), dtype=BF)
+    ends = [slice((1 << 30) - 9, (1 << 30) + 8), slice(n - 5, n), slice(0, 9)]
+    for t in (x[1], x):
+        up = t.flip(0) if t.dim() == 2 else t
+        out = ops.gated_silu_forward(t, up)
+        dg, du = ops.gated_silu_backward(up, t, up)
+        for part in ends:
+            want = R.gated(t[..., part], up[..., part], up[..., part])
+            for name, got in (("out", out), ("dgate", dg), ("dup", du)):
+                R.within(got[..., part], want[name], name)
+        assert int(out.count_nonzero()) == sum(int(out[..., p].count_nonzero()) for p in ends[:2])
+        del out, dg, du
+
+
 def test_gated_gradients():
     g = _gen(12)
     leaves = [_rand(g, 4, 13).requires_grad_(), _rand(g, 1, 13).requires_grad_()]

@@ -319,3 +319,17 @@ def test_updates_in_place_and_shifted(driver):  # noqa: F811
     for name in ("clip_gradients", "sgd_step"):
         good, bad = _launches(driver, f"{name},5,100,1,0", f"{name},5,100,1,4")
         assert good[0] == 0 and good[2] and bad[0] == E_ARG and not bad[2]
+
+
+@pytest.mark.parametrize("rows, columns, apart", [(1, (1 << 30) + 1, 0), (1, (1 << 32) - 1, 0), (2, (1 << 30) + 1, 0),
+                                                  (3, (1 << 31) + 5, 1), (256, (1 << 32) - 1, 1)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_activations_of_rows_past_a_launch(driver, rows, columns, apart, dtype):  # noqa: F811
+    """Rows of more than 2^30 values are taken in pieces: each value once."""
+    for way in ("forward", "backward"):
+        (rc, _, launches), = _launches(driver, f"gated_silu_{way},{rows},{columns},{dtype},{apart}")
+        per = 8 if dtype == BF16 else 4
+        threads = sum(x * t for _, x, t in launches)
+        least = rows * -(-columns // per)
+        assert rc == 0 and len(launches) == rows * -(-columns >> 30)
+        assert least <= threads < least + 256 * len(launches)
