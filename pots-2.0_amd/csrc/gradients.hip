@@ -278,15 +278,19 @@ int each_launch(const pots_gradients* a, uint32_t most, F&& f) {
 
 uint32_t blocks_of(uint64_t chunks) { return (uint32_t)std::min<uint64_t>(chunks, kBlocks); }
 
+// The sums that the launches of each_launch leave, counted without a list, which could find no memory.
 uint32_t parts_of(const pots_gradients* a) {
-  uint32_t parts = 0;
-  (void)each_launch(a, kNormed, [&](const uint32_t* some, uint32_t n) {
-    uint64_t chunks = 0;
-    for (uint32_t i = 0; i < n; i++) chunks += chunks_of(entries(a)[some[i]]);
-    parts += blocks_of(chunks);
-    return POTS_E_OK;
-  });
-  return parts;
+  uint32_t parts = 0, n = 0;
+  uint64_t chunks = 0;
+  for (uint32_t i = 0; i < a->tensors; i++) {
+    if (!entries(a)[i].count) continue;
+    chunks += chunks_of(entries(a)[i]);
+    if (++n % kNormed == 0) {
+      parts += blocks_of(chunks);
+      chunks = 0;
+    }
+  }
+  return parts + blocks_of(chunks);
 }
 
 template <class TABLE>
@@ -422,22 +426,23 @@ int change(const pots_gradients* a, void* work, void* stream) {
 
 using namespace pots;
 
-// (the lists that the entry points make may find no memory)
-template <class R, class F>
-static R guarded(R failed, F&& f) noexcept {
+// The lists that a call makes may find no memory; it says so in a text short enough to need none.
+template <class F>
+static int guarded(F&& f) noexcept {
   try {
     return f();
   } catch (...) {
-    return failed;
+    note_error("out of memory");
+    return POTS_E_NOMEM;
   }
 }
 
 extern "C" uint64_t pots_gradient_norm_work(const pots_gradients* a) {
-  return guarded<uint64_t>(0, [&] { return bad(a, false, false) ? 0 : 8ull * parts_of(a); });
+  return bad(a, false, false) ? 0 : 8ull * parts_of(a);
 }
 
 extern "C" int pots_gradient_norm(const pots_gradients* a, void* work, void* stream) {
-  return guarded<int>(POTS_E_NOMEM, [&] {
+  return guarded([&] {
     if (bad(a, false, false) || missing(a, false, false)) return POTS_E_ARG;
     if (parts_of(a) && !work) return POTS_E_ARG;
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -456,11 +461,11 @@ extern "C" uint64_t pots_clip_gradients_work(const pots_gradients* a) {
 }
 
 extern "C" int pots_clip_gradients(const pots_gradients* a, void* work, void* stream) {
-  return guarded<int>(POTS_E_NOMEM, [&] { return change<false>(a, work, stream); });
+  return guarded([&] { return change<false>(a, work, stream); });
 }
 
 extern "C" uint64_t pots_sgd_step_work(const pots_gradients* a) { return pots_gradient_norm_work(a); }
 
 extern "C" int pots_sgd_step(const pots_gradients* a, void* work, void* stream) {
-  return guarded<int>(POTS_E_NOMEM, [&] { return change<true>(a, work, stream); });
+  return guarded([&] { return change<true>(a, work, stream); });
 }

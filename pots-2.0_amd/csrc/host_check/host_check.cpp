@@ -17,8 +17,13 @@
 //                             case is a name and its sizes, joined by commas:
 //                             attention_{forward,backward},BATCH,HEADS,KV_HEADS,N,HEAD_DIM,DTYPE;
 //                             vocab_loss_{forward,backward},ROWS,DIM,VOCAB,DTYPE;
-//                             embedding_{forward,backward},TOKENS,DIM,VOCAB,DTYPE,ADD. Each
-//                             gives a line "= CASE" with its return code and its scratch, after the
+//                             embedding_{forward,backward},TOKENS,DIM,VOCAB,DTYPE,ADD;
+//                             rms_norm_{forward,quantized,backward},ROWS,DIM,BLOCK and the types of
+//                             x, the sum, the weight and y;
+//                             rotary_turn,BATCH,HEADS,KV_HEADS,N,HEAD_DIM,PAIRS,DTYPE;
+//                             gated_silu_{forward,backward},ROWS,COLUMNS,DTYPE,APART;
+//                             {gradient_norm,clip_gradients,sgd_step},TENSORS,VALUES,IN_PLACE,SHIFT.
+//                             Each gives a line "= CASE" with its return code and its scratch, after the
 //                             launches' lines: the kernel, its blocks and a block's threads.
 //
 // Exit status 0 when every result is as expected; the sanitizers abort on any finding.

@@ -10,7 +10,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from test_host_sanitize import driver  # noqa: F401  (a fixture)
+from test_host_sanitize import _run, driver  # noqa: F401  (a fixture)
 from test_operator_launches import _launches
 from verification.computation import operators as ops
 
@@ -319,6 +319,21 @@ def test_updates_in_place_and_shifted(driver):  # noqa: F811
     for name in ("clip_gradients", "sgd_step"):
         good, bad = _launches(driver, f"{name},5,100,1,0", f"{name},5,100,1,4")
         assert good[0] == 0 and good[2] and bad[0] == E_ARG and not bad[2]
+
+
+def test_lists_that_find_no_memory_say_so(driver):  # noqa: F811
+    """Each allocation of a call fails in turn: an error and its own text, not an earlier call's; and the
+    scratch's size is answered all the same."""
+    e_nomem = -1
+    seen = {}
+    for line in _run(driver.with_name("nomem")).splitlines():
+        name, rc, work, text = line.split(" ", 3)
+        seen.setdefault(name, []).append((int(rc), int(work), text.strip()))
+    assert seen.keys() == {"gradient_norm", "clip_gradients", "sgd_step"}
+    for name, calls in seen.items():
+        assert calls[-1][0] == 0 and len(calls) > 1, name
+        assert all(c[0] == e_nomem and c[2] == "out of memory" for c in calls[:-1]), (name, calls)
+        assert {c[1] for c in calls} == {8 * 200}, name  # 200 chunks, a sum a block
 
 
 @pytest.mark.parametrize("rows, columns, apart", [(1, (1 << 30) + 1, 0), (1, (1 << 32) - 1, 0), (2, (1 << 30) + 1, 0),
