@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+import step_operators_oracle as O
 from test_uncaptured_gpu import _grads, _step
 from verification.computation import operators
 from verification.computation.interface import load_weights, snapshot_weights
@@ -64,6 +65,44 @@ def test_a_step(dtype, bound, clipped):
         load_weights(c, model, w_t)
         proved = prove_step(c, model, w_t, records)
         assert abs(proved.loss - float(loss)) <= bound * abs(proved.loss)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("clipped", [False, True])
+def test_the_update_of_a_step(dtype, clipped):
+    """Each weight is the one before less its own gradient of the fused pass, which gives the same bits
+    again, by the factor and eta, within the roundings of that one formula."""
+    c, model, records = _step(True, True, dtype)
+    before = [p.detach().clone() for p in model.parameters()]
+    loss = c.uncaptured_loss(model, records, fused=True)
+    loss.backward()
+    grads = [p.grad.clone() for p in model.parameters()]
+    norm = float(O.total_norm(grads)[0])
+    max_norm = norm / 3 if clipped else math.inf
+    got, got_norm = uncaptured_step(c, model, records, max_norm=max_norm)
+    assert torch.equal(got, loss.detach())
+    O.within(got_norm, O.total_norm(grads), "norm")
+    names = [n for n, _ in model.named_parameters()]
+    for name, p, want in zip(names, model.parameters(), O.changed(grads, max_norm, before, c.eta)):
+        O.within(p.detach(), want, name)
+
+
+@pytest.mark.parametrize("tied, bias", [(True, True), (False, False)])
+def test_fused_gradients_in_bf16_are_as_near_as_the_captured_step_s(tied, bias):
+    """Against fp32, tensor by tensor: both passes round like tensors to bf16, the fused one fewer of them, so
+    that each's error is a sum of like many independent roundings; three times the other's allows
+    for their chance, and one rounding for a gradient that the other has by luck. A term that is missing, or has
+    the wrong sign, is as large as the gradient, a hundred times that."""
+    single, model, records = _step(tied, bias, torch.float32)
+    exact = _grads(model, single.loss(model, records))
+    weights = dict(model.named_parameters())
+    c, model, records = _step(tied, bias, torch.bfloat16)
+    assert all(torch.equal(p, weights[n]) for n, p in model.named_parameters())
+    captured = _grads(model, c.loss(model, records))
+    fused = _grads(model, c.uncaptured_loss(model, records, fused=True))
+    for name, g in exact.items():
+        off, other = float((fused[name] - g).norm()), float((captured[name] - g).norm())
+        assert off <= 3 * other + 2.0**-8 * float(g.norm()), (name, off, other, float(g.norm()))
 
 
 def test_steps_are_deterministic():
