@@ -355,10 +355,14 @@ class DecoderComputation(DeclaredComputation):
         """The model's features ``F`` from its embedded tokens ``[n_s, n, d]``: each layer's linear
         modules called as they are, and between them operators. The residual stream keeps the
         rows' type (the masters' fp32); norms read the branch in the products' type and write what
-        the next products read. Layers that are checkpointed, an activation other than silu, a
-        sliding window and frequencies that a call would rescale are refused."""
+        the next products read. Layers other than :meth:`build_model`'s (Llama's and Qwen2's), layers that are
+        checkpointed, an activation other than silu, a sliding window and frequencies that a call would rescale
+        are refused."""
         from verification.computation import operators
         body, cfg = model.model, model.config
+        if cfg.model_type not in ("llama", "qwen2"):
+            # (others norm their heads or scale their branches, in modules of the same names)
+            raise ValueError(f"the layers of {cfg.model_type!r} are not fused, only llama's and qwen2's")
         rope = body.rotary_emb
         if getattr(body, "gradient_checkpointing", False) and body.training:
             raise ValueError("fused layers are not checkpointed")

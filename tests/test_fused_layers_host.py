@@ -95,3 +95,19 @@ def test_what_fused_layers_refuse():
     from verification.computation.instances.mlp import MLPComputation
     with pytest.raises(ValueError, match="no uncaptured pass"):
         uncaptured_step(MLPComputation([4, 4], n_s=2, eta=0.1), model, records)
+
+
+@pytest.mark.parametrize("kind", ["qwen3", "granite", "mistral"])
+def test_layers_of_other_models_are_refused(kind):
+    """Their modules have the same names and do more between them: heads' norms, branches that are scaled."""
+    import transformers
+    from verification.computation.instances.attention import register
+    c, _, records = _step(False)
+    cfg = transformers.CONFIG_MAPPING[kind](
+        vocab_size=c.n_v, hidden_size=c.d, intermediate_size=c.d_f, num_hidden_layers=c.L,
+        num_attention_heads=c.n_h, num_key_value_heads=c.n_kv, head_dim=c.d_h, hidden_act="silu",
+        max_position_embeddings=64)
+    cfg._attn_implementation = register()
+    model = transformers.AutoModelForCausalLM.from_config(cfg).eval()
+    with pytest.raises(ValueError, match=kind):
+        c.uncaptured_loss(model, records, fused=True)
