@@ -508,7 +508,8 @@ int pots_embedding_backward(const pots_embedding *a, void *work, void *stream);
  * Quantized: y / scale in e4m3 or int8, to nearest (ties to even), with a scale for each `block`
  * columns (32, 64, 128 or 256; 0: the whole row): the largest size of y there over 448 or 127, at
  * least 2^-126. Where y holds a NaN the block's scale is NaN; where it holds an infinity the scale is
- * infinite.
+ * infinite, and what is finite in the block 0. y / scale is NaN of the whole block with a NaN scale and of the infinities: a
+ * NaN in e4m3, -128 in int8, whose numbers else are -127 to 127.
  * Backward, h = t s and g = dy weight: dt = dtotal + s (g - h mean(g h)), to dresidual in
  * total_type and to dx in x_type (each may be null, and so may dtotal), their rows following each
  * other; dweight (may be null) is the rows' sum of dy h, in weight_type. x, residual and y are not

@@ -545,7 +545,9 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e
     t)`` with ``y ≈ q · scale``, rounded to nearest from fp32. A scale (fp32 ``[..., blocks]``) is
     the largest size of a row (``block`` None), or of each ``block`` columns (32, 64, 128 or 256;
     the last may be fewer), over 448 or 127, and at least 2^-126. A block that holds a NaN has the
-    scale NaN; one that holds an infinity an infinite scale."""
+    scale NaN, and one that holds an infinity an infinite scale: there what is finite is 0. A ``y / scale``
+    that is NaN (all of the first, the infinities of the second) is NaN in e4m3 and −128 in int8, whose
+    numbers else are −127 to 127."""
     _norm_args(x, weight, eps, "x")
     _summands(x, residual)
     if dtype not in _EIGHT_BITS:

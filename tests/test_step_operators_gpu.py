@@ -279,6 +279,26 @@ def test_quantized_special_blocks(dtype, block):
     R.within(q.float(), R.quantized(x[1:], w, None, 1e-6, dtype, block)["q"], "q")
 
 
+@pytest.mark.parametrize("dtype", [E4M3, I8])
+def test_quantized_numbers_that_are_none(dtype):
+    """Where y / scale is NaN, the type's NaN or -128; int8 has that number for nothing else."""
+    x, w = _rand(_gen(14), 5, 96), torch.ones(96, device=DEV)
+
+    def none(q):
+        return q.float().isnan() if dtype == E4M3 else q == -128
+
+    q, _, _ = ops.rms_norm_quantized(x, w, dtype=dtype, block=32)
+    assert not bool(none(q).any())
+    for bad in (math.nan, math.inf, -math.inf):
+        w[40] = bad
+        q, _, _ = ops.rms_norm_quantized(x, w, dtype=dtype, block=32)
+        want = torch.zeros(96, dtype=torch.bool, device=DEV)
+        want[slice(32, 64) if math.isnan(bad) else 40] = True
+        assert torch.equal(none(q), want.expand(5, 96))
+        if not math.isnan(bad):
+            assert bool((q[:, 32:64].float()[:, torch.arange(32) != 8] == 0).all())
+
+
 # ---- rotary positions -----------------------------------------------------------------------
 
 def _rotary_check(q, k, positions, f, **kw):
