@@ -7,12 +7,13 @@
 //
 // Bound by memory: a row is read once into registers, four consecutive values of each 256 to a lane
 // (any width of type then fills whole lines), and everything follows from there. 8192 rows of 1536, x
-// and y bf16, r and t fp32: 27 us, 5.6 TB/s; the gradient 34, 4.6, and 4 for dw. (A copy of that size
-// reaches 5.0; the gradient finds part of t in the last cache, so stores past it lost 5 %.) In 8 bits, where a
-// value is one to three bytes, instructions count as well: the root, the scales and the divisions by
-// them are the hardware's approximations improved once (8192 x 1536 from bf16 to e4m3 in blocks of 128:
-// 17 us, with exact ones 20). Sums, the norm and y before its rounding are fp32; t is rounded to the
-// residual's type first, since the next layer reads that t, and so does the gradient.
+// and y bf16, r and t fp32: 27 us, 5.6 TB/s; the gradient 34, 5.9 of the 201 MB that it moves, and 4 for dw. (A
+// copy of that size reaches 5.0; the gradient finds part of t in the last cache, so stores past it lost 5 %.) In
+// 8 bits, where a value is one to three bytes, instructions bound it instead: 45 a value, which keep the vector units busy
+// for 0.65 of the launch (8192 x 1536 from bf16 to e4m3 in blocks of 128: 17 us, where the bytes take 7.6). The root, the
+// scales and the divisions by them are therefore the hardware's approximations improved once (with exact ones 20 us).
+// Sums, the norm and y before its rounding are fp32; t is rounded to the residual's type first, since the next layer reads
+// that t, and so does the gradient.
 //
 // dw: every wave adds up its own rows in registers, a block's waves join in LDS, and norm_join adds
 // the blocks' sums in their order, so that no atomics are needed.
@@ -47,7 +48,8 @@ __device__ __forceinline__ float sum_lanes(float v) {
   return v;
 }
 
-// 1 / √x of a normal number: the hardware's, off by a step at most, improved once. 0 of infinity.
+// 1 / √x of a normal number: the hardware's, off by a step at most, improved once; off by three quarters of a step
+// then, in rstd and y of every type. 0 of infinity.
 __device__ __forceinline__ float inverse_root(float x) {
   const float y = __builtin_amdgcn_rsqf(x);
   return x < INFINITY ? fmaf(0.5f * y, fmaf(-x * y, y, 1.f), y) : y;

@@ -4,7 +4,8 @@
 //
 // The gradient is the turn by −θ. Bound by memory: q and k are read and written once, in one
 // launch. θ is taken in whole turns and their fraction in 64 bits, so that far positions lose
-// nothing (below 2^-45 of a turn up to position 2^20); the sine and cosine of the fraction, less than
+// nothing that fp32 would hold (frequency / 2π is off by 2^-53 and 2^-54 of its size, so θ by at most 2^-35 of a turn
+// up to position 2^20 at frequencies up to 1); the sine and cosine of the fraction, less than
 // an eighth of a turn, are fp32. A block computes them for a few tokens into LDS, once for all heads; its
 // lanes then go over the tokens' heads, 16 bytes of u and 16 of v at a time, the first of them on their
 // way meanwhile (those 8192 tokens in bf16 12.4 us a call, 4.7 TB/s; with angles of each lane's own and no

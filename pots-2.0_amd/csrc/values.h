@@ -12,7 +12,8 @@
 
 namespace pots {
 
-// Quotients by a number that is the same for the launch, of numbers below 2^31.
+// Quotients by a number that is the same for the launch, of numbers below 2^31: a multiplication by its reciprocal rounded
+// up and a shift (Granlund and Montgomery, 1994).
 struct Divisor {
   uint32_t by, factor, shift;
 

@@ -523,7 +523,7 @@ def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6
     ``s = 1/√(mean t² + eps)``: ``(y, t, s)``. Each tensor has its own type, fp32 or bf16: ``t``
     the residual's (rounded to it once, and that is what is normed), ``y`` ``out_dtype``
     (``x``'s unless given), ``s`` fp32 ``[...]``. Without a residual ``t`` is ``x`` itself. Squares
-    are added in fp32: rows of sizes above 1e18 overflow."""
+    are added in fp32: a row whose 2-norm is 1.8e19 or more has an infinite sum, and comes out as zeros."""
     _norm_args(x, weight, eps, "x")
     _summands(x, residual)
     out_dtype = x.dtype if out_dtype is None else out_dtype
