@@ -572,6 +572,13 @@ def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, weight: torch.Tenso
     residual have the same gradient: ``dresidual`` in ``t``'s type, ``dx`` in ``x_dtype`` (``t``'s
     unless given; the same tensor where they are one type). ``dweight`` is summed in fp32 over all
     rows, in ``weight``'s type."""
+    return _norm_backward(dy, total, weight, rstd, dtotal, x_dtype, True)
+
+
+def _norm_backward(dy: torch.Tensor, total: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
+                   dtotal: torch.Tensor | None, x_dtype: torch.dtype | None, of_weight: bool
+                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """:func:`rms_norm_backward`, without ``dweight`` (None) unless ``of_weight``."""
     code = _norm_args(total, weight, 1.0, "total")
     _dtype(total, "total")
     if dy.shape != total.shape or dy.device != total.device:
@@ -587,7 +594,7 @@ def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, weight: torch.Tenso
     dresidual = dx = _new_like(total, total.dtype)
     if x_dtype != total.dtype:
         dx = _new_like(total, x_dtype)
-    dweight = _new_like(weight, weight.dtype)
+    dweight = _new_like(weight, weight.dtype) if of_weight else None
     (g, g_row), (t, t_row), own = _rows(dy), _rows(total), weight.contiguous()
     other, other_ptr, other_row = None, 0, 0
     if dtotal is not None:
@@ -596,7 +603,7 @@ def rms_norm_backward(dy: torch.Tensor, total: torch.Tensor, weight: torch.Tenso
     dim = total.shape[-1]
     args = _packed(_NORM, 0, 0, own.data_ptr(), t.data_ptr(), 0, rstd.data_ptr(), 0, g.data_ptr(),
                    other_ptr, 0 if dx is dresidual else dx.data_ptr(), dresidual.data_ptr(),
-                   dweight.data_ptr(), 0, 0, t_row, g_row, other_row, total.numel() // dim, dim, 0,
+                   0 if dweight is None else dweight.data_ptr(), 0, 0, t_row, g_row, other_row, total.numel() // dim, dim, 0,
                    _DTYPES[x_dtype], _DTYPES[total.dtype], code, dy_type, 1.0)
     native.get().operator("rms_norm_backward", args, total.device)
     return dx, dresidual, dweight
@@ -620,8 +627,8 @@ class _RmsNorm(torch.autograd.Function):
             return None, None, None, None, None
         if dy is None:  # nobody read the norm
             return dtotal.to(ctx.x_dtype), None, dtotal, None, None
-        dx, dresidual, dweight = rms_norm_backward(dy, total, weight, rstd, dtotal=dtotal,
-                                                   x_dtype=ctx.x_dtype)
+        dx, dresidual, dweight = _norm_backward(dy, total, weight, rstd, dtotal, ctx.x_dtype,
+                                                ctx.needs_input_grad[1])
         return dx, dweight, dresidual if ctx.added else None, None, None
 
 

@@ -222,6 +222,37 @@ def test_norm_gradients_where_one_output_is_unused():
     R.within(dr, R.norm_backward(o.to(BF), total.detach(), w.detach(), 1e-6, None, F32)["dx"], "dr")
 
 
+@pytest.mark.parametrize("rows, d", [(3, 40), (2000, 300), (700, 2100), (300, 9000)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_gradients_without_the_weights(rows, d, residual, monkeypatch):
+    """A gain that is frozen has no gradient, and nothing is summed for it; the others' bits are the same."""
+    from verification.commitment import native
+    g = _gen(15)
+    x, w = _rand(g, rows, d, dtype=BF), _rand(g, d)
+    res, o = _rand(g, rows, d) if residual else None, _rand(g, rows, d, dtype=BF)
+    calls = []
+    lib = native.get()
+    run = lib.operator
+
+    def operator(name, args, device):
+        calls.append((name, args))
+        return run(name, args, device)
+
+    monkeypatch.setattr(lib, "operator", operator)
+    got = []
+    for frozen in (False, True):
+        leaves = [t.detach().clone().requires_grad_() for t in (x, res) if t is not None]
+        gain = w.clone().requires_grad_(not frozen)
+        y = ops.rms_norm(leaves[0], gain, residual=leaves[1] if residual else None)
+        (y[0] if residual else y).backward(o)
+        got.append([t.grad for t in leaves])
+        name, args = calls.pop()
+        assert name == "rms_norm_backward" and (gain.grad is None) == frozen
+        assert (ops._NORM.unpack(args)[11] == 0) == frozen  # where dweight goes
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 # ---- 8 bits ---------------------------------------------------------------------------------
 
 def _quantized_check(x, w, residual, dtype, block):
